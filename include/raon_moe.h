@@ -45,6 +45,13 @@ extern "C" {
 /* Activations (host/backend.py:47-62 SiTU-GLU; kernels/moe/reference.py:127-180 SwiGLU). */
 #define RMOE_ACT_SITU 0
 #define RMOE_ACT_SWIGLU 1
+/* Activations of one value, for the products with an epilogue only (rmoe_linear_act_dev,
+ * rmoe_experts_linear_dev): the value itself, z sigmoid(z), z times the normal distribution
+ * function of z, and that with 0.5 (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3))) in its place. */
+#define RMOE_ACT_NONE 2
+#define RMOE_ACT_SILU 3
+#define RMOE_ACT_GELU 4
+#define RMOE_ACT_GELU_TANH 5
 
 /* Router score functions (host/raon.py:1233-1234 sigmoid; softmax for BASELINE configs). */
 #define RMOE_SCORE_SIGMOID 0
@@ -53,6 +60,11 @@ extern "C" {
 /* Weight formats of a dense matrix (BundleMeta.fmt, npu/backend.py:104-117). */
 #define RMOE_FMT_Q4NX 0  /* "q4nx_gemv": 5 bits per weight (quant/q4nx.py:335-393)       */
 #define RMOE_FMT_BFP16 1 /* "bfp16_gemv": bfp16ebs8, 9 bits per weight (quant/bfp16.py) */
+
+/* Element types of token rows. */
+#define RMOE_DT_BF16 0
+#define RMOE_DT_F16 1
+#define RMOE_DT_F32 2
 
 typedef struct rmoe_ctx rmoe_ctx;
 
@@ -117,6 +129,58 @@ int rmoe_linear(rmoe_ctx* ctx, int handle, const uint16_t* x, int T, int K_in, u
 int rmoe_linear_dev(rmoe_ctx* ctx, int handle, const void* x_dev, int T, void* y_dev, void* stream);
 /* Size the scratch that rmoe_linear_dev needs for up to T tokens on this matrix. */
 int rmoe_reserve_linear(rmoe_ctx* ctx, int handle, int T);
+
+/* Dense product with an epilogue, on device operands:
+ *   y = RTNE(act(x W^T + bias) + residual),
+ * fp32 throughout, rounded once.  x bf16 [T, K_in], K_in <= K a multiple of 8 (columns past
+ * it are zero), 16-byte aligned; bias fp32 [M] or NULL; residual bf16 of y's shape or NULL (y
+ * itself: added in place); y bf16 [T, M'].  act RMOE_ACT_NONE, _SILU, _GELU, _GELU_TANH:
+ * M' = M; RMOE_ACT_SWIGLU, _SITU (gate_beta, value_beta): M' = M / 2, row i of W the gate and
+ * row M/2 + i the up of output i, bias added to both.  (rmoe_linear_dev followed by the
+ * activation rounds gate and up to bf16 first; this call does not.)  Asynchronous on
+ * `stream`, never allocates.  The reference adds bias, activation and residual on the host
+ * (host/raon.py:1314-1330). */
+int rmoe_linear_act_dev(rmoe_ctx* ctx, int handle, const void* x_dev, int T, int K_in, const float* bias_dev, int act,
+                        float gate_beta, float value_beta, const void* residual_dev, void* y_dev, void* stream);
+/* Size the scratch that rmoe_linear_act_dev needs for up to T tokens on this matrix. */
+int rmoe_reserve_linear_act(rmoe_ctx* ctx, int handle, int T);
+
+/* ------------------------------------------------------------ tokens by expert --
+ * The steps around the experts' products on device operands, for an engine that puts work of
+ * its own between them.  T tokens of width H in RMOE_DT_* elements, any H >= 1, contiguous
+ * rows at any address of their type; k (1..16) routes per token, A = T k < 2^31 assignments
+ * a = t k + r.  Asynchronous on `stream`; nothing is allocated and no scratch of the context
+ * is used, so that calls on several streams or captured graphs share only the buffers the
+ * caller gives them.  Inputs and outputs of a call must not overlap. */
+
+/* Sort: rows[inv[a]] = x[t] for every assignment whose expert ids[a] is in 0..n_experts-1
+ * (n_experts <= 256), by expert and within an expert in ascending a; order[inv[a]] = a, and
+ * expert e's rows are [offsets[e], offsets[e+1]) (offsets int32 [n_experts + 1]).  A negative
+ * id is a route without an expert (padding, a dropped route, an expert of another GPU):
+ * inv[a] = -1 and no row.  The same expert may appear twice in a token.  rows [A, H], order
+ * [A] and inv [T, k] are written in full except rows and order from offsets[n_experts] on,
+ * which stay as they were.  An id past the experts has no row either, and the next
+ * synchronous call reports it.  The permutation is rmoe_dispatch's
+ * (kernels/moe_grouped/planner.py:76-108), the gather its jobs' (:184-240). */
+int rmoe_sort_tokens_dev(rmoe_ctx* ctx, const void* x_dev, int dtype, int T, int H, const void* ids_dev, int k,
+                         int n_experts, void* rows_dev, void* order_dev, void* inv_dev, void* offsets_dev,
+                         void* stream);
+/* The sort's gradient: dx[t] = sum of drows[inv[t][r]] over the routes with a row (none: zeros),
+ * fp32 in ascending sorted position, rounded once.  drows [A, H], dx [T, H]. */
+int rmoe_sort_tokens_backward_dev(rmoe_ctx* ctx, const void* drows_dev, int dtype, int T, int H, const void* inv_dev,
+                                  int k, void* dx_dev, void* stream);
+/* Combine: out[t] = sum of weights[t][r] rows[inv[t][r]] over the routes with a row, fp32 in
+ * ascending sorted position (= expert id, the order of rmoe_moe_experts_grouped), rounded
+ * once.  rows [A, H], weights fp32 [T, k], out [T, H].  A route without a row takes no part,
+ * whatever its weight. */
+int rmoe_combine_tokens_dev(rmoe_ctx* ctx, const void* rows_dev, int dtype, int T, int H, const void* inv_dev,
+                            const void* weights_dev, int k, void* out_dev, void* stream);
+/* Combine's gradient: drows[inv[t][r]] = weights[t][r] dout[t] (rows no route names stay as
+ * they were), dweights[t][r] = <dout[t], rows[inv[t][r]]> in fp32, 0 without a row.  inv as
+ * rmoe_sort_tokens_dev writes it: no position twice. */
+int rmoe_combine_tokens_backward_dev(rmoe_ctx* ctx, const void* dout_dev, const void* rows_dev, int dtype, int T, int H,
+                                     const void* inv_dev, const void* weights_dev, int k, void* drows_dev,
+                                     void* dweights_dev, void* stream);
 
 /* --------------------------------------------------------------- MoE layers --
  * One MoE layer: n_routed experts + n_shared (0 or 1) shared expert, hidden H,
@@ -285,6 +349,19 @@ int rmoe_moe_decode_stack(rmoe_ctx* ctx, const int* layers, int n_layers, const 
  * ascending expert, then token, then route) and offsets int32 [n_experts + 1]. */
 int rmoe_dispatch(rmoe_ctx* ctx, const int32_t* top_ids, int T, int k, int n_experts, int32_t* order,
                   int32_t* offsets);
+
+/* rmoe_linear_act_dev over sorted rows, each row with the matrix of its expert: for e in
+ * 0..n_routed-1 and offsets[e] <= p < offsets[e+1] (rmoe_sort_tokens_dev's offsets)
+ *   y[p] = RTNE(act(rows[p] W_e^T + bias[e]) + residual[p]).
+ * part RMOE_PART_GATE_UP: W_e [2I, H]; RMOE_PART_DOWN: W_e [H, Ipad], of which K_in = I columns
+ * (or up to Ipad) are read.  rows bf16 [n, K_in], 16-byte aligned, K_in a multiple of 8; bias
+ * fp32 [n_routed, M] or NULL; residual and y bf16 [n, M'].  Rows from offsets[n_routed] on
+ * stay as they were.  Both layer layouts (q4nx and weights-d) are served. */
+int rmoe_experts_linear_dev(rmoe_ctx* ctx, int layer, int part, const void* rows_dev, int n, int K_in,
+                            const void* offsets_dev, const float* bias_dev, int act, float gate_beta, float value_beta,
+                            const void* residual_dev, void* y_dev, void* stream);
+/* Size the scratch that rmoe_experts_linear_dev needs for up to n rows on this layer. */
+int rmoe_reserve_experts_linear(rmoe_ctx* ctx, int layer, int n);
 
 /* Grouped prefill MoE: NpuBackend.moe_experts_grouped (npu/backend.py:4845-4979).
  * x [T, H], top_ids [T, k] (distinct per token, 0..n_routed-1), top_weights fp32 [T, k],

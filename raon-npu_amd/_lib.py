@@ -20,6 +20,13 @@ RMOE_ENOMEM = 4
 
 ACT_SITU = 0
 ACT_SWIGLU = 1
+ACT_NONE = 2
+ACT_SILU = 3
+ACT_GELU = 4
+ACT_GELU_TANH = 5
+DT_BF16 = 0
+DT_F16 = 1
+DT_F32 = 2
 SCORE_SIGMOID = 0
 SCORE_SOFTMAX = 1
 FMT_Q4NX = 0
@@ -54,6 +61,12 @@ SIGNATURES: dict[str, list] = {
     "rmoe_linear": [_p, _i, _p, _i, _i, _p],
     "rmoe_linear_dev": [_p, _i, _p, _i, _p, _p],
     "rmoe_reserve_linear": [_p, _i, _i],
+    "rmoe_linear_act_dev": [_p, _i, _p, _i, _i, _p, _i, _f, _f, _p, _p, _p],
+    "rmoe_reserve_linear_act": [_p, _i, _i],
+    "rmoe_sort_tokens_dev": [_p, _p, _i, _i, _i, _p, _i, _i, _p, _p, _p, _p, _p],
+    "rmoe_sort_tokens_backward_dev": [_p, _p, _i, _i, _i, _p, _i, _p, _p],
+    "rmoe_combine_tokens_dev": [_p, _p, _i, _i, _i, _p, _p, _i, _p, _p],
+    "rmoe_combine_tokens_backward_dev": [_p, _p, _p, _i, _i, _i, _p, _p, _i, _p, _p, _p],
     "rmoe_layer_create": [_p, _i, _i, _i, _i, _i, _i],
     "rmoe_reserve": [_p, _i, _i],
     "rmoe_layer_upload_experts": [_p, _i, _p, _sz, _p, _sz],
@@ -81,6 +94,8 @@ SIGNATURES: dict[str, list] = {
     "rmoe_dispatch": [_p, _p, _i, _i, _i, _p, _p],
     "rmoe_moe_experts_grouped": [_p, _i, _p, _i, _p, _p, _p, _i, _f, _f, _p, _p],
     "rmoe_moe_prefill_dev": [_p, _i, _p, _i, _p, _i, _i, _f, _f, _p, _p, _p],
+    "rmoe_experts_linear_dev": [_p, _i, _i, _p, _i, _i, _p, _p, _i, _f, _f, _p, _p, _p],
+    "rmoe_reserve_experts_linear": [_p, _i, _i],
     "rmoe_moe_experts_grouped_dev": [_p, _i, _p, _i, _p, _p, _p, _i, _f, _f, _p, _p, _p],
 }
 _RESTYPES = {"rmoe_last_error": C.c_char_p, "rmoe_version": C.c_char_p, "rmoe_stream": _p}

@@ -1,0 +1,149 @@
+// y[n, M'] = RTNE(act(x[n, K] @ W^T + bias) + residual), q4nx or bfp16 weights, of one matrix
+// or of each row's expert, on bf16 MFMA (wave_gemm.h): exact products, fp32 sums, one
+// rounding at the end.  Gated activations pair weight row i (gate) with row M/2 + i.
+//
+// One workgroup takes 16 MF rows x 16 NF weight rows (half of them gate, half up when the
+// activation is gated), its W waves a W-th of K each; the waves' sums meet in LDS and are
+// added in wave order, where bias, activation and residual cost nothing but their own bytes.
+// By expert, a workgroup finds its rows from the experts' offsets itself (a wave scan over at
+// most 256 experts), so that the offsets stay on the device.
+#include <algorithm>
+
+#include "linear_act.h"
+#include "wave_gemm.h"
+
+namespace rmoe {
+namespace {
+
+constexpr int kPad = 4;  // floats of padding per row of the partial sums
+
+// Gated tiles hold NF / 2 fragments of gate rows, then the up rows of the same units.
+template <int kFmt, int MF, int NF, int XI, bool kGated>
+__global__ __launch_bounds__(512) void linear_act_kernel(LinAct a, int n_nt) {
+  extern __shared__ __attribute__((aligned(16))) float la_lds[];
+  constexpr int kTB = kFmt == RMOE_FMT_BFP16 ? kB16TileBytes : kTileBytes;
+  constexpr int kCols = 16 * NF, kStride = kCols + kPad, kOut = kGated ? kCols / 2 : kCols;
+  constexpr int BM = XI == 1 ? 4 : 16 * MF;  // rows of a tile
+  RowTiles<BM> rt;
+  const int n_mt = a.offsets ? rt.total(a.offsets, a.n_experts, a.n) : (a.n + BM - 1) / BM;
+  // XCD x takes a contiguous eighth of the tiles, the row tiles of one weight tile (by
+  // expert: the weight tiles of one row tile) back to back.
+  const int total = n_mt * n_nt, per = (total + 7) / 8, slot = (int)blockIdx.x / 8;
+  const int id = ((int)blockIdx.x % 8) * per + slot;
+  if (slot >= per || id >= total) return;
+  int nt, e = 0, row0, nrow;
+  if (a.offsets) {
+    nt = id % n_nt;
+    rt.find(id / n_nt, e, row0, nrow);
+  } else {
+    nt = id / n_mt;
+    row0 = (id % n_mt) * BM;
+    nrow = min(BM, a.n - row0);
+  }
+  const int tid = threadIdx.x, lane = tid & 63, wave = wave_id(), W = blockDim.x >> 6;
+  const int l16 = lane & 15, lq = lane >> 4;
+  const int nkt = a.K / kTileCols;
+  const uint8_t* tiles = a.tiles + (size_t)e * a.wstride;
+  WaveOperands<MF, NF, XI, true> o;
+#pragma unroll
+  for (int f = 0; f < NF; ++f) {
+    const int row = kGated ? nt * kOut + 16 * (f % (NF / 2 > 0 ? NF / 2 : 1)) + (f >= NF / 2 ? a.M / 2 : 0)
+                           : nt * kCols + 16 * f;
+    o.w[f] = tiles + (size_t)(row / kTileRows) * nkt * kTB + (row % kTileRows) * 16;
+  }
+  // Rows past the tile repeat its last one; their results are not stored.
+  o.x = reinterpret_cast<const uint8_t*>(a.x + (size_t)row0 * a.K_in);
+#pragma unroll
+  for (int m = 0; m < MF; ++m)
+#pragma unroll
+    for (int i = 0; i < XI; ++i)
+      o.xoff[m][i] = (uint32_t)min(16 * m + 4 * i + lq, nrow - 1) * (uint32_t)(2 * a.K_in) + 16u * (uint32_t)l16;
+  o.xchunks = (uint32_t)a.K_in / 8u;
+  o.lds = reinterpret_cast<uint8_t*>(la_lds) + (size_t)wave * 4096 * MF;
+  wg_f32x4 acc[MF][NF];
+#pragma unroll
+  for (int m = 0; m < MF; ++m)
+#pragma unroll
+    for (int f = 0; f < NF; ++f) acc[m][f] = wg_f32x4{0.f, 0.f, 0.f, 0.f};
+  wave_gemm<kFmt, MF, NF, XI>(o, wave * nkt / W, (wave + 1) * nkt / W, acc);
+  __syncthreads();  // the partial sums reuse the waves' activation regions
+  float* mine = la_lds + (size_t)wave * 16 * MF * kStride;
+#pragma unroll
+  for (int m = 0; m < MF; ++m)
+#pragma unroll
+    for (int f = 0; f < NF; ++f)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) mine[(16 * m + 4 * lq + i) * kStride + 16 * f + l16] = acc[m][f][i];
+  __syncthreads();
+  constexpr float kUnit = kFmt == RMOE_FMT_BFP16 ? 4.f : 1.f;  // see wave_gemm.h
+  auto sum = [&](int t, int c) {
+    float v = la_lds[t * kStride + c];
+    for (int w = 1; w < W; ++w) v += la_lds[(size_t)w * 16 * MF * kStride + t * kStride + c];
+    return kUnit * v;
+  };
+  const int width = kGated ? a.M / 2 : a.M;
+  const float* bias = a.bias ? a.bias + (size_t)e * a.M : nullptr;
+  for (int i = tid; i < nrow * kOut; i += blockDim.x) {
+    const int t = i / kOut, c = i % kOut, col = nt * kOut + c;
+    float z = sum(t, c);
+    if (bias) z += bias[col];
+    if constexpr (kGated) {
+      float u = sum(t, kOut + c);
+      if (bias) u += bias[a.M / 2 + col];
+      z = act_apply(a.act, z, u, a.gb, a.vb);
+    } else {
+      z = act_single(a.act, z);
+    }
+    const size_t at = (size_t)(row0 + t) * width + col;
+    if (a.residual) z += bf16_to_f32(a.residual[at]);
+    a.y[at] = (uint16_t)f32_to_bf16(z);
+  }
+}
+
+// Dynamic LDS of W waves: their activation regions, then in the same place their partial sums.
+constexpr size_t act_lds(int MF, int NF, int W) {
+  const size_t sums = (size_t)16 * MF * (16 * NF + kPad) * 4, rows = (size_t)4096 * MF;
+  return W * (sums > rows ? sums : rows);
+}
+
+template <int kFmt, int MF, int NF, int XI>
+hipError_t launch(const LinAct& a, hipStream_t st) {
+  const int nkt = a.K / kTileCols, W = std::min(nkt, nkt >= 64 ? 8 : 4);
+  constexpr int BM = XI == 1 ? 4 : 16 * MF;
+  const size_t mt = a.offsets ? std::min<size_t>(a.n, (size_t)a.n / BM + a.n_experts) : ((size_t)a.n + BM - 1) / BM;
+  const size_t total = mt * (a.M / (16 * NF)), grid = 8 * ((total + 7) / 8);
+  if (grid * 64 * W >= (size_t)1 << 32 || total >= (size_t)1 << 31) return hipErrorInvalidValue;
+  auto* kernel = act_gated(a.act) ? linear_act_kernel<kFmt, MF, NF, XI, (NF > 1)> : linear_act_kernel<kFmt, MF, NF, XI, false>;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(64 * W), act_lds(MF, NF, W), st, a, a.M / (16 * NF));
+  return hipGetLastError();
+}
+
+template <int kFmt>
+hipError_t pick(const LinAct& a, hipStream_t st) {
+  const bool gated = act_gated(a.act);
+  if (a.n <= 4) {
+    if (gated || a.M / 32 >= 448) return launch<kFmt, 1, 2, 1>(a, st);
+    return launch<kFmt, 1, 1, 1>(a, st);
+  }
+  return launch<kFmt, 2, 4, 4>(a, st);
+}
+
+}  // namespace
+
+hipError_t linear_act_setup() {
+  const void* fns[4] = {(const void*)linear_act_kernel<RMOE_FMT_Q4NX, 2, 4, 4, true>,
+                        (const void*)linear_act_kernel<RMOE_FMT_Q4NX, 2, 4, 4, false>,
+                        (const void*)linear_act_kernel<RMOE_FMT_BFP16, 2, 4, 4, true>,
+                        (const void*)linear_act_kernel<RMOE_FMT_BFP16, 2, 4, 4, false>};
+  for (const void* f : fns) {
+    const hipError_t e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, (int)act_lds(2, 4, 8));
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
+}
+
+hipError_t launch_linear_act(const LinAct& a, hipStream_t st) {
+  return a.fmt == RMOE_FMT_BFP16 ? pick<RMOE_FMT_BFP16>(a, st) : pick<RMOE_FMT_Q4NX>(a, st);
+}
+
+}  // namespace rmoe

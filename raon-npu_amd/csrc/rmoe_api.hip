@@ -254,6 +254,7 @@ int sync_and_check(rmoe_ctx* ctx, hipStream_t st) {
       }
       return fail(RMOE_EDEVICE, "persistent decode kernel timed out waiting for other workgroups");
     }
+    if (err & 16) return fail(RMOE_EINVAL, "sorted position out of range in inv");
     return fail(RMOE_EDEVICE, "device error flag 0x%x", err);
   }
   return RMOE_OK;
@@ -299,6 +300,76 @@ int check_ids(const int32_t* ids, int T, int k, int n_routed) {
     }
   }
   return RMOE_OK;
+}
+
+// The context's device for the launches of a call, the caller's current device afterwards.
+struct OnDevice {
+  int before = -1;
+  hipError_t status;
+  explicit OnDevice(const rmoe_ctx* ctx) {
+    status = hipGetDevice(&before);
+    if (status == hipSuccess && before != ctx->device) status = hipSetDevice(ctx->device);
+    else before = -1;
+  }
+  ~OnDevice() {
+    if (before >= 0) (void)hipSetDevice(before);
+  }
+};
+
+// An operand's bytes; operands may not overlap an output.
+struct Span {
+  const void* p;
+  size_t n;
+};
+bool overlap(const Span& a, const Span& b) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a.p), y = reinterpret_cast<uintptr_t>(b.p);
+  return a.p && b.p && x < y + b.n && y < x + a.n;
+}
+// Every output against every operand and the other outputs.
+int check_overlap(std::initializer_list<Span> in, std::initializer_list<Span> out) {
+  for (const Span* o = out.begin(); o != out.end(); ++o) {
+    for (const Span& i : in)
+      if (overlap(*o, i)) return fail(RMOE_EINVAL, "an output overlaps an input");
+    for (const Span* q = out.begin(); q != o; ++q)
+      if (overlap(*o, *q)) return fail(RMOE_EINVAL, "two outputs overlap");
+  }
+  return RMOE_OK;
+}
+
+// Token rows of the sort and combine calls.
+int check_tokens(rmoe_ctx* ctx, int dtype, int T, int H, int k, std::initializer_list<const void*> rows) {
+  if (!ctx) return fail(RMOE_EINVAL, "null context");
+  if (dtype != RMOE_DT_BF16 && dtype != RMOE_DT_F16 && dtype != RMOE_DT_F32)
+    return fail(RMOE_EINVAL, "unknown element type %d", dtype);
+  if (T < 1 || H < 1) return fail(RMOE_EINVAL, "T (%d) and H (%d) must be >= 1", T, H);
+  if (k < 1 || k > 16) return fail(RMOE_EINVAL, "k (%d) must be in 1..16", k);
+  if ((size_t)T * k >= (size_t)1 << 31) return fail(RMOE_EINVAL, "%d x %d routes are too many", T, k);
+  for (const void* p : rows)
+    if (reinterpret_cast<uintptr_t>(p) % (dtype == RMOE_DT_F32 ? 4 : 2))
+      return fail(RMOE_EINVAL, "rows must be aligned to their element type");
+  return RMOE_OK;
+}
+size_t row_bytes(int dtype, int H) { return (size_t)H * (dtype == RMOE_DT_F32 ? 4 : 2); }
+
+// Shapes and operands of a product with an epilogue (L: weights, rows and epilogue filled in).
+int check_linear_act(const rmoe::LinAct& L) {
+  if (!L.x || !L.y) return fail(RMOE_EINVAL, "null argument");
+  if (L.n < 1) return fail(RMOE_EINVAL, "the number of rows must be >= 1");
+  if (L.act < RMOE_ACT_SITU || L.act > RMOE_ACT_GELU_TANH) return fail(RMOE_EINVAL, "unknown activation %d", L.act);
+  if (L.K_in < 8 || L.K_in > L.K || L.K_in % 8)
+    return fail(RMOE_EINVAL, "input width %d must be a multiple of 8 and at most K=%d", L.K_in, L.K);
+  if (L.act == RMOE_ACT_SITU && (L.gb == 0.f || L.vb == 0.f)) return fail(RMOE_EINVAL, "SiTU betas must not be zero");
+  if (reinterpret_cast<uintptr_t>(L.x) & 15) return fail(RMOE_EINVAL, "the input rows must be 16-byte aligned");
+  if ((reinterpret_cast<uintptr_t>(L.y) | reinterpret_cast<uintptr_t>(L.residual)) & 1 ||
+      (reinterpret_cast<uintptr_t>(L.bias) | reinterpret_cast<uintptr_t>(L.offsets)) & 3)
+    return fail(RMOE_EINVAL, "operands must be aligned to their element type");
+  const bool gated = L.act == RMOE_ACT_SITU || L.act == RMOE_ACT_SWIGLU;
+  const Span y{L.y, (size_t)L.n * (gated ? L.M / 2 : L.M) * 2};
+  // The residual may be y itself (each element is read before it is written), not a part of it.
+  const Span res{L.residual == L.y ? nullptr : L.residual, y.n};
+  const size_t groups = L.offsets ? L.n_experts : 1;
+  return check_overlap({{L.x, (size_t)L.n * L.K_in * 2}, res, {L.bias, groups * L.M * 4},
+                        {L.offsets, (size_t)(L.n_experts + 1) * 4}}, {y});
 }
 
 // ------------------------------------------------------- static decode scratch --
@@ -382,7 +453,8 @@ int rmoe_create(int device, rmoe_ctx** out) {
   }
   bool ok = hipHostMalloc((void**)&ctx->pinned, kPinnedBytes, hipHostMallocDefault) == hipSuccess &&
             hipHostGetDevicePointer((void**)&ctx->pinned_dev, ctx->pinned, 0) == hipSuccess;
-  ok = ok && rmoe::prefill_setup() == hipSuccess && rmoe::linear_mfma_setup() == hipSuccess;
+  ok = ok && rmoe::prefill_setup() == hipSuccess && rmoe::linear_mfma_setup() == hipSuccess &&
+       rmoe::linear_act_setup() == hipSuccess;
   for (hipEvent_t& ev : ctx->chunk_done) ok = ok && hipEventCreateWithFlags(&ev, hipEventDisableTiming) == hipSuccess;
   if (!ok) {
     free_base(ctx);
@@ -635,6 +707,111 @@ int rmoe_reserve_linear(rmoe_ctx* ctx, int handle, int T) {
   linear_needs(m->M, m->K, T, f, c);
   TRY(grow(ctx->s.part, ctx->s.part_floats, f, ctx));
   TRY(grow(ctx->s.counters, ctx->s.n_counters, c, ctx));
+  return RMOE_OK;
+}
+
+static int run_linear_act(rmoe_ctx* ctx, const rmoe::LinAct& L, void* stream) {
+  TRY(check_linear_act(L));
+  OnDevice dev(ctx);
+  HIP_TRY(dev.status);
+  const hipError_t e = rmoe::launch_linear_act(L, pick_stream(ctx, stream));
+  if (e == hipErrorInvalidValue) return fail(RMOE_EINVAL, "%d rows of width %d are too many for one call", L.n, L.K_in);
+  HIP_TRY(e);
+  return RMOE_OK;
+}
+
+int rmoe_linear_act_dev(rmoe_ctx* ctx, int handle, const void* x_dev, int T, int K_in, const float* bias_dev, int act,
+                        float gate_beta, float value_beta, const void* residual_dev, void* y_dev, void* stream) {
+  RmoeMatrix* m;
+  TRY(find_matrix(ctx, handle, &m));
+  const rmoe::LinAct L{m->tiles, 0, m->fmt, m->M, m->K, (const uint16_t*)x_dev, T, K_in, nullptr, 0, bias_dev, act,
+                       gate_beta, value_beta, (const uint16_t*)residual_dev, (uint16_t*)y_dev};
+  return run_linear_act(ctx, L, stream);
+}
+
+int rmoe_reserve_linear_act(rmoe_ctx* ctx, int handle, int T) {
+  RmoeMatrix* m;
+  TRY(find_matrix(ctx, handle, &m));
+  if (T < 1) return fail(RMOE_EINVAL, "T must be >= 1");
+  return RMOE_OK;
+}
+
+int rmoe_experts_linear_dev(rmoe_ctx* ctx, int layer, int part, const void* rows_dev, int n, int K_in,
+                            const void* offsets_dev, const float* bias_dev, int act, float gate_beta, float value_beta,
+                            const void* residual_dev, void* y_dev, void* stream) {
+  RmoeLayer* l;
+  TRY(check_layer(ctx, layer, &l));
+  if (part != RMOE_PART_GATE_UP && part != RMOE_PART_DOWN)
+    return fail(RMOE_EINVAL, "part must be RMOE_PART_GATE_UP or RMOE_PART_DOWN, got %d", part);
+  if (!offsets_dev) return fail(RMOE_EINVAL, "null argument");
+  const bool up = part == RMOE_PART_GATE_UP;
+  const rmoe::LinAct L{up ? l->gu : l->dn, up ? l->gu_bytes : l->dn_bytes, up ? RMOE_FMT_Q4NX : l->dn_fmt,
+                       up ? 2 * l->I : l->H, up ? l->H : l->Ipad, (const uint16_t*)rows_dev, n, K_in,
+                       (const int32_t*)offsets_dev, l->n_routed, bias_dev, act, gate_beta, value_beta,
+                       (const uint16_t*)residual_dev, (uint16_t*)y_dev};
+  return run_linear_act(ctx, L, stream);
+}
+
+int rmoe_reserve_experts_linear(rmoe_ctx* ctx, int layer, int n) {
+  RmoeLayer* l;
+  TRY(check_layer(ctx, layer, &l));
+  if (n < 1) return fail(RMOE_EINVAL, "n must be >= 1");
+  return RMOE_OK;
+}
+
+// ----------------------------------------------------------- tokens by expert --
+int rmoe_sort_tokens_dev(rmoe_ctx* ctx, const void* x, int dtype, int T, int H, const void* ids, int k, int n_experts,
+                         void* rows, void* order, void* inv, void* offsets, void* stream) {
+  TRY(check_tokens(ctx, dtype, T, H, k, {x, rows}));
+  if (!x || !ids || !rows || !order || !inv || !offsets) return fail(RMOE_EINVAL, "null argument");
+  if (n_experts < 1 || n_experts > 256) return fail(RMOE_EINVAL, "n_experts (%d) must be in 1..256", n_experts);
+  const size_t rb = row_bytes(dtype, H), A = (size_t)T * k;
+  TRY(check_overlap({{x, T * rb}, {ids, A * 4}},
+                    {{rows, A * rb}, {order, A * 4}, {inv, A * 4}, {offsets, (size_t)(n_experts + 1) * 4}}));
+  OnDevice dev(ctx);
+  HIP_TRY(dev.status);
+  HIP_TRY(rmoe::launch_sort_tokens(x, dtype, T, H, (const int32_t*)ids, k, n_experts, rows, (int32_t*)order,
+                                   (int32_t*)inv, (int32_t*)offsets, ctx->s.err, pick_stream(ctx, stream)));
+  return RMOE_OK;
+}
+
+int rmoe_sort_tokens_backward_dev(rmoe_ctx* ctx, const void* drows, int dtype, int T, int H, const void* inv, int k,
+                                  void* dx, void* stream) {
+  TRY(check_tokens(ctx, dtype, T, H, k, {drows, dx}));
+  if (!drows || !inv || !dx) return fail(RMOE_EINVAL, "null argument");
+  const size_t rb = row_bytes(dtype, H), A = (size_t)T * k;
+  TRY(check_overlap({{drows, A * rb}, {inv, A * 4}}, {{dx, T * rb}}));
+  OnDevice dev(ctx);
+  HIP_TRY(dev.status);
+  HIP_TRY(rmoe::launch_sum_rows(drows, dtype, T, H, (const int32_t*)inv, nullptr, k, dx, ctx->s.err,
+                                pick_stream(ctx, stream)));
+  return RMOE_OK;
+}
+
+int rmoe_combine_tokens_dev(rmoe_ctx* ctx, const void* rows, int dtype, int T, int H, const void* inv,
+                            const void* weights, int k, void* out, void* stream) {
+  TRY(check_tokens(ctx, dtype, T, H, k, {rows, out}));
+  if (!rows || !inv || !weights || !out) return fail(RMOE_EINVAL, "null argument");
+  const size_t rb = row_bytes(dtype, H), A = (size_t)T * k;
+  TRY(check_overlap({{rows, A * rb}, {inv, A * 4}, {weights, A * 4}}, {{out, T * rb}}));
+  OnDevice dev(ctx);
+  HIP_TRY(dev.status);
+  HIP_TRY(rmoe::launch_sum_rows(rows, dtype, T, H, (const int32_t*)inv, (const float*)weights, k, out, ctx->s.err,
+                                pick_stream(ctx, stream)));
+  return RMOE_OK;
+}
+
+int rmoe_combine_tokens_backward_dev(rmoe_ctx* ctx, const void* dout, const void* rows, int dtype, int T, int H,
+                                     const void* inv, const void* weights, int k, void* drows, void* dweights,
+                                     void* stream) {
+  TRY(check_tokens(ctx, dtype, T, H, k, {dout, rows, drows}));
+  if (!dout || !rows || !inv || !weights || !drows || !dweights) return fail(RMOE_EINVAL, "null argument");
+  const size_t rb = row_bytes(dtype, H), A = (size_t)T * k;
+  TRY(check_overlap({{dout, T * rb}, {rows, A * rb}, {inv, A * 4}, {weights, A * 4}}, {{drows, A * rb}, {dweights, A * 4}}));
+  OnDevice dev(ctx);
+  HIP_TRY(dev.status);
+  HIP_TRY(rmoe::launch_combine_grad(dout, rows, dtype, T, H, (const int32_t*)inv, (const float*)weights, k, drows,
+                                    (float*)dweights, ctx->s.err, pick_stream(ctx, stream)));
   return RMOE_OK;
 }
 

@@ -517,6 +517,37 @@ hipError_t launch_router_prep(const uint16_t* x, int T, int H, const uint16_t* w
 hipError_t launch_topk(const float* logits, int T, int E, int k, int score, const float* bias, int renorm,
                        float scaling, int32_t* ids, float* wts, int32_t* counts, hipStream_t st);
 
+// Tokens to expert-sorted rows and back (token_sort.hip).  Up to kSortSmall assignments are
+// sorted by one launch in which every workgroup counts over all of them; beyond, by four.
+constexpr int kSortSmall = 1024;
+hipError_t launch_sort_tokens(const void* x, int dtype, int T, int H, const int32_t* ids, int k, int n_experts,
+                              void* rows, int32_t* order, int32_t* inv, int32_t* offsets, int* err, hipStream_t st);
+// wts null: ones (the gradient of the sort).
+hipError_t launch_sum_rows(const void* rows, int dtype, int T, int H, const int32_t* inv, const float* wts, int k,
+                           void* out, int* err, hipStream_t st);
+hipError_t launch_combine_grad(const void* dout, const void* rows, int dtype, int T, int H, const int32_t* inv,
+                               const float* wts, int k, void* drows, float* dwts, int* err, hipStream_t st);
+
+// y = act(x W^T + bias) + residual over n rows (linear_act.hip): of one matrix (offsets null),
+// or row p with the matrix of its expert e, offsets[e] <= p < offsets[e + 1], wstride bytes
+// and M biases apart.
+struct LinAct {
+  const uint8_t* tiles;
+  size_t wstride;
+  int fmt, M, K;
+  const uint16_t* x;  // [n, K_in], 16-byte aligned, K_in % 8 == 0; weights past K_in see zeros
+  int n, K_in;
+  const int32_t* offsets;
+  int n_experts;
+  const float* bias;
+  int act;
+  float gb, vb;
+  const uint16_t* residual;
+  uint16_t* y;
+};
+hipError_t linear_act_setup();  // once per device before the first call
+hipError_t launch_linear_act(const LinAct& a, hipStream_t st);
+
 // Persistent decode of n_layers (<= kMaxStack) layers of one geometry for one token
 // (moe_decode_stack.hip).  One workgroup per CU (grid n_cu).  ids_out/wts_out: [n_layers, k]
 // or null.  Scratch: stack_scratch_bytes / stack_counter_count; counters must be zero.

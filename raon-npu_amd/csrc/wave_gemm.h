@@ -59,12 +59,15 @@ __device__ __forceinline__ uint4 q4_pairs(uint32_t v, const Q4Masks& k) {
 // What a wave multiplies.  Lane (l16, lq) = (lane % 16, lane / 16).
 // XI: how many of a fragment's four row quartets are loaded (1 when at most 4 rows live; the
 // rows that are not loaded hold arbitrary values, which reach only their own results).
-template <int MF, int NF, int XI>
+// kTail: the activation rows end at column 8 xchunks, short of K; the columns past it are
+// taken as zero and not read.
+template <int MF, int NF, int XI, bool kTail = false>
 struct WaveOperands {
   const uint8_t* w[NF];   // fragment f's first K tile, advanced to its first row (uniform)
   const uint8_t* x;       // activations (uniform)
   uint32_t xoff[MF][XI];  // byte offset of activation row 16m + 4i + lq, plus 16 l16
   uint8_t* lds;           // 4096 MF bytes of the wave's own
+  uint32_t xchunks;       // kTail: 16-byte chunks per activation row
 };
 
 template <typename T>
@@ -82,7 +85,7 @@ __device__ __forceinline__ uint4 wg_load_weights(const uint8_t* base, uint32_t o
 // The activation rows of one K tile: global -> registers -> LDS -> MFMA operands.  In LDS
 // the 16-byte chunk c of row r sits at chunk c ^ (r % 16), so that both the writes (16
 // lanes on one row) and the reads (one chunk of 16 rows) cover all banks.
-template <int MF, int NF, int XI>
+template <int MF, int NF, int XI, bool kTail = false>
 struct WaveRows {
   uint4 raw[MF][XI];
   uint32_t wr, rd;
@@ -92,7 +95,18 @@ struct WaveRows {
     rd = 256u * l16 + 16u * (l16 ^ lq);
   }
   // live == false: every lane reads the same 16 bytes (the last tile's refill is not used).
-  __device__ __forceinline__ void load(const WaveOperands<MF, NF, XI>& o, int kt, bool live) {
+  __device__ __forceinline__ void load(const WaveOperands<MF, NF, XI, kTail>& o, int kt, bool live) {
+    if constexpr (kTail) {
+      const bool in = 16u * (uint32_t)kt + (threadIdx.x & 15u) < o.xchunks;
+#pragma unroll
+      for (int m = 0; m < MF; ++m)
+#pragma unroll
+        for (int i = 0; i < XI; ++i) {
+          const uint4 v = wg_load<uint4>(o.x, live && in ? o.xoff[m][i] + 256u * (uint32_t)kt : 0u);
+          raw[m][i] = in ? v : make_uint4(0u, 0u, 0u, 0u);
+        }
+      return;
+    }
     const uint8_t* xb = o.x + (size_t)kt * 256;
 #pragma unroll
     for (int m = 0; m < MF; ++m)
@@ -133,8 +147,8 @@ __device__ __forceinline__ uint4 b16_operand(uint32_t v0, uint32_t v1, float s) 
 // lq) holds activation rows 16m + 4lq + i (i = 0..3) of weight row l16 of fragment f.
 // The loads of tile kt + 1 are in flight under the MFMAs of tile kt (two register sets).
 // bfp16 sums are a quarter of the product's.
-template <int MF, int NF, int XI>
-__device__ __forceinline__ void wave_gemm_b16(const WaveOperands<MF, NF, XI>& o, int kt0, int kt1,
+template <int MF, int NF, int XI, bool kTail>
+__device__ __forceinline__ void wave_gemm_b16(const WaveOperands<MF, NF, XI, kTail>& o, int kt0, int kt1,
                                               wg_f32x4 (&acc)[MF][NF]) {
   const uint32_t lane = threadIdx.x & 63u, l16 = lane & 15u, lq = lane >> 4;
   if (kt0 >= kt1) return;
@@ -143,7 +157,7 @@ __device__ __forceinline__ void wave_gemm_b16(const WaveOperands<MF, NF, XI>& o,
   struct W {
     uint4 mt[NF][2], e[NF];
   } wa, wb;
-  WaveRows<MF, NF, XI> xr;
+  WaveRows<MF, NF, XI, kTail> xr;
   const uint32_t rd = 256u * l16 + 16u * (l16 ^ (2u * lq));
   auto load = [&](int kt, bool live, W& w) {
 #pragma unroll
@@ -200,8 +214,8 @@ __device__ __forceinline__ void wg_swap16(uint32_t& a, uint32_t& b) {
   b = r[1];
 }
 
-template <int MF, int NF, int XI>
-__device__ __forceinline__ void wave_gemm_q4(const WaveOperands<MF, NF, XI>& o, int kt0, int kt1,
+template <int MF, int NF, int XI, bool kTail>
+__device__ __forceinline__ void wave_gemm_q4(const WaveOperands<MF, NF, XI, kTail>& o, int kt0, int kt1,
                                              wg_f32x4 (&acc)[MF][NF]) {
   const uint32_t lane = threadIdx.x & 63u, l16 = lane & 15u, lq = lane >> 4;
   const Q4Masks masks = q4_masks();
@@ -212,7 +226,7 @@ __device__ __forceinline__ void wave_gemm_q4(const WaveOperands<MF, NF, XI>& o, 
     uint4 c[NF];   // codes of row l16, group lq
     uint4 sm[NF];  // scale | min words of row l16
   } wa, wb;
-  WaveRows<MF, NF, XI> xr;
+  WaveRows<MF, NF, XI, kTail> xr;
   auto load = [&](int kt, bool live, W& w) {
 #pragma unroll
     for (int f = 0; f < NF; ++f) {
@@ -378,12 +392,12 @@ __device__ __forceinline__ void wave_gemm_q4(const WaveOperands<MF, NF, XI>& o, 
   }
 }
 
-template <int kFmt, int MF, int NF, int XI>
-__device__ __forceinline__ void wave_gemm(const WaveOperands<MF, NF, XI>& o, int kt0, int kt1, wg_f32x4 (&acc)[MF][NF]) {
+template <int kFmt, int MF, int NF, int XI, bool kTail>
+__device__ __forceinline__ void wave_gemm(const WaveOperands<MF, NF, XI, kTail>& o, int kt0, int kt1, wg_f32x4 (&acc)[MF][NF]) {
   if constexpr (kFmt == RMOE_FMT_BFP16)
-    wave_gemm_b16<MF, NF, XI>(o, kt0, kt1, acc);
+    wave_gemm_b16<MF, NF, XI, kTail>(o, kt0, kt1, acc);
   else
-    wave_gemm_q4<MF, NF, XI>(o, kt0, kt1, acc);
+    wave_gemm_q4<MF, NF, XI, kTail>(o, kt0, kt1, acc);
 }
 
 }  // namespace rmoe

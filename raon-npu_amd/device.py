@@ -12,7 +12,8 @@ import ctypes as C
 import numpy as np
 
 from . import _lib
-from ._lib import ACT_SITU, ACT_SWIGLU, BUNDLE_B1, BUNDLE_B2, PART_DOWN, PART_GATE_UP, SCORE_SIGMOID, SCORE_SOFTMAX, call, new_bytes, ptr
+from ._lib import (ACT_GELU, ACT_GELU_TANH, ACT_NONE, ACT_SILU, ACT_SITU, ACT_SWIGLU, BUNDLE_B1, BUNDLE_B2, DT_BF16, DT_F16,
+                   DT_F32, PART_DOWN, PART_GATE_UP, SCORE_SIGMOID, SCORE_SOFTMAX, call, new_bytes, ptr)
 from .geometry import MoeGeometry
 
 
@@ -42,6 +43,47 @@ def _check_dev(t, shape: tuple, dtype_name: str, name: str):
         raise ValueError(f"{name} must be {dtype_name}, got {t.dtype}")
     if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
+
+
+_ROW_TYPES = {"bfloat16": DT_BF16, "int16": DT_BF16, "float16": DT_F16, "float32": DT_F32}
+_EPILOGUE_ACTS = {"none": ACT_NONE, "silu": ACT_SILU, "gelu": ACT_GELU, "gelu_tanh": ACT_GELU_TANH, "swiglu": ACT_SWIGLU,
+                  "situ": ACT_SITU}
+
+
+def _row_type(t, name: str) -> str:
+    """The element type of token rows: "bfloat16" (or its bits as "int16"), "float16" or "float32"."""
+    dt = str(getattr(t, "dtype", None)).split(".")[-1]
+    if dt not in _ROW_TYPES:
+        raise ValueError(f"{name} must be bfloat16 (or int16 bits), float16 or float32, got {dt}")
+    return dt
+
+
+def _shape2(t, name: str) -> tuple[int, int]:
+    shape = tuple(getattr(t, "shape", ()))
+    if len(shape) != 2:
+        raise ValueError(f"{name} must be a matrix, got shape {shape}")
+    return int(shape[0]), int(shape[1])
+
+
+def _check_on(ctx: "Context", named: dict):
+    """Tensors of a call live on the context's GPU (None: an operand left out)."""
+    for name, t in named.items():
+        if t is not None and t.device.index != ctx.device:
+            raise ValueError(f"{name} is on {t.device}, the context on cuda:{ctx.device}")
+
+
+def _check_bf16(t, shape: tuple, name: str):
+    """bf16 values of a given shape, as bfloat16 or as int16 bits."""
+    _check_dev(t, shape, "int16" if str(getattr(t, "dtype", None)) == "torch.int16" else "bfloat16", name)
+
+
+def _epilogue_act(act: str, gate_beta, value_beta) -> tuple[int, float, float, bool]:
+    """(code, gate_beta, value_beta, gated) of an epilogue's activation name."""
+    if act not in _EPILOGUE_ACTS:
+        raise ValueError(f"act must be one of {sorted(_EPILOGUE_ACTS)}, got {act!r}")
+    if (act == "situ") != (gate_beta is not None) or (act == "situ") != (value_beta is not None):
+        raise ValueError("gate_beta and value_beta go with act='situ', and only with it")
+    return (_EPILOGUE_ACTS[act], float(gate_beta or 0.0), float(value_beta or 0.0), act in ("swiglu", "situ"))
 
 
 _HIP_STREAM_LEGACY = 1  # hipStreamLegacy: the null stream, with its implicit ordering
@@ -185,6 +227,74 @@ class Context:
         call("rmoe_moe_decode_stack_dev", self._h, ptr(ids), ids.size, ptr(x_dev), ptr(out_dev), int(bool(residual)),
              act, gb, vb, ptr(ids_dev), ptr(wts_dev), _stream_ptr(stream))
 
+    # ---------------------------------------------------- tokens by expert --
+    def sort_tokens_dev(self, x_dev, ids_dev, n_experts: int, rows_dev, order_dev, inv_dev, offsets_dev, stream=None):
+        """Rows by expert: ``rows[inv[t, r]] = x[t]`` for ids int32 [T, k] (negative: no row,
+        inv -1), ascending expert, then assignment ``t * k + r`` (``order``); expert e's rows are
+        ``offsets[e]:offsets[e + 1]``.  x [T, H] and rows [T * k, H] bfloat16 (or int16 bits),
+        float16 or float32; order int32 [T * k], inv [T, k], offsets [n_experts + 1].  Rows and
+        order from ``offsets[n_experts]`` on stay as they were.  Asynchronous; allocates
+        nothing and uses no scratch (capturable, any number of calls at once)."""
+        dt = _row_type(x_dev, "x")
+        T, H = _shape2(x_dev, "x")
+        _, k = _shape2(ids_dev, "ids")
+        _check_dev(x_dev, (T, H), dt, "x")
+        _check_dev(ids_dev, (T, k), "int32", "ids")
+        _check_dev(rows_dev, (T * k, H), dt, "rows")
+        _check_dev(order_dev, (T * k,), "int32", "order")
+        _check_dev(inv_dev, (T, k), "int32", "inv")
+        _check_dev(offsets_dev, (int(n_experts) + 1,), "int32", "offsets")
+        _check_on(self, {"x": x_dev, "ids": ids_dev, "rows": rows_dev, "order": order_dev, "inv": inv_dev,
+                         "offsets": offsets_dev})
+        call("rmoe_sort_tokens_dev", self._h, ptr(x_dev), _ROW_TYPES[dt], T, H, ptr(ids_dev), k, int(n_experts),
+             ptr(rows_dev), ptr(order_dev), ptr(inv_dev), ptr(offsets_dev), _stream_ptr(stream))
+
+    def sort_tokens_backward_dev(self, drows_dev, inv_dev, dx_dev, stream=None):
+        """Gradient of ``sort_tokens_dev``: ``dx[t]`` = sum of ``drows[inv[t, r]]`` over the routes
+        with a row, in fp32, rounded once."""
+        dt = _row_type(drows_dev, "drows")
+        T, k = _shape2(inv_dev, "inv")
+        H = _shape2(drows_dev, "drows")[1]
+        _check_dev(drows_dev, (T * k, H), dt, "drows")
+        _check_dev(inv_dev, (T, k), "int32", "inv")
+        _check_dev(dx_dev, (T, H), dt, "dx")
+        _check_on(self, {"drows": drows_dev, "inv": inv_dev, "dx": dx_dev})
+        call("rmoe_sort_tokens_backward_dev", self._h, ptr(drows_dev), _ROW_TYPES[dt], T, H, ptr(inv_dev), k, ptr(dx_dev),
+             _stream_ptr(stream))
+
+    def combine_tokens_dev(self, rows_dev, inv_dev, wts_dev, out_dev, stream=None):
+        """``out[t]`` = sum of ``wts[t, r] * rows[inv[t, r]]`` over the routes with a row, in fp32
+        by ascending expert id, rounded once: rows [T * k, H], inv int32 [T, k] (of
+        ``sort_tokens_dev``), wts float32 [T, k], out [T, H]."""
+        dt = _row_type(rows_dev, "rows")
+        T, k = _shape2(inv_dev, "inv")
+        H = _shape2(rows_dev, "rows")[1]
+        _check_dev(rows_dev, (T * k, H), dt, "rows")
+        _check_dev(inv_dev, (T, k), "int32", "inv")
+        _check_dev(wts_dev, (T, k), "float32", "wts")
+        _check_dev(out_dev, (T, H), dt, "out")
+        _check_on(self, {"rows": rows_dev, "inv": inv_dev, "wts": wts_dev, "out": out_dev})
+        call("rmoe_combine_tokens_dev", self._h, ptr(rows_dev), _ROW_TYPES[dt], T, H, ptr(inv_dev), ptr(wts_dev), k,
+             ptr(out_dev), _stream_ptr(stream))
+
+    def combine_tokens_backward_dev(self, dout_dev, rows_dev, inv_dev, wts_dev, drows_dev, dwts_dev, stream=None):
+        """Gradients of ``combine_tokens_dev``: ``drows[inv[t, r]] = wts[t, r] * dout[t]`` (rows no
+        route names stay as they were) and ``dwts[t, r] = <dout[t], rows[inv[t, r]]>`` (float32,
+        0 without a row)."""
+        dt = _row_type(rows_dev, "rows")
+        T, k = _shape2(inv_dev, "inv")
+        H = _shape2(rows_dev, "rows")[1]
+        _check_dev(dout_dev, (T, H), dt, "dout")
+        _check_dev(rows_dev, (T * k, H), dt, "rows")
+        _check_dev(inv_dev, (T, k), "int32", "inv")
+        _check_dev(wts_dev, (T, k), "float32", "wts")
+        _check_dev(drows_dev, (T * k, H), dt, "drows")
+        _check_dev(dwts_dev, (T, k), "float32", "dwts")
+        _check_on(self, {"dout": dout_dev, "rows": rows_dev, "inv": inv_dev, "wts": wts_dev, "drows": drows_dev,
+                         "dwts": dwts_dev})
+        call("rmoe_combine_tokens_backward_dev", self._h, ptr(dout_dev), ptr(rows_dev), _ROW_TYPES[dt], T, H, ptr(inv_dev),
+             ptr(wts_dev), k, ptr(drows_dev), ptr(dwts_dev), _stream_ptr(stream))
+
     def dispatch(self, top_ids, n_experts: int) -> tuple[np.ndarray, np.ndarray]:
         ids = np.ascontiguousarray(top_ids, dtype=np.int32)
         if ids.ndim != 2:
@@ -230,6 +340,30 @@ class Matrix:
         _check_dev(x_dev, (T, self.K), "int16", "x")
         _check_dev(y_dev, (T, self.M), "int16", "y")
         call("rmoe_linear_dev", self.ctx.handle, self.handle, ptr(x_dev), int(T), ptr(y_dev), _stream_ptr(stream))
+
+    def reserve_act(self, T: int):
+        """Size the scratch of ``linear_act_dev`` for up to T tokens on this matrix."""
+        call("rmoe_reserve_linear_act", self.ctx.handle, self.handle, int(T))
+
+    def linear_act_dev(self, x_dev, T: int, y_dev, bias_dev=None, act: str = "none", residual_dev=None, gate_beta=None,
+                       value_beta=None, stream=None):
+        """``y = act(x @ W^T + bias) + residual`` in fp32, rounded once to bf16 (call
+        ``reserve_act(T)`` first).  x [T, K_in] bfloat16 or int16 bits (K_in <= K a multiple of 8;
+        columns past it are zero), bias float32 [M], residual of y's shape (y itself: in
+        place).  ``act`` "none", "silu", "gelu", "gelu_tanh": y [T, M]; "swiglu", "situ" (with the
+        betas): y [T, M / 2], the first M / 2 weight rows the gate, the others the up."""
+        code, gb, vb, gated = _epilogue_act(act, gate_beta, value_beta)
+        K_in = _shape2(x_dev, "x")[1]
+        width = self.M // 2 if gated else self.M
+        _check_bf16(x_dev, (T, K_in), "x")
+        _check_bf16(y_dev, (T, width), "y")
+        if bias_dev is not None:
+            _check_dev(bias_dev, (self.M,), "float32", "bias")
+        if residual_dev is not None:
+            _check_bf16(residual_dev, (T, width), "residual")
+        _check_on(self.ctx, {"x": x_dev, "y": y_dev, "bias": bias_dev, "residual": residual_dev})
+        call("rmoe_linear_act_dev", self.ctx.handle, self.handle, ptr(x_dev), int(T), K_in, ptr(bias_dev), code, gb, vb,
+             ptr(residual_dev), ptr(y_dev), _stream_ptr(stream))
 
     def free(self):
         call("rmoe_matrix_free", self.ctx.handle, self.handle)
@@ -465,6 +599,38 @@ class MoeLayer:
             _check_dev(wts_dev, (T, g.top_k), "float32", "wts")
         call("rmoe_moe_prefill_dev", self.ctx.handle, self.layer, ptr(x_dev), int(T), ptr(out_dev), int(bool(residual)),
              act, gb, vb, ptr(ids_dev), ptr(wts_dev), _stream_ptr(stream))
+
+    def reserve_experts_linear(self, n: int):
+        """Size the scratch of ``experts_linear_dev`` for up to n sorted rows."""
+        call("rmoe_reserve_experts_linear", self.ctx.handle, self.layer, int(n))
+
+    def experts_linear_dev(self, part: str, rows_dev, offsets_dev, y_dev, bias_dev=None, act: str = "none",
+                           residual_dev=None, gate_beta=None, value_beta=None, stream=None):
+        """``Matrix.linear_act_dev`` over sorted rows, each with its routed expert's matrix: row p
+        of ``offsets[e] <= p < offsets[e + 1]`` (int32 [n_routed + 1], of ``sort_tokens_dev``)
+        with expert e's ``part`` "gate_up" ([2I, H]) or "down" ([H, Ipad], rows of I columns).
+        rows [n, K_in], bias float32 [n_routed, M], y and residual [n, M] or, gated, [n, M / 2].
+        Rows from ``offsets[n_routed]`` on stay as they were.  Call
+        ``reserve_experts_linear(n)`` first."""
+        codes = {"gate_up": PART_GATE_UP, "down": PART_DOWN}
+        if part not in codes:
+            raise ValueError(f"part must be 'gate_up' or 'down', got {part!r}")
+        code, gb, vb, gated = _epilogue_act(act, gate_beta, value_beta)
+        g = self.geom
+        n, K_in = _shape2(rows_dev, "rows")
+        M = 2 * g.inter if part == "gate_up" else g.hidden
+        width = M // 2 if gated else M
+        _check_bf16(rows_dev, (n, K_in), "rows")
+        _check_dev(offsets_dev, (g.n_routed + 1,), "int32", "offsets")
+        _check_bf16(y_dev, (n, width), "y")
+        if bias_dev is not None:
+            _check_dev(bias_dev, (g.n_routed, M), "float32", "bias")
+        if residual_dev is not None:
+            _check_bf16(residual_dev, (n, width), "residual")
+        _check_on(self.ctx, {"rows": rows_dev, "offsets": offsets_dev, "y": y_dev, "bias": bias_dev,
+                             "residual": residual_dev})
+        call("rmoe_experts_linear_dev", self.ctx.handle, self.layer, codes[part], ptr(rows_dev), n, K_in, ptr(offsets_dev),
+             ptr(bias_dev), code, gb, vb, ptr(residual_dev), ptr(y_dev), _stream_ptr(stream))
 
     def free(self):
         call("rmoe_layer_free", self.ctx.handle, self.layer)

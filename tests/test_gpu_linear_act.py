@@ -1,0 +1,357 @@
+"""GPU: products of quantized weights with bias, activation and residual (csrc/linear_act.hip), dense and by
+expert, against the dequantized weights in 64 bits.
+
+Bounds.  A sum over K products in fp32 is off by at most (K + 64) 2^-23 sum |x w|; the weights' rounding to fp16 in
+the kernel of many rows adds at most 2^-11 sum |x w| (and 2^-37 of the largest |x| and |w| times K for values at the
+end of fp16's range).  z = that + bias carries d; an activation with |f'| <= L passes L d on and adds 32 steps of
+fp32; the sum with the residual and the rounding to bf16 add 2^-8 of the result."""
+
+from __future__ import annotations
+
+import math
+
+import numpy as np
+import pytest
+
+from oracle import bfp16 as B
+from oracle import q4nx as Q
+
+from raon_npu_amd.geometry import MoeGeometry
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+ACTS = ["none", "silu", "gelu", "gelu_tanh", "swiglu", "situ"]
+SITU = (4.0, 25.0)
+MANY = 32  # rows (of an expert or of the call) from which the kernel of many rows may run
+
+
+def _weights(fmt, M, K, seed, live=None, std=0.02):
+    rng = np.random.default_rng(seed)
+    w = rng.normal(0.0, std, (M, K)).astype(np.float32)
+    if live is not None:
+        w[:, live:] = 0
+    if fmt == "q4nx":
+        c, s, m = Q.quantize(w)
+        return Q.pack_gemv(c, s, m), torch.from_numpy(Q.dequantize_simple(c, s, m)).double()
+    blob = B.pack_gemv(w)
+    return blob, torch.from_numpy(B.dequantize_packed(blob, K, M)).double()
+
+
+def _reference(x, w, bias, act, residual, many):
+    """(y, bound) of y in float64."""
+    x = x.double()
+    K = x.shape[1]
+    absum = x.abs() @ w.abs().t()
+    z = x @ w.t()
+    d = (K + 64) * 2.0 ** -23 * absum
+    if many:
+        d += 2.0 ** -11 * absum + K * 2.0 ** -37 * x.abs().amax(1, keepdim=True) * w.abs().amax(1)[None]
+    if bias is not None:
+        z = z + bias.double()
+        d = d + 2.0 ** -24 * z.abs()
+    half = z.shape[1] // 2
+    if act in ("swiglu", "situ"):
+        g, u, dg, du = z[:, :half], z[:, half:], d[:, :half], d[:, half:]
+        if act == "swiglu":
+            f, L, h = g * torch.sigmoid(g), 1.1, u
+        else:
+            f, L, h = SITU[0] * torch.tanh(g / SITU[0]) * torch.sigmoid(g), 1.0 + SITU[0] / 4, SITU[1] * torch.tanh(u / SITU[1])
+        y = f * h
+        e = L * dg * (h.abs() + du) + f.abs() * du
+    else:
+        y = {"none": lambda: z, "silu": lambda: z * torch.sigmoid(z),
+             "gelu": lambda: z * 0.5 * torch.special.erfc(-z / math.sqrt(2.0)),
+             "gelu_tanh": lambda: z * torch.sigmoid(2 * math.sqrt(2 / math.pi) * (z + 0.044715 * z ** 3))}[act]()
+        e = 1.2 * d
+    e = e + 32 * 2.0 ** -24 * y.abs()
+    if residual is not None:
+        y = y + residual.double()
+        e = e + 2.0 ** -24 * y.abs()
+    return y, e
+
+
+def _check(got, ref, e, what=""):
+    got = got.cpu().double()
+    bound = 2.0 ** -8 * (ref.abs() + e) + e + 2.0 ** -133
+    bad = ~((got - ref).abs() <= bound)
+    assert not bad.any(), (what, bad.nonzero()[:4].tolist(), got[bad][:4].tolist(), ref[bad][:4].tolist())
+
+
+def _betas(act):
+    return {"gate_beta": SITU[0], "value_beta": SITU[1]} if act == "situ" else {}
+
+
+def _operands(T, M, K, act, bias, residual, seed):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(T, K, generator=g).to(torch.bfloat16)
+    b = torch.randn(M, generator=g) * 0.3 if bias else None
+    width = M // 2 if act in ("swiglu", "situ") else M
+    r = torch.randn(T, width, generator=g).to(torch.bfloat16) if residual else None
+    return x, b, r, width
+
+
+def _cuda(t):
+    return None if t is None else t.cuda()
+
+
+@pytest.mark.parametrize("fmt", ["q4nx", "bfp16"])
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("M,K", [(128, 256), (384, 768), (1536, 2048)])
+def test_dense(gpu_ctx, fmt, act, M, K):
+    blob, w = _weights(fmt, M, K, M + K)
+    mat = gpu_ctx.upload_matrix(blob, M, K, fmt=fmt)
+    mat.reserve_act(700)
+    for T, bias, residual in ((1, True, True), (4, False, False), (5, False, True), (33, True, False), (130, True, True),
+                              (700, True, True)):
+        x, b, r, width = _operands(T, M, K, act, bias, residual, 7 * T + M)
+        buf = torch.full((T + 1, width), 9.0, dtype=torch.bfloat16, device="cuda")
+        mat.linear_act_dev(_cuda(x), T, buf[:T], bias_dev=_cuda(b), act=act, residual_dev=_cuda(r),
+                           stream=torch.cuda.current_stream(), **_betas(act))
+        ref, e = _reference(x, w, b, act, r, T >= MANY)
+        _check(buf[:T], ref, e, T)
+        assert bool((buf[T] == 9).all())
+    mat.free()
+
+
+@pytest.mark.parametrize("fmt", ["q4nx", "bfp16"])
+@pytest.mark.parametrize("T", [1, 3, 40, 300])
+def test_input_narrower_than_the_matrix(gpu_ctx, fmt, T):
+    """K_in < K, also ending inside a tile of 128 columns; what lies behind a row is the next row."""
+    M, K = 256, 1280
+    blob, w = _weights(fmt, M, K, 3)
+    mat = gpu_ctx.upload_matrix(blob, M, K, fmt=fmt)
+    mat.reserve_act(T)
+    for K_in in (8, 120, 136, 1024, 1088, 1272, 1280):
+        x, b, r, width = _operands(T, M, K_in, "silu", True, True, K_in)
+        y = torch.zeros(T, width, dtype=torch.bfloat16, device="cuda")
+        mat.linear_act_dev(_cuda(x), T, y, bias_dev=_cuda(b), act="silu", residual_dev=_cuda(r),
+                           stream=torch.cuda.current_stream())
+        _check(y, *_reference(x, w[:, :K_in], b, "silu", r, T >= MANY), K_in)
+    mat.free()
+
+
+@pytest.mark.parametrize("T", [1, 40, 300])
+def test_residual_in_place_int16_and_odd_addresses(gpu_ctx, T):
+    """y is the residual; int16 bits are bfloat16 values; y at an address its 16-byte stores cannot take."""
+    M, K = 256, 512
+    blob, w = _weights("q4nx", M, K, 5)
+    mat = gpu_ctx.upload_matrix(blob, M, K)
+    mat.reserve_act(T)
+    x, b, r, _ = _operands(T, M, K, "gelu", True, True, 6)
+    st = torch.cuda.current_stream()
+    want = torch.zeros(T, M, dtype=torch.bfloat16, device="cuda")
+    mat.linear_act_dev(x.cuda(), T, want, bias_dev=b.cuda(), act="gelu", residual_dev=r.cuda(), stream=st)
+    _check(want, *_reference(x, w, b, "gelu", r, T >= MANY))
+    for shift in (0, 1, 4):
+        buf = torch.zeros(T * M + 16, dtype=torch.int16, device="cuda")
+        y = buf[shift:shift + T * M].view(T, M)
+        y.copy_(r.view(torch.int16))
+        mat.linear_act_dev(x.cuda().view(torch.int16), T, y, bias_dev=b.cuda(), act="gelu", residual_dev=y, stream=st)
+        assert torch.equal(y.view(torch.bfloat16), want)
+        assert not buf[:shift].any() and not buf[shift + T * M:].any()
+    mat.free()
+
+
+@pytest.mark.parametrize("fmt", ["q4nx", "bfp16"])
+@pytest.mark.parametrize("T", [2, 64, 300])
+def test_ranges_of_values(gpu_ctx, fmt, T):
+    """Rows of x and weights of very different sizes, as no type of 16 bits with a short exponent holds them:
+    2^-60 to 2^60, rows of zeros, and rows with one large value."""
+    M, K = 128, 512
+    for ws in (2.0 ** -40, 1.0, 2.0 ** 30):
+        blob, w = _weights(fmt, M, K, 9, std=ws)
+        mat = gpu_ctx.upload_matrix(blob, M, K, fmt=fmt)
+        mat.reserve_act(T)
+        g = torch.Generator().manual_seed(T)
+        x = torch.randn(T, K, generator=g) * 2.0 ** torch.linspace(-60, 60, T)[:, None].round()
+        x[T // 2] = 0
+        x[0, 5] = x[0, 5] * 2.0 ** 20
+        x = x.to(torch.bfloat16)
+        y = torch.zeros(T, M, dtype=torch.bfloat16, device="cuda")
+        mat.linear_act_dev(x.cuda(), T, y, stream=torch.cuda.current_stream())
+        _check(y, *_reference(x, w, None, "none", None, T >= MANY), ws)
+        assert not y[T // 2].any()
+        mat.free()
+
+
+@pytest.mark.parametrize("fmt", ["q4nx", "bfp16"])
+@pytest.mark.parametrize("T", [18, 200])
+def test_non_finite_rows_stay_in_their_row(gpu_ctx, fmt, T):
+    M, K = 128, 512
+    blob, w = _weights(fmt, M, K, 9)
+    mat = gpu_ctx.upload_matrix(blob, M, K, fmt=fmt)
+    mat.reserve_act(T)
+    x, _, _, _ = _operands(T, M, K, "none", False, False, 2)
+    st = torch.cuda.current_stream()
+    want, y = (torch.zeros(T, M, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    mat.linear_act_dev(x.cuda(), T, want, stream=st)
+    bad = x.clone()
+    bad[3, 7], bad[17, 300] = float("inf"), float("nan")
+    mat.linear_act_dev(bad.cuda(), T, y, stream=st)
+    keep = [t for t in range(T) if t not in (3, 17)]
+    assert torch.equal(y[keep], want[keep])
+    assert not y[[3, 17]].isfinite().any()
+    mat.free()
+
+
+def _layer(gpu_ctx, H, I, E, d_layout, seed):
+    """A layer and its float64 (gate_up [E, 2I, H], down [E, H, I]); weights-d layers have a bfp16 down."""
+    g = MoeGeometry(hidden=H, inter=I, n_routed=E, n_shared=1, top_k=min(4, E))
+    Ip = g.inter_pad
+    gu = [_weights("q4nx", 2 * I, H, seed + 2 * e) for e in range(E + 1)]
+    dn = [_weights("bfp16" if d_layout else "q4nx", H, Ip, seed + 2 * e + 1, live=I) for e in range(E + 1)]
+    if d_layout:
+        lyr = gpu_ctx.create_layer_d(7300, g)
+        lyr.upload_d(1, 0, b"".join(b for b, _ in gu[:E]))
+        lyr.upload_d(2, 0, b"".join(b for b, _ in dn))
+    else:
+        lyr = gpu_ctx.create_layer(7300, g)
+        lyr.upload_experts(b"".join(b for b, _ in gu), b"".join(b for b, _ in dn))
+    return lyr, [w for _, w in gu[:E]], [w[:, :I] for _, w in dn[:E]]
+
+
+COUNTS = [[1, 0, 0, 0, 0], [0, 0, 0, 0, 3], [1, 1, 1, 1, 1], [0, 17, 0, 5, 1], [4, 5, 16, 33, 0], [129, 0, 64, 65, 200],
+          [0, 700, 0, 0, 1], [0, 0, 0, 0, 0]]
+
+
+@pytest.mark.parametrize("d_layout", [False, True])
+@pytest.mark.parametrize("part", ["gate_up", "down"])
+def test_experts(gpu_ctx, d_layout, part):
+    """Each row with its expert's matrix; experts without rows, rows behind the last left as they were."""
+    H, I, E = 512, 320, 5
+    lyr, gu, dn = _layer(gpu_ctx, H, I, E, d_layout, 40)
+    ws, M, K = (gu, 2 * I, H) if part == "gate_up" else (dn, H, I)
+    lyr.reserve_experts_linear(1000)
+    for i, counts in enumerate(COUNTS):
+        live = sum(counts)
+        n = live + (3 if i % 2 else 0) or 2
+        offsets = torch.tensor([0] + list(np.cumsum(counts)), dtype=torch.int32)
+        act = ACTS[i % 6] if part == "gate_up" else ["none", "gelu"][i % 2]
+        x, _, r, width = _operands(n, M, K, act, False, i % 3 == 0, 60 + i)
+        x[live:] = float("nan")
+        b = torch.randn(E, M, generator=torch.Generator().manual_seed(i)) * 0.3 if i % 2 else None
+        y = torch.full((n, width), 9.0, dtype=torch.bfloat16, device="cuda")
+        lyr.experts_linear_dev(part, x.cuda(), offsets.cuda(), y, bias_dev=_cuda(b), act=act, residual_dev=_cuda(r),
+                               stream=torch.cuda.current_stream(), **_betas(act))
+        for e in range(E):
+            a, z = int(offsets[e]), int(offsets[e + 1])
+            if a < z:
+                ref, err = _reference(x[a:z], ws[e], None if b is None else b[e], act, None if r is None else r[a:z],
+                                      n >= MANY)
+                _check(y[a:z], ref, err, (counts, e))
+        assert bool((y[live:] == 9).all())
+    lyr.free()
+
+
+def test_experts_with_offsets_outside_the_rows(gpu_ctx):
+    """Offsets are device data: whatever they hold, nothing outside the rows is read or written."""
+    H, I, E = 256, 128, 5
+    lyr, gu, _ = _layer(gpu_ctx, H, I, E, False, 70)
+    n = 40
+    lyr.reserve_experts_linear(n)
+    x, _, _, width = _operands(n, 2 * I, H, "none", False, False, 3)
+    buf = torch.full((n + 64, width), 9.0, dtype=torch.bfloat16, device="cuda")
+    for offsets in ([-5, 3, 3, 900, 7, 2 ** 31 - 1], [50, 40, 30, 20, 10, 0], [2 ** 31 - 1] * 6, [-2 ** 31] * 6):
+        buf.fill_(9.0)
+        lyr.experts_linear_dev("gate_up", x.cuda(), torch.tensor(offsets, dtype=torch.int32, device="cuda"), buf[:n],
+                               stream=torch.cuda.current_stream())
+        assert bool((buf[n:] == 9).all())
+    torch.cuda.synchronize()
+    lyr.free()
+
+
+def test_one_token_sorted_through_its_experts(gpu_ctx):
+    """The operators in a row against the framework's closed call: route, sort, gate/up with SwiGLU, down, combine,
+    for one token and for batches; the closed call rounds gate and up to bf16 first, so both are compared with 64
+    bits at the parity bar (max-abs 1e-2, rel-L2 3e-3, of which roundings of h and of the result take
+    2^-8 / sqrt(3) each)."""
+    H, I, E, k = 512, 320, 8, 3
+    g = MoeGeometry(hidden=H, inter=I, n_routed=E, n_shared=1, top_k=k)
+    for d_layout in (False, True):
+        lyr, gu, dn = _layer(gpu_ctx, H, I, E, d_layout, 90)
+        for T in (1, 5, 77, 600):
+            gen = torch.Generator().manual_seed(T)
+            x = torch.randn(T, H, generator=gen).to(torch.bfloat16)
+            ids = torch.rand(T, E, generator=gen).argsort(1)[:, :k].to(torch.int32).contiguous()
+            if T > 5:
+                ids[3] = -1  # a padding token
+                ids[4, 1] = -1
+            w = torch.rand(T, k, generator=gen)
+            st = torch.cuda.Stream()
+            A = T * k
+            lyr.reserve_experts_linear(A)
+            dev = {"device": "cuda"}
+            rows = torch.zeros(A, H, dtype=torch.bfloat16, **dev)
+            order, off = torch.zeros(A, dtype=torch.int32, **dev), torch.zeros(E + 1, dtype=torch.int32, **dev)
+            inv = torch.zeros(T, k, dtype=torch.int32, **dev)
+            h = torch.zeros(A, I, dtype=torch.bfloat16, **dev)
+            d = torch.zeros(A, H, dtype=torch.bfloat16, **dev)
+            out = torch.zeros(T, H, dtype=torch.bfloat16, **dev)
+            xd, idd, wd = x.cuda(), ids.cuda(), w.cuda()
+            torch.cuda.synchronize()
+
+            def run():
+                gpu_ctx.sort_tokens_dev(xd, idd, E, rows, order, inv, off, stream=st)
+                lyr.experts_linear_dev("gate_up", rows, off, h, act="swiglu", stream=st)
+                lyr.experts_linear_dev("down", h, off, d, stream=st)
+                gpu_ctx.combine_tokens_dev(d, inv, wd, out, stream=st)
+
+            run()
+            torch.cuda.synchronize()
+            ref = torch.zeros(T, H, dtype=torch.float64)
+            for t in range(T):
+                for r in range(k):
+                    e = int(ids[t, r])
+                    if e >= 0:
+                        z = gu[e] @ x[t].double()
+                        hh = (z[:I] * torch.sigmoid(z[:I]) * z[I:]).to(torch.bfloat16).double()
+                        ref[t] += float(w[t, r]) * (dn[e] @ hh)
+            got = out.cpu().double()
+            assert float((got - ref).abs().max()) <= 1e-2
+            assert float((got - ref).norm()) <= 3e-3 * float(ref.norm())
+            if T > 5:
+                assert not out[3].any()
+            # captured and replayed, with new tokens
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=st):
+                run()
+            for i in range(3):
+                xd.copy_(x.roll(i, 0))
+                torch.cuda.synchronize()
+                graph.replay()
+                torch.cuda.synchronize()
+                replayed = out.clone()
+                run()
+                torch.cuda.synchronize()
+                assert torch.equal(out, replayed)
+        lyr.free()
+
+
+def test_refused_operands(gpu_ctx):
+    """What the entry points themselves refuse; nothing is launched."""
+    M, K, T = 128, 512, 4
+    blob, _ = _weights("q4nx", M, K, 1)
+    mat = gpu_ctx.upload_matrix(blob, M, K)
+    mat.reserve_act(T)
+    x = torch.zeros(T * K + 8, dtype=torch.bfloat16, device="cuda")
+    y = torch.zeros(T, M, dtype=torch.bfloat16, device="cuda")
+    buf = torch.zeros(2 * T * M, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(ValueError, match="16-byte"):
+        mat.linear_act_dev(x[1:1 + T * K].view(T, K), T, y)
+    with pytest.raises(ValueError, match="multiple of 8"):
+        mat.linear_act_dev(x[:T * 100].view(T, 100), T, y)
+    with pytest.raises(ValueError, match="at most K"):
+        mat.linear_act_dev(x.new_zeros(T, K + 8), T, y)
+    with pytest.raises(ValueError, match="overlaps"):
+        mat.linear_act_dev(x[:T * K].view(T, K), T, x[T * M:2 * T * M].view(T, M))
+    with pytest.raises(ValueError, match="overlaps"):
+        mat.linear_act_dev(x[:T * K].view(T, K), T, buf[:T * M].view(T, M), residual_dev=buf[M:M + T * M].view(T, M))
+    with pytest.raises(ValueError, match="betas"):
+        mat.linear_act_dev(x[:T * K].view(T, K), T, y[:, :64].contiguous(), act="situ", gate_beta=0.0, value_beta=25.0)
+    with pytest.raises(ValueError):
+        mat.reserve_act(0)
+    mat.free()
+    with pytest.raises(KeyError):
+        mat.linear_act_dev(x[:T * K].view(T, K), T, y)
