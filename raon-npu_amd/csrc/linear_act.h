@@ -11,10 +11,28 @@ __host__ __device__ constexpr bool act_gated(int act) { return act == RMOE_ACT_S
 
 // Activations of one value.  Each is z times a probability formed without cancellation: the
 // sigmoid from exp(-|z|), the normal distribution's from erfc, so that small results keep
-// their relative accuracy.
+// their relative accuracy.  exp2 and the reciprocal are the hardware's (1 ulp each; the
+// reciprocal with one Newton step), a few fp32 ulps below a bf16 rounding.
+__device__ __forceinline__ float recip(float d) {
+  const float r = __builtin_amdgcn_rcpf(d);
+  return fmaf(r, fmaf(-d, r, 1.0f), r);
+}
+__device__ __forceinline__ float exp_of(float z) { return __builtin_amdgcn_exp2f(1.44269504088896341f * z); }
 __device__ __forceinline__ float sigmoid_of(float z) {
-  const float e = expf(-fabsf(z));
-  return z >= 0.f ? 1.0f / (1.0f + e) : e / (1.0f + e);
+  const float e = exp_of(-fabsf(z)), r = recip(1.0f + e);
+  return z >= 0.f ? r : e * r;
+}
+// tanh: 1 - 2 / (1 + exp(2 |z|)), and below 0.3, where that cancels, its power series to z^9
+// (the next term is 4e-8 of z there).
+__device__ __forceinline__ float tanh_of(float z) {
+  const float a = fabsf(z), q = z * z;
+  const float big = 1.0f - 2.0f * recip(1.0f + exp_of(2.0f * fminf(a, 20.f)));
+  const float s = fmaf(q, fmaf(q, fmaf(q, fmaf(q, 62.f / 2835.f, -17.f / 315.f), 2.f / 15.f), -1.f / 3.f), 1.0f);
+  return a < 0.3f ? z * s : z != z ? z : copysignf(big, z);
+}
+__device__ __forceinline__ float act_pair(int act, float g, float u, float gb, float vb) {
+  if (act == RMOE_ACT_SWIGLU) return g * sigmoid_of(g) * u;
+  return gb * tanh_of(g / gb) * sigmoid_of(g) * (vb * tanh_of(u / vb));
 }
 __device__ __forceinline__ float act_single(int act, float z) {
   if (act == RMOE_ACT_SILU) return z * sigmoid_of(z);

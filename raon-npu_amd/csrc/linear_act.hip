@@ -90,7 +90,7 @@ __global__ __launch_bounds__(512) void linear_act_kernel(LinAct a, int n_nt) {
     if constexpr (kGated) {
       float u = sum(t, kOut + c);
       if (bias) u += bias[a.M / 2 + col];
-      z = act_apply(a.act, z, u, a.gb, a.vb);
+      z = act_pair(a.act, z, u, a.gb, a.vb);
     } else {
       z = act_single(a.act, z);
     }
@@ -142,7 +142,8 @@ hipError_t linear_act_setup() {
   return hipSuccess;
 }
 
-hipError_t launch_linear_act(const LinAct& a, hipStream_t st) {
+hipError_t launch_linear_act(const LinAct& a, uint8_t* scratch, size_t bytes, hipStream_t st) {
+  if (act_tiles_serve(a.fmt, a.M, a.K, a.offsets ? a.n_experts : 1, a.n)) return launch_act_tiles(a, scratch, bytes, st);
   return a.fmt == RMOE_FMT_BFP16 ? pick<RMOE_FMT_BFP16>(a, st) : pick<RMOE_FMT_Q4NX>(a, st);
 }
 

@@ -485,7 +485,7 @@ int rmoe_destroy(rmoe_ctx* ctx) {
   }
   RmoeScratch& s = ctx->s;
   void* bufs[] = {s.part, s.counters, s.h, s.ids, s.wts, s.logits, s.order, s.inv, s.offsets,
-                  s.chunk_counts, s.staging, s.pf, s.stack, s.stack_cnt};
+                  s.chunk_counts, s.staging, s.pf, s.stack, s.stack_cnt, s.act};
   for (void* b : bufs)
     if (b) hipFree(b);
   auto it = g_io.find(ctx);
@@ -710,11 +710,19 @@ int rmoe_reserve_linear(rmoe_ctx* ctx, int handle, int T) {
   return RMOE_OK;
 }
 
+static int reserve_act(rmoe_ctx* ctx, size_t bytes) {
+  HIP_TRY(hipSetDevice(ctx->device));
+  return bytes ? grow(ctx->s.act, ctx->s.act_bytes, bytes, ctx) : RMOE_OK;
+}
+
 static int run_linear_act(rmoe_ctx* ctx, const rmoe::LinAct& L, void* stream) {
   TRY(check_linear_act(L));
   OnDevice dev(ctx);
   HIP_TRY(dev.status);
-  const hipError_t e = rmoe::launch_linear_act(L, pick_stream(ctx, stream));
+  const hipError_t e = rmoe::launch_linear_act(L, ctx->s.act, ctx->s.act_bytes, pick_stream(ctx, stream));
+  if (e == hipErrorOutOfMemory)
+    return fail(RMOE_EINVAL, "scratch too small for %d rows: call %s first", L.n,
+                L.offsets ? "rmoe_reserve_experts_linear" : "rmoe_reserve_linear_act");
   if (e == hipErrorInvalidValue) return fail(RMOE_EINVAL, "%d rows of width %d are too many for one call", L.n, L.K_in);
   HIP_TRY(e);
   return RMOE_OK;
@@ -733,7 +741,7 @@ int rmoe_reserve_linear_act(rmoe_ctx* ctx, int handle, int T) {
   RmoeMatrix* m;
   TRY(find_matrix(ctx, handle, &m));
   if (T < 1) return fail(RMOE_EINVAL, "T must be >= 1");
-  return RMOE_OK;
+  return reserve_act(ctx, rmoe::act_tiles_scratch(m->fmt, m->M, m->K, 1, T));
 }
 
 int rmoe_experts_linear_dev(rmoe_ctx* ctx, int layer, int part, const void* rows_dev, int n, int K_in,
@@ -756,7 +764,8 @@ int rmoe_reserve_experts_linear(rmoe_ctx* ctx, int layer, int n) {
   RmoeLayer* l;
   TRY(check_layer(ctx, layer, &l));
   if (n < 1) return fail(RMOE_EINVAL, "n must be >= 1");
-  return RMOE_OK;
+  return reserve_act(ctx, std::max(rmoe::act_tiles_scratch(RMOE_FMT_Q4NX, 2 * l->I, l->H, l->n_routed, n),
+                                   rmoe::act_tiles_scratch(l->dn_fmt, l->H, l->Ipad, l->n_routed, n)));
 }
 
 // ----------------------------------------------------------- tokens by expert --

@@ -399,6 +399,8 @@ struct RmoeScratch {
   uint8_t* staging = nullptr;    // upload staging
   size_t staging_bytes = 0;
   int max_tokens = 0;
+  uint8_t* act = nullptr;        // products with an epilogue: fp16 rows, exponents
+  size_t act_bytes = 0;
   // persistent decode stack (moe_decode_stack.hip)
   uint8_t* stack = nullptr;      // per-layer hand-off buffers
   size_t stack_bytes = 0;
@@ -546,7 +548,13 @@ struct LinAct {
   uint16_t* y;
 };
 hipError_t linear_act_setup();  // once per device before the first call
-hipError_t launch_linear_act(const LinAct& a, hipStream_t st);
+// hipErrorOutOfMemory: scratch below act_tiles_scratch().
+hipError_t launch_linear_act(const LinAct& a, uint8_t* scratch, size_t bytes, hipStream_t st);
+// Many rows (linear_act_tiles.hip): whether it serves n rows over `groups` matrices, and the
+// scratch that takes (0 if it does not).
+bool act_tiles_serve(int fmt, int M, int K, int groups, size_t n);
+size_t act_tiles_scratch(int fmt, int M, int K, int groups, size_t n);
+hipError_t launch_act_tiles(const LinAct& a, uint8_t* scratch, size_t bytes, hipStream_t st);
 
 // Persistent decode of n_layers (<= kMaxStack) layers of one geometry for one token
 // (moe_decode_stack.hip).  One workgroup per CU (grid n_cu).  ids_out/wts_out: [n_layers, k]

@@ -13,7 +13,7 @@ import numpy as np
 
 from . import _lib
 from ._lib import (ACT_GELU, ACT_GELU_TANH, ACT_NONE, ACT_SILU, ACT_SITU, ACT_SWIGLU, BUNDLE_B1, BUNDLE_B2, DT_BF16, DT_F16,
-                   DT_F32, PART_DOWN, PART_GATE_UP, SCORE_SIGMOID, SCORE_SOFTMAX, call, new_bytes, ptr)
+                   DT_F32, PART_DOWN, PART_GATE_UP, SCORE_SIGMOID, SCORE_SOFTMAX, call, check, new_bytes, ptr)
 from .geometry import MoeGeometry
 
 
@@ -50,31 +50,50 @@ _EPILOGUE_ACTS = {"none": ACT_NONE, "silu": ACT_SILU, "gelu": ACT_GELU, "gelu_ta
                   "situ": ACT_SITU}
 
 
+_DTYPE_NAMES: dict = {}  # torch dtype -> its name, filled as types are seen (the module imports no torch)
+
+
+def _dtype_name(t) -> str:
+    dt = getattr(t, "dtype", None)
+    name = _DTYPE_NAMES.get(dt)
+    if name is None:
+        name = _DTYPE_NAMES[dt] = str(dt).split(".")[-1]
+    return name
+
+
 def _row_type(t, name: str) -> str:
     """The element type of token rows: "bfloat16" (or its bits as "int16"), "float16" or "float32"."""
-    dt = str(getattr(t, "dtype", None)).split(".")[-1]
+    dt = _dtype_name(t)
     if dt not in _ROW_TYPES:
         raise ValueError(f"{name} must be bfloat16 (or int16 bits), float16 or float32, got {dt}")
     return dt
 
 
 def _shape2(t, name: str) -> tuple[int, int]:
-    shape = tuple(getattr(t, "shape", ()))
-    if len(shape) != 2:
-        raise ValueError(f"{name} must be a matrix, got shape {shape}")
-    return int(shape[0]), int(shape[1])
+    try:
+        rows, cols = t.shape
+    except (AttributeError, ValueError):
+        raise ValueError(f"{name} must be a matrix, got shape {tuple(getattr(t, 'shape', ()))}") from None
+    return rows, cols
 
 
-def _check_on(ctx: "Context", named: dict):
-    """Tensors of a call live on the context's GPU (None: an operand left out)."""
-    for name, t in named.items():
-        if t is not None and t.device.index != ctx.device:
-            raise ValueError(f"{name} is on {t.device}, the context on cuda:{ctx.device}")
+def _operand(device: int, t, shape: tuple, dtype_name: str, name: str) -> int:
+    """The address of a device tensor with exactly the shape and type the kernel indexes, on the context's GPU.
+    A call of these operators takes 4 us on the GPU when it is small, and two microseconds of host time per operand
+    (``_check_dev``, then the device) made it 12: the checks are one expression, taken apart only to name a fault."""
+    try:
+        if (t.is_cuda and t.shape == shape and _dtype_name(t) == dtype_name and t.is_contiguous()
+                and t.get_device() == device):
+            return t.data_ptr()
+    except AttributeError:
+        pass
+    _check_dev(t, shape, dtype_name, name)
+    raise ValueError(f"{name} is on {t.device}, the context on cuda:{device}")
 
 
-def _check_bf16(t, shape: tuple, name: str):
+def _bf16_operand(device: int, t, shape: tuple, name: str) -> int:
     """bf16 values of a given shape, as bfloat16 or as int16 bits."""
-    _check_dev(t, shape, "int16" if str(getattr(t, "dtype", None)) == "torch.int16" else "bfloat16", name)
+    return _operand(device, t, shape, "int16" if _dtype_name(t) == "int16" else "bfloat16", name)
 
 
 def _epilogue_act(act: str, gate_beta, value_beta) -> tuple[int, float, float, bool]:
@@ -235,65 +254,52 @@ class Context:
         float16 or float32; order int32 [T * k], inv [T, k], offsets [n_experts + 1].  Rows and
         order from ``offsets[n_experts]`` on stay as they were.  Asynchronous; allocates
         nothing and uses no scratch (capturable, any number of calls at once)."""
-        dt = _row_type(x_dev, "x")
+        dt, dev, n_experts = _row_type(x_dev, "x"), self.device, int(n_experts)
         T, H = _shape2(x_dev, "x")
-        _, k = _shape2(ids_dev, "ids")
-        _check_dev(x_dev, (T, H), dt, "x")
-        _check_dev(ids_dev, (T, k), "int32", "ids")
-        _check_dev(rows_dev, (T * k, H), dt, "rows")
-        _check_dev(order_dev, (T * k,), "int32", "order")
-        _check_dev(inv_dev, (T, k), "int32", "inv")
-        _check_dev(offsets_dev, (int(n_experts) + 1,), "int32", "offsets")
-        _check_on(self, {"x": x_dev, "ids": ids_dev, "rows": rows_dev, "order": order_dev, "inv": inv_dev,
-                         "offsets": offsets_dev})
-        call("rmoe_sort_tokens_dev", self._h, ptr(x_dev), _ROW_TYPES[dt], T, H, ptr(ids_dev), k, int(n_experts),
-             ptr(rows_dev), ptr(order_dev), ptr(inv_dev), ptr(offsets_dev), _stream_ptr(stream))
+        k = _shape2(ids_dev, "ids")[1]
+        A = T * k
+        check(_lib.load().rmoe_sort_tokens_dev(
+            self._h, _operand(dev, x_dev, (T, H), dt, "x"), _ROW_TYPES[dt], T, H,
+            _operand(dev, ids_dev, (T, k), "int32", "ids"), k, n_experts,
+            _operand(dev, rows_dev, (A, H), dt, "rows"), _operand(dev, order_dev, (A,), "int32", "order"),
+            _operand(dev, inv_dev, (T, k), "int32", "inv"),
+            _operand(dev, offsets_dev, (n_experts + 1,), "int32", "offsets"), _stream_ptr(stream)))
 
     def sort_tokens_backward_dev(self, drows_dev, inv_dev, dx_dev, stream=None):
         """Gradient of ``sort_tokens_dev``: ``dx[t]`` = sum of ``drows[inv[t, r]]`` over the routes
         with a row, in fp32, rounded once."""
-        dt = _row_type(drows_dev, "drows")
+        dt, dev = _row_type(drows_dev, "drows"), self.device
         T, k = _shape2(inv_dev, "inv")
         H = _shape2(drows_dev, "drows")[1]
-        _check_dev(drows_dev, (T * k, H), dt, "drows")
-        _check_dev(inv_dev, (T, k), "int32", "inv")
-        _check_dev(dx_dev, (T, H), dt, "dx")
-        _check_on(self, {"drows": drows_dev, "inv": inv_dev, "dx": dx_dev})
-        call("rmoe_sort_tokens_backward_dev", self._h, ptr(drows_dev), _ROW_TYPES[dt], T, H, ptr(inv_dev), k, ptr(dx_dev),
-             _stream_ptr(stream))
+        check(_lib.load().rmoe_sort_tokens_backward_dev(
+            self._h, _operand(dev, drows_dev, (T * k, H), dt, "drows"), _ROW_TYPES[dt], T, H,
+            _operand(dev, inv_dev, (T, k), "int32", "inv"), k, _operand(dev, dx_dev, (T, H), dt, "dx"),
+            _stream_ptr(stream)))
 
     def combine_tokens_dev(self, rows_dev, inv_dev, wts_dev, out_dev, stream=None):
         """``out[t]`` = sum of ``wts[t, r] * rows[inv[t, r]]`` over the routes with a row, in fp32
         by ascending expert id, rounded once: rows [T * k, H], inv int32 [T, k] (of
         ``sort_tokens_dev``), wts float32 [T, k], out [T, H]."""
-        dt = _row_type(rows_dev, "rows")
+        dt, dev = _row_type(rows_dev, "rows"), self.device
         T, k = _shape2(inv_dev, "inv")
         H = _shape2(rows_dev, "rows")[1]
-        _check_dev(rows_dev, (T * k, H), dt, "rows")
-        _check_dev(inv_dev, (T, k), "int32", "inv")
-        _check_dev(wts_dev, (T, k), "float32", "wts")
-        _check_dev(out_dev, (T, H), dt, "out")
-        _check_on(self, {"rows": rows_dev, "inv": inv_dev, "wts": wts_dev, "out": out_dev})
-        call("rmoe_combine_tokens_dev", self._h, ptr(rows_dev), _ROW_TYPES[dt], T, H, ptr(inv_dev), ptr(wts_dev), k,
-             ptr(out_dev), _stream_ptr(stream))
+        check(_lib.load().rmoe_combine_tokens_dev(
+            self._h, _operand(dev, rows_dev, (T * k, H), dt, "rows"), _ROW_TYPES[dt], T, H,
+            _operand(dev, inv_dev, (T, k), "int32", "inv"), _operand(dev, wts_dev, (T, k), "float32", "wts"), k,
+            _operand(dev, out_dev, (T, H), dt, "out"), _stream_ptr(stream)))
 
     def combine_tokens_backward_dev(self, dout_dev, rows_dev, inv_dev, wts_dev, drows_dev, dwts_dev, stream=None):
         """Gradients of ``combine_tokens_dev``: ``drows[inv[t, r]] = wts[t, r] * dout[t]`` (rows no
         route names stay as they were) and ``dwts[t, r] = <dout[t], rows[inv[t, r]]>`` (float32,
         0 without a row)."""
-        dt = _row_type(rows_dev, "rows")
+        dt, dev = _row_type(rows_dev, "rows"), self.device
         T, k = _shape2(inv_dev, "inv")
         H = _shape2(rows_dev, "rows")[1]
-        _check_dev(dout_dev, (T, H), dt, "dout")
-        _check_dev(rows_dev, (T * k, H), dt, "rows")
-        _check_dev(inv_dev, (T, k), "int32", "inv")
-        _check_dev(wts_dev, (T, k), "float32", "wts")
-        _check_dev(drows_dev, (T * k, H), dt, "drows")
-        _check_dev(dwts_dev, (T, k), "float32", "dwts")
-        _check_on(self, {"dout": dout_dev, "rows": rows_dev, "inv": inv_dev, "wts": wts_dev, "drows": drows_dev,
-                         "dwts": dwts_dev})
-        call("rmoe_combine_tokens_backward_dev", self._h, ptr(dout_dev), ptr(rows_dev), _ROW_TYPES[dt], T, H, ptr(inv_dev),
-             ptr(wts_dev), k, ptr(drows_dev), ptr(dwts_dev), _stream_ptr(stream))
+        check(_lib.load().rmoe_combine_tokens_backward_dev(
+            self._h, _operand(dev, dout_dev, (T, H), dt, "dout"), _operand(dev, rows_dev, (T * k, H), dt, "rows"),
+            _ROW_TYPES[dt], T, H, _operand(dev, inv_dev, (T, k), "int32", "inv"),
+            _operand(dev, wts_dev, (T, k), "float32", "wts"), k, _operand(dev, drows_dev, (T * k, H), dt, "drows"),
+            _operand(dev, dwts_dev, (T, k), "float32", "dwts"), _stream_ptr(stream)))
 
     def dispatch(self, top_ids, n_experts: int) -> tuple[np.ndarray, np.ndarray]:
         ids = np.ascontiguousarray(top_ids, dtype=np.int32)
@@ -353,17 +359,13 @@ class Matrix:
         place).  ``act`` "none", "silu", "gelu", "gelu_tanh": y [T, M]; "swiglu", "situ" (with the
         betas): y [T, M / 2], the first M / 2 weight rows the gate, the others the up."""
         code, gb, vb, gated = _epilogue_act(act, gate_beta, value_beta)
-        K_in = _shape2(x_dev, "x")[1]
-        width = self.M // 2 if gated else self.M
-        _check_bf16(x_dev, (T, K_in), "x")
-        _check_bf16(y_dev, (T, width), "y")
-        if bias_dev is not None:
-            _check_dev(bias_dev, (self.M,), "float32", "bias")
-        if residual_dev is not None:
-            _check_bf16(residual_dev, (T, width), "residual")
-        _check_on(self.ctx, {"x": x_dev, "y": y_dev, "bias": bias_dev, "residual": residual_dev})
-        call("rmoe_linear_act_dev", self.ctx.handle, self.handle, ptr(x_dev), int(T), K_in, ptr(bias_dev), code, gb, vb,
-             ptr(residual_dev), ptr(y_dev), _stream_ptr(stream))
+        dev, T, K_in = self.ctx.device, int(T), _shape2(x_dev, "x")[1]
+        out = (T, self.M // 2 if gated else self.M)
+        check(_lib.load().rmoe_linear_act_dev(
+            self.ctx.handle, self.handle, _bf16_operand(dev, x_dev, (T, K_in), "x"), T, K_in,
+            None if bias_dev is None else _operand(dev, bias_dev, (self.M,), "float32", "bias"), code, gb, vb,
+            None if residual_dev is None else _bf16_operand(dev, residual_dev, out, "residual"),
+            _bf16_operand(dev, y_dev, out, "y"), _stream_ptr(stream)))
 
     def free(self):
         call("rmoe_matrix_free", self.ctx.handle, self.handle)
@@ -612,25 +614,22 @@ class MoeLayer:
         rows [n, K_in], bias float32 [n_routed, M], y and residual [n, M] or, gated, [n, M / 2].
         Rows from ``offsets[n_routed]`` on stay as they were.  Call
         ``reserve_experts_linear(n)`` first."""
-        codes = {"gate_up": PART_GATE_UP, "down": PART_DOWN}
-        if part not in codes:
+        g = self.geom
+        if part == "gate_up":
+            part_code, M = PART_GATE_UP, 2 * g.inter
+        elif part == "down":
+            part_code, M = PART_DOWN, g.hidden
+        else:
             raise ValueError(f"part must be 'gate_up' or 'down', got {part!r}")
         code, gb, vb, gated = _epilogue_act(act, gate_beta, value_beta)
-        g = self.geom
-        n, K_in = _shape2(rows_dev, "rows")
-        M = 2 * g.inter if part == "gate_up" else g.hidden
-        width = M // 2 if gated else M
-        _check_bf16(rows_dev, (n, K_in), "rows")
-        _check_dev(offsets_dev, (g.n_routed + 1,), "int32", "offsets")
-        _check_bf16(y_dev, (n, width), "y")
-        if bias_dev is not None:
-            _check_dev(bias_dev, (g.n_routed, M), "float32", "bias")
-        if residual_dev is not None:
-            _check_bf16(residual_dev, (n, width), "residual")
-        _check_on(self.ctx, {"rows": rows_dev, "offsets": offsets_dev, "y": y_dev, "bias": bias_dev,
-                             "residual": residual_dev})
-        call("rmoe_experts_linear_dev", self.ctx.handle, self.layer, codes[part], ptr(rows_dev), n, K_in, ptr(offsets_dev),
-             ptr(bias_dev), code, gb, vb, ptr(residual_dev), ptr(y_dev), _stream_ptr(stream))
+        dev, (n, K_in) = self.ctx.device, _shape2(rows_dev, "rows")
+        out = (n, M // 2 if gated else M)
+        check(_lib.load().rmoe_experts_linear_dev(
+            self.ctx.handle, self.layer, part_code, _bf16_operand(dev, rows_dev, (n, K_in), "rows"), n, K_in,
+            _operand(dev, offsets_dev, (g.n_routed + 1,), "int32", "offsets"),
+            None if bias_dev is None else _operand(dev, bias_dev, (g.n_routed, M), "float32", "bias"), code, gb, vb,
+            None if residual_dev is None else _bf16_operand(dev, residual_dev, out, "residual"),
+            _bf16_operand(dev, y_dev, out, "y"), _stream_ptr(stream)))
 
     def free(self):
         call("rmoe_layer_free", self.ctx.handle, self.layer)

@@ -25,6 +25,9 @@ class Tensor:
     def is_contiguous(self):
         return self._c
 
+    def get_device(self):
+        return self.device.index
+
     def data_ptr(self):
         return self._p
 
@@ -40,10 +43,14 @@ def f32(*shape, **kw):
 @pytest.fixture
 def ctx(monkeypatch):
     """A context without a device; a call that passes the wrapper's checks is a test's failure."""
-    def reached(name, *a):
-        raise AssertionError(f"{name} was called")
+    class Library:
+        def __getattr__(self, name):
+            def entry(*a):
+                raise AssertionError(f"{name} was called")
 
-    monkeypatch.setattr("raon_npu_amd.device.call", reached)
+            return entry
+
+    monkeypatch.setattr("raon_npu_amd._lib.load", Library)
     c = Context.__new__(Context)
     c._h, c.device = None, 0
     return c
