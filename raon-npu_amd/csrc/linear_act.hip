@@ -77,26 +77,54 @@ __global__ __launch_bounds__(512) void linear_act_kernel(LinAct a, int n_nt) {
   __syncthreads();
   constexpr float kUnit = kFmt == RMOE_FMT_BFP16 ? 4.f : 1.f;  // see wave_gemm.h
   auto sum = [&](int t, int c) {
-    float v = la_lds[t * kStride + c];
-    for (int w = 1; w < W; ++w) v += la_lds[(size_t)w * 16 * MF * kStride + t * kStride + c];
-    return kUnit * v;
+    const float* q = la_lds + t * kStride + c;
+    float4 v = *reinterpret_cast<const float4*>(q);
+    for (int w = 1; w < W; ++w) {
+      const float4 u = *reinterpret_cast<const float4*>(q + (size_t)w * 16 * MF * kStride);
+      v.x += u.x;
+      v.y += u.y;
+      v.z += u.z;
+      v.w += u.w;
+    }
+    return v;
   };
   const int width = kGated ? a.M / 2 : a.M;
   const float* bias = a.bias ? a.bias + (size_t)e * a.M : nullptr;
-  for (int i = tid; i < nrow * kOut; i += blockDim.x) {
-    const int t = i / kOut, c = i % kOut, col = nt * kOut + c;
-    float z = sum(t, c);
-    if (bias) z += bias[col];
-    if constexpr (kGated) {
-      float u = sum(t, kOut + c);
-      if (bias) u += bias[a.M / 2 + col];
-      z = act_pair(a.act, z, u, a.gb, a.vb);
-    } else {
-      z = act_single(a.act, z);
+  const bool wide = ((reinterpret_cast<uintptr_t>(a.y) | reinterpret_cast<uintptr_t>(a.residual)) & 7) == 0;
+  // Four columns a thread.
+  for (int i = tid; i < nrow * (kOut / 4); i += blockDim.x) {
+    const int t = i / (kOut / 4), c = 4 * (i % (kOut / 4)), col = nt * kOut + c;
+    float z[4], u[4];
+    *reinterpret_cast<float4*>(z) = sum(t, c);
+    if constexpr (kGated) *reinterpret_cast<float4*>(u) = sum(t, kOut + c);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      z[k] *= kUnit;
+      if (bias) z[k] += bias[col + k];
+      if constexpr (kGated) {
+        u[k] *= kUnit;
+        if (bias) u[k] += bias[a.M / 2 + col + k];
+        z[k] = act_pair(a.act, z[k], u[k], a.gb, a.vb);
+      } else {
+        z[k] = act_single(a.act, z[k]);
+      }
     }
     const size_t at = (size_t)(row0 + t) * width + col;
-    if (a.residual) z += bf16_to_f32(a.residual[at]);
-    a.y[at] = (uint16_t)f32_to_bf16(z);
+    if (wide) {
+      if (a.residual) {
+        const uint2 r = *reinterpret_cast<const uint2*>(a.residual + at);
+        z[0] += __uint_as_float(r.x << 16);
+        z[1] += __uint_as_float(r.x & 0xffff0000u);
+        z[2] += __uint_as_float(r.y << 16);
+        z[3] += __uint_as_float(r.y & 0xffff0000u);
+      }
+      *reinterpret_cast<uint2*>(a.y + at) =
+          make_uint2(f32_to_bf16(z[0]) | (f32_to_bf16(z[1]) << 16), f32_to_bf16(z[2]) | (f32_to_bf16(z[3]) << 16));
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        a.y[at + k] = (uint16_t)f32_to_bf16(a.residual ? z[k] + bf16_to_f32(a.residual[at + k]) : z[k]);
+    }
   }
 }
 
@@ -118,14 +146,31 @@ hipError_t launch(const LinAct& a, hipStream_t st) {
   return hipGetLastError();
 }
 
+// The largest tile that still gives the chip's 256 CUs kFillTiles workgroups, as for the
+// product without an epilogue (linear_mfma.hip); a gated tile needs a gate and an up fragment.
+// By expert, fewer rows than experts mostly come one to an expert: tiles of four rows then.
+constexpr int kFillTiles = 448;
+
 template <int kFmt>
 hipError_t pick(const LinAct& a, hipStream_t st) {
-  const bool gated = act_gated(a.act);
-  if (a.n <= 4) {
-    if (gated || a.M / 32 >= 448) return launch<kFmt, 1, 2, 1>(a, st);
+  const bool gated = act_gated(a.act), sparse = a.offsets && a.n < a.n_experts;
+  auto fills = [&](int rows, int nf) {
+    const size_t mt = sparse ? (size_t)a.n : ((size_t)a.n + rows - 1) / rows;
+    return mt * (size_t)(a.M / (16 * nf)) >= kFillTiles;
+  };
+  if (a.n <= 4 || sparse) {  // only the first row quartet of the fragment is loaded
+    if (fills(4, 4)) return launch<kFmt, 1, 4, 1>(a, st);
+    if (gated || fills(4, 2)) return launch<kFmt, 1, 2, 1>(a, st);
     return launch<kFmt, 1, 1, 1>(a, st);
   }
-  return launch<kFmt, 2, 4, 4>(a, st);
+  if (a.n > 16) {
+    if (fills(32, 4)) return launch<kFmt, 2, 4, 4>(a, st);
+    if (fills(32, 2)) return launch<kFmt, 2, 2, 4>(a, st);
+  } else if (fills(16, 4)) {
+    return launch<kFmt, 1, 4, 4>(a, st);
+  }
+  if (gated || fills(16, 2)) return launch<kFmt, 1, 2, 4>(a, st);
+  return launch<kFmt, 1, 1, 4>(a, st);
 }
 
 }  // namespace

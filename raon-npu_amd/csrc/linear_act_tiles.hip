@@ -22,15 +22,6 @@ typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 // --------------------------------------------------------------- preparation --
-// Workgroups 0..n_x-1: four rows of x each, to fp16 (zero past K_in) and their exponents; the
-// rest: the exponents of 256 weight rows each.
-struct PrepArgs {
-  LinAct a;
-  uint16_t* xh;
-  int32_t *xe, *we;
-  int n_x;
-};
-
 // The power of two e with v * 2^-e in [2^top, 2^(top+1)); 0 for zero and non-finite v.
 __device__ __forceinline__ int exponent_for(float v, int top) {
   const int be = (int)(__float_as_uint(v) >> 23) & 0xff;
@@ -45,45 +36,53 @@ __device__ __forceinline__ uint32_t bf16_pair_to_half(uint32_t v, int e) {
                    __builtin_amdgcn_ldexpf(__uint_as_float(v & 0xffff0000u), -e));
 }
 
-__global__ __launch_bounds__(256) void act_prep_kernel(PrepArgs p) {
-  const LinAct& a = p.a;
+// Rows of x to fp16 (zero past K_in) and their exponents, one wave a row.  A copy's work: 53,600
+// rows of 2,048 take 90 us (4.9 TB/s).
+__global__ __launch_bounds__(256) void act_prep_kernel(LinAct a, uint16_t* __restrict__ xh, int32_t* __restrict__ xe) {
   const int lane = threadIdx.x & 63, wave = wave_id();
-  if ((int)blockIdx.x < p.n_x) {
-    const size_t t = (size_t)blockIdx.x * 4 + wave;
-    if (t >= (size_t)a.n) return;
-    const uint4* src = reinterpret_cast<const uint4*>(a.x + t * a.K_in);
-    uint4* dst = reinterpret_cast<uint4*>(p.xh + t * a.K);
-    const int nch = a.K_in / 8, nout = a.K / 8;
-    float mx = 0.f;
-    for (int c = lane; c < nch; c += 64) {
-      const uint4 v = src[c];
-      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  const size_t t = (size_t)blockIdx.x * 4 + wave;
+  if (t >= (size_t)a.n) return;
+  const uint4* src = reinterpret_cast<const uint4*>(a.x + t * a.K_in);
+  uint4* dst = reinterpret_cast<uint4*>(xh + t * a.K);
+  const int nch = a.K_in / 8, nout = a.K / 8;
+  constexpr int kKeep = 5;  // 16-byte chunks a lane keeps between the two passes (2,560 columns)
+  uint4 v[kKeep];
+  float mx = 0.f;
+  auto largest = [&](const uint4& q) {
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        mx = fmaxf(mx, fmaxf(fabsf(__uint_as_float(w[i] << 16)), fabsf(__uint_as_float(w[i] & 0xffff0000u))));
-    }
+    for (int i = 0; i < 4; ++i)
+      mx = fmaxf(mx, fmaxf(fabsf(__uint_as_float(w[i] << 16)), fabsf(__uint_as_float(w[i] & 0xffff0000u))));
+  };
 #pragma unroll
-    for (int off = 32; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor(mx, off, 64));
-    const int e = exponent_for(mx, 14);
-    for (int c = lane; c < nout; c += 64) {
-      uint4 v = make_uint4(0u, 0u, 0u, 0u);
-      if (c < nch) {
-        const uint4 s = src[c];
-        v = make_uint4(bf16_pair_to_half(s.x, e), bf16_pair_to_half(s.y, e), bf16_pair_to_half(s.z, e),
-                       bf16_pair_to_half(s.w, e));
-      }
-      dst[c] = v;
-    }
-    if (lane == 0) p.xe[t] = e;
-    return;
+  for (int i = 0; i < kKeep; ++i) {
+    v[i] = lane + 64 * i < nch ? src[lane + 64 * i] : make_uint4(0u, 0u, 0u, 0u);
+    largest(v[i]);
   }
-  const size_t r = ((size_t)blockIdx.x - p.n_x) * 256 + threadIdx.x;  // row r % M of matrix r / M
-  const size_t rows = (size_t)a.M * (a.offsets ? a.n_experts : 1);
-  if (r >= rows) return;
-  const int row = (int)(r % a.M), nkt = a.K / kTileCols;
-  const bool b16 = a.fmt == RMOE_FMT_BFP16;
+  for (int c = lane + 64 * kKeep; c < nch; c += 64) largest(src[c]);
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor(mx, off, 64));
+  const int e = exponent_for(mx, 14);
+  auto half = [&](const uint4& q) {
+    return make_uint4(bf16_pair_to_half(q.x, e), bf16_pair_to_half(q.y, e), bf16_pair_to_half(q.z, e),
+                      bf16_pair_to_half(q.w, e));
+  };
+#pragma unroll
+  for (int i = 0; i < kKeep; ++i)
+    if (lane + 64 * i < nout) dst[lane + 64 * i] = half(v[i]);
+  for (int c = lane + 64 * kKeep; c < nout; c += 64) dst[c] = c < nch ? half(src[c]) : make_uint4(0u, 0u, 0u, 0u);
+  if (lane == 0) xe[t] = e;
+}
+
+// The exponent of each weight row, from its scale | min words or its blocks' exponents.
+__global__ __launch_bounds__(256) void row_exponents_kernel(const uint8_t* __restrict__ tiles, int fmt, int M, int K,
+                                                            int16_t* __restrict__ out) {
+  const int row = blockIdx.x * 256 + threadIdx.x;
+  if (row >= M) return;
+  const int nkt = K / kTileCols;
+  const bool b16 = fmt == RMOE_FMT_BFP16;
   const int tb = b16 ? kB16TileBytes : kTileBytes, at = b16 ? kB16MantBytes : kCodeBytes;
-  const uint8_t* q = a.tiles + (r / a.M) * a.wstride + (size_t)(row / kTileRows) * nkt * tb + at + (row % kTileRows) * 16;
+  const uint8_t* q = tiles + (size_t)(row / kTileRows) * nkt * tb + at + (row % kTileRows) * 16;
   float mx = 0.f;
   uint32_t emax = 7u;
 #pragma unroll 4
@@ -102,28 +101,33 @@ __global__ __launch_bounds__(256) void act_prep_kernel(PrepArgs p) {
     }
   }
   // |m| <= 2^7 in bfp16
-  p.we[r] = b16 ? (int)emax - 133 + 7 - 10 : exponent_for(mx, 10);
+  out[row] = (int16_t)(b16 ? (int)emax - 133 + 7 - 10 : exponent_for(mx, 10));
 }
 
 // ---------------------------------------------------------------------- tiles --
 struct TileArgs {
   LinAct a;
   const uint16_t* xh;
-  const int32_t *xe, *we;
+  const int32_t* xe;
   int n_nt;
 };
 
-constexpr int kActBM = 128;
-constexpr int kStage = kActBM * 128;  // bytes of 128 rows x 64 columns of fp16
-constexpr int kEpilogueLds = 65536;
+constexpr int kActBM = 128;  // rows of the largest tile
+// A kernel's tiles have up to 16 BF rows (BF = 2, 4, 8 fragments); a stage in LDS holds 64
+// columns of them in fp16.
+template <int BF>
+constexpr int kStage = 16 * BF * 128;
 
 // A wave's weights in LDS, as its tiles hold them: its 64 weight rows' sub-blocks of half a K
-// tile (64 columns: two of codes, four of mantissas; 1 KB each, two stages), then the 1 KB of
+// tile (64 columns: two of codes, four of mantissas; 1 KB each) in a ring, then the 1 KB of
 // scale | min words or exponents of a whole K tile (two, by the tile's parity).
 template <int kFmt>
 constexpr int kHalfBlocks = kFmt == RMOE_FMT_BFP16 ? 4 : 2;
+// Stages in LDS, of rows and of weights.  Three (where two workgroups a CU still fit) gained
+// nothing: 53,600 x gate/up 529 us with two, 537 with three.
+constexpr int kRing = 2;
 template <int kFmt>
-constexpr int kWaveWeights = 2 * 1024 * kHalfBlocks<kFmt> + 2 * 1024;
+constexpr int kWaveWeights = 1024 * kHalfBlocks<kFmt> * kRing + 2 * 1024;
 
 __device__ __forceinline__ f16x2 as_f16x2(uint32_t v) { return __builtin_bit_cast(f16x2, v); }
 __device__ __forceinline__ uint32_t as_u32(f16x2 v) { return __builtin_bit_cast(uint32_t, v); }
@@ -252,29 +256,43 @@ struct StageWeights<RMOE_FMT_BFP16, NF> {
   static __device__ __forceinline__ uint32_t chunk(int g) { return 2u * ((threadIdx.x & 63u) >> 4) + g; }
 };
 
-// One step of 32 columns: MF x NF products with the operands b, and under them the 2 NF
-// halves of the next step's operands n (from `from`, its step g), spread evenly: an MFMA takes
-// 16 cycles and its issue 4, so a wave's vector instructions fit between its own.  Chunk c
-// (16 bytes) of row r of a stage sits at chunk c ^ (r / 2 % 8): the 16 rows of a fragment then
-// cover all 64 banks.
-template <int kFmt, int MF, int NF>
-__device__ __forceinline__ void mfma_step(const uint8_t* stage, uint32_t chunk, const uint4 (&b)[NF],
-                                          const StageWeights<kFmt, NF>& from, int g, const int (&we)[NF],
-                                          const CodeMasks& masks, uint4 (&n)[NF], f32x4 (&acc)[8][NF]) {
+// One stage: two steps of 32 columns, each MF x NF products, the first with the operands b0.
+// Under the first step the second's operands b1 are formed from cur, under the second the next
+// stage's b0 from next, whose words are read halfway through the first; the forming is spread
+// evenly: an MFMA takes 16 cycles and its issue 4, so a wave's vector instructions fit between
+// its own.  Rows are read two fragments ahead.  Chunk c (16 bytes) of row r of a stage sits at
+// chunk c ^ (r / 2 % 8): the 16 rows of a fragment then cover all 64 banks.
+template <int kFmt, int BF, int MF, int NF, typename Copy, typename Read>
+__device__ __forceinline__ void mfma_stage(const uint8_t* stage, uint4 (&b0)[NF], const StageWeights<kFmt, NF>& cur,
+                                           StageWeights<kFmt, NF>& next, const int (&we)[NF], const CodeMasks& masks,
+                                           f32x4 (&acc)[BF][NF], Copy copy, Read read) {
   const uint32_t l16 = threadIdx.x & 15u;
-  const uint8_t* p = stage + 128u * l16 + 16u * (chunk ^ (l16 >> 1));
-  uint4 x[MF];
+  const uint8_t* p[2];
 #pragma unroll
-  for (int m = 0; m < 2; ++m) x[m] = *reinterpret_cast<const uint4*>(p + 2048 * m);
+  for (int g = 0; g < 2; ++g) p[g] = stage + 128u * l16 + 16u * (StageWeights<kFmt, NF>::chunk(g) ^ (l16 >> 1));
+  auto row = [&](int i) { return *reinterpret_cast<const uint4*>(p[i / MF] + 2048 * (i % MF)); };
+  uint4 x[2 * MF], b1[NF];
+  x[0] = row(0);
+  x[1] = row(1);
 #pragma unroll
-  for (int m = 0; m < MF; ++m) {
-    if (m + 2 < MF) x[m + 2] = *reinterpret_cast<const uint4*>(p + 2048 * (m + 2));
+  for (int i = 0; i < 2 * MF; ++i) {
+    const int m = i % MF;
+    if (i + 2 < 2 * MF) x[i + 2] = row(i + 2);
+    if (i == MF / 2) read();
+    if (i == MF) {
+      next.arrange();
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // read()'s place may be copied to from here on
+    }
+    copy(i);
 #pragma unroll
     for (int f = 0; f < NF; ++f)
-      acc[m][f] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, x[m]), __builtin_bit_cast(f16x8, b[f]),
-                                                         acc[m][f], 0, 0, 0);
+      acc[m][f] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, x[i]),
+                                                         __builtin_bit_cast(f16x8, i < MF ? b0[f] : b1[f]), acc[m][f], 0, 0, 0);
 #pragma unroll
-    for (int q = 2 * NF * m / MF; q < 2 * NF * (m + 1) / MF; ++q) from.form(g, q / 2, q % 2, we, masks, n[q / 2]);
+    for (int q = 2 * NF * m / MF; q < 2 * NF * (m + 1) / MF; ++q) {
+      if (i < MF) cur.form(1, q / 2, q % 2, we, masks, b1[q / 2]);
+      else next.form(0, q / 2, q % 2, we, masks, b0[q / 2]);
+    }
     __builtin_amdgcn_sched_barrier(0);
   }
 }
@@ -295,25 +313,29 @@ __device__ __forceinline__ void copy16(const void* base, uint32_t offset, uint32
       : "v"(offset), "s"(base), "s"(__builtin_amdgcn_readfirstlane(lds))
       : "memory");
 }
-// Every copy of this wave has landed, then the workgroup meets.
+// All but the last kPending copies of this wave have landed, then the workgroup meets.
+template <int kPending>
 __device__ __forceinline__ void copies_landed() {
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kPending) : "memory");
   __syncthreads();
 }
 
 // One tile of up to 16 MF rows x 64 NF weight rows; wave w takes all rows and 16 NF = 64
 // weight rows of its own (w: the matrix; wo: byte offset of weight row `lane` of the 64).
-// Stages of 64 columns, two in LDS: a stage's rows are copied under the one before, its
-// weights, which no other wave reads, under the one before that, so that their operands are
-// formed under products throughout.  One barrier a stage.
-template <int kFmt, int MF, int NF>
+// Stages s of 64 columns.  Rows are copied R - 1 stages ahead into a ring of R = kRing, and
+// weights, which no other wave reads, R + 1 ahead into the place that stage s + 1's left when
+// their words went to registers, so that operands are formed under products throughout.  A
+// wave waits in the order of its copies: at a stage's end for those issued by the end of the
+// stage R - 1 before.  One barrier a stage.  Copies past the end repeat the last stage's.
+template <int kFmt, int BF, int MF, int NF>
 __device__ __forceinline__ void tile_product(const TileArgs& t, const uint8_t* w, uint32_t wo, int we_lane,
-                                             const int (&we)[NF], int row0, uint8_t* lds, f32x4 (&acc)[8][NF]) {
+                                             const int (&we)[NF], int row0, uint8_t* lds, f32x4 (&acc)[BF][NF]) {
   static_assert(NF == 4, "64 weight rows a wave");
   constexpr int kTB = kFmt == RMOE_FMT_BFP16 ? kB16TileBytes : kTileBytes, kBlocks = kHalfBlocks<kFmt>;
-  const int lane = threadIdx.x & 63, wave = wave_id(), nkt = t.a.K / kTileCols;
+  constexpr int R = kRing, kAhead = R - 1;
+  const int lane = threadIdx.x & 63, wave = wave_id(), nkt = t.a.K / kTileCols, ns = 2 * nkt;
   const uint32_t lds0 = (uint32_t)(uintptr_t)lds;
-  const int wbase = 2 * kStage + wave * kWaveWeights<kFmt>, pbase = wbase + 2 * 1024 * kBlocks;
+  const int wbase = R * kStage<BF> + wave * kWaveWeights<kFmt>, pbase = wbase + R * 1024 * kBlocks;
   // Copy q = wave + 4i fills LDS rows 8q..8q+7 (1 KB): lane L brings row 8q + L / 8 the chunk
   // that sits at position L % 8.  Rows past the tile are the next tiles' or, behind the last
   // row, the kActBM spare rows of the scratch; their results are not stored.
@@ -322,78 +344,99 @@ __device__ __forceinline__ void tile_product(const TileArgs& t, const uint8_t* w
   const uint32_t xo = (uint32_t)(8 * wave + lane / 8) * ld + 16u * (uint32_t)((lane % 8) ^ ((4 * wave + lane / 16) % 8));
   uint32_t rows0 = lds0 + 1024u * (uint32_t)wave;
   asm volatile("" : "+s"(rows0));  // kept in a scalar register
-  auto load_rows = [&](const uint8_t* x, int slot) {
-#pragma unroll
-    for (int i = 0; i < MF / 2; ++i) copy16(x + (size_t)(32 * i) * ld, xo, rows0 + (uint32_t)(slot * kStage + 4096 * i));
+  auto row_copy = [&](int i, int s, uint32_t slot) {
+    copy16(xb + 128 * min(s, ns - 1) + (size_t)(32 * i) * ld, xo, rows0 + slot + (uint32_t)(4096 * i));
   };
-  auto load_weights = [&](const uint8_t* tile, int j) {
-#pragma unroll
-    for (int i = 0; i < kBlocks; ++i)
-      copy16(tile + 1024 * (kBlocks * j + i), wo, lds0 + (uint32_t)(wbase + 1024 * (kBlocks * j + i)));
+  // Stage q's weights, q of the parity j, at byte `at` of the wave's ring: kBlocks + 1 - j copies.
+  auto weight_copy = [&](int i, int q, uint32_t at) {
+    const int j = q & 1;
+    const uint8_t* tile = w + (size_t)min(q >> 1, nkt - 1) * kTB;
+    if (i < kBlocks) copy16(tile + 1024 * (kBlocks * j + i), wo, lds0 + (uint32_t)wbase + at + (uint32_t)(1024 * i));
+    else copy16(tile + 2048 * kBlocks, wo, lds0 + (uint32_t)(pbase + 1024 * ((q >> 1) & 1)));
   };
-  auto load_words = [&](const uint8_t* tile, int par) {
-    copy16(tile + 2048 * kBlocks, wo, lds0 + (uint32_t)(pbase + 1024 * par));
+  auto load_weights = [&](int q, uint32_t at) {
+#pragma unroll
+    for (int i = 0; i < kBlocks; ++i) weight_copy(i, q, at);
+    if ((q & 1) == 0) weight_copy(kBlocks, q, at);
+  };
+  // A stage's copies, spread over its 2 MF turns (a wave stands still at a copy until the
+  // copies before it are taken up): rows under the first step, weights under the second.
+  auto copies = [&](int i, int s, int q, int nw, uint32_t there, uint32_t at) {
+#pragma unroll
+    for (int c = 0; c < MF / 2; ++c)
+      if (i == 2 * c + 1) row_copy(c, s, there);
+#pragma unroll
+    for (int c = 0; c < nw; ++c)
+      if (i == MF + (c + 1) * (MF - 1) / nw) weight_copy(c, q, at);
   };
   const CodeMasks masks = code_masks();
-  load_rows(xb, 0);
-  load_weights(w, 0);
-  load_weights(w, 1);
-  load_words(w, 0);
-  copies_landed();
+#pragma unroll
+  for (int s = 0; s < kAhead; ++s)
+#pragma unroll
+    for (int i = 0; i < MF / 2; ++i) row_copy(i, s, (uint32_t)(s * kStage<BF>));
+#pragma unroll
+  for (int s = 0; s < R; ++s) load_weights(s, (uint32_t)(s * 1024 * kBlocks));
+  copies_landed<0>();
   if constexpr (kFmt == RMOE_FMT_Q4NX) convert_words(lds + pbase, we_lane);
   StageWeights<kFmt, NF> cur, next;
-  uint4 b0[NF], b1[NF];
+  uint4 b0[NF];
   cur.read(lds + wbase, lds + pbase, 0);
   cur.arrange();
 #pragma unroll
   for (int q = 0; q < 2 * NF; ++q) cur.form(0, q / 2, q % 2, we, masks, b0[q / 2]);
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  load_weights(R, 0u);
+  // Ring offsets: stage s's rows, stage s + kAhead's rows, stage s + 1's weights.
+  uint32_t here = 0u, there = (uint32_t)(kAhead * kStage<BF>), ws = (uint32_t)(1024 * kBlocks);
+  auto turn = [&]() {
+    here = here == (uint32_t)((R - 1) * kStage<BF>) ? 0u : here + (uint32_t)kStage<BF>;
+    there = there == (uint32_t)((R - 1) * kStage<BF>) ? 0u : there + (uint32_t)kStage<BF>;
+    ws = ws == (uint32_t)((R - 1) * 1024 * kBlocks) ? 0u : ws + (uint32_t)(1024 * kBlocks);
+  };
+  // Copies that may be in flight at the end of a stage: R - 2 stages' rows and the weights of
+  // the last R - 1, with words every second stage (for R = 2: with the even stage q alone).
+  constexpr int kRows = (R - 2) * (MF / 2);
+  constexpr int kEvenEnd = R == 2 ? kBlocks : kRows + 2 * kBlocks + 1, kOddEnd = R == 2 ? kBlocks + 1 : kEvenEnd;
 #pragma unroll 1
   for (int kt = 0; kt < nkt; ++kt) {
     const uint8_t* wp = lds + pbase + 1024 * (kt & 1);
     const uint8_t* wp_next = lds + pbase + 1024 * ((kt + 1) & 1);
-    const bool more = kt + 1 < nkt;
-    // First half of the tile.  Its weights are in registers; their place in LDS takes the
-    // next tile's.
-    load_rows(xb + 128, 1);
-    if (more) {
-      load_weights(w + kTB, 0);
-      load_words(w + kTB, (kt + 1) & 1);
-    }
-    mfma_step<kFmt, MF, NF>(lds, StageWeights<kFmt, NF>::chunk(0), b0, cur, 1, we, masks, b1, acc);
-    next.read(lds + wbase + 1024 * kBlocks, wp, 1);
-    next.arrange();
-    mfma_step<kFmt, MF, NF>(lds, StageWeights<kFmt, NF>::chunk(1), b1, next, 0, we, masks, b0, acc);
-    copies_landed();
-    // Second half; past the last tile the operands formed are of old weights and not used.
-    if (more) {
-      xb += 256;
-      w += kTB;
-      load_rows(xb, 0);
-      load_weights(w, 1);
-      if constexpr (kFmt == RMOE_FMT_Q4NX) convert_words(lds + pbase + 1024 * ((kt + 1) & 1), we_lane);
-    }
-    mfma_step<kFmt, MF, NF>(lds + kStage, StageWeights<kFmt, NF>::chunk(0), b0, next, 1, we, masks, b1, acc);
-    cur.read(lds + wbase, wp_next, 0);
-    cur.arrange();
-    mfma_step<kFmt, MF, NF>(lds + kStage, StageWeights<kFmt, NF>::chunk(1), b1, cur, 0, we, masks, b0, acc);
-    copies_landed();
+    const int s = 2 * kt;
+    mfma_stage<kFmt, BF, MF, NF>(
+        lds + here, b0, cur, next, we, masks, acc,
+        [&](int i) { copies(i, s + kAhead, s + 1 + R, kBlocks + R % 2, there, ws); },
+        [&] { next.read(lds + wbase + ws, wp, 1); });
+    copies_landed<kEvenEnd>();
+    turn();
+    mfma_stage<kFmt, BF, MF, NF>(
+        lds + here, b0, next, cur, we, masks, acc,
+        [&](int i) {
+          // The next tile's words have landed (past the last tile the operands are not used).
+          if (kFmt == RMOE_FMT_Q4NX && i == 0) convert_words(lds + pbase + 1024 * ((kt + 1) & 1), we_lane);
+          copies(i, s + 1 + kAhead, s + 2 + R, kBlocks + 1 - R % 2, there, ws);
+        },
+        [&] { cur.read(lds + wbase + ws, wp_next, 0); });
+    copies_landed<kOddEnd>();
+    turn();
   }
+  copies_landed<0>();  // the epilogue reuses the memory
 }
 
-template <int kFmt, int NF, bool kGated>
-__global__ __launch_bounds__(256, 2) void act_tile_kernel(TileArgs t) {
-  constexpr int kLds = 2 * kStage + 4 * kWaveWeights<kFmt>;
-  __shared__ __attribute__((aligned(16))) uint8_t lds[kLds > kEpilogueLds ? kLds : kEpilogueLds];
+template <int kFmt, int NF, bool kGated, int BF>
+__global__ __launch_bounds__(256, BF == 8 ? 2 : BF == 4 ? 3 : 4) void act_tile_kernel(TileArgs t) {
+  constexpr int kLds = kRing * kStage<BF> + 4 * kWaveWeights<kFmt>, kTile = 16 * BF;
+  static_assert(kLds <= 80 * 1024, "two workgroups a CU");
+  __shared__ __attribute__((aligned(16))) uint8_t lds[kLds];
   constexpr int kCols = 64 * NF, kOut = kGated ? kCols / 2 : kCols;
   constexpr int kTB = kFmt == RMOE_FMT_BFP16 ? kB16TileBytes : kTileBytes;
   const LinAct& a = t.a;
-  RowTiles<kActBM> rt;
-  const int n_mt = a.offsets ? rt.total(a.offsets, a.n_experts, a.n) : (a.n + kActBM - 1) / kActBM;
+  RowTiles<kTile> rt;
+  const int n_mt = a.offsets ? rt.total(a.offsets, a.n_experts, a.n) : (a.n + kTile - 1) / kTile;
   const int total = n_mt * t.n_nt, per = (total + 7) / 8, slot = (int)blockIdx.x / 8;
   const int id = ((int)blockIdx.x % 8) * per + slot;
   if (slot >= per || id >= total) return;
   const int nt = id % t.n_nt;
-  int e = 0, row0 = id / t.n_nt * kActBM, nrow = min(kActBM, a.n - row0);
+  int e = 0, row0 = id / t.n_nt * kTile, nrow = min(kTile, a.n - row0);
   if (a.offsets) rt.find(id / t.n_nt, e, row0, nrow);
   const int wave = wave_id(), nkt = a.K / kTileCols, width = kGated ? a.M / 2 : a.M;
   const uint8_t* tiles = a.tiles + (size_t)e * a.wstride;
@@ -403,24 +446,24 @@ __global__ __launch_bounds__(256, 2) void act_tile_kernel(TileArgs t) {
   auto row_of = [&](int r) { return kGated && r >= 32 ? width + base + r - 32 : base + r; };
   const int wr = row_of(threadIdx.x & 63);
   const uint32_t wo = (uint32_t)(wr / kTileRows) * (uint32_t)(nkt * kTB) + (uint32_t)(wr % kTileRows) * 16u;
-  const int32_t* wes = t.we + (size_t)e * a.M;
+  const int16_t* wes = a.exps + (size_t)e * a.M;
   int we[NF];
 #pragma unroll
   for (int f = 0; f < NF; ++f) we[f] = wes[row_of(16 * f + (threadIdx.x & 15))];
-  f32x4 acc[8][NF];
+  f32x4 acc[BF][NF];
 #pragma unroll
-  for (int m = 0; m < 8; ++m)
+  for (int m = 0; m < BF; ++m)
 #pragma unroll
     for (int f = 0; f < NF; ++f) acc[m][f] = f32x4{0.f, 0.f, 0.f, 0.f};
   // A short tile multiplies only the fragments that hold rows.
-  if (nrow > 64) tile_product<kFmt, 8, NF>(t, tiles, wo, wes[wr], we, row0, lds, acc);
-  else if (nrow > 32) tile_product<kFmt, 4, NF>(t, tiles, wo, wes[wr], we, row0, lds, acc);
-  else tile_product<kFmt, 2, NF>(t, tiles, wo, wes[wr], we, row0, lds, acc);
+  if (BF == 8 && nrow > 64) tile_product<kFmt, BF, BF, NF>(t, tiles, wo, wes[wr], we, row0, lds, acc);
+  else if (BF >= 4 && nrow > 32) tile_product<kFmt, BF, BF < 4 ? BF : 4, NF>(t, tiles, wo, wes[wr], we, row0, lds, acc);
+  else tile_product<kFmt, BF, 2, NF>(t, tiles, wo, wes[wr], we, row0, lds, acc);
 
   // Epilogue: sums and bias through LDS as fp32, kRows rows at a time, so that the activation
   // has its operands at hand and residual and y move 16 bytes a thread.  Columns of
   // different lq go to different banks: column c of row r sits at c ^ 16 (r / 4 % 4).
-  constexpr int kRows = kEpilogueLds / 4 / kCols;
+  constexpr int kRows = kLds >= kTile * kCols * 4 ? kTile : kLds >= kTile / 2 * kCols * 4 ? kTile / 2 : kTile / 4;
   int tid = threadIdx.x;
   asm volatile("" : "+v"(tid));  // what follows from it is computed here, not kept across the products
   const int l16 = tid & 15, lq = (tid & 63) >> 4;
@@ -432,7 +475,7 @@ __global__ __launch_bounds__(256, 2) void act_tile_kernel(TileArgs t) {
   for (int f = 0; f < NF; ++f) bias[f] = a.bias ? a.bias[(size_t)e * a.M + row_of(16 * f + l16)] : 0.f;
   const bool wide = ((reinterpret_cast<uintptr_t>(a.y) | reinterpret_cast<uintptr_t>(a.residual)) & 15) == 0;
 #pragma unroll
-  for (int r0 = 0; r0 < kActBM; r0 += kRows) {
+  for (int r0 = 0; r0 < kTile; r0 += kRows) {
     if (r0 >= nrow) break;
     if (r0) __syncthreads();
 #pragma unroll
@@ -492,47 +535,65 @@ __global__ __launch_bounds__(256, 2) void act_tile_kernel(TileArgs t) {
   }
 }
 
-template <int kFmt, int NF>
+template <int kFmt, int BF>
 hipError_t launch_tiles(const TileArgs& t0, hipStream_t st) {
+  constexpr int NF = 4, kTile = 16 * BF;
   TileArgs t = t0;
   const LinAct& a = t.a;
   t.n_nt = (a.M + 64 * NF - 1) / (64 * NF);
-  const size_t mt = a.offsets ? std::min<size_t>(a.n, (size_t)a.n / kActBM + a.n_experts) : ((size_t)a.n + kActBM - 1) / kActBM;
+  const size_t mt = a.offsets ? std::min<size_t>(a.n, (size_t)a.n / kTile + a.n_experts) : ((size_t)a.n + kTile - 1) / kTile;
   const size_t grid = 8 * ((mt * t.n_nt + 7) / 8);
   if (grid * 256 >= (size_t)1 << 32) return hipErrorInvalidValue;
-  auto* kernel = act_gated(a.act) ? act_tile_kernel<kFmt, NF, true> : act_tile_kernel<kFmt, NF, false>;
+  auto* kernel = act_gated(a.act) ? act_tile_kernel<kFmt, NF, true, BF> : act_tile_kernel<kFmt, NF, false, BF>;
   hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(256), 0, st, t);
   return hipGetLastError();
+}
+// By the rows an expert has in the mean (128 experts, q4nx gate/up [1536, 2048], tiles of 32, 64
+// and 128 rows: 28 rows 80, 78 and 85 us, 44 rows 120, 91 and 101, 62 rows 149, 125 and 125, 94
+// rows 195, 160 and 143; bfp16 down [2560, 1088]: 12 rows 99, 108 and 108, 47 rows 149, 143 and 143,
+// 70 rows 183, 179 and 169); one matrix has rows enough for the largest.
+template <int kFmt>
+hipError_t pick_tiles(const TileArgs& t, hipStream_t st) {
+  const size_t rows = t.a.offsets ? (size_t)t.a.n / t.a.n_experts : (size_t)t.a.n;
+  if (rows <= 24) return launch_tiles<kFmt, 2>(t, st);
+  if (rows <= 64) return launch_tiles<kFmt, 4>(t, st);
+  return launch_tiles<kFmt, 8>(t, st);
 }
 
 size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 
 }  // namespace
 
-// The rule, and the scratch of n rows with it (0: the kernel of few rows, which needs none).
+hipError_t launch_row_exponents(const uint8_t* tiles, int fmt, int M, int K, int16_t* exps, hipStream_t st) {
+  hipLaunchKernelGGL(row_exponents_kernel, dim3((M + 255) / 256), dim3(256), 0, st, tiles, fmt, M, K, exps);
+  return hipGetLastError();
+}
+
+// Which rows this kernel serves, against linear_act_kernel (whose cost grows with every 32 rows).
+// One matrix: from 144 tiles of 128 x 256 ([2176, 2560]: 2,048 rows 60 / 67 us, 4,096 rows 88 /
+// 120; [1536, 2048], 1,024 rows, 48 tiles: 47 / 19).  By expert: from one row an expert
+// (128 experts, gate/up [1536, 2048]: 32 rows 35 / 23 us, 128 rows 46 / 52, 2,048 rows 66 / 78,
+// 8,000 rows 125 / 206).
 bool act_tiles_serve(int fmt, int M, int K, int groups, size_t n) {
   const size_t bytes = fmt == RMOE_FMT_BFP16 ? matrix_bytes_bfp16(M, K) : matrix_bytes(M, K);
   if (bytes >= (size_t)1 << 32) return false;  // 32-bit byte offsets into a matrix
-  return n >= (groups == 1 ? 128 : (size_t)16 * groups);
+  if (groups > 1) return n >= (size_t)groups;
+  return (n + kActBM - 1) / kActBM * ((M + 255) / 256) >= 144;
 }
 size_t act_tiles_scratch(int fmt, int M, int K, int groups, size_t n) {
   if (!act_tiles_serve(fmt, M, K, groups, n)) return 0;
-  return round256((n + kActBM) * K * 2) + round256(n * 4) + round256((size_t)groups * M * 4);
+  return round256((n + kActBM) * K * 2) + round256(n * 4);
 }
 
 hipError_t launch_act_tiles(const LinAct& a, uint8_t* scratch, size_t bytes, hipStream_t st) {
-  const int groups = a.offsets ? a.n_experts : 1;
-  if (act_tiles_scratch(a.fmt, a.M, a.K, groups, a.n) > bytes) return hipErrorOutOfMemory;
+  if (act_tiles_scratch(a.fmt, a.M, a.K, a.offsets ? a.n_experts : 1, a.n) > bytes) return hipErrorOutOfMemory;
   uint16_t* xh = reinterpret_cast<uint16_t*>(scratch);
   int32_t* xe = reinterpret_cast<int32_t*>(scratch + round256(((size_t)a.n + kActBM) * a.K * 2));
-  int32_t* we = reinterpret_cast<int32_t*>(reinterpret_cast<uint8_t*>(xe) + round256((size_t)a.n * 4));
-  const size_t n_x = ((size_t)a.n + 3) / 4, n_w = ((size_t)groups * a.M + 255) / 256;
-  if ((n_x + n_w) * 256 >= (size_t)1 << 32) return hipErrorInvalidValue;
-  hipLaunchKernelGGL(act_prep_kernel, dim3((unsigned)(n_x + n_w)), dim3(256), 0, st, PrepArgs{a, xh, xe, we, (int)n_x});
+  hipLaunchKernelGGL(act_prep_kernel, dim3((unsigned)(((size_t)a.n + 3) / 4)), dim3(256), 0, st, a, xh, xe);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  const TileArgs t{a, xh, xe, we, 0};
-  return a.fmt == RMOE_FMT_BFP16 ? launch_tiles<RMOE_FMT_BFP16, 4>(t, st) : launch_tiles<RMOE_FMT_Q4NX, 4>(t, st);
+  const TileArgs t{a, xh, xe, 0};
+  return a.fmt == RMOE_FMT_BFP16 ? pick_tiles<RMOE_FMT_BFP16>(t, st) : pick_tiles<RMOE_FMT_Q4NX>(t, st);
 }
 
 }  // namespace rmoe

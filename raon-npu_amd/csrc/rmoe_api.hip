@@ -260,15 +260,35 @@ int sync_and_check(rmoe_ctx* ctx, hipStream_t st) {
   return RMOE_OK;
 }
 
+// The tiles of an [M, K] matrix of `need` bytes, and behind them the exponents of its rows.
+bool alloc_matrix(RmoeMatrix& m, size_t need) {
+  if (hipMalloc((void**)&m.tiles, need + (size_t)m.M * sizeof(int16_t)) != hipSuccess) return false;
+  m.exps = reinterpret_cast<int16_t*>(m.tiles + need);
+  return true;
+}
+// The exponents of freshly written weights (queued behind them).
+hipError_t matrix_exponents(const RmoeMatrix& m, hipStream_t st) {
+  return rmoe::launch_row_exponents(m.tiles, m.fmt, m.M, m.K, m.exps, st);
+}
+hipError_t gu_exponents(const RmoeLayer& L, size_t e, hipStream_t st) {
+  return rmoe::launch_row_exponents(L.gu + e * L.gu_bytes, RMOE_FMT_Q4NX, 2 * L.I, L.H, L.gu_exps + e * 2 * L.I, st);
+}
+hipError_t dn_exponents(const RmoeLayer& L, size_t e, hipStream_t st) {
+  return rmoe::launch_row_exponents(L.dn + e * L.dn_bytes, L.dn_fmt, L.H, L.Ipad, L.dn_exps + e * L.H, st);
+}
+
 // Allocate the expert storage of L and register it as `layer` (replacing nothing:
 // the caller freed any previous layer of that id).
 int place_layer(rmoe_ctx* ctx, int layer, RmoeLayer& L) {
-  if (hipMalloc((void**)&L.gu, (size_t)L.gu_experts * L.gu_bytes) != hipSuccess)
-    return fail(RMOE_ENOMEM, "hipMalloc of expert gate_up failed");
-  if (hipMalloc((void**)&L.dn, (size_t)L.dn_experts * L.dn_bytes) != hipSuccess) {
+  const size_t gub = (size_t)L.gu_experts * L.gu_bytes, gue = (size_t)L.gu_experts * 2 * L.I * sizeof(int16_t);
+  const size_t dnb = (size_t)L.dn_experts * L.dn_bytes, dne = (size_t)L.dn_experts * L.H * sizeof(int16_t);
+  if (hipMalloc((void**)&L.gu, gub + gue) != hipSuccess) return fail(RMOE_ENOMEM, "hipMalloc of expert gate_up failed");
+  if (hipMalloc((void**)&L.dn, dnb + dne) != hipSuccess) {
     hipFree(L.gu);
     return fail(RMOE_ENOMEM, "hipMalloc of expert down failed");
   }
+  L.gu_exps = reinterpret_cast<int16_t*>(L.gu + gub);
+  L.dn_exps = reinterpret_cast<int16_t*>(L.dn + dnb);
   if (L.dn_fmt == RMOE_FMT_BFP16 &&
       (hipMalloc((void**)&L.dn_rowexp, (size_t)L.dn_experts * L.H) != hipSuccess ||
        hipMemset(L.dn_rowexp, 7, (size_t)L.dn_experts * L.H) != hipSuccess)) {
@@ -522,10 +542,11 @@ int rmoe_matrix_upload(rmoe_ctx* ctx, const void* bytes, size_t nbytes, int M, i
   RmoeMatrix m;
   m.M = M;
   m.K = K;
-  if (hipMalloc((void**)&m.tiles, need) != hipSuccess) return fail(RMOE_ENOMEM, "hipMalloc of %zu bytes failed", need);
+  if (!alloc_matrix(m, need)) return fail(RMOE_ENOMEM, "hipMalloc of %zu bytes failed", need);
   TRY(grow(ctx->s.staging, ctx->s.staging_bytes, need, ctx));
   HIP_TRY(hipMemcpyAsync(ctx->s.staging, bytes, need, hipMemcpyHostToDevice, ctx->stream));
   HIP_TRY(rmoe::launch_relayout_in(ctx->s.staging, m.tiles, M, K, ctx->stream));
+  HIP_TRY(matrix_exponents(m, ctx->stream));
   HIP_TRY(hipStreamSynchronize(ctx->stream));
   *handle = ctx->next_handle++;
   ctx->mats[*handle] = m;
@@ -541,7 +562,7 @@ int rmoe_matrix_upload_q4k(rmoe_ctx* ctx, const void* bytes, size_t nbytes, int 
   RmoeMatrix m;
   m.M = M;
   m.K = K;
-  if (hipMalloc((void**)&m.tiles, tb) != hipSuccess) return fail(RMOE_ENOMEM, "hipMalloc of %zu bytes failed", tb);
+  if (!alloc_matrix(m, tb)) return fail(RMOE_ENOMEM, "hipMalloc of %zu bytes failed", tb);
   int r = grow(ctx->s.staging, ctx->s.staging_bytes, need, ctx);
   if (r != RMOE_OK) {
     hipFree(m.tiles);
@@ -549,6 +570,7 @@ int rmoe_matrix_upload_q4k(rmoe_ctx* ctx, const void* bytes, size_t nbytes, int 
   }
   HIP_TRY(hipMemcpyAsync(ctx->s.staging, bytes, need, hipMemcpyHostToDevice, ctx->stream));
   HIP_TRY(rmoe::launch_q4k_to_tiles(ctx->s.staging, M, K, m.tiles, K, 0, ctx->stream));
+  HIP_TRY(matrix_exponents(m, ctx->stream));
   HIP_TRY(hipStreamSynchronize(ctx->stream));
   *handle = ctx->next_handle++;
   ctx->mats[*handle] = m;
@@ -566,7 +588,7 @@ int rmoe_matrix_upload_bfp16(rmoe_ctx* ctx, const void* bytes, size_t nbytes, in
   m.M = M;
   m.K = K;
   m.fmt = RMOE_FMT_BFP16;
-  if (hipMalloc((void**)&m.tiles, need) != hipSuccess) return fail(RMOE_ENOMEM, "hipMalloc of %zu bytes failed", need);
+  if (!alloc_matrix(m, need)) return fail(RMOE_ENOMEM, "hipMalloc of %zu bytes failed", need);
   int r = grow(ctx->s.staging, ctx->s.staging_bytes, need, ctx);
   if (r != RMOE_OK) {
     hipFree(m.tiles);
@@ -574,6 +596,7 @@ int rmoe_matrix_upload_bfp16(rmoe_ctx* ctx, const void* bytes, size_t nbytes, in
   }
   HIP_TRY(hipMemcpyAsync(ctx->s.staging, bytes, need, hipMemcpyHostToDevice, ctx->stream));
   HIP_TRY(rmoe::launch_b16_relayout_in(ctx->s.staging, m.tiles, M, K, ctx->stream));
+  HIP_TRY(matrix_exponents(m, ctx->stream));
   HIP_TRY(hipStreamSynchronize(ctx->stream));
   *handle = ctx->next_handle++;
   ctx->mats[*handle] = m;
@@ -588,10 +611,11 @@ int rmoe_matrix_quantize_dev(rmoe_ctx* ctx, const float* w_dev, int M, int K, in
   m.M = M;
   m.K = K;
   const size_t need = rmoe::matrix_bytes(M, K);
-  if (hipMalloc((void**)&m.tiles, need) != hipSuccess) return fail(RMOE_ENOMEM, "hipMalloc of %zu bytes failed", need);
+  if (!alloc_matrix(m, need)) return fail(RMOE_ENOMEM, "hipMalloc of %zu bytes failed", need);
   hipStream_t st = pick_stream(ctx, stream);
   if (!stream) HIP_TRY(hipDeviceSynchronize());  // the context's stream is ordered with no other
   HIP_TRY(rmoe::launch_quantize(w_dev, M, K, K, K, m.tiles, ctx->s.err, st));
+  HIP_TRY(matrix_exponents(m, st));
   int r = sync_and_check(ctx, st);
   if (r != RMOE_OK) {
     hipFree(m.tiles);
@@ -732,7 +756,7 @@ int rmoe_linear_act_dev(rmoe_ctx* ctx, int handle, const void* x_dev, int T, int
                         float gate_beta, float value_beta, const void* residual_dev, void* y_dev, void* stream) {
   RmoeMatrix* m;
   TRY(find_matrix(ctx, handle, &m));
-  const rmoe::LinAct L{m->tiles, 0, m->fmt, m->M, m->K, (const uint16_t*)x_dev, T, K_in, nullptr, 0, bias_dev, act,
+  const rmoe::LinAct L{m->tiles, m->exps, 0, m->fmt, m->M, m->K, (const uint16_t*)x_dev, T, K_in, nullptr, 0, bias_dev, act,
                        gate_beta, value_beta, (const uint16_t*)residual_dev, (uint16_t*)y_dev};
   return run_linear_act(ctx, L, stream);
 }
@@ -753,7 +777,7 @@ int rmoe_experts_linear_dev(rmoe_ctx* ctx, int layer, int part, const void* rows
     return fail(RMOE_EINVAL, "part must be RMOE_PART_GATE_UP or RMOE_PART_DOWN, got %d", part);
   if (!offsets_dev) return fail(RMOE_EINVAL, "null argument");
   const bool up = part == RMOE_PART_GATE_UP;
-  const rmoe::LinAct L{up ? l->gu : l->dn, up ? l->gu_bytes : l->dn_bytes, up ? RMOE_FMT_Q4NX : l->dn_fmt,
+  const rmoe::LinAct L{up ? l->gu : l->dn, up ? l->gu_exps : l->dn_exps, up ? l->gu_bytes : l->dn_bytes, up ? RMOE_FMT_Q4NX : l->dn_fmt,
                        up ? 2 * l->I : l->H, up ? l->H : l->Ipad, (const uint16_t*)rows_dev, n, K_in,
                        (const int32_t*)offsets_dev, l->n_routed, bias_dev, act, gate_beta, value_beta,
                        (const uint16_t*)residual_dev, (uint16_t*)y_dev};
@@ -894,11 +918,13 @@ int rmoe_layer_upload_d(rmoe_ctx* ctx, int layer, int bundle, int expert0, int n
     const size_t e = (size_t)expert0 + i;
     HIP_TRY(hipMemcpyAsync(ctx->s.staging, (const uint8_t*)bytes + (size_t)i * per, per, hipMemcpyHostToDevice,
                            ctx->stream));
-    if (b1)
+    if (b1) {
       HIP_TRY(rmoe::launch_relayout_in(ctx->s.staging, base + e * per, 2 * L->I, L->H, ctx->stream));
-    else {
+      HIP_TRY(gu_exponents(*L, e, ctx->stream));
+    } else {
       HIP_TRY(rmoe::launch_b16_relayout_in(ctx->s.staging, base + e * per, L->H, L->Ipad, ctx->stream));
       HIP_TRY(rmoe::launch_b16_rowexp(base + e * per, L->H, L->Ipad, L->I, L->dn_rowexp + e * L->H, ctx->stream));
+      HIP_TRY(dn_exponents(*L, e, ctx->stream));
     }
     // The staging buffer is reused by the next expert: wait for the re-layout.
     HIP_TRY(hipStreamSynchronize(ctx->stream));
@@ -935,6 +961,7 @@ int rmoe_layer_expert_matrix(rmoe_ctx* ctx, int layer, int expert, int part, int
     if (expert < 0 || expert >= L->gu_experts)
       return fail(RMOE_EINVAL, "expert %d has no gate/up in layer %d (0..%d)", expert, layer, L->gu_experts - 1);
     m.tiles = L->gu + (size_t)expert * L->gu_bytes;
+    m.exps = L->gu_exps + (size_t)expert * 2 * L->I;
     m.M = 2 * L->I;
     m.K = L->H;
     m.fmt = RMOE_FMT_Q4NX;
@@ -942,6 +969,7 @@ int rmoe_layer_expert_matrix(rmoe_ctx* ctx, int layer, int expert, int part, int
     if (expert < 0 || expert >= L->dn_experts)
       return fail(RMOE_EINVAL, "expert %d has no down projection in layer %d (0..%d)", expert, layer, L->dn_experts - 1);
     m.tiles = L->dn + (size_t)expert * L->dn_bytes;
+    m.exps = L->dn_exps + (size_t)expert * L->H;
     m.M = L->H;
     m.K = L->Ipad;
     m.fmt = L->dn_fmt;
@@ -978,8 +1006,10 @@ int rmoe_layer_upload_experts(rmoe_ctx* ctx, int layer, const void* gate_up, siz
   for (size_t e = 0; e < ne; ++e) {
     HIP_TRY(hipMemcpyAsync(ctx->s.staging, (const uint8_t*)gate_up + e * L->gu_bytes, L->gu_bytes, hipMemcpyHostToDevice, ctx->stream));
     HIP_TRY(rmoe::launch_relayout_in(ctx->s.staging, L->gu + e * L->gu_bytes, 2 * L->I, L->H, ctx->stream));
+    HIP_TRY(gu_exponents(*L, e, ctx->stream));
     HIP_TRY(hipMemcpyAsync(ctx->s.staging, (const uint8_t*)down + e * L->dn_bytes, L->dn_bytes, hipMemcpyHostToDevice, ctx->stream));
     HIP_TRY(rmoe::launch_relayout_in(ctx->s.staging, L->dn + e * L->dn_bytes, L->H, L->Ipad, ctx->stream));
+    HIP_TRY(dn_exponents(*L, e, ctx->stream));
     // The staging buffer is reused by the next expert: wait for the re-layout.
     HIP_TRY(hipStreamSynchronize(ctx->stream));
   }
@@ -1010,6 +1040,7 @@ int rmoe_layer_upload_expert_q4k(rmoe_ctx* ctx, int layer, int expert, int part,
   TRY(grow(ctx->s.staging, ctx->s.staging_bytes, need, ctx));
   HIP_TRY(hipMemcpyAsync(ctx->s.staging, bytes, need, hipMemcpyHostToDevice, ctx->stream));
   HIP_TRY(rmoe::launch_q4k_to_tiles(ctx->s.staging, M, K, dst, Kt, row0, ctx->stream));
+  HIP_TRY(part == RMOE_PART_DOWN ? dn_exponents(*L, expert, ctx->stream) : gu_exponents(*L, expert, ctx->stream));
   HIP_TRY(hipStreamSynchronize(ctx->stream));
   return RMOE_OK;
 }
@@ -1028,6 +1059,8 @@ int rmoe_layer_quantize_expert_dev(rmoe_ctx* ctx, int layer, int expert, const f
                                 ctx->s.err, st));
   HIP_TRY(rmoe::launch_quantize(down_dev, L->H, L->Ipad, L->I, L->I, L->dn + (size_t)expert * L->dn_bytes, ctx->s.err,
                                 st));
+  HIP_TRY(gu_exponents(*L, expert, st));
+  HIP_TRY(dn_exponents(*L, expert, st));
   return sync_and_check(ctx, st);
 }
 
@@ -1044,6 +1077,8 @@ int rmoe_layer_synthesize_dev(rmoe_ctx* ctx, int layer, uint64_t seed, float std
     const uint64_t s_dn = seed * 1000003ull + (uint64_t)e * 2ull + 2ull;
     HIP_TRY(rmoe::launch_synth_quantize(s_gu, std, 2 * L->I, L->H, L->H, L->gu + (size_t)e * L->gu_bytes, ctx->s.err, st));
     HIP_TRY(rmoe::launch_synth_quantize(s_dn, std, L->H, L->Ipad, L->I, L->dn + (size_t)e * L->dn_bytes, ctx->s.err, st));
+    HIP_TRY(gu_exponents(*L, e, st));
+    HIP_TRY(dn_exponents(*L, e, st));
   }
   return sync_and_check(ctx, st);
 }
