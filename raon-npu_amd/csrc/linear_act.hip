@@ -18,7 +18,8 @@ namespace {
 constexpr int kPad = 4;  // floats of padding per row of the partial sums
 
 // Gated tiles hold NF / 2 fragments of gate rows, then the up rows of the same units.
-template <int kFmt, int MF, int NF, int XI, bool kGated>
+// kTail: the rows end short of K (K_in < K).
+template <int kFmt, int MF, int NF, int XI, bool kGated, bool kTail>
 __global__ __launch_bounds__(512) void linear_act_kernel(LinAct a, int n_nt) {
   extern __shared__ __attribute__((aligned(16))) float la_lds[];
   constexpr int kTB = kFmt == RMOE_FMT_BFP16 ? kB16TileBytes : kTileBytes;
@@ -44,7 +45,7 @@ __global__ __launch_bounds__(512) void linear_act_kernel(LinAct a, int n_nt) {
   const int l16 = lane & 15, lq = lane >> 4;
   const int nkt = a.K / kTileCols;
   const uint8_t* tiles = a.tiles + (size_t)e * a.wstride;
-  WaveOperands<MF, NF, XI, true> o;
+  WaveOperands<MF, NF, XI, kTail> o;
 #pragma unroll
   for (int f = 0; f < NF; ++f) {
     const int row = kGated ? nt * kOut + 16 * (f % (NF / 2 > 0 ? NF / 2 : 1)) + (f >= NF / 2 ? a.M / 2 : 0)
@@ -141,7 +142,11 @@ hipError_t launch(const LinAct& a, hipStream_t st) {
   const size_t mt = a.offsets ? std::min<size_t>(a.n, (size_t)a.n / BM + a.n_experts) : ((size_t)a.n + BM - 1) / BM;
   const size_t total = mt * (a.M / (16 * NF)), grid = 8 * ((total + 7) / 8);
   if (grid * 64 * W >= (size_t)1 << 32 || total >= (size_t)1 << 31) return hipErrorInvalidValue;
-  auto* kernel = act_gated(a.act) ? linear_act_kernel<kFmt, MF, NF, XI, (NF > 1)> : linear_act_kernel<kFmt, MF, NF, XI, false>;
+  constexpr bool kPair = NF > 1;
+  auto* kernel = a.K_in < a.K ? (act_gated(a.act) ? linear_act_kernel<kFmt, MF, NF, XI, kPair, true>
+                                                  : linear_act_kernel<kFmt, MF, NF, XI, false, true>)
+                              : (act_gated(a.act) ? linear_act_kernel<kFmt, MF, NF, XI, kPair, false>
+                                                  : linear_act_kernel<kFmt, MF, NF, XI, false, false>);
   hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(64 * W), act_lds(MF, NF, W), st, a, a.M / (16 * NF));
   return hipGetLastError();
 }
@@ -175,16 +180,22 @@ hipError_t pick(const LinAct& a, hipStream_t st) {
 
 }  // namespace
 
-hipError_t linear_act_setup() {
-  const void* fns[4] = {(const void*)linear_act_kernel<RMOE_FMT_Q4NX, 2, 4, 4, true>,
-                        (const void*)linear_act_kernel<RMOE_FMT_Q4NX, 2, 4, 4, false>,
-                        (const void*)linear_act_kernel<RMOE_FMT_BFP16, 2, 4, 4, true>,
-                        (const void*)linear_act_kernel<RMOE_FMT_BFP16, 2, 4, 4, false>};
+template <int kFmt>
+static hipError_t setup() {
+  const void* fns[4] = {(const void*)linear_act_kernel<kFmt, 2, 4, 4, true, true>,
+                        (const void*)linear_act_kernel<kFmt, 2, 4, 4, true, false>,
+                        (const void*)linear_act_kernel<kFmt, 2, 4, 4, false, true>,
+                        (const void*)linear_act_kernel<kFmt, 2, 4, 4, false, false>};
   for (const void* f : fns) {
     const hipError_t e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, (int)act_lds(2, 4, 8));
     if (e != hipSuccess) return e;
   }
   return hipSuccess;
+}
+// Allow the 32 x 64 tiles of eight waves their 68 KB of dynamic LDS (the others stay under 64).
+hipError_t linear_act_setup() {
+  const hipError_t e = setup<RMOE_FMT_Q4NX>();
+  return e == hipSuccess ? setup<RMOE_FMT_BFP16>() : e;
 }
 
 hipError_t launch_linear_act(const LinAct& a, uint8_t* scratch, size_t bytes, hipStream_t st) {
