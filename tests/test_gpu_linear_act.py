@@ -355,3 +355,110 @@ def test_refused_operands(gpu_ctx):
     mat.free()
     with pytest.raises(KeyError):
         mat.linear_act_dev(x[:T * K].view(T, K), T, y)
+
+
+@pytest.mark.parametrize("fmt", ["q4nx", "bfp16"])
+@pytest.mark.parametrize("M", [128, 14336, 28672])
+@pytest.mark.parametrize("K,widths", [(256, (256, 136)), (1280, (1280, 1088, 520))])
+def test_every_tile_of_few_rows(gpu_ctx, fmt, M, K, widths):
+    """The tile shapes that the rule picks by rows and weight rows (16 x 16 to 32 x 64, up to four rows or more,
+    gated or not, narrower rows or not), with K splits of one to three K tiles a wave."""
+    parts = [_weights(fmt, 128, K, s) for s in (1, 2, 3)]
+    order = [0, 1, 2, 1] * (M // 512) + [2] * (M // 128 % 4)
+    mat = gpu_ctx.upload_matrix(b"".join(parts[i][0] for i in order), M, K, fmt=fmt)
+    w = torch.cat([p[1] for p in parts]).cuda()
+    rows = torch.cat([torch.arange(128) + 128 * i for i in order]).cuda()  # weight row -> row of w
+    st = torch.cuda.current_stream()
+    for T in (3, 9, 17, 40, 100):
+        mat.reserve_act(T)
+        for K_in in widths:
+            x = torch.randn(T, K_in, generator=torch.Generator().manual_seed(T + K_in)).to(torch.bfloat16).cuda()
+            absum = (x.double().abs() @ w[:, :K_in].abs().t())[:, rows]
+            z = (x.double() @ w[:, :K_in].t())[:, rows]
+            many = 2.0 ** -11 * absum if T >= MANY else 0.0
+            d = (K_in + 64) * 2.0 ** -23 * absum + many
+            y = torch.zeros(T, M, dtype=torch.bfloat16, device="cuda")
+            mat.linear_act_dev(x, T, y, stream=st)
+            assert bool(((y.double() - z).abs() <= 2.0 ** -8 * (z.abs() + d) + d).all()), (T, K_in)
+            g, u, dg, du = z[:, :M // 2], z[:, M // 2:], d[:, :M // 2], d[:, M // 2:]
+            f = g * torch.sigmoid(g)
+            e = 1.1 * dg * (u.abs() + du) + f.abs() * du + 32 * 2.0 ** -24 * (f * u).abs()
+            h = torch.zeros(T, M // 2, dtype=torch.bfloat16, device="cuda")
+            mat.linear_act_dev(x, T, h, act="swiglu", stream=st)
+            assert bool(((h.double() - f * u).abs() <= 2.0 ** -8 * ((f * u).abs() + e) + e).all()), (T, K_in)
+    mat.free()
+
+
+@pytest.mark.parametrize("part,act", [("gate_up", "swiglu"), ("down", "none")])
+@pytest.mark.parametrize("d_layout", [False, True])
+def test_experts_by_rows_an_expert(gpu_ctx, part, act, d_layout):
+    """Row counts on both sides of every change of kernel and tile: fewer rows than experts, then 24 and 64 an expert
+    in the mean, spread evenly and all on two experts."""
+    H, I, E = 256, 192, 6
+    lyr, gu, dn = _layer(gpu_ctx, H, I, E, d_layout, 120)
+    ws, M, K = (gu, 2 * I, H) if part == "gate_up" else (dn, H, I)
+    for n in (1, 4, 5, 6, 7, 149, 150, 389, 390, 391, 1200):
+        lyr.reserve_experts_linear(n)
+        x, _, _, width = _operands(n, M, K, act, False, False, n)
+        for counts in ([n // E + (e < n % E) for e in range(E)], [0, n // 3, 0, 0, n - n // 3, 0]):
+            offsets = torch.tensor([0] + list(np.cumsum(counts)), dtype=torch.int32)
+            y = torch.full((n, width), 9.0, dtype=torch.bfloat16, device="cuda")
+            lyr.experts_linear_dev(part, x.cuda(), offsets.cuda(), y, act=act, stream=torch.cuda.current_stream())
+            for e in range(E):
+                a, z = int(offsets[e]), int(offsets[e + 1])
+                if a < z:
+                    ref, err = _reference(x[a:z], ws[e], None, act, None, True)
+                    _check(y[a:z], ref, err, (n, counts, e))
+    lyr.free()
+
+
+@pytest.mark.parametrize("fmt", ["q4nx", "bfp16"])
+def test_dense_of_many_rows(gpu_ctx, fmt):
+    """Enough rows for the kernel of many rows, whole and ragged tiles, widths that end inside a tile of 256 weight
+    rows, every epilogue; a token's neighbours do not matter."""
+    K = 512
+    for M, T, act in ((256, 128 * 144, "none"), (384, 128 * 72 + 5, "gelu"), (1280, 128 * 29 + 77, "situ"),
+                      (2176, 128 * 16 + 1, "swiglu")):
+        blob, w = _weights(fmt, M, K, M)
+        mat = gpu_ctx.upload_matrix(blob, M, K, fmt=fmt)
+        mat.reserve_act(T)
+        x, b, r, width = _operands(T, M, K, act, True, True, T)
+        y = torch.zeros(T, width, dtype=torch.bfloat16, device="cuda")
+        st = torch.cuda.current_stream()
+        mat.linear_act_dev(x.cuda(), T, y, bias_dev=b.cuda(), act=act, residual_dev=r.cuda(), stream=st, **_betas(act))
+        pick = torch.cat([torch.arange(300), torch.arange(T - 300, T)])
+        _check(y[pick], *_reference(x[pick], w, b, act, r[pick], True), (M, T))
+        in_place = r.cuda()
+        mat.linear_act_dev(x.cuda(), T, in_place, bias_dev=b.cuda(), act=act, residual_dev=in_place, stream=st, **_betas(act))
+        assert torch.equal(in_place, y)
+        odd = torch.zeros(T * width + 9, dtype=torch.bfloat16, device="cuda")
+        mat.linear_act_dev(x.cuda(), T, odd[1:1 + T * width].view(T, width), bias_dev=b.cuda(), act=act,
+                           residual_dev=r.cuda(), stream=st, **_betas(act))
+        assert torch.equal(odd[1:1 + T * width].view(T, width), y) and not odd[0] and not odd[1 + T * width:].any()
+        mat.free()
+
+
+def test_exponents_follow_the_weights(gpu_ctx):
+    """Weights written anew under the same layer (another size by 2^12) are served with their own exponents."""
+    H, I, E, n = 256, 128, 2, 64
+    g = MoeGeometry(hidden=H, inter=I, n_routed=E, n_shared=1, top_k=1)
+    lyr = gpu_ctx.create_layer(7301, g)
+    lyr.reserve_experts_linear(n)
+    x = torch.randn(n, H, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16)
+    offsets = torch.tensor([0, n // 2, n], dtype=torch.int32, device="cuda")
+    y = torch.zeros(n, 2 * I, dtype=torch.bfloat16, device="cuda")
+    for std in (0.02, 0.02 * 2.0 ** 12, 0.02 * 2.0 ** -20):
+        parts = [_weights("q4nx", 2 * I, H, e, std=std) for e in range(E + 1)]
+        dn = [_weights("q4nx", H, 256, 9, live=I)[0]] * (E + 1)
+        lyr.upload_experts(b"".join(p[0] for p in parts), b"".join(dn))
+        lyr.experts_linear_dev("gate_up", x.cuda(), offsets, y, stream=torch.cuda.current_stream())
+        for e in range(E):
+            s = slice(e * n // 2, (e + 1) * n // 2)
+            _check(y[s], *_reference(x[s], parts[e][1], None, "none", None, True), std)
+        w = torch.randn(2 * I, H, generator=torch.Generator().manual_seed(5)) * std * 2.0 ** 5
+        lyr.quantize_expert(1, w.cuda(), torch.zeros(H, I, device="cuda"))
+        c, s, m = Q.quantize(w.numpy())
+        lyr.experts_linear_dev("gate_up", x.cuda(), offsets, y, stream=torch.cuda.current_stream())
+        _check(y[n // 2:], *_reference(x[n // 2:], torch.from_numpy(Q.dequantize_simple(c, s, m)).double(), None, "none",
+                                       None, True), std)
+    lyr.free()
