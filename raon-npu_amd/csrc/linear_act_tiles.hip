@@ -320,32 +320,36 @@ __device__ __forceinline__ void copies_landed() {
   __syncthreads();
 }
 
-// One tile of up to 16 MF rows x 64 NF weight rows; wave w takes all rows and 16 NF = 64
-// weight rows of its own (w: the matrix; wo: byte offset of weight row `lane` of the 64).
+// One tile of up to 16 MF rows x 64 NW weight rows over the K tiles [kt0, kt0 + nkt); each of
+// its NW waves takes all rows and 16 NF = 64 weight rows of its own (w: the matrix; wo: byte
+// offset of weight row `lane` of the 64).
 // Stages s of 64 columns.  Rows are copied R - 1 stages ahead into a ring of R = kRing, and
 // weights, which no other wave reads, R + 1 ahead into the place that stage s + 1's left when
 // their words went to registers, so that operands are formed under products throughout.  A
 // wave waits in the order of its copies: at a stage's end for those issued by the end of the
 // stage R - 1 before.  One barrier a stage.  Copies past the end repeat the last stage's.
-template <int kFmt, int BF, int MF, int NF>
+template <int kFmt, int BF, int MF, int NF, int NW>
 __device__ __forceinline__ void tile_product(const TileArgs& t, const uint8_t* w, uint32_t wo, int we_lane,
-                                             const int (&we)[NF], int row0, uint8_t* lds, f32x4 (&acc)[BF][NF]) {
+                                             const int (&we)[NF], int row0, int kt0, int nkt, uint8_t* lds,
+                                             f32x4 (&acc)[BF][NF]) {
   static_assert(NF == 4, "64 weight rows a wave");
   constexpr int kTB = kFmt == RMOE_FMT_BFP16 ? kB16TileBytes : kTileBytes, kBlocks = kHalfBlocks<kFmt>;
   constexpr int R = kRing, kAhead = R - 1;
-  const int lane = threadIdx.x & 63, wave = wave_id(), nkt = t.a.K / kTileCols, ns = 2 * nkt;
+  const int lane = threadIdx.x & 63, wave = wave_id() % NW, ns = 2 * nkt;
+  w += (size_t)kt0 * kTB;
   const uint32_t lds0 = (uint32_t)(uintptr_t)lds;
   const int wbase = R * kStage<BF> + wave * kWaveWeights<kFmt>, pbase = wbase + R * 1024 * kBlocks;
-  // Copy q = wave + 4i fills LDS rows 8q..8q+7 (1 KB): lane L brings row 8q + L / 8 the chunk
+  // Copy q = wave + NW i fills LDS rows 8q..8q+7 (1 KB): lane L brings row 8q + L / 8 the chunk
   // that sits at position L % 8.  Rows past the tile are the next tiles' or, behind the last
   // row, the kActBM spare rows of the scratch; their results are not stored.
-  const uint8_t* xb = reinterpret_cast<const uint8_t*>(t.xh + (size_t)row0 * t.a.K);
+  constexpr int kRowCopies = 2 * MF / NW;
+  const uint8_t* xb = reinterpret_cast<const uint8_t*>(t.xh + (size_t)row0 * t.a.K) + (size_t)kt0 * 256;
   const uint32_t ld = 2u * (uint32_t)t.a.K;
   const uint32_t xo = (uint32_t)(8 * wave + lane / 8) * ld + 16u * (uint32_t)((lane % 8) ^ ((4 * wave + lane / 16) % 8));
   uint32_t rows0 = lds0 + 1024u * (uint32_t)wave;
   asm volatile("" : "+s"(rows0));  // kept in a scalar register
   auto row_copy = [&](int i, int s, uint32_t slot) {
-    copy16(xb + 128 * min(s, ns - 1) + (size_t)(32 * i) * ld, xo, rows0 + slot + (uint32_t)(4096 * i));
+    copy16(xb + 128 * min(s, ns - 1) + (size_t)(8 * NW * i) * ld, xo, rows0 + slot + (uint32_t)(1024 * NW * i));
   };
   // Stage q's weights, q of the parity j, at byte `at` of the wave's ring: kBlocks + 1 - j copies.
   auto weight_copy = [&](int i, int q, uint32_t at) {
@@ -363,8 +367,8 @@ __device__ __forceinline__ void tile_product(const TileArgs& t, const uint8_t* w
   // copies before it are taken up): rows under the first step, weights under the second.
   auto copies = [&](int i, int s, int q, int nw, uint32_t there, uint32_t at) {
 #pragma unroll
-    for (int c = 0; c < MF / 2; ++c)
-      if (i == 2 * c + 1) row_copy(c, s, there);
+    for (int c = 0; c < kRowCopies; ++c)
+      if (i == (2 * c + 1) * MF / (2 * kRowCopies)) row_copy(c, s, there);
 #pragma unroll
     for (int c = 0; c < nw; ++c)
       if (i == MF + (c + 1) * (MF - 1) / nw) weight_copy(c, q, at);
@@ -373,7 +377,7 @@ __device__ __forceinline__ void tile_product(const TileArgs& t, const uint8_t* w
 #pragma unroll
   for (int s = 0; s < kAhead; ++s)
 #pragma unroll
-    for (int i = 0; i < MF / 2; ++i) row_copy(i, s, (uint32_t)(s * kStage<BF>));
+    for (int i = 0; i < kRowCopies; ++i) row_copy(i, s, (uint32_t)(s * kStage<BF>));
 #pragma unroll
   for (int s = 0; s < R; ++s) load_weights(s, (uint32_t)(s * 1024 * kBlocks));
   copies_landed<0>();
@@ -393,10 +397,10 @@ __device__ __forceinline__ void tile_product(const TileArgs& t, const uint8_t* w
     there = there == (uint32_t)((R - 1) * kStage<BF>) ? 0u : there + (uint32_t)kStage<BF>;
     ws = ws == (uint32_t)((R - 1) * 1024 * kBlocks) ? 0u : ws + (uint32_t)(1024 * kBlocks);
   };
-  // Copies that may be in flight at the end of a stage: R - 2 stages' rows and the weights of
-  // the last R - 1, with words every second stage (for R = 2: with the even stage q alone).
-  constexpr int kRows = (R - 2) * (MF / 2);
-  constexpr int kEvenEnd = R == 2 ? kBlocks : kRows + 2 * kBlocks + 1, kOddEnd = R == 2 ? kBlocks + 1 : kEvenEnd;
+  // Copies that may be in flight at the end of a stage: the last, of its weights, with words
+  // every second stage.
+  static_assert(R == 2, "counts of the copies in flight");
+  constexpr int kEvenEnd = kBlocks, kOddEnd = kBlocks + 1;
 #pragma unroll 1
   for (int kt = 0; kt < nkt; ++kt) {
     const uint8_t* wp = lds + pbase + 1024 * (kt & 1);
@@ -422,12 +426,13 @@ __device__ __forceinline__ void tile_product(const TileArgs& t, const uint8_t* w
   copies_landed<0>();  // the epilogue reuses the memory
 }
 
-template <int kFmt, int NF, bool kGated, int BF>
-__global__ __launch_bounds__(256, BF == 8 ? 2 : BF == 4 ? 3 : 4) void act_tile_kernel(TileArgs t) {
-  constexpr int kLds = kRing * kStage<BF> + 4 * kWaveWeights<kFmt>, kTile = 16 * BF;
-  static_assert(kLds <= 80 * 1024, "two workgroups a CU");
-  __shared__ __attribute__((aligned(16))) uint8_t lds[kLds];
-  constexpr int kCols = 64 * NF, kOut = kGated ? kCols / 2 : kCols;
+// Tiles of 16 BF rows x 64 NW weight rows by KS groups of NW waves, which take a KS-th of K each.
+template <int kFmt, int NF, bool kGated, int BF, int NW, int KS>
+__global__ __launch_bounds__(64 * NW * KS, BF == 8 ? 2 : BF == 4 ? 3 : 4) void act_tile_kernel(TileArgs t) {
+  constexpr int kLds = kRing * kStage<BF> + NW * kWaveWeights<kFmt>, kTile = 16 * BF;
+  static_assert(kLds <= 80 * 1024, "two groups a CU");
+  __shared__ __attribute__((aligned(16))) uint8_t lds[KS * kLds];
+  constexpr int kCols = 16 * NF * NW, kOut = kGated ? kCols / 2 : kCols;
   constexpr int kTB = kFmt == RMOE_FMT_BFP16 ? kB16TileBytes : kTileBytes;
   const LinAct& a = t.a;
   RowTiles<kTile> rt;
@@ -438,11 +443,11 @@ __global__ __launch_bounds__(256, BF == 8 ? 2 : BF == 4 ? 3 : 4) void act_tile_k
   const int nt = id % t.n_nt;
   int e = 0, row0 = id / t.n_nt * kTile, nrow = min(kTile, a.n - row0);
   if (a.offsets) rt.find(id / t.n_nt, e, row0, nrow);
-  const int wave = wave_id(), nkt = a.K / kTileCols, width = kGated ? a.M / 2 : a.M;
+  const int wave = wave_id() % NW, group = wave_id() / NW, nkt = a.K / kTileCols, width = kGated ? a.M / 2 : a.M;
   const uint8_t* tiles = a.tiles + (size_t)e * a.wstride;
   // The wave's weight rows: 64 consecutive ones, or 32 gate rows and their up rows.  Columns
   // past the matrix (its width is a multiple of 64) repeat its first rows.
-  const int c0 = nt * kOut + wave * (kOut / 4), base = c0 < width ? c0 : 0;
+  const int c0 = nt * kOut + wave * (kOut / NW), base = c0 < width ? c0 : 0;
   auto row_of = [&](int r) { return kGated && r >= 32 ? width + base + r - 32 : base + r; };
   const int wr = row_of(threadIdx.x & 63);
   const uint32_t wo = (uint32_t)(wr / kTileRows) * (uint32_t)(nkt * kTB) + (uint32_t)(wr % kTileRows) * 16u;
@@ -456,14 +461,18 @@ __global__ __launch_bounds__(256, BF == 8 ? 2 : BF == 4 ? 3 : 4) void act_tile_k
 #pragma unroll
     for (int f = 0; f < NF; ++f) acc[m][f] = f32x4{0.f, 0.f, 0.f, 0.f};
   // A short tile multiplies only the fragments that hold rows.
-  if (BF == 8 && nrow > 64) tile_product<kFmt, BF, BF, NF>(t, tiles, wo, wes[wr], we, row0, lds, acc);
-  else if (BF >= 4 && nrow > 32) tile_product<kFmt, BF, BF < 4 ? BF : 4, NF>(t, tiles, wo, wes[wr], we, row0, lds, acc);
-  else tile_product<kFmt, BF, 2, NF>(t, tiles, wo, wes[wr], we, row0, lds, acc);
+  const int nk = nkt / KS, kt0 = group * nk;  // K % 256 == 0
+  uint8_t* mine = lds + group * kLds;
+  if (BF == 8 && nrow > 64) tile_product<kFmt, BF, BF, NF, NW>(t, tiles, wo, wes[wr], we, row0, kt0, nk, mine, acc);
+  else if (BF >= 4 && nrow > 32)
+    tile_product<kFmt, BF, BF < 4 ? BF : 4, NF, NW>(t, tiles, wo, wes[wr], we, row0, kt0, nk, mine, acc);
+  else tile_product<kFmt, BF, 2, NF, NW>(t, tiles, wo, wes[wr], we, row0, kt0, nk, mine, acc);
 
   // Epilogue: sums and bias through LDS as fp32, kRows rows at a time, so that the activation
   // has its operands at hand and residual and y move 16 bytes a thread.  Columns of
   // different lq go to different banks: column c of row r sits at c ^ 16 (r / 4 % 4).
-  constexpr int kRows = kLds >= kTile * kCols * 4 ? kTile : kLds >= kTile / 2 * kCols * 4 ? kTile / 2 : kTile / 4;
+  constexpr int kAll = KS * kLds;
+  constexpr int kRows = kAll >= kTile * kCols * 4 ? kTile : kAll >= kTile / 2 * kCols * 4 ? kTile / 2 : kTile / 4;
   int tid = threadIdx.x;
   asm volatile("" : "+v"(tid));  // what follows from it is computed here, not kept across the products
   const int l16 = tid & 15, lq = (tid & 63) >> 4;
@@ -478,23 +487,40 @@ __global__ __launch_bounds__(256, BF == 8 ? 2 : BF == 4 ? 3 : 4) void act_tile_k
   for (int r0 = 0; r0 < kTile; r0 += kRows) {
     if (r0 >= nrow) break;
     if (r0) __syncthreads();
+    auto at_column = [&](int f) {
+      return wave * (kOut / NW) + l16 + (kGated ? 16 * (f % (NF / 2)) + (f >= NF / 2 ? kOut : 0) : 16 * f);
+    };
+    if constexpr (KS > 1) {  // the second group's sums first
+      if (group == 1) {
 #pragma unroll
-    for (int m = r0 / 16; m < (r0 + kRows) / 16; ++m)
+        for (int m = r0 / 16; m < (r0 + kRows) / 16; ++m)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = 16 * m + 4 * lq + i;
-        const int xe = t.xe[row0 + min(r, nrow - 1)];
-        float* o = out + (r - r0) * kCols;
+          for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int f = 0; f < NF; ++f) {
-          const int c = kGated ? wave * (kOut / 4) + 16 * (f % (NF / 2)) + (f >= NF / 2 ? kOut : 0) : wave * (kOut / 4) + 16 * f;
-          o[(c + l16) ^ (16 * lq)] = __builtin_amdgcn_ldexpf(acc[m][f][i], xe + we[f]) + bias[f];
-        }
+            for (int f = 0; f < NF; ++f)
+              out[(16 * m + 4 * lq + i - r0) * kCols + (at_column(f) ^ (16 * lq))] = acc[m][f][i];
       }
+      __syncthreads();
+    }
+    if (group == 0) {
+#pragma unroll
+      for (int m = r0 / 16; m < (r0 + kRows) / 16; ++m)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = 16 * m + 4 * lq + i;
+          const int xe = t.xe[row0 + min(r, nrow - 1)];
+          float* o = out + (r - r0) * kCols;
+#pragma unroll
+          for (int f = 0; f < NF; ++f) {
+            float& v = o[at_column(f) ^ (16 * lq)];
+            v = __builtin_amdgcn_ldexpf(KS > 1 ? acc[m][f][i] + v : acc[m][f][i], xe + we[f]) + bias[f];
+          }
+        }
+    }
     __syncthreads();
     const int rows = min(kRows, nrow - r0), cols = min(kOut, width - nt * kOut);
 #pragma unroll 1
-    for (int i = tid; i < rows * (kOut / 8); i += 256) {
+    for (int i = tid; i < rows * (kOut / 8); i += 64 * NW * KS) {
       const int r = i / (kOut / 8), c = 8 * (i % (kOut / 8));
       if (c >= cols) continue;
       const float* o = out + r * kCols + (c ^ (16 * ((r >> 2) & 3)));
@@ -535,26 +561,38 @@ __global__ __launch_bounds__(256, BF == 8 ? 2 : BF == 4 ? 3 : 4) void act_tile_k
   }
 }
 
-template <int kFmt, int BF>
+template <int kFmt, int BF, int NW = 4, int KS = 1>
 hipError_t launch_tiles(const TileArgs& t0, hipStream_t st) {
   constexpr int NF = 4, kTile = 16 * BF;
   TileArgs t = t0;
   const LinAct& a = t.a;
-  t.n_nt = (a.M + 64 * NF - 1) / (64 * NF);
+  t.n_nt = (a.M + 16 * NF * NW - 1) / (16 * NF * NW);
   const size_t mt = a.offsets ? std::min<size_t>(a.n, (size_t)a.n / kTile + a.n_experts) : ((size_t)a.n + kTile - 1) / kTile;
   const size_t grid = 8 * ((mt * t.n_nt + 7) / 8);
-  if (grid * 256 >= (size_t)1 << 32) return hipErrorInvalidValue;
-  auto* kernel = act_gated(a.act) ? act_tile_kernel<kFmt, NF, true, BF> : act_tile_kernel<kFmt, NF, false, BF>;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(256), 0, st, t);
+  constexpr int kThreads = 64 * NW * KS;
+  if (grid * kThreads >= (size_t)1 << 32) return hipErrorInvalidValue;
+  auto* kernel = act_gated(a.act) ? act_tile_kernel<kFmt, NF, true, BF, NW, KS> : act_tile_kernel<kFmt, NF, false, BF, NW, KS>;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(kThreads), 0, st, t);
   return hipGetLastError();
 }
-// By the rows an expert has in the mean (128 experts, q4nx gate/up [1536, 2048], tiles of 32, 64
-// and 128 rows: 28 rows 80, 78 and 85 us, 44 rows 120, 91 and 101, 62 rows 149, 125 and 125, 94
-// rows 195, 160 and 143; bfp16 down [2560, 1088]: 12 rows 99, 108 and 108, 47 rows 149, 143 and 143,
-// 70 rows 183, 179 and 169); one matrix has rows enough for the largest.
+// Tiles of 128 x 256 and of 64 x 128 weight rows over one matrix of M rows.
+size_t large_tiles(int M, size_t n) { return (n + 127) / 128 * ((M + 255) / 256); }
+size_t small_tiles(int M, size_t n) { return (n + 63) / 64 * (M / 128); }
+constexpr size_t kFillLarge = 200, kFillSmall = 256;
+
+// By expert: by the rows an expert has in the mean (128 experts, q4nx gate/up [1536, 2048], tiles
+// of 32, 64 and 128 rows: 28 rows 68, 67 and 77 us, 44 rows 108, 81 and 93, 62 rows 135, 113 and
+// 112, 94 rows 184, 139 and 128; bfp16 down [2560, 1088]: 12 rows 100, 108 and 108, 47 rows 147,
+// 138 and 137, 70 rows 180, 164 and 158).
+// One matrix: 128 x 256 from kFillLarge tiles of it on, below that 64 x 128 by two groups of K,
+// which make 3.75 times the workgroups (q4nx [2176, 2560], SwiGLU, 64 x 128 / 128 x 256: 1,024
+// rows 35 / 50 us, 2,048 (144 large tiles) 54 / 54, 3,000 (216) 66 / 58, 4,096 83 / 81).
 template <int kFmt>
 hipError_t pick_tiles(const TileArgs& t, hipStream_t st) {
-  const size_t rows = t.a.offsets ? (size_t)t.a.n / t.a.n_experts : (size_t)t.a.n;
+  const LinAct& a = t.a;
+  if (!a.offsets || a.n_experts == 1)
+    return large_tiles(a.M, a.n) >= kFillLarge ? launch_tiles<kFmt, 8>(t, st) : launch_tiles<kFmt, 4, 2, 2>(t, st);
+  const size_t rows = (size_t)a.n / a.n_experts;
   if (rows <= 24) return launch_tiles<kFmt, 2>(t, st);
   if (rows <= 64) return launch_tiles<kFmt, 4>(t, st);
   return launch_tiles<kFmt, 8>(t, st);
@@ -570,15 +608,15 @@ hipError_t launch_row_exponents(const uint8_t* tiles, int fmt, int M, int K, int
 }
 
 // Which rows this kernel serves, against linear_act_kernel (whose cost grows with every 32 rows).
-// One matrix: from 144 tiles of 128 x 256 ([2176, 2560]: 2,048 rows 60 / 67 us, 4,096 rows 88 /
-// 120; [1536, 2048], 1,024 rows, 48 tiles: 47 / 19).  By expert: from one row an expert
-// (128 experts, gate/up [1536, 2048]: 32 rows 35 / 23 us, 128 rows 46 / 52, 2,048 rows 66 / 78,
-// 8,000 rows 125 / 206).
+// One matrix: from kFillSmall tiles of 64 x 128 on (this kernel / that one, q4nx with SwiGLU:
+// [2176, 2560], 700 rows (187 tiles) 26 / 27 us, 1,024 rows (272) 35 / 40, 1,500 rows 38 / 56;
+// [1536, 2048], 1,024 rows (192) 23 / 23, 1,500 rows (288) 31 / 34; [512, 2048], 3,000 rows (188)
+// 29 / 24).  By expert: from one row an expert on (128 experts, q4nx gate/up [1536, 2048]: 128 rows
+// 39 / 52 us, 2,048 rows 55 / 78, 8,000 rows 112 / 206).
 bool act_tiles_serve(int fmt, int M, int K, int groups, size_t n) {
   const size_t bytes = fmt == RMOE_FMT_BFP16 ? matrix_bytes_bfp16(M, K) : matrix_bytes(M, K);
   if (bytes >= (size_t)1 << 32) return false;  // 32-bit byte offsets into a matrix
-  if (groups > 1) return n >= (size_t)groups;
-  return (n + kActBM - 1) / kActBM * ((M + 255) / 256) >= 144;
+  return groups > 1 ? n >= (size_t)groups : small_tiles(M, n) >= kFillSmall;
 }
 size_t act_tiles_scratch(int fmt, int M, int K, int groups, size_t n) {
   if (!act_tiles_serve(fmt, M, K, groups, n)) return 0;
@@ -587,9 +625,11 @@ size_t act_tiles_scratch(int fmt, int M, int K, int groups, size_t n) {
 
 hipError_t launch_act_tiles(const LinAct& a, uint8_t* scratch, size_t bytes, hipStream_t st) {
   if (act_tiles_scratch(a.fmt, a.M, a.K, a.offsets ? a.n_experts : 1, a.n) > bytes) return hipErrorOutOfMemory;
+  const size_t groups = ((size_t)a.n + 3) / 4;
+  if (groups * 256 >= (size_t)1 << 32) return hipErrorInvalidValue;
   uint16_t* xh = reinterpret_cast<uint16_t*>(scratch);
   int32_t* xe = reinterpret_cast<int32_t*>(scratch + round256(((size_t)a.n + kActBM) * a.K * 2));
-  hipLaunchKernelGGL(act_prep_kernel, dim3((unsigned)(((size_t)a.n + 3) / 4)), dim3(256), 0, st, a, xh, xe);
+  hipLaunchKernelGGL(act_prep_kernel, dim3((unsigned)groups), dim3(256), 0, st, a, xh, xe);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   const TileArgs t{a, xh, xe, 0};
