@@ -137,19 +137,22 @@ int rmoe_reserve_linear(rmoe_ctx* ctx, int handle, int T);
  * itself: added in place); y bf16 [T, M'].  act RMOE_ACT_NONE, _SILU, _GELU, _GELU_TANH:
  * M' = M; RMOE_ACT_SWIGLU, _SITU (gate_beta, value_beta): M' = M / 2, row i of W the gate and
  * row M/2 + i the up of output i, bias added to both.  (rmoe_linear_dev followed by the
- * activation rounds gate and up to bf16 first; this call does not.)  Asynchronous on
- * `stream`, never allocates.  The reference adds bias, activation and residual on the host
+ * activation rounds gate and up to bf16 first; this call does not.)  Many rows are multiplied
+ * in fp16 with a power of two per row of x and of W: q4nx weights are rounded once to fp16's 11
+ * bits of their row's largest.  Asynchronous on `stream`, never allocates; products of many
+ * rows use context scratch, so that overlapping ones need a context each.  The reference adds bias, activation and residual on the host
  * (host/raon.py:1314-1330). */
 int rmoe_linear_act_dev(rmoe_ctx* ctx, int handle, const void* x_dev, int T, int K_in, const float* bias_dev, int act,
                         float gate_beta, float value_beta, const void* residual_dev, void* y_dev, void* stream);
-/* Size the scratch that rmoe_linear_act_dev needs for up to T tokens on this matrix. */
+/* Size the scratch that rmoe_linear_act_dev needs for up to T tokens on this matrix.  Graphs
+ * captured before stay valid. */
 int rmoe_reserve_linear_act(rmoe_ctx* ctx, int handle, int T);
 
 /* ------------------------------------------------------------ tokens by expert --
  * The steps around the experts' products on device operands, for an engine that puts work of
  * its own between them.  T tokens of width H in RMOE_DT_* elements, any H >= 1, contiguous
  * rows at any address of their type; k (1..16) routes per token, A = T k < 2^31 assignments
- * a = t k + r.  Asynchronous on `stream`; nothing is allocated and no scratch of the context
+ * a = t k + r; H at most 2^30.  Asynchronous on `stream`; nothing is allocated and no scratch of the context
  * is used, so that calls on several streams or captured graphs share only the buffers the
  * caller gives them.  Inputs and outputs of a call must not overlap. */
 
@@ -360,7 +363,8 @@ int rmoe_dispatch(rmoe_ctx* ctx, const int32_t* top_ids, int T, int k, int n_exp
 int rmoe_experts_linear_dev(rmoe_ctx* ctx, int layer, int part, const void* rows_dev, int n, int K_in,
                             const void* offsets_dev, const float* bias_dev, int act, float gate_beta, float value_beta,
                             const void* residual_dev, void* y_dev, void* stream);
-/* Size the scratch that rmoe_experts_linear_dev needs for up to n rows on this layer. */
+/* Size the scratch that rmoe_experts_linear_dev needs for up to n rows on this layer (the same
+ * scratch as rmoe_reserve_linear_act's). */
 int rmoe_reserve_experts_linear(rmoe_ctx* ctx, int layer, int n);
 
 /* Grouped prefill MoE: NpuBackend.moe_experts_grouped (npu/backend.py:4845-4979).

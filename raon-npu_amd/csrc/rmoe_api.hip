@@ -362,6 +362,7 @@ int check_tokens(rmoe_ctx* ctx, int dtype, int T, int H, int k, std::initializer
   if (dtype != RMOE_DT_BF16 && dtype != RMOE_DT_F16 && dtype != RMOE_DT_F32)
     return fail(RMOE_EINVAL, "unknown element type %d", dtype);
   if (T < 1 || H < 1) return fail(RMOE_EINVAL, "T (%d) and H (%d) must be >= 1", T, H);
+  if (H > 1 << 30) return fail(RMOE_EINVAL, "H (%d) must be at most 2^30", H);
   if (k < 1 || k > 16) return fail(RMOE_EINVAL, "k (%d) must be in 1..16", k);
   if ((size_t)T * k >= (size_t)1 << 31) return fail(RMOE_EINVAL, "%d x %d routes are too many", T, k);
   for (const void* p : rows)
@@ -508,6 +509,7 @@ int rmoe_destroy(rmoe_ctx* ctx) {
                   s.chunk_counts, s.staging, s.pf, s.stack, s.stack_cnt, s.act};
   for (void* b : bufs)
     if (b) hipFree(b);
+  for (uint8_t* b : s.act_before) hipFree(b);
   auto it = g_io.find(ctx);
   if (it != g_io.end()) {
     hipFree(it->second.p);
@@ -736,7 +738,16 @@ int rmoe_reserve_linear(rmoe_ctx* ctx, int handle, int T) {
 
 static int reserve_act(rmoe_ctx* ctx, size_t bytes) {
   HIP_TRY(hipSetDevice(ctx->device));
-  return bytes ? grow(ctx->s.act, ctx->s.act_bytes, bytes, ctx) : RMOE_OK;
+  if (bytes <= ctx->s.act_bytes) return RMOE_OK;
+  // A graph captured before keeps the buffer it was captured with: growing gives a new one, of
+  // at least twice the size, so that the old ones together are smaller.
+  uint8_t* p = nullptr;
+  size_t cap = 0;
+  TRY(grow(p, cap, std::max(bytes, 2 * ctx->s.act_bytes), ctx));
+  if (ctx->s.act) ctx->s.act_before.push_back(ctx->s.act);
+  ctx->s.act = p;
+  ctx->s.act_bytes = cap;
+  return RMOE_OK;
 }
 
 static int run_linear_act(rmoe_ctx* ctx, const rmoe::LinAct& L, void* stream) {

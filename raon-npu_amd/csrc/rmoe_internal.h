@@ -405,6 +405,7 @@ struct RmoeScratch {
   int max_tokens = 0;
   uint8_t* act = nullptr;        // products with an epilogue: fp16 rows, exponents
   size_t act_bytes = 0;
+  std::vector<uint8_t*> act_before;  // smaller ones, which captured graphs may hold
   // persistent decode stack (moe_decode_stack.hip)
   uint8_t* stack = nullptr;      // per-layer hand-off buffers
   size_t stack_bytes = 0;
@@ -523,9 +524,7 @@ hipError_t launch_router_prep(const uint16_t* x, int T, int H, const uint16_t* w
 hipError_t launch_topk(const float* logits, int T, int E, int k, int score, const float* bias, int renorm,
                        float scaling, int32_t* ids, float* wts, int32_t* counts, hipStream_t st);
 
-// Tokens to expert-sorted rows and back (token_sort.hip).  Up to kSortSmall assignments are
-// sorted by one launch in which every workgroup counts over all of them; beyond, by four.
-constexpr int kSortSmall = 1024;
+// Tokens to expert-sorted rows and back (token_sort.hip).
 hipError_t launch_sort_tokens(const void* x, int dtype, int T, int H, const int32_t* ids, int k, int n_experts,
                               void* rows, int32_t* order, int32_t* inv, int32_t* offsets, int* err, hipStream_t st);
 // wts null: ones (the gradient of the sort).

@@ -25,6 +25,14 @@ namespace {
 constexpr int kMaxRoutes = 16;
 constexpr int kErrExpert = 4, kErrPosition = 16;
 
+// Few assignments are sorted by one launch in which every token's workgroup counts over all
+// of them, k comparisons each; more by four launches.  One / four (H 256, by events and, in
+// brackets, replayed in a graph): 1,024 assignments 7.5 us; 2,048 of k = 8 10.1 / 15.2 (9.7 /
+// 10.9), of k = 2 7.4 / 15.0 (7.5 / 10.7), of k = 16 14.6 / 15.4 (14.9 / 11.2); 4,096 of k = 8
+// 17.3 / 15.6 (17.6 / 11.7).
+constexpr int kSmallRoutes = 2048, kSmallWork = 16384;  // n, n k
+bool sort_is_small(int n, int k) { return n <= kSmallRoutes && n * k <= kSmallWork; }
+
 // One element of a type as fp32, and fp32 rounded to it (RTNE).
 template <int DT>
 struct Elem;
@@ -76,8 +84,8 @@ __device__ __forceinline__ int route_expert(int id, int E, int* err) {
   return id < 0 || id >= E ? -1 : id;
 }
 
-// Up to kSmall assignments: workgroup t counts its own token's positions over all ids (4 KB
-// at 1,024, read from L2), workgroup T the offsets; one launch, no workspace.
+// Few assignments: workgroup t counts its own token's positions over all ids (4 KB at 1,024,
+// read from L2), workgroup T the offsets; one launch, no workspace.
 struct SortArgs {
   const int32_t* ids;
   int T, k, E, n;
@@ -88,9 +96,15 @@ __device__ void small_offsets(const SortArgs& a, int* hist) {
   const int tid = threadIdx.x;
   hist[tid] = 0;
   __syncthreads();
-  for (int j = tid; j < a.n; j += 256) {
-    const int e = route_expert(a.ids[j], a.E, a.err);
-    if (e >= 0) atomicAdd(&hist[e], 1);
+  for (int j0 = tid; j0 < a.n; j0 += 8 * 256) {  // eight loads in flight
+    int id[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) id[u] = j0 + 256 * u < a.n ? a.ids[j0 + 256 * u] : -1;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int e = route_expert(id[u], a.E, a.err);
+      if (e >= 0) atomicAdd(&hist[e], 1);
+    }
   }
   __syncthreads();
   if (tid < 64) {
@@ -139,11 +153,18 @@ __global__ __launch_bounds__(256) void sort_small_kernel(SortArgs a, const uint8
     e[r] = id >= a.E ? -1 : id;
     cnt[r] = 0;
   }
-  for (int j0 = 64 * wave; j0 < a.n; j0 += 256) {
-    const int j = j0 + lane, ej = j < a.n ? a.ids[j] : -1;
+  for (int j0 = 64 * wave; j0 < a.n; j0 += 4 * 256) {
+    int ej[4];
 #pragma unroll
-    for (int r = 0; r < kMaxRoutes; ++r)
-      if (r < a.k) cnt[r] += __popcll(__ballot(ej >= 0 && (ej < e[r] || (ej == e[r] && j < t * a.k + r))));
+    for (int u = 0; u < 4; ++u) ej[u] = j0 + 256 * u + lane < a.n ? a.ids[j0 + 256 * u + lane] : -1;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (j0 + 256 * u >= a.n) break;
+      const int j = j0 + 256 * u + lane;
+#pragma unroll
+      for (int r = 0; r < kMaxRoutes; ++r)
+        if (r < a.k) cnt[r] += __popcll(__ballot(ej[u] >= 0 && (ej[u] < e[r] || (ej[u] == e[r] && j < t * a.k + r))));
+    }
   }
   if (lane == 0)
 #pragma unroll
@@ -465,11 +486,11 @@ constexpr size_t kMaxGroups = ((size_t)1 << 32) / 256 - 1;
 
 template <typename U>
 hipError_t sort_with(const SortArgs& a, const void* x, void* rows, size_t rb, hipStream_t st) {
-  if (a.n <= kSortSmall) {
+  if (sort_is_small(a.n, a.k)) {
     hipLaunchKernelGGL(sort_small_kernel<U>, dim3(a.T + 1), dim3(256), 0, st, a, (const uint8_t*)x, (uint8_t*)rows, rb);
     return hipGetLastError();
   }
-  const int nchunks = (a.n + kDispatchChunk - 1) / kDispatchChunk;
+  const int nchunks = (int)(((size_t)a.n + kDispatchChunk - 1) / kDispatchChunk);
   hipLaunchKernelGGL(sort_count_kernel, dim3(nchunks - 1), dim3(256), 0, st, a);
   hipLaunchKernelGGL(sort_scan_kernel, dim3(1), dim3(1024), 0, st, a, nchunks);
   hipLaunchKernelGGL(sort_place_kernel, dim3(nchunks), dim3(256), 0, st, a, nchunks);

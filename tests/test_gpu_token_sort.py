@@ -54,9 +54,11 @@ def _buffers(T, k, E, H, dtype, fill=7):
             torch.full((E + 1,), -9, dtype=torch.int32, device="cuda"))
 
 
-# One workgroup's assignments (1,024) and one chunk's on both sides; a last chunk shorter than the experts.
+# Both sides of one launch and four (2,048 assignments, 1,024 of 16 routes) and of a chunk of 1,024; a last chunk
+# shorter than the experts.
 SHAPES = [(1, 1, 1, 1), (1, 8, 128, 2048), (4, 8, 128, 2048), (3, 16, 256, 33), (128, 8, 128, 64), (129, 8, 128, 64),
-          (1024, 1, 256, 8), (1025, 1, 256, 8), (445, 6, 128, 2560), (300, 7, 9, 1027), (2049, 3, 64, 136),
+          (1024, 1, 256, 8), (1025, 1, 256, 8), (64, 16, 128, 8), (65, 16, 128, 8),
+          (256, 8, 128, 8), (257, 8, 128, 8), (2048, 1, 200, 8), (2049, 1, 200, 8), (445, 6, 128, 2560), (300, 7, 9, 1027), (2049, 3, 64, 136),
           (4100, 16, 255, 24)]
 
 

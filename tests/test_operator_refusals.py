@@ -135,6 +135,7 @@ BF16, F32 = _lib.DT_BF16, _lib.DT_F32
     ((P[0], 3, T, H, P[1], k, E, P[2], P[3], P[4], P[5]), "element type"),
     ((P[0], BF16, 0, H, P[1], k, E, P[2], P[3], P[4], P[5]), "T"),
     ((P[0], BF16, T, 0, P[1], k, E, P[2], P[3], P[4], P[5]), "H"),
+    ((P[0], BF16, 1, (1 << 30) + 1, P[1], k, E, P[2], P[3], P[4], P[5]), "H"),
     ((P[0], BF16, T, H, P[1], 0, E, P[2], P[3], P[4], P[5]), "k"),
     ((P[0], BF16, T, H, P[1], 17, E, P[2], P[3], P[4], P[5]), "k"),
     ((P[0], BF16, 1 << 30, H, P[1], 2, E, P[2], P[3], P[4], P[5]), "too many"),
