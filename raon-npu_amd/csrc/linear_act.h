@@ -12,12 +12,17 @@ __host__ __device__ constexpr bool act_gated(int act) { return act == RMOE_ACT_S
 // Activations of one value.  Each is z times a probability formed without cancellation: the
 // sigmoid from exp(-|z|), the normal distribution's from erfc, so that small results keep
 // their relative accuracy.  exp2 and the reciprocal are the hardware's (1 ulp each; the
-// reciprocal with one Newton step), a few fp32 ulps below a bf16 rounding.
+// reciprocal with one Newton step); with the exponent's own rounding exp(z) is off by
+// (2 + |z|) 2^-23 of it, far below a bf16 rounding.
 __device__ __forceinline__ float recip(float d) {
   const float r = __builtin_amdgcn_rcpf(d);
   return fmaf(r, fmaf(-d, r, 1.0f), r);
 }
-__device__ __forceinline__ float exp_of(float z) { return __builtin_amdgcn_exp2f(1.44269504088896341f * z); }
+__device__ __forceinline__ float exp_of(float z) {
+  const float t = 1.44269504088896341f * z;
+  const int s = t < -100.f ? 40 : 0;  // the instruction gives 0 for a subnormal result
+  return __builtin_amdgcn_ldexpf(__builtin_amdgcn_exp2f(t + (float)s), -s);
+}
 __device__ __forceinline__ float sigmoid_of(float z) {
   const float e = exp_of(-fabsf(z)), r = recip(1.0f + e);
   return z >= 0.f ? r : e * r;

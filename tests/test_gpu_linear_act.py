@@ -24,7 +24,7 @@ torch = pytest.importorskip("torch")
 
 ACTS = ["none", "silu", "gelu", "gelu_tanh", "swiglu", "situ"]
 SITU = (4.0, 25.0)
-MANY = 32  # rows (of an expert or of the call) from which the kernel of many rows may run
+MANY = 32  # rows of one matrix from which the kernel of many rows may run; by expert: one an expert in the mean
 
 
 def _weights(fmt, M, K, seed, live=None, std=0.02):
@@ -239,7 +239,7 @@ def test_experts(gpu_ctx, d_layout, part):
             a, z = int(offsets[e]), int(offsets[e + 1])
             if a < z:
                 ref, err = _reference(x[a:z], ws[e], None if b is None else b[e], act, None if r is None else r[a:z],
-                                      n >= MANY)
+                                      n >= E)
                 _check(y[a:z], ref, err, (counts, e))
         assert bool((y[live:] == 9).all())
     lyr.free()
@@ -462,3 +462,100 @@ def test_exponents_follow_the_weights(gpu_ctx):
         _check(y[n // 2:], *_reference(x[n // 2:], torch.from_numpy(Q.dequantize_simple(c, s, m)).double(), None, "none",
                                        None, True), std)
     lyr.free()
+
+
+@pytest.mark.parametrize("act", ACTS)
+def test_activations_over_their_range(gpu_ctx, act):
+    """y = act(bias) for z from -300 to 300, where exp(z) ends fp32's range and the results bf16's: x is zero, so z
+    is the bias itself.  Relative to the result exp(z) is off by (2 + |z|) 2^-23 and the rest by 32 steps of fp32,
+    then half a step of bf16; a probability below fp32's normal numbers is off by one subnormal step, 2^-149, more
+    (times |z|, and SiTU's or the gate's other factor), a bf16 subnormal by 2^-134."""
+    M, K, E = 4096, 256, 2
+    blob, _ = _weights("q4nx", M, K, 1)
+    mat = gpu_ctx.upload_matrix(blob, M, K)
+    gated = act in ("swiglu", "situ")
+    half = M // 2 if gated else M
+    z = torch.cat([torch.linspace(-300, 300, half // 2), torch.linspace(-3, 3, half - half // 2)])
+    z[5], z[6], z[half // 2], z[half // 2 + 1] = 0.0, -0.0, 1e-30, -1e-30
+    u = torch.linspace(-40, 40, half).roll(half // 3)
+    b = torch.cat([z, u]) if gated else z
+    x = torch.zeros(2, K, dtype=torch.bfloat16, device="cuda")
+    y = torch.zeros(2, half, dtype=torch.bfloat16, device="cuda")
+    mat.reserve_act(2)
+    mat.linear_act_dev(x, 2, y, bias_dev=b.cuda(), act=act, stream=torch.cuda.current_stream(), **_betas(act))
+    zd, ud = z.double(), u.double()
+    p = torch.sigmoid(zd)
+    ref = {"none": lambda: zd, "silu": lambda: zd * p, "gelu": lambda: zd * 0.5 * torch.special.erfc(-zd / math.sqrt(2.0)),
+           "gelu_tanh": lambda: zd * torch.sigmoid(2 * math.sqrt(2 / math.pi) * (zd + 0.044715 * zd ** 3)),
+           "swiglu": lambda: zd * p * ud,
+           "situ": lambda: SITU[0] * torch.tanh(zd / SITU[0]) * p * SITU[1] * torch.tanh(ud / SITU[1])}[act]()
+    # gelu's exponent is z^2 / 2, gelu_tanh's 1.6 (z + 0.045 z^3)
+    arg = {"gelu": zd * zd, "gelu_tanh": 2 * (zd.abs() + 0.05 * zd.abs() ** 3)}.get(act, zd.abs())
+    e = ref.abs() * (34 + arg.clamp(max=200.0)) * 2.0 ** -23 + 2.0 ** -149 * 1000.0 * zd.abs().clamp(min=1.0)
+    got = y.cpu().double()
+    bound = 2.0 ** -8 * (ref.abs() + e) + e + 2.0 ** -134
+    for row in got:
+        bad = ~((row - ref).abs() <= bound)
+        assert not bad.any(), (z[bad][:4].tolist(), row[bad][:4].tolist(), ref[bad][:4].tolist())
+    mat.free()
+
+
+def test_graph_captured_before_a_larger_reserve(gpu_ctx):
+    """A captured product of many rows replays as before after the scratch has grown, and other rows have gone
+    through the new one.  (The same rows in a larger batch may be summed in another order.)"""
+    M, K, T = 1024, 512, 2100
+    blob, _ = _weights("q4nx", M, K, 3)
+    mat = gpu_ctx.upload_matrix(blob, M, K)
+    mat.reserve_act(T)
+    st = torch.cuda.Stream()
+    x = torch.randn(3 * T, K, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).cuda()
+    y, big = torch.zeros(T, M, dtype=torch.bfloat16, device="cuda"), torch.zeros(3 * T, M, dtype=torch.bfloat16, device="cuda")
+    torch.cuda.synchronize()
+    mat.linear_act_dev(x[:T], T, y, act="silu", stream=st)
+    torch.cuda.synchronize()
+    want = y.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=st):
+        mat.linear_act_dev(x[:T], T, y, act="silu", stream=st)
+    for grown in (T, 2 * T, 3 * T):
+        mat.reserve_act(grown)
+        mat.linear_act_dev(x[:grown], grown, big[:grown], act="silu", stream=st)
+        junk = torch.full((grown, 4 * K), float("nan"), dtype=torch.bfloat16, device="cuda")
+        y.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, want)
+        del junk
+    mat.free()
+
+
+def test_two_contexts_on_two_streams(gpu_ctx):
+    """Products of many rows that overlap, a context each: the same bits as one after the other."""
+    from raon_npu_amd import Context
+
+    M, K, T = 1024, 1024, 3000
+    blob, _ = _weights("bfp16", M, K, 3)
+    runs = []
+    for seed, c in ((1, gpu_ctx), (2, Context(0))):
+        mat = c.upload_matrix(blob, M, K, fmt="bfp16")
+        mat.reserve_act(T)
+        x = torch.randn(T, K, generator=torch.Generator().manual_seed(seed)).to(torch.bfloat16).cuda()
+        y = torch.zeros(T, M, dtype=torch.bfloat16, device="cuda")
+        runs.append((c, mat, x, y, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    want = []
+    for c, mat, x, y, st in runs:
+        mat.linear_act_dev(x, T, y, act="gelu", stream=st)
+        torch.cuda.synchronize()
+        want.append(y.clone())
+        y.zero_()
+    torch.cuda.synchronize()
+    for _ in range(8):
+        for c, mat, x, y, st in runs:
+            mat.linear_act_dev(x, T, y, act="gelu", stream=st)
+    torch.cuda.synchronize()
+    for w, (c, mat, x, y, st) in zip(want, runs):
+        assert torch.equal(y, w)
+        mat.free()
+    runs[1][0].close()
