@@ -36,9 +36,12 @@ __device__ __forceinline__ uint32_t bf16_pair_to_half(uint32_t v, int e) {
                    __builtin_amdgcn_ldexpf(__uint_as_float(v & 0xffff0000u), -e));
 }
 
-// Rows of x to fp16 (zero past K_in) and their exponents, one wave a row.  A copy's work: 53,600
-// rows of 2,048 take 90 us (4.9 TB/s).
-__global__ __launch_bounds__(256) void act_prep_kernel(LinAct a, uint16_t* __restrict__ xh, int32_t* __restrict__ xe) {
+// Rows of x to fp16 (zero past K_in) and their exponents, one wave a row; clears the counters
+// of split tiles (256 at `arrived`, if any).  A copy's work: 53,600 rows of 2,048 take 90 us
+// (4.9 TB/s).
+__global__ __launch_bounds__(256) void act_prep_kernel(LinAct a, uint16_t* __restrict__ xh, int32_t* __restrict__ xe,
+                                                       int* __restrict__ arrived) {
+  if (arrived && blockIdx.x == 0) arrived[threadIdx.x] = 0;
   const int lane = threadIdx.x & 63, wave = wave_id();
   const size_t t = (size_t)blockIdx.x * 4 + wave;
   if (t >= (size_t)a.n) return;
@@ -110,6 +113,10 @@ struct TileArgs {
   const uint16_t* xh;
   const int32_t* xe;
   int n_nt;
+  // One matrix's last tiles, `slices` parts of K each (kSplit; see split_tail()).
+  int n_whole, slices;
+  uint64_t* part;
+  int* arrived;
 };
 
 constexpr int kActBM = 128;  // rows of the largest tile
@@ -427,7 +434,9 @@ __device__ __forceinline__ void tile_product(const TileArgs& t, const uint8_t* w
 }
 
 // Tiles of 16 BF rows x 64 NW weight rows by KS groups of NW waves, which take a KS-th of K each.
-template <int kFmt, int NF, bool kGated, int BF, int NW, int KS>
+// kSplit: the workgroups behind those of n_whole tiles take a slice of K each of the last
+// tiles, and the last of a tile to arrive adds their sums in the order of the slices.
+template <int kFmt, int NF, bool kGated, int BF, int NW, int KS, bool kSplit>
 __global__ __launch_bounds__(64 * NW * KS, BF == 8 ? 2 : BF == 4 ? 3 : 4) void act_tile_kernel(TileArgs t) {
   constexpr int kLds = kRing * kStage<BF> + NW * kWaveWeights<kFmt>, kTile = 16 * BF;
   static_assert(kLds <= 80 * 1024, "two groups a CU");
@@ -437,9 +446,17 @@ __global__ __launch_bounds__(64 * NW * KS, BF == 8 ? 2 : BF == 4 ? 3 : 4) void a
   const LinAct& a = t.a;
   RowTiles<kTile> rt;
   const int n_mt = a.offsets ? rt.total(a.offsets, a.n_experts, a.n) : (a.n + kTile - 1) / kTile;
-  const int total = n_mt * t.n_nt, per = (total + 7) / 8, slot = (int)blockIdx.x / 8;
-  const int id = ((int)blockIdx.x % 8) * per + slot;
-  if (slot >= per || id >= total) return;
+  const int total = kSplit ? t.n_whole : n_mt * t.n_nt, per = (total + 7) / 8, slot = (int)blockIdx.x / 8;
+  int id = ((int)blockIdx.x % 8) * per + slot, slice = 0, slices = 1;
+  if (kSplit && (int)blockIdx.x >= 8 * per) {
+    const int p = (int)blockIdx.x - 8 * per;
+    slices = t.slices;
+    id = total + p / slices;
+    slice = p % slices;
+    if (id >= n_mt * t.n_nt) return;
+  } else if (slot >= per || id >= total) {
+    return;
+  }
   const int nt = id % t.n_nt;
   int e = 0, row0 = id / t.n_nt * kTile, nrow = min(kTile, a.n - row0);
   if (a.offsets) rt.find(id / t.n_nt, e, row0, nrow);
@@ -461,12 +478,58 @@ __global__ __launch_bounds__(64 * NW * KS, BF == 8 ? 2 : BF == 4 ? 3 : 4) void a
 #pragma unroll
     for (int f = 0; f < NF; ++f) acc[m][f] = f32x4{0.f, 0.f, 0.f, 0.f};
   // A short tile multiplies only the fragments that hold rows.
-  const int nk = nkt / KS, kt0 = group * nk;  // K % 256 == 0
+  static_assert(!kSplit || KS == 1, "one way to split K");
+  const int kt0 = kSplit ? slice * nkt / slices : group * (nkt / KS);  // K % 256 == 0
+  const int nk = kSplit ? (slice + 1) * nkt / slices - kt0 : nkt / KS;
   uint8_t* mine = lds + group * kLds;
   if (BF == 8 && nrow > 64) tile_product<kFmt, BF, BF, NF, NW>(t, tiles, wo, wes[wr], we, row0, kt0, nk, mine, acc);
   else if (BF >= 4 && nrow > 32)
     tile_product<kFmt, BF, BF < 4 ? BF : 4, NF, NW>(t, tiles, wo, wes[wr], we, row0, kt0, nk, mine, acc);
   else tile_product<kFmt, BF, 2, NF, NW>(t, tiles, wo, wes[wr], we, row0, kt0, nk, mine, acc);
+
+  if constexpr (kSplit) {
+    if (slices > 1) {
+      // Stores of device scope go past the XCD's L2: no fence has to write it back (all of it, for
+      // every slice: 25 us more).  The few that read invalidate theirs.
+      constexpr int kPairs = 2 * BF * NF;
+      uint64_t* p = t.part + (size_t)(id - total) * slices * (kPairs * 256) + threadIdx.x;
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i) {
+        const f32x4 v = acc[i / 2 / NF][i / 2 % NF];
+        const uint64_t q = (uint64_t)__float_as_uint(v[2 * (i % 2) + 1]) << 32 | __float_as_uint(v[2 * (i % 2)]);
+        __hip_atomic_store(p + ((size_t)slice * kPairs + i) * 256, q, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      }
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();
+      int* last = reinterpret_cast<int*>(lds);
+      if (threadIdx.x == 0) *last = atomicAdd(t.arrived + (id - total), 1) == slices - 1;
+      __syncthreads();
+      if (!*last) return;
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+#pragma unroll
+      for (int i = 0; i < BF * NF; ++i) acc[i / NF][i % NF] = f32x4{0.f, 0.f, 0.f, 0.f};
+      constexpr int kBatch = 32;  // loads in flight
+#pragma unroll 1
+      for (int s = 0; s < slices; ++s) {
+#pragma unroll
+        for (int i0 = 0; i0 < kPairs; i0 += kBatch) {
+          uint64_t q[kBatch];
+#pragma unroll
+          for (int i = 0; i < kBatch; ++i) q[i] = p[(size_t)(i0 + i) * 256];
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int i = 0; i < kBatch; ++i) {
+            f32x4& v = acc[(i0 + i) / 2 / NF][(i0 + i) / 2 % NF];
+            v[2 * (i % 2)] += __uint_as_float((uint32_t)q[i]);
+            v[2 * (i % 2) + 1] += __uint_as_float((uint32_t)(q[i] >> 32));
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        p += (size_t)kPairs * 256;
+      }
+      __syncthreads();  // the epilogue reuses the memory
+    }
+  }
 
   // Epilogue: sums and bias through LDS as fp32, kRows rows at a time, so that the activation
   // has its operands at hand and residual and y move 16 bytes a thread.  Columns of
@@ -561,17 +624,19 @@ __global__ __launch_bounds__(64 * NW * KS, BF == 8 ? 2 : BF == 4 ? 3 : 4) void a
   }
 }
 
-template <int kFmt, int BF, int NW = 4, int KS = 1>
+template <int kFmt, int BF, int NW = 4, int KS = 1, bool kSplit = false>
 hipError_t launch_tiles(const TileArgs& t0, hipStream_t st) {
   constexpr int NF = 4, kTile = 16 * BF;
   TileArgs t = t0;
   const LinAct& a = t.a;
   t.n_nt = (a.M + 16 * NF * NW - 1) / (16 * NF * NW);
   const size_t mt = a.offsets ? std::min<size_t>(a.n, (size_t)a.n / kTile + a.n_experts) : ((size_t)a.n + kTile - 1) / kTile;
-  const size_t grid = 8 * ((mt * t.n_nt + 7) / 8);
+  size_t grid = 8 * ((mt * t.n_nt + 7) / 8);
+  if (kSplit) grid = 8 * (((size_t)t.n_whole + 7) / 8) + (mt * t.n_nt - t.n_whole) * t.slices;
   constexpr int kThreads = 64 * NW * KS;
   if (grid * kThreads >= (size_t)1 << 32) return hipErrorInvalidValue;
-  auto* kernel = act_gated(a.act) ? act_tile_kernel<kFmt, NF, true, BF, NW, KS> : act_tile_kernel<kFmt, NF, false, BF, NW, KS>;
+  auto* kernel = act_gated(a.act) ? act_tile_kernel<kFmt, NF, true, BF, NW, KS, kSplit>
+                                  : act_tile_kernel<kFmt, NF, false, BF, NW, KS, kSplit>;
   hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(kThreads), 0, st, t);
   return hipGetLastError();
 }
@@ -579,6 +644,20 @@ hipError_t launch_tiles(const TileArgs& t0, hipStream_t st) {
 size_t large_tiles(int M, size_t n) { return (n + 127) / 128 * ((M + 255) / 256); }
 size_t small_tiles(int M, size_t n) { return (n + 63) / 64 * (M / 128); }
 constexpr size_t kFillLarge = 200, kFillSmall = 256;
+
+// Large tiles past a multiple of 256: a CU takes 50 us for one of [2176, 2560] alone and 72 for
+// two, so a few of them beyond are cut along K into three or four slices, of two K tiles at
+// least, and as many as there are CUs.  4,096 rows of [2176, 2560] (32 beyond) 82 us whole, in 3,
+// 4, 6 and 8 slices 70, 67, 70 and 76; 6,000 of [1536, 2048] (26) 70, and 61, 60, 63 and 66; 5,060
+// of [2176, 2560] (104) 85, in 2 slices 85.  Returns the slices (1: none are cut).
+constexpr size_t kCus = 256, kMinSlices = 3, kMaxSlices = 4;
+size_t split_tail(size_t tiles, int K) {
+  const size_t over = tiles % kCus;
+  if (tiles < kCus || over == 0) return 1;
+  const size_t slices = std::min<size_t>({kCus / over, kMaxSlices, (size_t)K / (2 * kTileCols)});
+  return slices < kMinSlices ? 1 : slices;
+}
+constexpr size_t kTailBytes = kCus * kActBM * 256 * 4;  // the sums of at most kCus slices
 
 // By expert: by the rows an expert has in the mean (128 experts, q4nx gate/up [1536, 2048], tiles
 // of 32, 64 and 128 rows: 28 rows 68, 67 and 77 us, 44 rows 108, 81 and 93, 62 rows 135, 113 and
@@ -590,6 +669,7 @@ constexpr size_t kFillLarge = 200, kFillSmall = 256;
 template <int kFmt>
 hipError_t pick_tiles(const TileArgs& t, hipStream_t st) {
   const LinAct& a = t.a;
+  if (t.slices > 1) return launch_tiles<kFmt, 8, 4, 1, true>(t, st);
   if (!a.offsets || a.n_experts == 1)
     return large_tiles(a.M, a.n) >= kFillLarge ? launch_tiles<kFmt, 8>(t, st) : launch_tiles<kFmt, 4, 2, 2>(t, st);
   const size_t rows = (size_t)a.n / a.n_experts;
@@ -620,7 +700,8 @@ bool act_tiles_serve(int fmt, int M, int K, int groups, size_t n) {
 }
 size_t act_tiles_scratch(int fmt, int M, int K, int groups, size_t n) {
   if (!act_tiles_serve(fmt, M, K, groups, n)) return 0;
-  return round256((n + kActBM) * K * 2) + round256(n * 4);
+  const bool tail = groups == 1 && large_tiles(M, n) >= kCus;
+  return round256((n + kActBM) * K * 2) + round256(n * 4) + (tail ? kTailBytes + kCus * 4 : 0);
 }
 
 hipError_t launch_act_tiles(const LinAct& a, uint8_t* scratch, size_t bytes, hipStream_t st) {
@@ -629,10 +710,16 @@ hipError_t launch_act_tiles(const LinAct& a, uint8_t* scratch, size_t bytes, hip
   if (groups * 256 >= (size_t)1 << 32) return hipErrorInvalidValue;
   uint16_t* xh = reinterpret_cast<uint16_t*>(scratch);
   int32_t* xe = reinterpret_cast<int32_t*>(scratch + round256(((size_t)a.n + kActBM) * a.K * 2));
-  hipLaunchKernelGGL(act_prep_kernel, dim3((unsigned)groups), dim3(256), 0, st, a, xh, xe);
+  TileArgs t{a, xh, xe, 0, 0, 1, nullptr, nullptr};
+  const size_t tiles = large_tiles(a.M, a.n);
+  if (!a.offsets && (t.slices = (int)split_tail(tiles, a.K)) > 1) {
+    t.n_whole = (int)(tiles / kCus * kCus);
+    t.part = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(xe) + round256((size_t)a.n * 4));
+    t.arrived = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(t.part) + kTailBytes);
+  }
+  hipLaunchKernelGGL(act_prep_kernel, dim3((unsigned)groups), dim3(256), 0, st, a, xh, xe, t.arrived);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  const TileArgs t{a, xh, xe, 0};
   return a.fmt == RMOE_FMT_BFP16 ? pick_tiles<RMOE_FMT_BFP16>(t, st) : pick_tiles<RMOE_FMT_Q4NX>(t, st);
 }
 

@@ -559,3 +559,70 @@ def test_two_contexts_on_two_streams(gpu_ctx):
         assert torch.equal(y, w)
         mat.free()
     runs[1][0].close()
+
+
+@pytest.mark.parametrize("M,K,T", [
+    (256, 512, 128 * 211 + 5),   # 212 tiles of 128 x 256, no whole round of 256
+    (256, 512, 128 * 256 + 3),   # one tile past a round, ragged, of a K too short to cut
+    (256, 2048, 128 * 256 + 100),  # the same, in four slices of four K tiles
+    (1280, 1280, 128 * 54 - 60),  # 270 tiles: 14 past a round, four slices of two and three K tiles
+    (2176, 1280, 128 * 40),      # 360: 104 past a round, too many to cut
+    (768, 2560, 128 * 113 + 1),  # 342: 86, the same
+    (1280, 768, 128 * 68),       # 340: 84, in three slices of two
+    (512, 1792, 128 * 161),      # 322: 66, in three slices of four and five
+    (2560, 1024, 128 * 55),      # 550: 38 past two rounds, in four
+    (512, 512, 128 * 193)])      # 386: 130 past a round
+@pytest.mark.parametrize("act", ["none", "swiglu"])
+def test_dense_around_whole_rounds_of_tiles(gpu_ctx, M, K, T, act):
+    """Tile counts on both sides of multiples of the CUs, where the last tiles' sums are cut along K: every row against
+    64 bits, rows behind the last as they were, and the same bits each time."""
+    for fmt in ("q4nx", "bfp16"):
+        blob, w = _weights(fmt, M, K, M + K)
+        mat = gpu_ctx.upload_matrix(blob, M, K, fmt=fmt)
+        mat.reserve_act(T)
+        gated = act == "swiglu"
+        width = M // 2 if gated else M
+        x = torch.randn(T, K, generator=torch.Generator().manual_seed(T)).to(torch.bfloat16).cuda()
+        b = torch.randn(M, generator=torch.Generator().manual_seed(1)).cuda()
+        y = torch.full((T + 1, width), 9.0, dtype=torch.bfloat16, device="cuda")
+        st = torch.cuda.current_stream()
+        mat.linear_act_dev(x, T, y[:T], bias_dev=b, act=act, stream=st)
+        w = w.cuda()
+        for t0 in range(0, T, 4096):
+            ref, e = _reference(x[t0:t0 + 4096], w, b, act, None, True)
+            _check(y[t0:min(t0 + 4096, T)], ref.cpu(), e.cpu(), (fmt, t0))
+        assert bool((y[T] == 9).all())
+        first = y.clone()
+        for _ in range(5):
+            y[:T].zero_()
+            mat.linear_act_dev(x, T, y[:T], bias_dev=b, act=act, stream=st)
+            assert torch.equal(y, first)
+        mat.free()
+
+
+def test_split_tiles_in_a_graph(gpu_ctx):
+    """The cut tiles' counters are cleared by each call, captured or not, also after a call of other rows."""
+    M, K, T = 2176, 1280, 128 * 32
+    blob, _ = _weights("q4nx", M, K, 3)
+    mat = gpu_ctx.upload_matrix(blob, M, K)
+    mat.reserve_act(T)
+    st = torch.cuda.Stream()
+    x = torch.randn(T, K, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).cuda()
+    y, other = (torch.zeros(T, M, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    torch.cuda.synchronize()
+    mat.linear_act_dev(x, T, y, stream=st)
+    torch.cuda.synchronize()
+    want = y.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=st):
+        mat.linear_act_dev(x, T, y, stream=st)
+    for n in (T, 128 * 30, 128 * 31, 7):
+        mat.linear_act_dev(x[:n], n, other[:n], stream=st)
+        torch.cuda.synchronize()
+        y.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, want)
+    mat.free()
