@@ -135,8 +135,8 @@ int rmoe_reserve_linear(rmoe_ctx* ctx, int handle, int T);
  * fp32 throughout, rounded once.  x bf16 [T, K_in], K_in <= K a multiple of 8 (columns past
  * it are zero), 16-byte aligned; bias fp32 [M] or NULL; residual bf16 of y's shape or NULL (y
  * itself: added in place); y bf16 [T, M'].  act RMOE_ACT_NONE, _SILU, _GELU, _GELU_TANH:
- * M' = M; RMOE_ACT_SWIGLU, _SITU (gate_beta, value_beta): M' = M / 2, row i of W the gate and
- * row M/2 + i the up of output i, bias added to both.  (rmoe_linear_dev followed by the
+ * M' = M; RMOE_ACT_SWIGLU, _SITU (gate_beta, value_beta, 2^-100 to 2^100 in magnitude):
+ * M' = M / 2, row i of W the gate and row M/2 + i the up of output i, bias added to both.  (rmoe_linear_dev followed by the
  * activation rounds gate and up to bf16 first; this call does not.)  Many rows are multiplied
  * in fp16 with a power of two per row of x and of W: q4nx weights are rounded once to fp16's 11
  * bits of their row's largest.  Asynchronous on `stream`, never allocates; products of many

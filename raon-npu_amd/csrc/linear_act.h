@@ -11,13 +11,11 @@ __host__ __device__ constexpr bool act_gated(int act) { return act == RMOE_ACT_S
 
 // Activations of one value.  Each is z times a probability formed without cancellation: the
 // sigmoid from exp(-|z|), the normal distribution's from erfc, so that small results keep
-// their relative accuracy.  exp2 and the reciprocal are the hardware's (1 ulp each; the
-// reciprocal with one Newton step); with the exponent's own rounding exp(z) is off by
-// (2 + |z|) 2^-23 of it, far below a bf16 rounding.
-__device__ __forceinline__ float recip(float d) {
-  const float r = __builtin_amdgcn_rcpf(d);
-  return fmaf(r, fmaf(-d, r, 1.0f), r);
-}
+// their relative accuracy.  exp2 and the reciprocal are the hardware's (1 ulp each); with the
+// exponent's own rounding exp(z) is off by (2 + |z|) 2^-23 of it, far below a bf16 rounding.
+// They are kept short: a product with 4,096 x 1,088 SiTU outputs took 83 us with IEEE
+// divisions, Newton steps and clamps, and 77 without.
+__device__ __forceinline__ float recip(float d) { return __builtin_amdgcn_rcpf(d); }
 __device__ __forceinline__ float exp_of(float z) {
   const float t = 1.44269504088896341f * z;
   const int s = t < -100.f ? 40 : 0;  // the instruction gives 0 for a subnormal result
@@ -27,17 +25,17 @@ __device__ __forceinline__ float sigmoid_of(float z) {
   const float e = exp_of(-fabsf(z)), r = recip(1.0f + e);
   return z >= 0.f ? r : e * r;
 }
-// tanh: 1 - 2 / (1 + exp(2 |z|)), and below 0.3, where that cancels, its power series to z^9
-// (the next term is 4e-8 of z there).
+// tanh: 1 - 2 / (1 + exp(2 |z|)), which an infinite exp makes 1, and below 0.3, where that
+// cancels, its power series to z^9 (the next term is 4e-8 of z there).
 __device__ __forceinline__ float tanh_of(float z) {
   const float a = fabsf(z), q = z * z;
-  const float big = 1.0f - 2.0f * recip(1.0f + exp_of(2.0f * fminf(a, 20.f)));
+  const float big = fmaf(-2.0f, recip(1.0f + __builtin_amdgcn_exp2f(2.88539008177792681f * a)), 1.0f);
   const float s = fmaf(q, fmaf(q, fmaf(q, fmaf(q, 62.f / 2835.f, -17.f / 315.f), 2.f / 15.f), -1.f / 3.f), 1.0f);
-  return a < 0.3f ? z * s : z != z ? z : copysignf(big, z);
+  return a < 0.3f ? z * s : copysignf(big, z);
 }
 __device__ __forceinline__ float act_pair(int act, float g, float u, float gb, float vb) {
   if (act == RMOE_ACT_SWIGLU) return g * sigmoid_of(g) * u;
-  return gb * tanh_of(g / gb) * sigmoid_of(g) * (vb * tanh_of(u / vb));
+  return gb * tanh_of(g * (1.0f / gb)) * sigmoid_of(g) * (vb * tanh_of(u * (1.0f / vb)));
 }
 __device__ __forceinline__ float act_single(int act, float z) {
   if (act == RMOE_ACT_SILU) return z * sigmoid_of(z);

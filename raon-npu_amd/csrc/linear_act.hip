@@ -18,7 +18,7 @@ namespace {
 constexpr int kPad = 4;  // floats of padding per row of the partial sums
 
 // Gated tiles hold NF / 2 fragments of gate rows, then the up rows of the same units.
-// kTail: the rows end short of K (K_in < K).
+// kTail: the rows end inside a K tile.
 template <int kFmt, int MF, int NF, int XI, bool kGated, bool kTail>
 __global__ __launch_bounds__(512) void linear_act_kernel(LinAct a, int n_nt) {
   extern __shared__ __attribute__((aligned(16))) float la_lds[];
@@ -43,7 +43,7 @@ __global__ __launch_bounds__(512) void linear_act_kernel(LinAct a, int n_nt) {
   }
   const int tid = threadIdx.x, lane = tid & 63, wave = wave_id(), W = blockDim.x >> 6;
   const int l16 = lane & 15, lq = lane >> 4;
-  const int nkt = a.K / kTileCols;
+  const int nkt = a.K / kTileCols, nkt_in = (a.K_in + kTileCols - 1) / kTileCols;
   const uint8_t* tiles = a.tiles + (size_t)e * a.wstride;
   WaveOperands<MF, NF, XI, kTail> o;
 #pragma unroll
@@ -66,7 +66,7 @@ __global__ __launch_bounds__(512) void linear_act_kernel(LinAct a, int n_nt) {
   for (int m = 0; m < MF; ++m)
 #pragma unroll
     for (int f = 0; f < NF; ++f) acc[m][f] = wg_f32x4{0.f, 0.f, 0.f, 0.f};
-  wave_gemm<kFmt, MF, NF, XI>(o, wave * nkt / W, (wave + 1) * nkt / W, acc);
+  wave_gemm<kFmt, MF, NF, XI>(o, wave * nkt_in / W, (wave + 1) * nkt_in / W, acc);
   __syncthreads();  // the partial sums reuse the waves' activation regions
   float* mine = la_lds + (size_t)wave * 16 * MF * kStride;
 #pragma unroll
@@ -137,16 +137,16 @@ constexpr size_t act_lds(int MF, int NF, int W) {
 
 template <int kFmt, int MF, int NF, int XI>
 hipError_t launch(const LinAct& a, hipStream_t st) {
-  const int nkt = a.K / kTileCols, W = std::min(nkt, nkt >= 64 ? 8 : 4);
+  const int nkt = (a.K_in + kTileCols - 1) / kTileCols, W = std::min(nkt, nkt >= 64 ? 8 : 4);
   constexpr int BM = XI == 1 ? 4 : 16 * MF;
   const size_t mt = a.offsets ? std::min<size_t>(a.n, (size_t)a.n / BM + a.n_experts) : ((size_t)a.n + BM - 1) / BM;
   const size_t total = mt * (a.M / (16 * NF)), grid = 8 * ((total + 7) / 8);
   if (grid * 64 * W >= (size_t)1 << 32 || total >= (size_t)1 << 31) return hipErrorInvalidValue;
   constexpr bool kPair = NF > 1;
-  auto* kernel = a.K_in < a.K ? (act_gated(a.act) ? linear_act_kernel<kFmt, MF, NF, XI, kPair, true>
-                                                  : linear_act_kernel<kFmt, MF, NF, XI, false, true>)
-                              : (act_gated(a.act) ? linear_act_kernel<kFmt, MF, NF, XI, kPair, false>
-                                                  : linear_act_kernel<kFmt, MF, NF, XI, false, false>);
+  auto* kernel = a.K_in % kTileCols ? (act_gated(a.act) ? linear_act_kernel<kFmt, MF, NF, XI, kPair, true>
+                                                        : linear_act_kernel<kFmt, MF, NF, XI, false, true>)
+                                    : (act_gated(a.act) ? linear_act_kernel<kFmt, MF, NF, XI, kPair, false>
+                                                        : linear_act_kernel<kFmt, MF, NF, XI, false, false>);
   hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(64 * W), act_lds(MF, NF, W), st, a, a.M / (16 * NF));
   return hipGetLastError();
 }

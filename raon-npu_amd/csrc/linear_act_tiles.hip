@@ -36,7 +36,7 @@ __device__ __forceinline__ uint32_t bf16_pair_to_half(uint32_t v, int e) {
                    __builtin_amdgcn_ldexpf(__uint_as_float(v & 0xffff0000u), -e));
 }
 
-// Rows of x to fp16 (zero past K_in) and their exponents, one wave a row; clears the counters
+// Rows of x to fp16 (zero past K_in to the end of its pair of K tiles) and their exponents, one wave a row; clears the counters
 // of split tiles (256 at `arrived`, if any).  A copy's work: 53,600 rows of 2,048 take 90 us
 // (4.9 TB/s).
 __global__ __launch_bounds__(256) void act_prep_kernel(LinAct a, uint16_t* __restrict__ xh, int32_t* __restrict__ xe,
@@ -47,7 +47,7 @@ __global__ __launch_bounds__(256) void act_prep_kernel(LinAct a, uint16_t* __res
   if (t >= (size_t)a.n) return;
   const uint4* src = reinterpret_cast<const uint4*>(a.x + t * a.K_in);
   uint4* dst = reinterpret_cast<uint4*>(xh + t * a.K);
-  const int nch = a.K_in / 8, nout = a.K / 8;
+  const int nch = a.K_in / 8, nout = (a.K_in + 2 * kTileCols - 1) / (2 * kTileCols) * (2 * kTileCols / 8);
   constexpr int kKeep = 5;  // 16-byte chunks a lane keeps between the two passes (2,560 columns)
   uint4 v[kKeep];
   float mx = 0.f;
@@ -479,8 +479,9 @@ __global__ __launch_bounds__(64 * NW * KS, BF == 8 ? 2 : BF == 4 ? 3 : 4) void a
     for (int f = 0; f < NF; ++f) acc[m][f] = f32x4{0.f, 0.f, 0.f, 0.f};
   // A short tile multiplies only the fragments that hold rows.
   static_assert(!kSplit || KS == 1, "one way to split K");
-  const int kt0 = kSplit ? slice * nkt / slices : group * (nkt / KS);  // K % 256 == 0
-  const int nk = kSplit ? (slice + 1) * nkt / slices - kt0 : nkt / KS;
+  const int nkt_in = (a.K_in + kTileCols - 1) / kTileCols, half = (nkt_in + KS - 1) / KS;  // K % 256 == 0
+  const int kt0 = kSplit ? slice * nkt_in / slices : group * half;
+  const int nk = kSplit ? (slice + 1) * nkt_in / slices - kt0 : half;
   uint8_t* mine = lds + group * kLds;
   if (BF == 8 && nrow > 64) tile_product<kFmt, BF, BF, NF, NW>(t, tiles, wo, wes[wr], we, row0, kt0, nk, mine, acc);
   else if (BF >= 4 && nrow > 32)
@@ -651,10 +652,10 @@ constexpr size_t kFillLarge = 200, kFillSmall = 256;
 // 4, 6 and 8 slices 70, 67, 70 and 76; 6,000 of [1536, 2048] (26) 70, and 61, 60, 63 and 66; 5,060
 // of [2176, 2560] (104) 85, in 2 slices 85.  Returns the slices (1: none are cut).
 constexpr size_t kCus = 256, kMinSlices = 3, kMaxSlices = 4;
-size_t split_tail(size_t tiles, int K) {
+size_t split_tail(size_t tiles, int K_in) {
   const size_t over = tiles % kCus;
   if (tiles < kCus || over == 0) return 1;
-  const size_t slices = std::min<size_t>({kCus / over, kMaxSlices, (size_t)K / (2 * kTileCols)});
+  const size_t slices = std::min<size_t>({kCus / over, kMaxSlices, (size_t)K_in / (2 * kTileCols)});
   return slices < kMinSlices ? 1 : slices;
 }
 constexpr size_t kTailBytes = kCus * kActBM * 256 * 4;  // the sums of at most kCus slices
@@ -712,7 +713,7 @@ hipError_t launch_act_tiles(const LinAct& a, uint8_t* scratch, size_t bytes, hip
   int32_t* xe = reinterpret_cast<int32_t*>(scratch + round256(((size_t)a.n + kActBM) * a.K * 2));
   TileArgs t{a, xh, xe, 0, 0, 1, nullptr, nullptr};
   const size_t tiles = large_tiles(a.M, a.n);
-  if (!a.offsets && (t.slices = (int)split_tail(tiles, a.K)) > 1) {
+  if (!a.offsets && (t.slices = (int)split_tail(tiles, a.K_in)) > 1) {
     t.n_whole = (int)(tiles / kCus * kCus);
     t.part = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(xe) + round256((size_t)a.n * 4));
     t.arrived = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(t.part) + kTailBytes);

@@ -2,6 +2,7 @@
 // and the entry points.  Host entry points validate every shape before any kernel
 // is launched; "_dev" entry points validate shapes and scratch capacity and never
 // allocate.
+#include <math.h>
 #include <stdarg.h>
 #include <stdio.h>
 #include <string.h>
@@ -379,7 +380,9 @@ int check_linear_act(const rmoe::LinAct& L) {
   if (L.act < RMOE_ACT_SITU || L.act > RMOE_ACT_GELU_TANH) return fail(RMOE_EINVAL, "unknown activation %d", L.act);
   if (L.K_in < 8 || L.K_in > L.K || L.K_in % 8)
     return fail(RMOE_EINVAL, "input width %d must be a multiple of 8 and at most K=%d", L.K_in, L.K);
-  if (L.act == RMOE_ACT_SITU && (L.gb == 0.f || L.vb == 0.f)) return fail(RMOE_EINVAL, "SiTU betas must not be zero");
+  for (float b : {L.gb, L.vb})
+    if (L.act == RMOE_ACT_SITU && !(fabsf(b) >= 0x1p-100f && fabsf(b) <= 0x1p100f))
+      return fail(RMOE_EINVAL, "SiTU betas must be between 2^-100 and 2^100 in magnitude");
   if (reinterpret_cast<uintptr_t>(L.x) & 15) return fail(RMOE_EINVAL, "the input rows must be 16-byte aligned");
   if ((reinterpret_cast<uintptr_t>(L.y) | reinterpret_cast<uintptr_t>(L.residual)) & 1 ||
       (reinterpret_cast<uintptr_t>(L.bias) | reinterpret_cast<uintptr_t>(L.offsets)) & 3)

@@ -542,7 +542,7 @@ struct LinAct {
   size_t wstride;
   int fmt, M, K;
   const uint16_t* x;  // [n, K_in], 16-byte aligned, K_in % 8 == 0; weights past K_in see zeros
-  int n, K_in;
+  int n, K_in;        // (their K tiles are not read)
   const int32_t* offsets;
   int n_experts;
   const float* bias;

@@ -82,17 +82,26 @@ def _operand(device: int, t, shape: tuple, dtype_name: str, name: str) -> int:
     A call of these operators takes 4 us on the GPU when it is small, and two microseconds of host time per operand
     (``_check_dev``, then the device) made it 12: the checks are one expression, taken apart only to name a fault."""
     try:
-        if (t.is_cuda and t.shape == shape and _dtype_name(t) == dtype_name and t.is_contiguous()
-                and t.get_device() == device):
+        if (t.get_device() == device and t.shape == shape and _DTYPE_NAMES.get(t.dtype) == dtype_name
+                and t.is_contiguous()):
             return t.data_ptr()
     except AttributeError:
         pass
     _check_dev(t, shape, dtype_name, name)
-    raise ValueError(f"{name} is on {t.device}, the context on cuda:{device}")
+    if t.get_device() != device:
+        raise ValueError(f"{name} is on {t.device}, the context on cuda:{device}")
+    _dtype_name(t)  # a type seen for the first time
+    return t.data_ptr()
 
 
 def _bf16_operand(device: int, t, shape: tuple, name: str) -> int:
     """bf16 values of a given shape, as bfloat16 or as int16 bits."""
+    try:
+        if (t.get_device() == device and t.shape == shape and _DTYPE_NAMES.get(t.dtype) in ("bfloat16", "int16")
+                and t.is_contiguous()):
+            return t.data_ptr()
+    except AttributeError:
+        pass
     return _operand(device, t, shape, "int16" if _dtype_name(t) == "int16" else "bfloat16", name)
 
 

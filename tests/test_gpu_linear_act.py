@@ -626,3 +626,21 @@ def test_split_tiles_in_a_graph(gpu_ctx):
         torch.cuda.synchronize()
         assert torch.equal(y, want)
     mat.free()
+
+
+@pytest.mark.parametrize("fmt", ["q4nx", "bfp16"])
+@pytest.mark.parametrize("T", [128 * 64 + 1, 128 * 256 + 3])
+def test_many_rows_narrower_than_the_matrix(gpu_ctx, fmt, T):
+    """K_in < K with tiles by two groups of K, which may get unequal shares, and with the last tiles cut along K."""
+    M, K = 256, 1280
+    blob, w = _weights(fmt, M, K, 3)
+    mat = gpu_ctx.upload_matrix(blob, M, K, fmt=fmt)
+    mat.reserve_act(T)
+    w = w.cuda()
+    for K_in in (8, 128, 136, 640, 1024, 1088, 1152, 1272):
+        x = torch.randn(T, K_in, generator=torch.Generator().manual_seed(K_in)).to(torch.bfloat16).cuda()
+        y = torch.zeros(T, M, dtype=torch.bfloat16, device="cuda")
+        mat.linear_act_dev(x, T, y, act="silu", stream=torch.cuda.current_stream())
+        ref, e = _reference(x, w[:, :K_in], None, "silu", None, True)
+        _check(y, ref.cpu(), e.cpu(), K_in)
+    mat.free()
