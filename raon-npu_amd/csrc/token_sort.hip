@@ -25,13 +25,13 @@ namespace {
 constexpr int kMaxRoutes = 16;
 constexpr int kErrExpert = 4, kErrPosition = 16;
 
-// Few assignments are sorted by one launch in which every token's workgroup counts over all
-// of them, k comparisons each; more by four launches.  One / four (H 256, by events and, in
-// brackets, replayed in a graph): 1,024 assignments 7.5 us; 2,048 of k = 8 10.1 / 15.2 (9.7 /
-// 10.9), of k = 2 7.4 / 15.0 (7.5 / 10.7), of k = 16 14.6 / 15.4 (14.9 / 11.2); 4,096 of k = 8
-// 17.3 / 15.6 (17.6 / 11.7).
-constexpr int kSmallRoutes = 2048, kSmallWork = 16384;  // n, n k
-bool sort_is_small(int n, int k) { return n <= kSmallRoutes && n * k <= kSmallWork; }
+// Assignments up to which every token's workgroup finds its own positions by k comparisons
+// with each of them, in one launch with the rows; up to which every chunk's workgroup counts
+// all of them, in two launches; beyond, four.  H 256, k 8, by events / replayed in a graph: 1,024
+// assignments in one 7.4 / 6.6 us, in two 9.6 / 7.0; 2,048 9.6 / 9.7 and 9.8 / 7.2; 4,096 in two
+// 9.7 / 7.5, in four 14.9 / 11.4; 32,768 12.9 and 16.3; 53,600 16.8 and 18.8; 72,000 20.0 and 19.7;
+// 128,000 31 and 27.
+constexpr int kOneLaunch = 1024, kTwoLaunches = 65536;
 
 // One element of a type as fp32, and fp32 rounded to it (RTNE).
 template <int DT>
@@ -84,8 +84,8 @@ __device__ __forceinline__ int route_expert(int id, int E, int* err) {
   return id < 0 || id >= E ? -1 : id;
 }
 
-// Few assignments: workgroup t counts its own token's positions over all ids (4 KB at 1,024,
-// read from L2), workgroup T the offsets; one launch, no workspace.
+// Up to kOneLaunch assignments: workgroup t counts its own token's positions over all ids (4 KB
+// at most, read from L2), workgroup T the offsets; no workspace.
 struct SortArgs {
   const int32_t* ids;
   int T, k, E, n;
@@ -179,6 +179,74 @@ __global__ __launch_bounds__(256) void sort_small_kernel(SortArgs a, const uint8
   }
   __syncthreads();
   scatter_row<U>(x + (size_t)t * rb, rows, rb, pos, a.k, tid, 256);
+}
+
+// Up to kTwoLaunches: one places them, one moves the rows.  Workgroup c takes chunk c and counts
+// the assignments before and behind it itself (n reads from L2 a workgroup, no workspace).  Its
+// 16 waves take 64 assignments each and rank the lanes of equal expert by ballots on the id's
+// bits (stable, no order of atomics in the result).
+__global__ __launch_bounds__(1024) void sort_place_all_kernel(SortArgs a) {
+  __shared__ int before[256], total[256], slot[16][256];
+  const int c = blockIdx.x, tid = threadIdx.x, wave = wave_id(), lane = tid & 63;
+  if (tid < 256) before[tid] = total[tid] = 0;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) slot[w * 4 + tid / 256][tid % 256] = 0;
+  const int i = c * kDispatchChunk + tid, ev = i < a.n ? route_expert(a.ids[i], a.E, a.err) : -1;
+  __syncthreads();
+  constexpr int kAhead = 8;  // loads in flight
+  for (int c0 = 0; c0 * kDispatchChunk < a.n; c0 += kAhead) {
+    int id[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int j = (c0 + u) * kDispatchChunk + tid;
+      id[u] = j < a.n ? a.ids[j] : -1;
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      if (id[u] >= 0 && id[u] < a.E) atomicAdd(c0 + u < c ? &before[id[u]] : &total[id[u]], 1);
+  }
+  unsigned long long same = __ballot(ev >= 0);
+#pragma unroll
+  for (int b = 0; b < 8; ++b) {
+    const unsigned long long bb = __ballot((ev >> b) & 1);
+    same &= ((ev >> b) & 1) ? bb : ~bb;
+  }
+  if (ev < 0) same = 0ull;
+  if (same && (same >> lane) == 1ull) slot[wave][ev] = __popcll(same);  // one writer per expert
+  __syncthreads();
+  if (tid < 64) {  // offsets: exclusive sums over the experts
+    int run = 0;
+#pragma unroll
+    for (int e0 = 0; e0 < 256; e0 += 64) {
+      const int e = e0 + tid, own = before[e] + total[e];
+      int incl = own;
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        const int y = __shfl_up(incl, d, 64);
+        if (tid >= d) incl += y;
+      }
+      const int first = run + incl - own;
+      before[e] += first;  // the chunk's first position
+      if (c == 0 && e < a.E) a.offsets[e] = first;
+      run += __shfl(incl, 63, 64);
+    }
+    if (c == 0 && tid == 0) a.offsets[a.E] = run;
+  }
+  __syncthreads();
+  if (tid < 256) {
+    int run = before[tid];
+#pragma unroll
+    for (int w = 0; w < 16; ++w) {
+      const int v = slot[w][tid];
+      slot[w][tid] = run;
+      run += v;
+    }
+  }
+  __syncthreads();
+  int pos = -1;
+  if (same) pos = slot[wave][ev] + __popcll(same & ((1ull << lane) - 1ull));
+  if (i < a.n) a.inv[i] = pos;
+  if (pos >= 0) a.order[pos] = i;
 }
 
 // More assignments: chunks of kDispatchChunk are counted, the counts summed over the chunks
@@ -453,7 +521,11 @@ __global__ __launch_bounds__(256) void combine_grad_kernel(CombineGradArgs a) {
       Pack<DT, N> o;
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        o.v[i] = Elem<DT>::put(__fmul_rn(w, df[i]));
+        float p = __fmul_rn(w, df[i]);
+        // The product is rounded to fp32 first, at every address and column: the compiler makes one
+        // instruction with a single rounding of some products with their conversion to fp16.
+        if constexpr (DT == RMOE_DT_F16) asm("" : "+v"(p));
+        o.v[i] = Elem<DT>::put(p);
         dot[r] = fmaf(df[i], Elem<DT>::get(v.v[i]), dot[r]);
       }
       store_pack<DT, N>(static_cast<E*>(a.drows) + (size_t)p * a.H + c, o);
@@ -486,14 +558,18 @@ constexpr size_t kMaxGroups = ((size_t)1 << 32) / 256 - 1;
 
 template <typename U>
 hipError_t sort_with(const SortArgs& a, const void* x, void* rows, size_t rb, hipStream_t st) {
-  if (sort_is_small(a.n, a.k)) {
+  if (a.n <= kOneLaunch) {
     hipLaunchKernelGGL(sort_small_kernel<U>, dim3(a.T + 1), dim3(256), 0, st, a, (const uint8_t*)x, (uint8_t*)rows, rb);
     return hipGetLastError();
   }
   const int nchunks = (int)(((size_t)a.n + kDispatchChunk - 1) / kDispatchChunk);
-  hipLaunchKernelGGL(sort_count_kernel, dim3(nchunks - 1), dim3(256), 0, st, a);
-  hipLaunchKernelGGL(sort_scan_kernel, dim3(1), dim3(1024), 0, st, a, nchunks);
-  hipLaunchKernelGGL(sort_place_kernel, dim3(nchunks), dim3(256), 0, st, a, nchunks);
+  if (a.n <= kTwoLaunches) {
+    hipLaunchKernelGGL(sort_place_all_kernel, dim3(nchunks), dim3(1024), 0, st, a);
+  } else {
+    hipLaunchKernelGGL(sort_count_kernel, dim3(nchunks - 1), dim3(256), 0, st, a);
+    hipLaunchKernelGGL(sort_scan_kernel, dim3(1), dim3(1024), 0, st, a, nchunks);
+    hipLaunchKernelGGL(sort_place_kernel, dim3(nchunks), dim3(256), 0, st, a, nchunks);
+  }
   hipError_t e = hipGetLastError();
   const int threads = (int)std::min<size_t>(256, (rb / sizeof(U) + 63) / 64 * 64);
   for (size_t t0 = 0; e == hipSuccess && t0 < (size_t)a.T; t0 += kMaxGroups) {

@@ -54,12 +54,13 @@ def _buffers(T, k, E, H, dtype, fill=7):
             torch.full((E + 1,), -9, dtype=torch.int32, device="cuda"))
 
 
-# Both sides of one launch and four (2,048 assignments, 1,024 of 16 routes) and of a chunk of 1,024; a last chunk
-# shorter than the experts.
+# Both sides of one launch and two (1,024 assignments), of two and four (65,536) and of a chunk of 1,024; a last
+# chunk shorter than the experts.
 SHAPES = [(1, 1, 1, 1), (1, 8, 128, 2048), (4, 8, 128, 2048), (3, 16, 256, 33), (128, 8, 128, 64), (129, 8, 128, 64),
           (1024, 1, 256, 8), (1025, 1, 256, 8), (64, 16, 128, 8), (65, 16, 128, 8),
           (256, 8, 128, 8), (257, 8, 128, 8), (2048, 1, 200, 8), (2049, 1, 200, 8), (445, 6, 128, 2560), (300, 7, 9, 1027), (2049, 3, 64, 136),
-          (4100, 16, 255, 24)]
+          (4096, 16, 255, 24),
+          (4100, 16, 255, 24), (65537, 1, 256, 8), (9400, 7, 9, 24)]
 
 
 @pytest.mark.parametrize("T,k,E,H", SHAPES)
@@ -78,7 +79,7 @@ def test_sort(gpu_ctx, T, k, E, H, dtype):
 
 
 def test_sort_without_any_route_and_all_on_one_expert(gpu_ctx):
-    for T, k, E, H in ((5, 2, 4, 16), (3000, 2, 4, 16)):
+    for T, k, E, H in ((5, 2, 4, 16), (3000, 2, 4, 16), (33000, 2, 4, 16)):
         x = torch.randn(T, H, device="cuda").to(torch.bfloat16)
         st = torch.cuda.current_stream()
         for ids in (torch.full((T, k), -1, dtype=torch.int32), torch.full((T, k), 2, dtype=torch.int32),
@@ -99,7 +100,7 @@ def test_sort_without_any_route_and_all_on_one_expert(gpu_ctx):
 
 def test_expert_past_the_last_is_reported(gpu_ctx):
     """Its route has no row; the next synchronous call raises, once."""
-    for T in (4, 2000):
+    for T in (4, 2000, 40000):
         x = torch.randn(T, 32, device="cuda").to(torch.bfloat16)
         ids = _ids(T, 2, 8, 5, drop=0.0)
         ids[1, 1] = 8
@@ -263,6 +264,33 @@ def test_rows_at_odd_addresses(gpu_ctx, dtype, shift):
     # another order of the dot product's sum
     S = (_gather(want[0].cpu(), inv.cpu()) * x.cpu().double()[:, None]).abs().sum(2)
     assert bool(((outs[0][2] - outs[1][2]).cpu().double().abs() <= 2 * H * 2.0 ** -23 * S).all())
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_the_same_bits_at_every_address(gpu_ctx, dtype):
+    """Sums and products round alike whether 16-byte accesses take them or single elements: 100,000 products, of
+    which, with 13 bits between fp32 and fp16, some 2^-14 round otherwise once than twice."""
+    T, k, E, H = 64, 4, 8, 512
+    g = torch.Generator().manual_seed(21)
+    rows, dout = torch.randn(T * k, H, generator=g).to(dtype).cuda(), torch.randn(T, H, generator=g).to(dtype).cuda()
+    w = (torch.rand(T, k, generator=g) - 0.3).cuda()
+    inv = _plain_sort(_ids(T, k, E, 4), E)[1].cuda()
+    st = torch.cuda.current_stream()
+
+    def odd(v):
+        b = torch.zeros(v.numel() + 1, dtype=v.dtype, device="cuda")
+        b[1:].copy_(v.reshape(-1))
+        return b[1:].view(v.shape)
+
+    got = []
+    for f in (lambda v: v, odd):
+        out, dx, dr, dw = f(torch.zeros_like(dout)), f(torch.zeros_like(dout)), f(torch.zeros_like(rows)), torch.zeros_like(w)
+        gpu_ctx.combine_tokens_dev(f(rows), inv, w, out, stream=st)
+        gpu_ctx.sort_tokens_backward_dev(f(rows), inv, dx, stream=st)
+        gpu_ctx.combine_tokens_backward_dev(f(dout), f(rows), inv, w, dr, dw, stream=st)
+        got.append((out.clone(), dx.clone(), dr.clone()))
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
 
 
 def test_non_finite_values(gpu_ctx):
