@@ -77,19 +77,20 @@ __global__ __launch_bounds__(256) void act_prep_kernel(LinAct a, uint16_t* __res
   if (lane == 0) xe[t] = e;
 }
 
-// The exponent of each weight row, from its scale | min words or its blocks' exponents.
+// The exponent of each weight row, from its scale | min words or its blocks' exponents.  64 rows a
+// workgroup, every fourth K tile a wave: the words of 128 experts of [1536, 2048], 50 MB, at once.
 __global__ __launch_bounds__(256) void row_exponents_kernel(const uint8_t* __restrict__ tiles, int fmt, int M, int K,
                                                             int16_t* __restrict__ out) {
-  const int row = blockIdx.x * 256 + threadIdx.x;
-  if (row >= M) return;
-  const int nkt = K / kTileCols;
+  __shared__ uint32_t part[4][64];
+  const int lane = threadIdx.x & 63, wave = wave_id(), nkt = K / kTileCols;
+  const size_t row = (size_t)blockIdx.x * kTileRows + lane;  // M % 64 == 0
   const bool b16 = fmt == RMOE_FMT_BFP16;
   const int tb = b16 ? kB16TileBytes : kTileBytes, at = b16 ? kB16MantBytes : kCodeBytes;
-  const uint8_t* q = tiles + (size_t)(row / kTileRows) * nkt * tb + at + (row % kTileRows) * 16;
+  const uint8_t* q = tiles + (size_t)blockIdx.x * nkt * tb + at + lane * 16;
   float mx = 0.f;
   uint32_t emax = 7u;
 #pragma unroll 4
-  for (int kt = 0; kt < nkt; ++kt) {
+  for (int kt = wave; kt < nkt; kt += 4) {
     const uint4 v = *reinterpret_cast<const uint4*>(q + (size_t)kt * tb);
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
@@ -103,6 +104,13 @@ __global__ __launch_bounds__(256) void row_exponents_kernel(const uint8_t* __res
       }
     }
   }
+  // The bits of positive floats are ordered as they are.
+  part[wave][lane] = b16 ? emax : __float_as_uint(mx);
+  __syncthreads();
+  if (wave) return;
+  const uint32_t m = max(max(part[0][lane], part[1][lane]), max(part[2][lane], part[3][lane]));
+  emax = m;
+  mx = __uint_as_float(m);
   // |m| <= 2^7 in bfp16
   out[row] = (int16_t)(b16 ? (int)emax - 133 + 7 - 10 : exponent_for(mx, 10));
 }
@@ -684,7 +692,7 @@ size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 }  // namespace
 
 hipError_t launch_row_exponents(const uint8_t* tiles, int fmt, int M, int K, int16_t* exps, hipStream_t st) {
-  hipLaunchKernelGGL(row_exponents_kernel, dim3((M + 255) / 256), dim3(256), 0, st, tiles, fmt, M, K, exps);
+  hipLaunchKernelGGL(row_exponents_kernel, dim3(M / kTileRows), dim3(256), 0, st, tiles, fmt, M, K, exps);
   return hipGetLastError();
 }
 

@@ -271,11 +271,12 @@ bool alloc_matrix(RmoeMatrix& m, size_t need) {
 hipError_t matrix_exponents(const RmoeMatrix& m, hipStream_t st) {
   return rmoe::launch_row_exponents(m.tiles, m.fmt, m.M, m.K, m.exps, st);
 }
-hipError_t gu_exponents(const RmoeLayer& L, size_t e, hipStream_t st) {
-  return rmoe::launch_row_exponents(L.gu + e * L.gu_bytes, RMOE_FMT_Q4NX, 2 * L.I, L.H, L.gu_exps + e * 2 * L.I, st);
+// The same of n experts from e on, whose tiles stand one behind the other.
+hipError_t gu_exponents(const RmoeLayer& L, size_t e, int n, hipStream_t st) {
+  return rmoe::launch_row_exponents(L.gu + e * L.gu_bytes, RMOE_FMT_Q4NX, n * 2 * L.I, L.H, L.gu_exps + e * 2 * L.I, st);
 }
-hipError_t dn_exponents(const RmoeLayer& L, size_t e, hipStream_t st) {
-  return rmoe::launch_row_exponents(L.dn + e * L.dn_bytes, L.dn_fmt, L.H, L.Ipad, L.dn_exps + e * L.H, st);
+hipError_t dn_exponents(const RmoeLayer& L, size_t e, int n, hipStream_t st) {
+  return rmoe::launch_row_exponents(L.dn + e * L.dn_bytes, L.dn_fmt, n * L.H, L.Ipad, L.dn_exps + e * L.H, st);
 }
 
 // Allocate the expert storage of L and register it as `layer` (replacing nothing:
@@ -934,15 +935,15 @@ int rmoe_layer_upload_d(rmoe_ctx* ctx, int layer, int bundle, int expert0, int n
                            ctx->stream));
     if (b1) {
       HIP_TRY(rmoe::launch_relayout_in(ctx->s.staging, base + e * per, 2 * L->I, L->H, ctx->stream));
-      HIP_TRY(gu_exponents(*L, e, ctx->stream));
     } else {
       HIP_TRY(rmoe::launch_b16_relayout_in(ctx->s.staging, base + e * per, L->H, L->Ipad, ctx->stream));
       HIP_TRY(rmoe::launch_b16_rowexp(base + e * per, L->H, L->Ipad, L->I, L->dn_rowexp + e * L->H, ctx->stream));
-      HIP_TRY(dn_exponents(*L, e, ctx->stream));
     }
     // The staging buffer is reused by the next expert: wait for the re-layout.
     HIP_TRY(hipStreamSynchronize(ctx->stream));
   }
+  HIP_TRY(b1 ? gu_exponents(*L, expert0, n, ctx->stream) : dn_exponents(*L, expert0, n, ctx->stream));
+  HIP_TRY(hipStreamSynchronize(ctx->stream));
   return RMOE_OK;
 }
 
@@ -1020,13 +1021,14 @@ int rmoe_layer_upload_experts(rmoe_ctx* ctx, int layer, const void* gate_up, siz
   for (size_t e = 0; e < ne; ++e) {
     HIP_TRY(hipMemcpyAsync(ctx->s.staging, (const uint8_t*)gate_up + e * L->gu_bytes, L->gu_bytes, hipMemcpyHostToDevice, ctx->stream));
     HIP_TRY(rmoe::launch_relayout_in(ctx->s.staging, L->gu + e * L->gu_bytes, 2 * L->I, L->H, ctx->stream));
-    HIP_TRY(gu_exponents(*L, e, ctx->stream));
     HIP_TRY(hipMemcpyAsync(ctx->s.staging, (const uint8_t*)down + e * L->dn_bytes, L->dn_bytes, hipMemcpyHostToDevice, ctx->stream));
     HIP_TRY(rmoe::launch_relayout_in(ctx->s.staging, L->dn + e * L->dn_bytes, L->H, L->Ipad, ctx->stream));
-    HIP_TRY(dn_exponents(*L, e, ctx->stream));
     // The staging buffer is reused by the next expert: wait for the re-layout.
     HIP_TRY(hipStreamSynchronize(ctx->stream));
   }
+  HIP_TRY(gu_exponents(*L, 0, (int)ne, ctx->stream));
+  HIP_TRY(dn_exponents(*L, 0, (int)ne, ctx->stream));
+  HIP_TRY(hipStreamSynchronize(ctx->stream));
   return RMOE_OK;
 }
 
@@ -1054,7 +1056,7 @@ int rmoe_layer_upload_expert_q4k(rmoe_ctx* ctx, int layer, int expert, int part,
   TRY(grow(ctx->s.staging, ctx->s.staging_bytes, need, ctx));
   HIP_TRY(hipMemcpyAsync(ctx->s.staging, bytes, need, hipMemcpyHostToDevice, ctx->stream));
   HIP_TRY(rmoe::launch_q4k_to_tiles(ctx->s.staging, M, K, dst, Kt, row0, ctx->stream));
-  HIP_TRY(part == RMOE_PART_DOWN ? dn_exponents(*L, expert, ctx->stream) : gu_exponents(*L, expert, ctx->stream));
+  HIP_TRY(part == RMOE_PART_DOWN ? dn_exponents(*L, expert, 1, ctx->stream) : gu_exponents(*L, expert, 1, ctx->stream));
   HIP_TRY(hipStreamSynchronize(ctx->stream));
   return RMOE_OK;
 }
@@ -1073,8 +1075,8 @@ int rmoe_layer_quantize_expert_dev(rmoe_ctx* ctx, int layer, int expert, const f
                                 ctx->s.err, st));
   HIP_TRY(rmoe::launch_quantize(down_dev, L->H, L->Ipad, L->I, L->I, L->dn + (size_t)expert * L->dn_bytes, ctx->s.err,
                                 st));
-  HIP_TRY(gu_exponents(*L, expert, st));
-  HIP_TRY(dn_exponents(*L, expert, st));
+  HIP_TRY(gu_exponents(*L, expert, 1, st));
+  HIP_TRY(dn_exponents(*L, expert, 1, st));
   return sync_and_check(ctx, st);
 }
 
@@ -1091,9 +1093,9 @@ int rmoe_layer_synthesize_dev(rmoe_ctx* ctx, int layer, uint64_t seed, float std
     const uint64_t s_dn = seed * 1000003ull + (uint64_t)e * 2ull + 2ull;
     HIP_TRY(rmoe::launch_synth_quantize(s_gu, std, 2 * L->I, L->H, L->H, L->gu + (size_t)e * L->gu_bytes, ctx->s.err, st));
     HIP_TRY(rmoe::launch_synth_quantize(s_dn, std, L->H, L->Ipad, L->I, L->dn + (size_t)e * L->dn_bytes, ctx->s.err, st));
-    HIP_TRY(gu_exponents(*L, e, st));
-    HIP_TRY(dn_exponents(*L, e, st));
   }
+  HIP_TRY(gu_exponents(*L, 0, ne, st));
+  HIP_TRY(dn_exponents(*L, 0, ne, st));
   return sync_and_check(ctx, st);
 }
 

@@ -644,3 +644,94 @@ def test_many_rows_narrower_than_the_matrix(gpu_ctx, fmt, T):
         ref, e = _reference(x, w[:, :K_in], None, "silu", None, True)
         _check(y, ref.cpu(), e.cpu(), K_in)
     mat.free()
+
+
+def test_layer_of_one_expert(gpu_ctx):
+    """One expert with all rows, some of them, or none: the tiles of one matrix, found from its offsets."""
+    H, I = 256, 192
+    g = MoeGeometry(hidden=H, inter=I, n_routed=1, n_shared=1, top_k=1)
+    lyr = gpu_ctx.create_layer(7302, g)
+    gu = [_weights("q4nx", 2 * I, H, s) for s in (1, 2)]
+    dn = [_weights("q4nx", H, 256, s, live=I)[0] for s in (3, 4)]
+    lyr.upload_experts(b"".join(b for b, _ in gu), b"".join(dn))
+    w = gu[0][1]
+    n = 128 * 64 + 77
+    lyr.reserve_experts_linear(n)
+    x = torch.randn(n, H, generator=torch.Generator().manual_seed(2)).to(torch.bfloat16)
+    for rows, first, last in ((n, 0, n), (n, 100, n - 900), (n, 5, 5), (9, 0, 9), (9, 3, 4)):
+        y = torch.full((rows, I), 9.0, dtype=torch.bfloat16, device="cuda")
+        lyr.experts_linear_dev("gate_up", x[:rows].cuda(), torch.tensor([first, last], dtype=torch.int32, device="cuda"), y,
+                               act="swiglu", stream=torch.cuda.current_stream())
+        if first < last:
+            _check(y[first:last], *_reference(x[first:last], w, None, "swiglu", None, rows > 9), (rows, first, last))
+        assert bool((y[:first] == 9).all()) and bool((y[last:] == 9).all())
+    lyr.free()
+
+
+def _agree(a, b):
+    """Two bf16 roundings of sums that differ by the weights' rounding to fp16: each rounding is uniform in half a step,
+    2^-8 / sqrt(3) of a value at most, the sums differ by 2^-11 / sqrt(3) of the terms' rms."""
+    a, b = a.double(), b.double()
+    return float((a - b).norm()) <= (2 ** 0.5 * 2.0 ** -8 + 2.0 ** -11) / 3 ** 0.5 * float(b.norm())
+
+
+def test_every_way_to_write_weights(gpu_ctx):
+    """Many rows, which use the exponents kept with the weights, against a few rows of the same weights, which do not:
+    layers synthesized, quantized on the device or from Q4_K, and matrices of every kind, views of experts included."""
+    st = torch.cuda.current_stream()
+    H, I, E, n = 512, 256, 3, 96
+    g = MoeGeometry(hidden=H, inter=I, n_routed=E, n_shared=1, top_k=1)
+    lyr = gpu_ctx.create_layer(7303, g)
+    lyr.reserve_experts_linear(n)
+    offsets = torch.tensor([0, 32, 64, 96], dtype=torch.int32, device="cuda")
+
+    def check_layer(what):
+        for part, M, K in (("gate_up", 2 * I, H), ("down", H, I)):
+            x = torch.randn(n, K, generator=torch.Generator().manual_seed(K)).to(torch.bfloat16).cuda()
+            y, few = (torch.zeros(n, M, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+            lyr.experts_linear_dev(part, x, offsets, y, stream=st)
+            for e in range(E):
+                view = lyr.expert_matrix(e, part)
+                view.reserve_act(32)
+                view.linear_act_dev(x[32 * e:32 * e + 32], 32, few[32 * e:32 * e + 32], stream=st)
+                big_n = 64 * (256 * 128 // M + 1)
+                view.reserve_act(big_n)
+                big = torch.zeros(big_n, M, dtype=torch.bfloat16, device="cuda")
+                view.linear_act_dev(x[32 * e:32 * e + 32].repeat(big_n // 32, 1).contiguous(), big_n, big, stream=st)
+                assert _agree(big[:32], few[32 * e:32 * e + 32]) and torch.equal(big[-32:], big[:32]), (what, part, e)
+                view.free()
+            assert bool(y.any()) and _agree(y, few), (what, part)
+
+    lyr.synthesize(3, std=0.5, stream=st)
+    check_layer("synthesized")
+    lyr.synthesize(4, std=2.0 ** -12)
+    check_layer("synthesized smaller")
+    for e in range(E):
+        lyr.quantize_expert(e, torch.randn(2 * I, H, device="cuda") * 2.0 ** (3 * e), torch.randn(H, I, device="cuda"))
+    check_layer("quantized")
+    rng = np.random.default_rng(5)
+
+    def q4k(rows, cols, d):  # random 144-byte super-blocks with sane scales
+        b = rng.integers(0, 256, (rows * cols // 256, 144), dtype=np.uint8)
+        b[:, :4] = np.frombuffer(np.array([d, d / 2], dtype=np.float16).tobytes(), dtype=np.uint8)
+        return b.tobytes()
+
+    for e in range(E):
+        lyr.upload_expert_q4k(e, "gate", q4k(I, H, 0.01 * 4 ** e))
+        lyr.upload_expert_q4k(e, "up", q4k(I, H, 0.3))
+        lyr.upload_expert_q4k(e, "down", q4k(H, I, 0.002))
+    check_layer("Q4_K")
+    lyr.free()
+    M, K = 512, 768
+    T = 64 * 65
+    x = torch.randn(T, K, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).cuda()
+    for mat in (gpu_ctx.quantize_matrix(torch.randn(M, K, device="cuda") * 300, M, K),
+                gpu_ctx.upload_matrix(_weights("q4nx", M, K, 1)[0], M, K),
+                gpu_ctx.upload_matrix(_weights("bfp16", M, K, 1, std=2.0 ** -30)[0], M, K, fmt="bfp16"),
+                gpu_ctx.upload_matrix(q4k(M, K, 0.02), M, K, fmt="q4k")):
+        mat.reserve_act(T)
+        y, few = torch.zeros(T, M, dtype=torch.bfloat16, device="cuda"), torch.zeros(32, M, dtype=torch.bfloat16, device="cuda")
+        mat.linear_act_dev(x, T, y, stream=st)
+        mat.linear_act_dev(x[:32], 32, few, stream=st)
+        assert bool(few.any()) and _agree(y[:32], few), mat.fmt
+        mat.free()
