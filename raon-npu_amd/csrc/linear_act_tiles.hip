@@ -4,9 +4,11 @@
 // Operands.  A row of x becomes fp16 times a power of two that brings its largest value into
 // [2^14, 2^15): bf16's 8 significant bits fit, values down to 2^-31 of the largest are exact.
 // A weight is formed in fp16 as its row's power of two brings the row's largest into
-// [2^10, 2^11): bfp16's m * 2^(e-133) exactly, q4nx's m + s * n by one fused multiply-add,
-// rounded once to fp16's 11 bits.  That rounding, at most 2^-11 of a weight (and 2^-35 of the
-// row's largest), adds to a sum what is an eighth of its bf16 rounding in the mean (rel-L2
+// [2^10, 2^11) or, q4nx, [2^14, 2^15): bfp16's m * 2^(e-133) exactly in blocks whose largest is
+// no less than 2^-27 of the row's, q4nx's m + s * n by one fused multiply-add, rounded once to
+// fp16's 11 bits, in groups whose scale is no less than 2^-27 of the row's largest (below, s and
+// s / 16 are subnormal and the weight is off by up to 2^-31 of it).  That rounding, at most 2^-11
+// of a weight, adds to a sum what is an eighth of its bf16 rounding in the mean (rel-L2
 // against 64 bits 1.65e-3 with and without it); keeping s * (n - 8) exact instead costs a
 // second product over the group sums of x (one MFMA in five) and their preparation.  Sums
 // are fp32; the powers of two are taken back exactly.
@@ -112,7 +114,7 @@ __global__ __launch_bounds__(256) void row_exponents_kernel(const uint8_t* __res
   emax = m;
   mx = __uint_as_float(m);
   // |m| <= 2^7 in bfp16
-  out[row] = (int16_t)(b16 ? (int)emax - 133 + 7 - 10 : exponent_for(mx, 10));
+  out[row] = (int16_t)(b16 ? (int)emax - 133 + 7 - 10 : exponent_for(mx, 14));
 }
 
 // ---------------------------------------------------------------------- tiles --

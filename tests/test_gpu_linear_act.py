@@ -2,8 +2,8 @@
 expert, against the dequantized weights in 64 bits.
 
 Bounds.  A sum over K products in fp32 is off by at most (K + 64) 2^-23 sum |x w|; the weights' rounding to fp16 in
-the kernel of many rows adds at most 2^-11 sum |x w| (and 2^-37 of the largest |x| and |w| times K for values at the
-end of fp16's range).  z = that + bias carries d; an activation with |f'| <= L passes L d on and adds 32 steps of
+the kernel of many rows adds at most 2^-11 sum |x w| (and K times 2^-30 of the largest |x| and |w| for values at the
+end of fp16's range: x is off by 2^-38 of its row's largest there, a q4nx weight by 2^-31).  z = that + bias carries d; an activation with |f'| <= L passes L d on and adds 32 steps of
 fp32; the sum with the residual and the rounding to bf16 add 2^-8 of the result."""
 
 from __future__ import annotations
@@ -47,7 +47,7 @@ def _reference(x, w, bias, act, residual, many):
     z = x @ w.t()
     d = (K + 64) * 2.0 ** -23 * absum
     if many:
-        d += 2.0 ** -11 * absum + K * 2.0 ** -37 * x.abs().amax(1, keepdim=True) * w.abs().amax(1)[None]
+        d += 2.0 ** -11 * absum + K * 2.0 ** -30 * x.abs().amax(1, keepdim=True) * w.abs().amax(1)[None]
     if bias is not None:
         z = z + bias.double()
         d = d + 2.0 ** -24 * z.abs()
@@ -735,3 +735,34 @@ def test_every_way_to_write_weights(gpu_ctx):
         mat.linear_act_dev(x[:32], 32, few, stream=st)
         assert bool(few.any()) and _agree(y[:32], few), mat.fmt
         mat.free()
+
+
+@pytest.mark.parametrize("fmt", ["q4nx", "bfp16"])
+def test_groups_of_very_different_sizes(gpu_ctx, fmt):
+    """Rows whose groups' weights differ by 2^20, met by tokens that are zero where the large ones are: the small ones
+    keep their precision, so that the bound is 2^-11 of the terms alone."""
+    M, K, T = 512, 512, 64 * 65
+    rng = np.random.default_rng(3)
+    w = rng.normal(0.0, 0.5, (M, K)).astype(np.float32)
+    scale = 2.0 ** -rng.integers(0, 21, (M, K // 32))
+    scale[:, 0] = 1.0
+    scale[:, 1:9] = 2.0 ** -20
+    w *= np.repeat(scale, 32, 1).astype(np.float32)
+    if fmt == "q4nx":
+        c, s, m = Q.quantize(w)
+        blob, wd = Q.pack_gemv(c, s, m), torch.from_numpy(Q.dequantize_simple(c, s, m)).double()
+    else:
+        blob = B.pack_gemv(w)
+        wd = torch.from_numpy(B.dequantize_packed(blob, K, M)).double()
+    mat = gpu_ctx.upload_matrix(blob, M, K, fmt=fmt)
+    mat.reserve_act(T)
+    x = torch.randn(T, K, generator=torch.Generator().manual_seed(4)).to(torch.bfloat16)
+    x[::2, :32] = 0
+    x[::2, 288:] = 0
+    y = torch.zeros(T, M, dtype=torch.bfloat16, device="cuda")
+    mat.linear_act_dev(x.cuda(), T, y, stream=torch.cuda.current_stream())
+    xd = x.double()
+    z, absum = xd @ wd.t(), xd.abs() @ wd.abs().t()
+    d = ((K + 64) * 2.0 ** -23 + 2.0 ** -11) * absum
+    _check(y, z, d, fmt)
+    mat.free()
