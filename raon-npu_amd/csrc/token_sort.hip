@@ -55,12 +55,20 @@ struct Elem<RMOE_DT_F32> {
   static __device__ __forceinline__ T put(float v) { return v; }
 };
 
+// Sorted rows of this many bytes and more are summed with non-temporal loads: they are read once
+// and do not fit the caches anyway (6,700 tokens alone, other buffers each time: 58 -> 49 us; the
+// combine's gradient gains nothing).  H 2,048, k 8, sort and combine in turn (the same buffers /
+// others each time): 220 MB of rows 92 / 100 us without the hint, 89 / 93 with it; 67 MB 35 / 36 and
+// 36 / 33; 34 MB 20 / 22 and 23 / 22.  (Storing them so makes the sort alone 60 -> 54 us and the two
+// 100 -> 113: what comes next finds less of them in the cache.)
+constexpr size_t kOnceBytes = (size_t)64 << 20;
+
 // N elements in one load: 16 bytes, or (N = 1) one element where rows are not 16-byte aligned.
 template <int DT, int N>
 struct Pack {
   typename Elem<DT>::T v[N];
 };
-template <int DT, int N>
+template <int DT, int N, bool kOnce = false>
 __device__ __forceinline__ Pack<DT, N> load_pack(const typename Elem<DT>::T* p) {
   if constexpr (N == 1) {
     Pack<DT, N> r;
@@ -68,7 +76,10 @@ __device__ __forceinline__ Pack<DT, N> load_pack(const typename Elem<DT>::T* p) 
     return r;
   } else {
     static_assert(sizeof(Pack<DT, N>) == 16, "16-byte packs");
-    return __builtin_bit_cast(Pack<DT, N>, *reinterpret_cast<const u32x4_t*>(p));
+    if constexpr (kOnce)
+      return __builtin_bit_cast(Pack<DT, N>, __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(p)));
+    else
+      return __builtin_bit_cast(Pack<DT, N>, *reinterpret_cast<const u32x4_t*>(p));
   }
 }
 template <int DT, int N>
@@ -430,7 +441,7 @@ struct SumArgs {
 
 // out[t] = sum over the token's rows in ascending position; one wave per (token, slab of 64 N
 // columns), up to kMaxRoutes / 2 row loads in flight.
-template <int DT, int N, bool kWeighted>
+template <int DT, int N, bool kWeighted, bool kOnce>
 __global__ __launch_bounds__(256) void sum_rows_kernel(SumArgs a) {
   typedef typename Elem<DT>::T E;
   const size_t id = (size_t)blockIdx.x * 4 + wave_id();
@@ -453,7 +464,7 @@ __global__ __launch_bounds__(256) void sum_rows_kernel(SumArgs a) {
         const int r = __ffsll((unsigned long long)__ballot(q.rank == s0 + s)) - 1;
         const int p = __builtin_amdgcn_readlane(q.pos, r);
         w[s] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(q.w), r));
-        if (in) v[s] = load_pack<DT, N>(static_cast<const E*>(a.rows) + (size_t)p * a.H + c);
+        if (in) v[s] = load_pack<DT, N, kOnce>(static_cast<const E*>(a.rows) + (size_t)p * a.H + c);
       }
     }
 #pragma unroll
@@ -584,13 +595,15 @@ template <int DT, int N>
 hipError_t sum_with(SumArgs a, hipStream_t st) {
   a.nslab = (a.H + 64 * N - 1) / (64 * N);
   const int total = a.T;
+  const bool once = (size_t)a.n * a.H * dtype_bytes(DT) >= kOnceBytes;
   const size_t step = std::max<size_t>(1, kMaxGroups * 4 / a.nslab);
   for (size_t t0 = 0; t0 < (size_t)total; t0 += step) {
     a.t0 = (int)t0;
     a.T = (int)std::min(step, (size_t)total - t0);
     const dim3 grid((unsigned)(((size_t)a.T * a.nslab + 3) / 4)), block(256);
-    if (a.wts) hipLaunchKernelGGL((sum_rows_kernel<DT, N, true>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((sum_rows_kernel<DT, N, false>), grid, block, 0, st, a);
+    auto* kernel = once ? (a.wts ? sum_rows_kernel<DT, N, true, N != 1> : sum_rows_kernel<DT, N, false, N != 1>)
+                        : (a.wts ? sum_rows_kernel<DT, N, true, false> : sum_rows_kernel<DT, N, false, false>);
+    hipLaunchKernelGGL(kernel, grid, block, 0, st, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }

@@ -371,3 +371,32 @@ def test_rows_past_4_gib(gpu_ctx):
     out = torch.zeros_like(x)
     gpu_ctx.combine_tokens_dev(rows, inv, torch.full((T, k), 0.25, device="cuda"), out, stream=st)
     assert torch.equal(out, x)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_rows_larger_than_the_caches(gpu_ctx, dtype):
+    """Rows of 64 MB and more are read with another hint: the same bits as in pieces that are not."""
+    T, k, E, H = 2200, 8, 32, 2056
+    g = torch.Generator().manual_seed(6)
+    ids = _ids(T, k, E, 6).cuda()
+    x = torch.randn(T, H, generator=g).to(dtype).cuda()
+    w = torch.rand(T, k, generator=g).cuda()
+    rows, order, inv, off = _buffers(T, k, E, H, dtype)
+    st = torch.cuda.current_stream()
+    gpu_ctx.sort_tokens_dev(x, ids, E, rows, order, inv, off, stream=st)
+    out, dx, dr, dw = torch.zeros_like(x), torch.zeros_like(x), torch.zeros_like(rows), torch.zeros_like(w)
+    gpu_ctx.combine_tokens_dev(rows, inv, w, out, stream=st)
+    gpu_ctx.sort_tokens_backward_dev(rows, inv, dx, stream=st)
+    gpu_ctx.combine_tokens_backward_dev(x, rows, inv, w, dr, dw, stream=st)
+    for t0 in (0, 1000, 2100):
+        n = 100
+        s = slice(t0, t0 + n)
+        part = _buffers(n, k, E, H, dtype)
+        gpu_ctx.sort_tokens_dev(x[s], ids[s], E, *part, stream=st)
+        o, d, r, q = torch.zeros_like(x[s]), torch.zeros_like(x[s]), torch.zeros_like(part[0]), torch.zeros_like(w[s])
+        gpu_ctx.combine_tokens_dev(part[0], part[2], w[s], o, stream=st)
+        gpu_ctx.sort_tokens_backward_dev(part[0], part[2], d, stream=st)
+        gpu_ctx.combine_tokens_backward_dev(x[s], part[0], part[2], w[s], r, q, stream=st)
+        assert torch.equal(o, out[s]) and torch.equal(d, dx[s]) and torch.equal(q, dw[s])
+        live = part[2] >= 0
+        assert torch.equal(r[part[2][live].long()], dr[inv[s][live].long()])
