@@ -5,6 +5,10 @@
 // One workgroup takes 16 MF rows x 16 NF weight rows (half of them gate, half up when the
 // activation is gated), its W waves a W-th of K each; the waves' sums meet in LDS and are
 // added in wave order, where bias, activation and residual cost nothing but their own bytes.
+// One row of q4nx [2048, 768] takes 4.4 us, the 8 experts of a token's gate/up (15.7 MB) 8.5; 445
+// rows of [1536, 2048] with SwiGLU 12.8 us (220 TFLOP/s), bound by the vector instructions around
+// the MFMAs (one FMA per group and output, the unpacking), which grow with the rows.  Eight
+// waves a tile 17.1, 32 x 64 tiles 14.3 (336 of them).
 // By expert, a workgroup finds its rows from the experts' offsets itself (a wave scan over at
 // most 256 experts), so that the offsets stay on the device.
 #include <algorithm>

@@ -12,6 +12,12 @@
 // against 64 bits 1.65e-3 with and without it); keeping s * (n - 8) exact instead costs a
 // second product over the group sums of x (one MFMA in five) and their preparation.  Sums
 // are fp32; the powers of two are taken back exactly.
+//
+// Bound by the matrix pipes and the vector instructions between them, which form the weights.
+// 53,600 rows of 128 experts' q4nx [1536, 2048], SwiGLU: 360 to 390 us (337 GFLOP, 870 to 940
+// TFLOP/s; torch's bf16 8192^3 reaches 1,210) behind 64 for the rows of x; 8,192 rows of
+// [8192, 4096] 575 us in all (957 TFLOP/s); 128 experts' bfp16 [2560, 1088] of 21 rows each 97 us,
+// in which 425 MB of weights stream at 4.7 TB/s.
 #include <algorithm>
 
 #include "linear_act.h"
@@ -39,8 +45,8 @@ __device__ __forceinline__ uint32_t bf16_pair_to_half(uint32_t v, int e) {
 }
 
 // Rows of x to fp16 (zero past K_in to the end of its pair of K tiles) and their exponents, one wave a row; clears the counters
-// of split tiles (256 at `arrived`, if any).  A copy's work: 53,600 rows of 2,048 take 90 us
-// (4.9 TB/s).
+// of split tiles (256 at `arrived`, if any).  A copy's work: 53,600 rows of 2,048 (440 MB) take 64
+// us where half of them are in the caches, 90 where not.
 __global__ __launch_bounds__(256) void act_prep_kernel(LinAct a, uint16_t* __restrict__ xh, int32_t* __restrict__ xe,
                                                        int* __restrict__ arrived) {
   if (arrived && blockIdx.x == 0) arrived[threadIdx.x] = 0;
