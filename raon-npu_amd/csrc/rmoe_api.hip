@@ -358,8 +358,9 @@ int check_overlap(std::initializer_list<Span> in, std::initializer_list<Span> ou
   return RMOE_OK;
 }
 
-// Token rows of the sort and combine calls.
-int check_tokens(rmoe_ctx* ctx, int dtype, int T, int H, int k, std::initializer_list<const void*> rows) {
+// Token rows of the sort and combine calls, and their int32 and fp32 operands.
+int check_tokens(rmoe_ctx* ctx, int dtype, int T, int H, int k, std::initializer_list<const void*> rows,
+                 std::initializer_list<const void*> words) {
   if (!ctx) return fail(RMOE_EINVAL, "null context");
   if (dtype != RMOE_DT_BF16 && dtype != RMOE_DT_F16 && dtype != RMOE_DT_F32)
     return fail(RMOE_EINVAL, "unknown element type %d", dtype);
@@ -370,6 +371,8 @@ int check_tokens(rmoe_ctx* ctx, int dtype, int T, int H, int k, std::initializer
   for (const void* p : rows)
     if (reinterpret_cast<uintptr_t>(p) % (dtype == RMOE_DT_F32 ? 4 : 2))
       return fail(RMOE_EINVAL, "rows must be aligned to their element type");
+  for (const void* p : words)
+    if (reinterpret_cast<uintptr_t>(p) % 4) return fail(RMOE_EINVAL, "int32 and fp32 operands must be aligned to 4 bytes");
   return RMOE_OK;
 }
 size_t row_bytes(int dtype, int H) { return (size_t)H * (dtype == RMOE_DT_F32 ? 4 : 2); }
@@ -513,7 +516,7 @@ int rmoe_destroy(rmoe_ctx* ctx) {
                   s.chunk_counts, s.staging, s.pf, s.stack, s.stack_cnt, s.act};
   for (void* b : bufs)
     if (b) hipFree(b);
-  for (uint8_t* b : s.act_before) hipFree(b);
+  for (int i = 0; i < s.n_act_before; ++i) hipFree(s.act_before[i]);
   auto it = g_io.find(ctx);
   if (it != g_io.end()) {
     hipFree(it->second.p);
@@ -748,7 +751,7 @@ static int reserve_act(rmoe_ctx* ctx, size_t bytes) {
   uint8_t* p = nullptr;
   size_t cap = 0;
   TRY(grow(p, cap, std::max(bytes, 2 * ctx->s.act_bytes), ctx));
-  if (ctx->s.act) ctx->s.act_before.push_back(ctx->s.act);
+  if (ctx->s.act) ctx->s.act_before[ctx->s.n_act_before++] = ctx->s.act;
   ctx->s.act = p;
   ctx->s.act_bytes = cap;
   return RMOE_OK;
@@ -810,7 +813,7 @@ int rmoe_reserve_experts_linear(rmoe_ctx* ctx, int layer, int n) {
 // ----------------------------------------------------------- tokens by expert --
 int rmoe_sort_tokens_dev(rmoe_ctx* ctx, const void* x, int dtype, int T, int H, const void* ids, int k, int n_experts,
                          void* rows, void* order, void* inv, void* offsets, void* stream) {
-  TRY(check_tokens(ctx, dtype, T, H, k, {x, rows}));
+  TRY(check_tokens(ctx, dtype, T, H, k, {x, rows}, {ids, order, inv, offsets}));
   if (!x || !ids || !rows || !order || !inv || !offsets) return fail(RMOE_EINVAL, "null argument");
   if (n_experts < 1 || n_experts > 256) return fail(RMOE_EINVAL, "n_experts (%d) must be in 1..256", n_experts);
   const size_t rb = row_bytes(dtype, H), A = (size_t)T * k;
@@ -825,7 +828,7 @@ int rmoe_sort_tokens_dev(rmoe_ctx* ctx, const void* x, int dtype, int T, int H, 
 
 int rmoe_sort_tokens_backward_dev(rmoe_ctx* ctx, const void* drows, int dtype, int T, int H, const void* inv, int k,
                                   void* dx, void* stream) {
-  TRY(check_tokens(ctx, dtype, T, H, k, {drows, dx}));
+  TRY(check_tokens(ctx, dtype, T, H, k, {drows, dx}, {inv}));
   if (!drows || !inv || !dx) return fail(RMOE_EINVAL, "null argument");
   const size_t rb = row_bytes(dtype, H), A = (size_t)T * k;
   TRY(check_overlap({{drows, A * rb}, {inv, A * 4}}, {{dx, T * rb}}));
@@ -838,7 +841,7 @@ int rmoe_sort_tokens_backward_dev(rmoe_ctx* ctx, const void* drows, int dtype, i
 
 int rmoe_combine_tokens_dev(rmoe_ctx* ctx, const void* rows, int dtype, int T, int H, const void* inv,
                             const void* weights, int k, void* out, void* stream) {
-  TRY(check_tokens(ctx, dtype, T, H, k, {rows, out}));
+  TRY(check_tokens(ctx, dtype, T, H, k, {rows, out}, {inv, weights}));
   if (!rows || !inv || !weights || !out) return fail(RMOE_EINVAL, "null argument");
   const size_t rb = row_bytes(dtype, H), A = (size_t)T * k;
   TRY(check_overlap({{rows, A * rb}, {inv, A * 4}, {weights, A * 4}}, {{out, T * rb}}));
@@ -852,7 +855,7 @@ int rmoe_combine_tokens_dev(rmoe_ctx* ctx, const void* rows, int dtype, int T, i
 int rmoe_combine_tokens_backward_dev(rmoe_ctx* ctx, const void* dout, const void* rows, int dtype, int T, int H,
                                      const void* inv, const void* weights, int k, void* drows, void* dweights,
                                      void* stream) {
-  TRY(check_tokens(ctx, dtype, T, H, k, {dout, rows, drows}));
+  TRY(check_tokens(ctx, dtype, T, H, k, {dout, rows, drows}, {inv, weights, dweights}));
   if (!dout || !rows || !inv || !weights || !drows || !dweights) return fail(RMOE_EINVAL, "null argument");
   const size_t rb = row_bytes(dtype, H), A = (size_t)T * k;
   TRY(check_overlap({{dout, T * rb}, {rows, A * rb}, {inv, A * 4}, {weights, A * 4}}, {{drows, A * rb}, {dweights, A * 4}}));

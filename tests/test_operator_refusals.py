@@ -141,6 +141,9 @@ BF16, F32 = _lib.DT_BF16, _lib.DT_F32
     ((P[0], BF16, 1 << 30, H, P[1], 2, E, P[2], P[3], P[4], P[5]), "too many"),
     ((P[0] + 1, BF16, T, H, P[1], k, E, P[2], P[3], P[4], P[5]), "aligned"),
     ((P[0] + 2, F32, T, H, P[1], k, E, P[2], P[3], P[4], P[5]), "aligned"),
+    ((P[0], BF16, T, H, P[1] + 2, k, E, P[2], P[3], P[4], P[5]), "aligned to 4"),
+    ((P[0], BF16, T, H, P[1], k, E, P[2], P[3] + 1, P[4], P[5]), "aligned to 4"),
+    ((P[0], BF16, T, H, P[1], k, E, P[2], P[3], P[4], P[5] + 2), "aligned to 4"),
     ((P[0], BF16, T, H, P[1], k, 0, P[2], P[3], P[4], P[5]), "n_experts"),
     ((P[0], BF16, T, H, P[1], k, 257, P[2], P[3], P[4], P[5]), "n_experts"),
     ((None, BF16, T, H, P[1], k, E, P[2], P[3], P[4], P[5]), "null"),
@@ -158,6 +161,9 @@ def test_sort_entry_point(raw, args, what):
     ("rmoe_sort_tokens_backward_dev", (P[0], BF16, T, H, P[1], k, P[0]), "overlaps"),
     ("rmoe_sort_tokens_backward_dev", (P[0], BF16, T, H, None, k, P[2]), "null"),
     ("rmoe_combine_tokens_dev", (P[0], BF16, T, H, P[1], None, k, P[2]), "null"),
+    ("rmoe_sort_tokens_backward_dev", (P[0], BF16, T, H, P[1] + 2, k, P[2]), "aligned to 4"),
+    ("rmoe_combine_tokens_dev", (P[0], BF16, T, H, P[1], P[3] + 2, k, P[2]), "aligned to 4"),
+    ("rmoe_combine_tokens_backward_dev", (P[0], P[1], BF16, T, H, P[2], P[3], k, P[4], P[5] + 2), "aligned to 4"),
     ("rmoe_combine_tokens_dev", (P[0], BF16, T, H, P[1], P[3], 17, P[2]), "k"),
     ("rmoe_combine_tokens_dev", (P[0], BF16, T, H, P[1], P[3], k, P[0] + 64), "overlaps"),
     ("rmoe_combine_tokens_backward_dev", (P[0], P[1], BF16, T, H, P[2], P[3], k, P[1], P[5]), "overlaps"),
