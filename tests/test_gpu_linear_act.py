@@ -766,3 +766,70 @@ def test_groups_of_very_different_sizes(gpu_ctx, fmt):
     d = ((K + 64) * 2.0 ** -23 + 2.0 ** -11) * absum
     _check(y, z, d, fmt)
     mat.free()
+
+
+@pytest.mark.parametrize("E", [255, 256])
+def test_the_most_experts(gpu_ctx, E):
+    """As many experts as the wave that finds a row's expert holds, the last with and without rows, few and many."""
+    H, I = 256, 64
+    g = MoeGeometry(hidden=H, inter=I, n_routed=E, n_shared=1, top_k=8)
+    lyr = gpu_ctx.create_layer(7304, g)
+    gu = [_weights("q4nx", 2 * I, H, s) for s in range(5)]
+    dn = [_weights("q4nx", H, 256, s, live=I) for s in range(5)]
+    lyr.upload_experts(b"".join(gu[e % 5][0] for e in range(E + 1)), b"".join(dn[e % 5][0] for e in range(E + 1)))
+    st = torch.cuda.current_stream()
+    rng = np.random.default_rng(E)
+    for counts in (np.eye(E, dtype=int)[E - 1], rng.integers(0, 2, E), rng.integers(0, 90, E), np.eye(E, dtype=int)[0] * 700,
+                   np.eye(E, dtype=int)[E - 1] * 700):
+        n = int(counts.sum())
+        lyr.reserve_experts_linear(n)
+        offsets = torch.tensor([0] + list(np.cumsum(counts)), dtype=torch.int32)
+        expert = torch.repeat_interleave(torch.arange(E), torch.from_numpy(counts))
+        for part, ws, M, K in (("gate_up", gu, 2 * I, H), ("down", dn, H, I)):
+            x = torch.randn(n, K, generator=torch.Generator().manual_seed(n + K)).to(torch.bfloat16)
+            y = torch.zeros(n, M, dtype=torch.bfloat16, device="cuda")
+            lyr.experts_linear_dev(part, x.cuda(), offsets.cuda(), y, stream=st)
+            for s in range(5):
+                rows = (expert % 5 == s).nonzero()[:, 0]
+                if len(rows):
+                    _check(y.cpu()[rows], *_reference(x[rows], ws[s][1][:, :K], None, "none", None, n >= E), (E, n, part, s))
+    lyr.free()
+
+
+def test_rows_past_4_gib(gpu_ctx):
+    """x, its fp16 form and (by expert) y of more than 4 GiB: rows on both sides of that offset, the first and the
+    last, against 64 bits."""
+    st = torch.cuda.current_stream()
+    K, T = 8192, 262144 + 77
+    blob, w = _weights("q4nx", 128, K, 13)
+    mat = gpu_ctx.upload_matrix(blob, 128, K)
+    mat.reserve_act(T)
+    x = torch.empty(T, K, dtype=torch.bfloat16, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(14)
+    for t0 in range(0, T, 65536):
+        rows = x[t0:t0 + 65536]
+        rows.copy_(torch.randn(rows.shape, device="cuda", generator=g))
+    y = torch.zeros(T, 128, dtype=torch.bfloat16, device="cuda")
+    mat.linear_act_dev(x, T, y, stream=st)
+    for s in (slice(0, 64), slice(262144 - 64, 262144 + 77)):
+        _check(y[s], *[t.cpu() for t in _reference(x[s], w.cuda(), None, "none", None, True)], s)
+    assert bool((y != 0).any(1).all())
+    mat.free()
+    del x, y
+    H, I, E, n = 256, 2048, 2, 2 ** 19 + 300  # y [n, 4096]
+    g = MoeGeometry(hidden=H, inter=I, n_routed=E, n_shared=1, top_k=1)
+    lyr = gpu_ctx.create_layer(7305, g)
+    lyr.synthesize(3)
+    lyr.reserve_experts_linear(n)
+    x = torch.empty(n, H, dtype=torch.bfloat16, device="cuda")
+    x.copy_(torch.randn(4096, H, generator=torch.Generator().manual_seed(1)).repeat(n // 4096 + 1, 1)[:n])
+    y = torch.zeros(n, 2 * I, dtype=torch.bfloat16, device="cuda")
+    # expert 1 begins before the 4 GiB of y and ends behind them
+    lyr.experts_linear_dev("gate_up", x, torch.tensor([0, n - 4096, n], dtype=torch.int32, device="cuda"), y, stream=st)
+    for e, rows in ((0, slice(2 ** 19 - 8192, 2 ** 19 - 8192 + 64)), (1, slice(n - 4096, n - 4000)), (1, slice(n - 64, n))):
+        view = lyr.expert_matrix(e, "gate_up")
+        few = torch.zeros(rows.stop - rows.start, 2 * I, dtype=torch.bfloat16, device="cuda")
+        view.linear_act_dev(x[rows], len(few), few, stream=st)
+        assert _agree(y[rows], few)
+        view.free()
+    lyr.free()
