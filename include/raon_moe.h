@@ -139,7 +139,8 @@ int rmoe_reserve_linear(rmoe_ctx* ctx, int handle, int T);
  * M' = M / 2, row i of W the gate and row M/2 + i the up of output i, bias added to both.  (rmoe_linear_dev followed by the
  * activation rounds gate and up to bf16 first; this call does not.)  Many rows are multiplied
  * in fp16 with a power of two per row of x and of W: a q4nx weight is rounded once to fp16's 11
- * bits, and values below about 2^-27 of their row's largest keep fewer.  Asynchronous on `stream`, never allocates; products of many
+ * bits, and values below about 2^-27 of their row's largest keep fewer.  A row's last bits may
+ * so depend on how many rows the call has (rmoe_linear_dev's do not).  Asynchronous on `stream`, never allocates; products of many
  * rows use context scratch, so that overlapping ones need a context each.  The reference adds bias, activation and residual on the host
  * (host/raon.py:1314-1330). */
 int rmoe_linear_act_dev(rmoe_ctx* ctx, int handle, const void* x_dev, int T, int K_in, const float* bias_dev, int act,
