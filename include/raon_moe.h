@@ -132,17 +132,18 @@ int rmoe_reserve_linear(rmoe_ctx* ctx, int handle, int T);
 
 /* Dense product with an epilogue, on device operands:
  *   y = RTNE(act(x W^T + bias) + residual),
- * fp32 throughout, rounded once.  x bf16 [T, K_in], K_in <= K a multiple of 8 (columns past
- * it are zero), 16-byte aligned; bias fp32 [M] or NULL; residual bf16 of y's shape or NULL (y
- * itself: added in place); y bf16 [T, M'].  act RMOE_ACT_NONE, _SILU, _GELU, _GELU_TANH:
+ * sums and epilogue in fp32, rounded once.  x bf16 [T, K_in], K_in <= K a multiple of 8 (columns
+ * past it are zero), 16-byte aligned; bias fp32 [M] or NULL; residual bf16 of y's shape or NULL
+ * (y itself: added in place); y bf16 [T, M'].  act RMOE_ACT_NONE, _SILU, _GELU, _GELU_TANH:
  * M' = M; RMOE_ACT_SWIGLU, _SITU (gate_beta, value_beta, 2^-100 to 2^100 in magnitude):
- * M' = M / 2, row i of W the gate and row M/2 + i the up of output i, bias added to both.  (rmoe_linear_dev followed by the
- * activation rounds gate and up to bf16 first; this call does not.)  Many rows are multiplied
- * in fp16 with a power of two per row of x and of W: a q4nx weight is rounded once to fp16's 11
- * bits, and values below about 2^-27 of their row's largest keep fewer.  A row's last bits may
- * so depend on how many rows the call has (rmoe_linear_dev's do not).  Asynchronous on `stream`, never allocates; products of many
- * rows use context scratch, so that overlapping ones need a context each.  The reference adds bias, activation and residual on the host
- * (host/raon.py:1314-1330). */
+ * M' = M / 2, row i of W the gate and row M/2 + i the up of output i, bias added to both.
+ * (rmoe_linear_dev followed by the activation rounds gate and up to bf16 first; this call does
+ * not.)  Many rows are multiplied in fp16 with a power of two per row of x and of W: a q4nx
+ * weight is rounded once to fp16's 11 bits, and values below about 2^-27 of their row's largest
+ * keep fewer.  A row's last bits may so depend on how many rows the call has (rmoe_linear_dev's
+ * do not).  Asynchronous on `stream`, never allocates; products of many rows use context
+ * scratch, so that overlapping ones need a context each.  The reference adds bias, activation
+ * and residual on the host (host/raon.py:1314-1330). */
 int rmoe_linear_act_dev(rmoe_ctx* ctx, int handle, const void* x_dev, int T, int K_in, const float* bias_dev, int act,
                         float gate_beta, float value_beta, const void* residual_dev, void* y_dev, void* stream);
 /* Size the scratch that rmoe_linear_act_dev needs for up to T tokens on this matrix.  Graphs
