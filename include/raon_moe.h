@@ -132,11 +132,13 @@ int rmoe_reserve_linear(rmoe_ctx* ctx, int handle, int T);
 
 /* Dense product with an epilogue, on device operands:
  *   y = RTNE(act(x W^T + bias) + residual),
- * sums and epilogue in fp32, rounded once.  x bf16 [T, K_in], K_in <= K a multiple of 8 (columns
- * past it are zero), 16-byte aligned; bias fp32 [M] or NULL; residual bf16 of y's shape or NULL
- * (y itself: added in place); y bf16 [T, M'].  act RMOE_ACT_NONE, _SILU, _GELU, _GELU_TANH:
- * M' = M; RMOE_ACT_SWIGLU, _SITU (gate_beta, value_beta, 2^-100 to 2^100 in magnitude):
- * M' = M / 2, row i of W the gate and row M/2 + i the up of output i, bias added to both.
+ * sums and epilogue in fp32, rounded once.  x bf16 [T, K_in], K_in <= K a multiple of 8, 16-byte
+ * aligned; W's columns past K_in take no part, whatever they hold, nor do those past I of an
+ * expert's down, which are padding (x's columns there count for nothing).  bias fp32 [M] or NULL;
+ * residual bf16 of y's shape or NULL (y itself: added in place); y bf16 [T, M'].  act
+ * RMOE_ACT_NONE, _SILU, _GELU, _GELU_TANH: M' = M; RMOE_ACT_SWIGLU, _SITU (gate_beta, value_beta,
+ * 2^-100 to 2^100 in magnitude): M' = M / 2, row i of W the gate and row M/2 + i the up of output
+ * i, bias added to both.
  * (rmoe_linear_dev followed by the activation rounds gate and up to bf16 first; this call does
  * not.)  Many rows are multiplied in fp16 with a power of two per row of x and of W: a q4nx
  * weight is rounded once to fp16's 11 bits, and values below about 2^-27 of their row's largest
@@ -358,8 +360,8 @@ int rmoe_dispatch(rmoe_ctx* ctx, const int32_t* top_ids, int T, int k, int n_exp
 /* rmoe_linear_act_dev over sorted rows, each row with the matrix of its expert: for e in
  * 0..n_routed-1 and offsets[e] <= p < offsets[e+1] (rmoe_sort_tokens_dev's offsets)
  *   y[p] = RTNE(act(rows[p] W_e^T + bias[e]) + residual[p]).
- * part RMOE_PART_GATE_UP: W_e [2I, H]; RMOE_PART_DOWN: W_e [H, Ipad], of which K_in = I columns
- * (or up to Ipad) are read.  rows bf16 [n, K_in], 16-byte aligned, K_in a multiple of 8; bias
+ * part RMOE_PART_GATE_UP: W_e [2I, H]; RMOE_PART_DOWN: W_e [H, I], rows of K_in = I columns or
+ * more, up to Ipad: what they and the padded weights hold past I takes no part.  rows bf16 [n, K_in], 16-byte aligned, K_in a multiple of 8; bias
  * fp32 [n_routed, M] or NULL; residual and y bf16 [n, M'].  Rows from offsets[n_routed] on
  * stay as they were.  Both layer layouts (q4nx and weights-d) are served. */
 int rmoe_experts_linear_dev(rmoe_ctx* ctx, int layer, int part, const void* rows_dev, int n, int K_in,

@@ -57,12 +57,12 @@ __global__ __launch_bounds__(512) void linear_act_kernel(LinAct a, int n_nt) {
     o.w[f] = tiles + (size_t)(row / kTileRows) * nkt * kTB + (row % kTileRows) * 16;
   }
   // Rows past the tile repeat its last one; their results are not stored.
-  o.x = reinterpret_cast<const uint8_t*>(a.x + (size_t)row0 * a.K_in);
+  o.x = reinterpret_cast<const uint8_t*>(a.x + (size_t)row0 * a.ldx);
 #pragma unroll
   for (int m = 0; m < MF; ++m)
 #pragma unroll
     for (int i = 0; i < XI; ++i)
-      o.xoff[m][i] = (uint32_t)min(16 * m + 4 * i + lq, nrow - 1) * (uint32_t)(2 * a.K_in) + 16u * (uint32_t)l16;
+      o.xoff[m][i] = (uint32_t)min(16 * m + 4 * i + lq, nrow - 1) * (uint32_t)(2 * a.ldx) + 16u * (uint32_t)l16;
   o.xchunks = (uint32_t)a.K_in / 8u;
   o.lds = reinterpret_cast<uint8_t*>(la_lds) + (size_t)wave * 4096 * MF;
   wg_f32x4 acc[MF][NF];

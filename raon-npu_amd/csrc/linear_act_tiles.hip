@@ -53,7 +53,7 @@ __global__ __launch_bounds__(256) void act_prep_kernel(LinAct a, uint16_t* __res
   const int lane = threadIdx.x & 63, wave = wave_id();
   const size_t t = (size_t)blockIdx.x * 4 + wave;
   if (t >= (size_t)a.n) return;
-  const uint4* src = reinterpret_cast<const uint4*>(a.x + t * a.K_in);
+  const uint4* src = reinterpret_cast<const uint4*>(a.x + t * a.ldx);
   uint4* dst = reinterpret_cast<uint4*>(xh + t * a.K);
   const int nch = a.K_in / 8, nout = (a.K_in + 2 * kTileCols - 1) / (2 * kTileCols) * (2 * kTileCols / 8);
   constexpr int kKeep = 5;  // 16-byte chunks a lane keeps between the two passes (2,560 columns)
@@ -85,28 +85,32 @@ __global__ __launch_bounds__(256) void act_prep_kernel(LinAct a, uint16_t* __res
   if (lane == 0) xe[t] = e;
 }
 
-// The exponent of each weight row, from its scale | min words or its blocks' exponents.  64 rows a
+// The exponent of each weight row, from the scale | min words or block exponents of its first
+// K_live columns: those behind do not count (a down's padding, whose bytes may be anything).  64 rows a
 // workgroup, every fourth K tile a wave: the words of 128 experts of [1536, 2048], 50 MB, at once.
 __global__ __launch_bounds__(256) void row_exponents_kernel(const uint8_t* __restrict__ tiles, int fmt, int M, int K,
-                                                            int16_t* __restrict__ out) {
+                                                            int K_live, int16_t* __restrict__ out) {
   __shared__ uint32_t part[4][64];
   const int lane = threadIdx.x & 63, wave = wave_id(), nkt = K / kTileCols;
   const size_t row = (size_t)blockIdx.x * kTileRows + lane;  // M % 64 == 0
   const bool b16 = fmt == RMOE_FMT_BFP16;
   const int tb = b16 ? kB16TileBytes : kTileBytes, at = b16 ? kB16MantBytes : kCodeBytes;
+  const int per = b16 ? 16 : 4, unit = b16 ? 8 : 32, nlive = (K_live + unit - 1) / unit;  // a tile's blocks or groups
+  const int nkt_live = (K_live + kTileCols - 1) / kTileCols;
   const uint8_t* q = tiles + (size_t)blockIdx.x * nkt * tb + at + lane * 16;
   float mx = 0.f;
   uint32_t emax = 7u;
 #pragma unroll 4
-  for (int kt = wave; kt < nkt; kt += 4) {
+  for (int kt = wave; kt < nkt_live; kt += 4) {
     const uint4 v = *reinterpret_cast<const uint4*>(q + (size_t)kt * tb);
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       if (b16) {
 #pragma unroll
-        for (int b = 0; b < 4; ++b) emax = max(emax, (w[i] >> (8 * b)) & 0xffu);
-      } else {
+        for (int b = 0; b < 4; ++b)
+          if (per * kt + 4 * i + b < nlive) emax = max(emax, (w[i] >> (8 * b)) & 0xffu);
+      } else if (per * kt + i < nlive) {
         const float s = __uint_as_float(w[i] << 16), m = __uint_as_float(w[i] & 0xffff0000u);
         mx = fmaxf(mx, fmaxf(fabsf(m), fabsf(fmaf(15.f, s, m))));
       }
@@ -199,15 +203,17 @@ __device__ __forceinline__ void swap16(uint32_t& a, uint32_t& b) {
 }
 
 // q4nx: the scale | min words of a K tile in the wave's LDS, brought to the row's power of two
-// and to fp16 once for all that read them (lane = weight row; four words).
-__device__ __forceinline__ void convert_words(uint8_t* wp, int we) {
+// and to fp16 once for all that read them (lane = weight row; four words, the first `live` of
+// them: the words behind x's columns meet zeros, and are taken as zero, since they may be anything).
+__device__ __forceinline__ void convert_words(uint8_t* wp, int we, int live) {
   uint4* p = reinterpret_cast<uint4*>(wp) + (threadIdx.x & 63u);
   uint4 v = *p;
-  auto half = [&](uint32_t w) {
-    return half_pair(__builtin_amdgcn_ldexpf(__uint_as_float(w << 16), -we),
-                     __builtin_amdgcn_ldexpf(__uint_as_float(w & 0xffff0000u), -we));
+  auto half = [&](uint32_t w, int i) {
+    const uint32_t h = half_pair(__builtin_amdgcn_ldexpf(__uint_as_float(w << 16), -we),
+                                 __builtin_amdgcn_ldexpf(__uint_as_float(w & 0xffff0000u), -we));
+    return i < live ? h : 0u;
   };
-  *p = make_uint4(half(v.x), half(v.y), half(v.z), half(v.w));
+  *p = make_uint4(half(v.x, 0), half(v.y, 1), half(v.z, 2), half(v.w, 3));
 }
 
 // What a wave keeps of a stage's weights while it forms MFMA operands from them: 64 columns
@@ -269,7 +275,9 @@ struct StageWeights<RMOE_FMT_BFP16, NF> {
   __device__ __forceinline__ void arrange() {}
   __device__ __forceinline__ void form(int g, int f, int part, const int (&we)[NF], const CodeMasks&, uint4& b) const {
     const uint32_t lq = (threadIdx.x & 63u) >> 4;
-    const int e = (int)max((ex[f] >> (16u * (lq & 1u) + 8u * g)) & 0xffu, 7u) - 133 - we[f];
+    // No more than the row's own shift, 10 - 7: blocks behind x's columns may hold any exponent, and
+    // their weights, which meet zeros, stay finite.
+    const int e = min((int)max((ex[f] >> (16u * (lq & 1u) + 8u * g)) & 0xffu, 7u) - 133 - we[f], 3);
     const float s = __builtin_amdgcn_ldexpf(1.f, e);
     const uint32_t w = g ? (part ? v[f].w : v[f].z) : (part ? v[f].y : v[f].x);
     const uint2 r = b16_operand_half(w, as_f16x2(half_pair(s, s)));
@@ -404,7 +412,8 @@ __device__ __forceinline__ void tile_product(const TileArgs& t, const uint8_t* w
 #pragma unroll
   for (int s = 0; s < R; ++s) load_weights(s, (uint32_t)(s * 1024 * kBlocks));
   copies_landed<0>();
-  if constexpr (kFmt == RMOE_FMT_Q4NX) convert_words(lds + pbase, we_lane);
+  const int groups = (t.a.K_in + 31) / 32 - 4 * kt0;  // that x's columns reach, from this slice's first on
+  if constexpr (kFmt == RMOE_FMT_Q4NX) convert_words(lds + pbase, we_lane, groups);
   StageWeights<kFmt, NF> cur, next;
   uint4 b0[NF];
   cur.read(lds + wbase, lds + pbase, 0);
@@ -439,7 +448,8 @@ __device__ __forceinline__ void tile_product(const TileArgs& t, const uint8_t* w
         lds + here, b0, next, cur, we, masks, acc,
         [&](int i) {
           // The next tile's words have landed (past the last tile the operands are not used).
-          if (kFmt == RMOE_FMT_Q4NX && i == 0) convert_words(lds + pbase + 1024 * ((kt + 1) & 1), we_lane);
+          if (kFmt == RMOE_FMT_Q4NX && i == 0)
+            convert_words(lds + pbase + 1024 * ((kt + 1) & 1), we_lane, groups - 4 * (kt + 1));
           copies(i, s + 1 + kAhead, s + 2 + R, kBlocks + 1 - R % 2, there, ws);
         },
         [&] { cur.read(lds + wbase + ws, wp_next, 0); });
@@ -699,8 +709,8 @@ size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 
 }  // namespace
 
-hipError_t launch_row_exponents(const uint8_t* tiles, int fmt, int M, int K, int16_t* exps, hipStream_t st) {
-  hipLaunchKernelGGL(row_exponents_kernel, dim3(M / kTileRows), dim3(256), 0, st, tiles, fmt, M, K, exps);
+hipError_t launch_row_exponents(const uint8_t* tiles, int fmt, int M, int K, int K_live, int16_t* exps, hipStream_t st) {
+  hipLaunchKernelGGL(row_exponents_kernel, dim3(M / kTileRows), dim3(256), 0, st, tiles, fmt, M, K, K_live, exps);
   return hipGetLastError();
 }
 
@@ -718,7 +728,8 @@ bool act_tiles_serve(int fmt, int M, int K, int groups, size_t n) {
 size_t act_tiles_scratch(int fmt, int M, int K, int groups, size_t n) {
   if (!act_tiles_serve(fmt, M, K, groups, n)) return 0;
   const bool tail = groups == 1 && large_tiles(M, n) >= kCus;
-  return round256((n + kActBM) * K * 2) + round256(n * 4) + (tail ? kTailBytes + kCus * 4 : 0);
+  return round256((n + kActBM) * K * 2) + round256(n * 4) + (size_t)groups * M * sizeof(int16_t) +
+         (tail ? kTailBytes + kCus * 4 : 0);
 }
 
 hipError_t launch_act_tiles(const LinAct& a, uint8_t* scratch, size_t bytes, hipStream_t st) {
@@ -728,10 +739,21 @@ hipError_t launch_act_tiles(const LinAct& a, uint8_t* scratch, size_t bytes, hip
   uint16_t* xh = reinterpret_cast<uint16_t*>(scratch);
   int32_t* xe = reinterpret_cast<int32_t*>(scratch + round256(((size_t)a.n + kActBM) * a.K * 2));
   TileArgs t{a, xh, xe, 0, 0, 1, nullptr, nullptr};
+  uint8_t* next = reinterpret_cast<uint8_t*>(xe) + round256((size_t)a.n * 4);
+  // Narrower x: the kept exponents count weights that take no part, which may be of any size.  Those
+  // of the columns that do are taken for this call.
+  const int unit = a.fmt == RMOE_FMT_BFP16 ? 8 : 32, rows = (a.offsets ? a.n_experts : 1) * a.M;
+  if ((a.K_in + unit - 1) / unit != (a.live + unit - 1) / unit) {
+    int16_t* exps = reinterpret_cast<int16_t*>(next);
+    t.a.exps = exps;
+    const hipError_t e = launch_row_exponents(a.tiles, a.fmt, rows, a.K, a.K_in, exps, st);
+    if (e != hipSuccess) return e;
+  }
+  next += (size_t)rows * sizeof(int16_t);  // M is a multiple of 128
   const size_t tiles = large_tiles(a.M, a.n);
   if (!a.offsets && (t.slices = (int)split_tail(tiles, a.K_in)) > 1) {
     t.n_whole = (int)(tiles / kCus * kCus);
-    t.part = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(xe) + round256((size_t)a.n * 4));
+    t.part = reinterpret_cast<uint64_t*>(next);
     t.arrived = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(t.part) + kTailBytes);
   }
   hipLaunchKernelGGL(act_prep_kernel, dim3((unsigned)groups), dim3(256), 0, st, a, xh, xe, t.arrived);

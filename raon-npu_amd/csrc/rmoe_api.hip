@@ -265,18 +265,20 @@ int sync_and_check(rmoe_ctx* ctx, hipStream_t st) {
 bool alloc_matrix(RmoeMatrix& m, size_t need) {
   if (hipMalloc((void**)&m.tiles, need + (size_t)m.M * sizeof(int16_t)) != hipSuccess) return false;
   m.exps = reinterpret_cast<int16_t*>(m.tiles + need);
+  m.live = m.K;
   return true;
 }
 // The exponents of freshly written weights (queued behind them).
 hipError_t matrix_exponents(const RmoeMatrix& m, hipStream_t st) {
-  return rmoe::launch_row_exponents(m.tiles, m.fmt, m.M, m.K, m.exps, st);
+  return rmoe::launch_row_exponents(m.tiles, m.fmt, m.M, m.K, m.live, m.exps, st);
 }
 // The same of n experts from e on, whose tiles stand one behind the other.
 hipError_t gu_exponents(const RmoeLayer& L, size_t e, int n, hipStream_t st) {
-  return rmoe::launch_row_exponents(L.gu + e * L.gu_bytes, RMOE_FMT_Q4NX, n * 2 * L.I, L.H, L.gu_exps + e * 2 * L.I, st);
+  return rmoe::launch_row_exponents(L.gu + e * L.gu_bytes, RMOE_FMT_Q4NX, n * 2 * L.I, L.H, L.H, L.gu_exps + e * 2 * L.I,
+                                    st);
 }
 hipError_t dn_exponents(const RmoeLayer& L, size_t e, int n, hipStream_t st) {
-  return rmoe::launch_row_exponents(L.dn + e * L.dn_bytes, L.dn_fmt, n * L.H, L.Ipad, L.dn_exps + e * L.H, st);
+  return rmoe::launch_row_exponents(L.dn + e * L.dn_bytes, L.dn_fmt, n * L.H, L.Ipad, L.I, L.dn_exps + e * L.H, st);
 }
 
 // Allocate the expert storage of L and register it as `layer` (replacing nothing:
@@ -382,8 +384,8 @@ int check_linear_act(const rmoe::LinAct& L) {
   if (!L.x || !L.y) return fail(RMOE_EINVAL, "null argument");
   if (L.n < 1) return fail(RMOE_EINVAL, "the number of rows must be >= 1");
   if (L.act < RMOE_ACT_SITU || L.act > RMOE_ACT_GELU_TANH) return fail(RMOE_EINVAL, "unknown activation %d", L.act);
-  if (L.K_in < 8 || L.K_in > L.K || L.K_in % 8)
-    return fail(RMOE_EINVAL, "input width %d must be a multiple of 8 and at most K=%d", L.K_in, L.K);
+  if (L.ldx < 8 || L.ldx > L.K || L.ldx % 8)
+    return fail(RMOE_EINVAL, "input width %d must be a multiple of 8 and at most K=%d", L.ldx, L.K);
   for (float b : {L.gb, L.vb})
     if (L.act == RMOE_ACT_SITU && !(fabsf(b) >= 0x1p-100f && fabsf(b) <= 0x1p100f))
       return fail(RMOE_EINVAL, "SiTU betas must be between 2^-100 and 2^100 in magnitude");
@@ -396,7 +398,7 @@ int check_linear_act(const rmoe::LinAct& L) {
   // The residual may be y itself (each element is read before it is written), not a part of it.
   const Span res{L.residual == L.y ? nullptr : L.residual, y.n};
   const size_t groups = L.offsets ? L.n_experts : 1;
-  return check_overlap({{L.x, (size_t)L.n * L.K_in * 2}, res, {L.bias, groups * L.M * 4},
+  return check_overlap({{L.x, (size_t)L.n * L.ldx * 2}, res, {L.bias, groups * L.M * 4},
                         {L.offsets, (size_t)(L.n_experts + 1) * 4}}, {y});
 }
 
@@ -765,7 +767,7 @@ static int run_linear_act(rmoe_ctx* ctx, const rmoe::LinAct& L, void* stream) {
   if (e == hipErrorOutOfMemory)
     return fail(RMOE_EINVAL, "scratch too small for %d rows: call %s first", L.n,
                 L.offsets ? "rmoe_reserve_experts_linear" : "rmoe_reserve_linear_act");
-  if (e == hipErrorInvalidValue) return fail(RMOE_EINVAL, "%d rows of width %d are too many for one call", L.n, L.K_in);
+  if (e == hipErrorInvalidValue) return fail(RMOE_EINVAL, "%d rows of width %d are too many for one call", L.n, L.ldx);
   HIP_TRY(e);
   return RMOE_OK;
 }
@@ -774,8 +776,8 @@ int rmoe_linear_act_dev(rmoe_ctx* ctx, int handle, const void* x_dev, int T, int
                         float gate_beta, float value_beta, const void* residual_dev, void* y_dev, void* stream) {
   RmoeMatrix* m;
   TRY(find_matrix(ctx, handle, &m));
-  const rmoe::LinAct L{m->tiles, m->exps, 0, m->fmt, m->M, m->K, (const uint16_t*)x_dev, T, K_in, nullptr, 0, bias_dev, act,
-                       gate_beta, value_beta, (const uint16_t*)residual_dev, (uint16_t*)y_dev};
+  const rmoe::LinAct L{m->tiles, m->exps, 0, m->fmt, m->M, m->K, m->live, (const uint16_t*)x_dev, T, K_in,
+                       std::min(K_in, m->live), nullptr, 0, bias_dev, act, gate_beta, value_beta, (const uint16_t*)residual_dev, (uint16_t*)y_dev};
   return run_linear_act(ctx, L, stream);
 }
 
@@ -795,9 +797,10 @@ int rmoe_experts_linear_dev(rmoe_ctx* ctx, int layer, int part, const void* rows
     return fail(RMOE_EINVAL, "part must be RMOE_PART_GATE_UP or RMOE_PART_DOWN, got %d", part);
   if (!offsets_dev) return fail(RMOE_EINVAL, "null argument");
   const bool up = part == RMOE_PART_GATE_UP;
+  const int live = up ? l->H : l->I;
   const rmoe::LinAct L{up ? l->gu : l->dn, up ? l->gu_exps : l->dn_exps, up ? l->gu_bytes : l->dn_bytes, up ? RMOE_FMT_Q4NX : l->dn_fmt,
-                       up ? 2 * l->I : l->H, up ? l->H : l->Ipad, (const uint16_t*)rows_dev, n, K_in,
-                       (const int32_t*)offsets_dev, l->n_routed, bias_dev, act, gate_beta, value_beta,
+                       up ? 2 * l->I : l->H, up ? l->H : l->Ipad, live, (const uint16_t*)rows_dev, n, K_in,
+                       std::min(K_in, live), (const int32_t*)offsets_dev, l->n_routed, bias_dev, act, gate_beta, value_beta,
                        (const uint16_t*)residual_dev, (uint16_t*)y_dev};
   return run_linear_act(ctx, L, stream);
 }
@@ -981,7 +984,7 @@ int rmoe_layer_expert_matrix(rmoe_ctx* ctx, int layer, int expert, int part, int
     m.tiles = L->gu + (size_t)expert * L->gu_bytes;
     m.exps = L->gu_exps + (size_t)expert * 2 * L->I;
     m.M = 2 * L->I;
-    m.K = L->H;
+    m.K = m.live = L->H;
     m.fmt = RMOE_FMT_Q4NX;
   } else if (part == RMOE_PART_DOWN) {
     if (expert < 0 || expert >= L->dn_experts)
@@ -990,6 +993,7 @@ int rmoe_layer_expert_matrix(rmoe_ctx* ctx, int layer, int expert, int part, int
     m.exps = L->dn_exps + (size_t)expert * L->H;
     m.M = L->H;
     m.K = L->Ipad;
+    m.live = L->I;
     m.fmt = L->dn_fmt;
   } else {
     return fail(RMOE_EINVAL, "part must be RMOE_PART_GATE_UP or RMOE_PART_DOWN, got %d", part);

@@ -343,7 +343,8 @@ struct RmoeMatrix {
   uint8_t* tiles = nullptr;  // device, tile layout of the format
   int M = 0, K = 0;
   int fmt = 0;               // RMOE_FMT_Q4NX or RMOE_FMT_BFP16
-  int16_t* exps = nullptr;   // [M] exponents of the rows, in the tiles' allocation
+  int16_t* exps = nullptr;   // [M] exponents of the rows' first `live` columns, in the tiles' allocation
+  int live = 0;              // columns that are weights: K, or I of a down view (those behind are padding)
   // A view (rmoe_layer_expert_matrix) borrows the tiles of one expert of this layer and
   // owns no memory; -1 for a matrix that owns its tiles.
   int view_of_layer = -1;
@@ -362,8 +363,8 @@ struct RmoeLayer {
   int dn_fmt = 0;                     // RMOE_FMT_Q4NX or RMOE_FMT_BFP16
   uint8_t* gu = nullptr;              // gu_experts experts, tile layout
   uint8_t* dn = nullptr;              // dn_experts experts, tile layout of dn_fmt
-  // Exponents of the weight rows ([gu_experts][2I], [dn_experts][H]), in gu's and dn's
-  // allocations.
+  // Exponents of the weight rows ([gu_experts][2I], [dn_experts][H]; down: of the first I
+  // columns), in gu's and dn's allocations.
   int16_t *gu_exps = nullptr, *dn_exps = nullptr;
   // bfp16 down only: per expert and row, the largest max(e, 7) over the blocks of the
   // first I columns ([dn_experts][H]; filled on upload).
@@ -539,11 +540,12 @@ hipError_t launch_combine_grad(const void* dout, const void* rows, int dtype, in
 // and M biases apart.
 struct LinAct {
   const uint8_t* tiles;
-  const int16_t* exps;  // of the weight rows (launch_row_exponents), M apart by expert
+  const int16_t* exps;  // of the weight rows' first `live` columns (launch_row_exponents), M apart by expert
   size_t wstride;
-  int fmt, M, K;
-  const uint16_t* x;  // [n, K_in], 16-byte aligned, K_in % 8 == 0; weights past K_in see zeros
-  int n, K_in;        // (their K tiles are not read)
+  int fmt, M, K, live;  // columns from `live` on are padding of any bytes
+  const uint16_t* x;    // [n, ldx], 16-byte aligned, ldx % 8 == 0
+  int n, ldx, K_in;     // columns of x that are multiplied, K_in <= live, K_in % 8 == 0; weights past
+                        // them take no part, whatever they hold
   const int32_t* offsets;
   int n_experts;
   const float* bias;
@@ -559,9 +561,10 @@ hipError_t launch_linear_act(const LinAct& a, uint8_t* scratch, size_t bytes, hi
 // scratch that takes (0 if it does not).
 bool act_tiles_serve(int fmt, int M, int K, int groups, size_t n);
 size_t act_tiles_scratch(int fmt, int M, int K, int groups, size_t n);
-// The power of two of each weight row of a matrix that the kernel of many rows divides it by:
-// taken whenever the weights are written, and kept behind them.
-hipError_t launch_row_exponents(const uint8_t* tiles, int fmt, int M, int K, int16_t* exps, hipStream_t st);
+// The power of two of each weight row of a matrix that the kernel of many rows divides it by,
+// from the row's first K_live columns: taken whenever the weights are written, and kept behind
+// them.  M: the rows of all matrices that stand one behind the other.
+hipError_t launch_row_exponents(const uint8_t* tiles, int fmt, int M, int K, int K_live, int16_t* exps, hipStream_t st);
 hipError_t launch_act_tiles(const LinAct& a, uint8_t* scratch, size_t bytes, hipStream_t st);
 
 // Persistent decode of n_layers (<= kMaxStack) layers of one geometry for one token

@@ -59,8 +59,10 @@ __device__ __forceinline__ uint4 q4_pairs(uint32_t v, const Q4Masks& k) {
 // What a wave multiplies.  Lane (l16, lq) = (lane % 16, lane / 16).
 // XI: how many of a fragment's four row quartets are loaded (1 when at most 4 rows live; the
 // rows that are not loaded hold arbitrary values, which reach only their own results).
-// kTail: the activation rows end at column 8 xchunks, short of K; the columns past it are
-// taken as zero and not read.
+// kTail: the activation rows end at column 8 xchunks, inside a K tile; the columns past it are
+// taken as zero and not read.  Weights there take no part, whatever they hold: q4nx's words of
+// the groups behind are taken as zero too (an infinite scale would make 0 * inf of their sums);
+// bfp16's 2^(e - 133) is finite at every e.
 template <int MF, int NF, int XI, bool kTail = false>
 struct WaveOperands {
   const uint8_t* w[NF];   // fragment f's first K tile, advanced to its first row (uniform)
@@ -268,7 +270,12 @@ __device__ __forceinline__ void wave_gemm_q4(const WaveOperands<MF, NF, XI, kTai
       wg_swap32(c[f][1], c[f][3]);
       wg_swap16(c[f][0], c[f][1]);
       wg_swap16(c[f][2], c[f][3]);
-      const uint32_t w[4] = {wt.sm[f].x, wt.sm[f].y, wt.sm[f].z, wt.sm[f].w};
+      uint32_t w[4] = {wt.sm[f].x, wt.sm[f].y, wt.sm[f].z, wt.sm[f].w};
+      if constexpr (kTail) {
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          if (16u * (uint32_t)kt + 4u * g >= o.xchunks) w[g] = 0u;
+      }
 #pragma unroll
       for (int g = 0; g < 4; ++g) s16[f][g] = 16.f * __uint_as_float(w[g] << 16);
 #pragma unroll

@@ -364,7 +364,7 @@ class Matrix:
                        value_beta=None, stream=None):
         """``y = act(x @ W^T + bias) + residual`` in fp32, rounded once to bf16 (call
         ``reserve_act(T)`` first).  x [T, K_in] bfloat16 or int16 bits (K_in <= K a multiple of 8;
-        columns past it are zero), bias float32 [M], residual of y's shape (y itself: in
+        W's columns past it take no part, nor do those past I of an expert's down), bias float32 [M], residual of y's shape (y itself: in
         place).  ``act`` "none", "silu", "gelu", "gelu_tanh": y [T, M]; "swiglu", "situ" (with the
         betas): y [T, M / 2], the first M / 2 weight rows the gate, the others the up.  Many rows are
         multiplied in fp16 (q4nx weights rounded to 11 bits), so a row's last bits may depend on T;
@@ -621,7 +621,8 @@ class MoeLayer:
                            residual_dev=None, gate_beta=None, value_beta=None, stream=None):
         """``Matrix.linear_act_dev`` over sorted rows, each with its routed expert's matrix: row p
         of ``offsets[e] <= p < offsets[e + 1]`` (int32 [n_routed + 1], of ``sort_tokens_dev``)
-        with expert e's ``part`` "gate_up" ([2I, H]) or "down" ([H, Ipad], rows of I columns).
+        with expert e's ``part`` "gate_up" ([2I, H]) or "down" ([H, I]; rows of I columns, or more up
+        to Ipad, of which the first I count).
         rows [n, K_in], bias float32 [n_routed, M], y and residual [n, M] or, gated, [n, M / 2].
         Rows from ``offsets[n_routed]`` on stay as they were.  Call
         ``reserve_experts_linear(n)`` first."""
