@@ -140,12 +140,13 @@ int rmoe_reserve_linear(rmoe_ctx* ctx, int handle, int T);
  * 2^-100 to 2^100 in magnitude): M' = M / 2, row i of W the gate and row M/2 + i the up of output
  * i, bias added to both.
  * (rmoe_linear_dev followed by the activation rounds gate and up to bf16 first; this call does
- * not.)  Many rows are multiplied in fp16 with a power of two per row of x and of W: a q4nx
- * weight is rounded once to fp16's 11 bits, and values below about 2^-27 of their row's largest
- * keep fewer.  A row's last bits may so depend on how many rows the call has (rmoe_linear_dev's
- * do not).  Asynchronous on `stream`, never allocates; products of many rows use context
- * scratch, so that overlapping ones need a context each.  The reference adds bias, activation
- * and residual on the host (host/raon.py:1314-1330). */
+ * not.)  Products of weights and values are exact; many rows are multiplied in fp16 with a power
+ * of two per row of x and of W, where weights below 2^-27 of their row's largest (values of x:
+ * 2^-30) keep fewer bits.  Sums of many rows are added in another order, so that a row's last
+ * bits may depend on how many rows the call has (rmoe_linear_dev's do not).  Asynchronous on
+ * `stream`, never allocates; products of many rows use context scratch, so that overlapping ones
+ * need a context each.  The reference adds bias, activation and residual on the host
+ * (host/raon.py:1314-1330). */
 int rmoe_linear_act_dev(rmoe_ctx* ctx, int handle, const void* x_dev, int T, int K_in, const float* bias_dev, int act,
                         float gate_beta, float value_beta, const void* residual_dev, void* y_dev, void* stream);
 /* Size the scratch that rmoe_linear_act_dev needs for up to T tokens on this matrix.  Graphs

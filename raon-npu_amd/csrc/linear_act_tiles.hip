@@ -2,16 +2,17 @@
 // each row's expert, on fp16 MFMA.
 //
 // Operands.  A row of x becomes fp16 times a power of two that brings its largest value into
-// [2^14, 2^15): bf16's 8 significant bits fit, values down to 2^-31 of the largest are exact.
-// A weight is formed in fp16 as its row's power of two brings the row's largest into
-// [2^10, 2^11) or, q4nx, [2^14, 2^15): bfp16's m * 2^(e-133) exactly in blocks whose largest is
-// no less than 2^-27 of the row's, q4nx's m + s * n by one fused multiply-add, rounded once to
-// fp16's 11 bits, in groups whose scale is no less than 2^-27 of the row's largest (below, s and
-// s / 16 are subnormal and the weight is off by up to 2^-31 of it).  That rounding, at most 2^-11
-// of a weight, adds to a sum what is an eighth of its bf16 rounding in the mean (rel-L2
-// against 64 bits 1.65e-3 with and without it); keeping s * (n - 8) exact instead costs a
-// second product over the group sums of x (one MFMA in five) and their preparation.  Sums
-// are fp32; the powers of two are taken back exactly.
+// [2^kXTop, 2^(kXTop + 1)): bf16's 8 significant bits fit, values down to 2^-30 of the largest are exact
+// (those below are cut by at most 2^-37 of it).  A weight row is brought to a power of two as well:
+// bfp16's m * 2^(e-133) into [2^10, 2^11), exactly in blocks whose largest is no less than 2^-27 of the
+// row's.  q4nx's m + s * n is s * (n - 8) + (m + 8 s): the first has 8 bits times 4, which fp16 holds
+// exactly in groups whose scale is no less than 2^-27 of the row's largest (below, a weight is off by
+// up to 2^-35 of it), and the second meets the sum of x over the group of 32 columns, of which the
+// preparation keeps 22 bits: a product of its own whose 32 steps are eight groups' 8 s and m, each
+// with both halves of the sum, one MFMA in nine.  Sums are fp32; the powers of two are taken back exactly.
+// (With the weight rounded to fp16's 11 bits, 53,600 rows of gate/up take 425 us and not 467, but
+// results depend on which kernel a number of rows selects: 3.3e-4 off in rel-L2, now 6e-5, which the
+// order of the sums leaves.)
 //
 // Bound by the matrix pipes and the vector instructions between them, which form the weights.
 // 53,600 rows of 128 experts' q4nx [1536, 2048], SwiGLU: 360 to 390 us (337 GFLOP, 870 to 940
@@ -30,6 +31,14 @@ typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 // --------------------------------------------------------------- preparation --
+// A row of x is brought to [2^kXTop, 2^(kXTop + 1)).  q4nx's sums of 32 of its values then reach 2^19, 16
+// times too much for fp16: they are divided by that, and so are the scales that meet the values
+// themselves; the result is 2^kShift times the accumulated sums.
+template <int kFmt>
+constexpr int kXTop = kFmt == RMOE_FMT_BFP16 ? 14 : 13;
+template <int kFmt>
+constexpr int kShift = kFmt == RMOE_FMT_BFP16 ? 0 : 4;
+
 // The power of two e with v * 2^-e in [2^top, 2^(top+1)); 0 for zero and non-finite v.
 __device__ __forceinline__ int exponent_for(float v, int top) {
   const int be = (int)(__float_as_uint(v) >> 23) & 0xff;
@@ -44,11 +53,14 @@ __device__ __forceinline__ uint32_t bf16_pair_to_half(uint32_t v, int e) {
                    __builtin_amdgcn_ldexpf(__uint_as_float(v & 0xffff0000u), -e));
 }
 
-// Rows of x to fp16 (zero past K_in to the end of its pair of K tiles) and their exponents, one wave a row; clears the counters
-// of split tiles (256 at `arrived`, if any).  A copy's work: 53,600 rows of 2,048 (440 MB) take 64
+// Rows of x to fp16 (zero past K_in to the end of its pair of K tiles) and their exponents, one wave
+// a row; clears the counters of split tiles (256 at `arrived`, if any).  A copy's work: 53,600 rows of 2,048 (440 MB) take 64
 // us where half of them are in the caches, 90 where not.
+// kSums: also, per group of 32 columns, the sum of its fp16 values times 2^-4 as two fp16 values (22
+// bits), at xs [n][K / 128 tiles][first, second][4 groups], zero like the columns past K_in.
+template <bool kSums>
 __global__ __launch_bounds__(256) void act_prep_kernel(LinAct a, uint16_t* __restrict__ xh, int32_t* __restrict__ xe,
-                                                       int* __restrict__ arrived) {
+                                                       uint16_t* __restrict__ xs, int* __restrict__ arrived) {
   if (arrived && blockIdx.x == 0) arrived[threadIdx.x] = 0;
   const int lane = threadIdx.x & 63, wave = wave_id();
   const size_t t = (size_t)blockIdx.x * 4 + wave;
@@ -73,15 +85,35 @@ __global__ __launch_bounds__(256) void act_prep_kernel(LinAct a, uint16_t* __res
   for (int c = lane + 64 * kKeep; c < nch; c += 64) largest(src[c]);
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor(mx, off, 64));
-  const int e = exponent_for(mx, 14);
+  const int e = exponent_for(mx, kXTop<kSums ? RMOE_FMT_Q4NX : RMOE_FMT_BFP16>);
   auto half = [&](const uint4& q) {
     return make_uint4(bf16_pair_to_half(q.x, e), bf16_pair_to_half(q.y, e), bf16_pair_to_half(q.z, e),
                       bf16_pair_to_half(q.w, e));
   };
+  // Chunk c's eight columns; nout is a multiple of 32, so that all four lanes of a group are here.
+  auto put = [&](int c, const uint4& h) {
+    dst[c] = h;
+    if constexpr (kSums) {
+      const uint32_t w[4] = {h.x, h.y, h.z, h.w};
+      float s = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const f16x2 p = __builtin_bit_cast(f16x2, w[i]);
+        s += (float)p[0] + (float)p[1];
+      }
+      s += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(s), 0xB1, 0xF, 0xF, false));  // lane ^ 1
+      s += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(s), 0x4E, 0xF, 0xF, false));  // lane ^ 2
+      s *= 0x1p-4f;
+      const _Float16 hi = (_Float16)s, lo = (_Float16)(s - (float)hi);
+      const int part = c & 3;  // the group's first lane writes the first value, its second the other
+      if (part < 2)
+        xs[(t * (a.K / kTileCols) + c / 16) * 8 + 4 * part + (c / 4) % 4] = __builtin_bit_cast(uint16_t, part ? lo : hi);
+    }
+  };
 #pragma unroll
   for (int i = 0; i < kKeep; ++i)
-    if (lane + 64 * i < nout) dst[lane + 64 * i] = half(v[i]);
-  for (int c = lane + 64 * kKeep; c < nout; c += 64) dst[c] = c < nch ? half(src[c]) : make_uint4(0u, 0u, 0u, 0u);
+    if (lane + 64 * i < nout) put(lane + 64 * i, half(v[i]));
+  for (int c = lane + 64 * kKeep; c < nout; c += 64) put(c, c < nch ? half(src[c]) : make_uint4(0u, 0u, 0u, 0u));
   if (lane == 0) xe[t] = e;
 }
 
@@ -132,6 +164,7 @@ struct TileArgs {
   LinAct a;
   const uint16_t* xh;
   const int32_t* xe;
+  const uint16_t* xs;  // q4nx: see act_prep_kernel
   int n_nt;
   // One matrix's last tiles, `slices` parts of K each (kSplit; see split_tail()).
   int n_whole, slices;
@@ -153,6 +186,9 @@ constexpr int kHalfBlocks = kFmt == RMOE_FMT_BFP16 ? 4 : 2;
 // Stages in LDS, of rows and of weights.  Three (where two workgroups a CU still fit) gained
 // nothing: 53,600 x gate/up 529 us with two, 537 with three.
 constexpr int kRing = 2;
+// q4nx: the group sums of a pair of K tiles, 32 bytes a row.
+template <int kFmt, int BF>
+constexpr int kSumBytes = kFmt == RMOE_FMT_BFP16 ? 0 : 16 * BF * 32;
 template <int kFmt>
 constexpr int kWaveWeights = 1024 * kHalfBlocks<kFmt> * kRing + 2 * 1024;
 
@@ -160,27 +196,25 @@ __device__ __forceinline__ f16x2 as_f16x2(uint32_t v) { return __builtin_bit_cas
 __device__ __forceinline__ uint32_t as_u32(f16x2 v) { return __builtin_bit_cast(uint32_t, v); }
 
 __device__ __forceinline__ f16x2 low2(f16x2 v) { return __builtin_shufflevector(v, v, 0, 0); }
-__device__ __forceinline__ f16x2 high2(f16x2 v) { return __builtin_shufflevector(v, v, 1, 1); }
 
 // Masks of the code unpacking in registers: (x & m) | o is one instruction then, which takes
 // no literal and one scalar register.
 struct CodeMasks {
-  uint32_t lo, hi, magic;  // 0x000f000f, 0x00f000f0 (scalar), 0x64006400 (vector)
+  uint32_t lo, hi, magic_lo, magic_hi;  // 0x000f000f, 0x00f000f0 (scalar), 0x48004800, 0x38003800 (vector)
 };
 __device__ __forceinline__ CodeMasks code_masks() {
   CodeMasks k;
-  asm volatile("s_mov_b32 %0, 0xf000f\n\ts_mov_b32 %1, 0xf000f0\n\tv_mov_b32 %2, 0x64006400"
-               : "=&s"(k.lo), "=&s"(k.hi), "=&v"(k.magic));
+  asm volatile("s_mov_b32 %0, 0xf000f\n\ts_mov_b32 %1, 0xf000f0\n\tv_mov_b32 %2, 0x48004800\n\tv_mov_b32 %3, 0x38003800"
+               : "=&s"(k.lo), "=&s"(k.hi), "=&v"(k.magic_lo), "=&v"(k.magic_hi));
   return k;
 }
-// Four codes times s plus m (sm: s low, m high), in the low 16 bits' nibble order: one nibble
-// pair of the dword sits where the bits 0x6400 make it 1024 + n, one where they make it
-// 1024 + 16 n, which meets s / 16.
+// Four codes less 8, times s 2^-4 (sm: 8 s low), in the low 16 bits' nibble order: the exponents 0x4800
+// and 0x3800 make the nibble pairs of the dword 8 + n / 128 and 0.5 + n / 128, from which (n - 8) / 128
+// is left exactly.  It has 4 bits and s bf16's 8: fp16 holds their product.
 __device__ __forceinline__ uint2 q4_operand(uint32_t c, f16x2 sm, const CodeMasks& k) {
-  const f16x2 k1024 = {(_Float16)1024.f, (_Float16)1024.f}, sixteenth = {(_Float16)0.0625f, (_Float16)0.0625f};
-  const f16x2 s = low2(sm), s16 = s * sixteenth, m = high2(sm);
-  const f16x2 n0 = as_f16x2((c & k.lo) | k.magic) - k1024, n1 = as_f16x2((c & k.hi) | k.magic) - k1024;
-  return make_uint2(as_u32(__builtin_elementwise_fma(n0, s, m)), as_u32(__builtin_elementwise_fma(n1, s16, m)));
+  const f16x2 k0 = {(_Float16)8.0625f, (_Float16)8.0625f}, k1 = {(_Float16)0.5625f, (_Float16)0.5625f};
+  const f16x2 s = low2(sm);
+  return make_uint2(as_u32((as_f16x2((c & k.lo) | k.magic_lo) - k0) * s), as_u32((as_f16x2((c & k.hi) | k.magic_hi) - k1) * s));
 }
 // Four int8 mantissas times s, a power of two: a byte u = m + 128 below 0x64 is 1024 + u, and
 // (1024 + u) s - 1152 s = m s without a rounding.
@@ -203,13 +237,13 @@ __device__ __forceinline__ void swap16(uint32_t& a, uint32_t& b) {
 }
 
 // q4nx: the scale | min words of a K tile in the wave's LDS, brought to the row's power of two
-// and to fp16 once for all that read them (lane = weight row; four words, the first `live` of
+// and to fp16, as 8 s and m, once for all that read them (lane = weight row; four words, the first `live` of
 // them: the words behind x's columns meet zeros, and are taken as zero, since they may be anything).
 __device__ __forceinline__ void convert_words(uint8_t* wp, int we, int live) {
   uint4* p = reinterpret_cast<uint4*>(wp) + (threadIdx.x & 63u);
   uint4 v = *p;
   auto half = [&](uint32_t w, int i) {
-    const uint32_t h = half_pair(__builtin_amdgcn_ldexpf(__uint_as_float(w << 16), -we),
+    const uint32_t h = half_pair(__builtin_amdgcn_ldexpf(__uint_as_float(w << 16), 3 - we),
                                  __builtin_amdgcn_ldexpf(__uint_as_float(w & 0xffff0000u), -we));
     return i < live ? h : 0u;
   };
@@ -404,6 +438,47 @@ __device__ __forceinline__ void tile_product(const TileArgs& t, const uint8_t* w
     for (int c = 0; c < nw; ++c)
       if (i == MF + (c + 1) * (MF - 1) / nw) weight_copy(c, q, at);
   };
+  // q4nx: sum over the groups of (m + 8 s) X, X the group's sum of x, by products whose 32 steps are the words
+  // (8 s, m) of two K tiles' groups, met by X's first part (lane quarters 0, 1: tile 0, 1) and its
+  // second (2, 3).  Tile kt's sums and the next one's (past the last tile its own again, met by zeros).
+  const uint8_t* sb = reinterpret_cast<const uint8_t*>(t.xs) + (size_t)row0 * (t.a.K / kTileCols) * 16;
+  const int sbase = R * kStage<BF> + NW * kWaveWeights<kFmt>;
+  // The lane, as a value that the compiler does not know: the addresses below are formed where they are
+  // used, not kept in registers across the products.
+  auto lane_here = [&]() {
+    uint32_t l = threadIdx.x & 63u;
+    asm volatile("" : "+v"(l));
+    return l;
+  };
+  auto sums_copy = [&](int kt) {
+    const uint32_t l = lane_here(), n = (uint32_t)t.a.K / kTileCols;
+    const int part = wave % (MF / 2);  // 32 rows
+    copy16(sb, ((32u * (uint32_t)part + l / 2) * n + (uint32_t)kt0 + min((uint32_t)kt + l % 2, (uint32_t)nkt - 1u)) * 16u,
+           lds0 + (uint32_t)(sbase + 1024 * part));
+  };
+  auto add_mins = [&](int kt) {
+    const uint32_t l = lane_here(), l16 = l & 15u, lq = l >> 4;
+    const bool in = (lq & 1u) == 0u || kt + 1 < nkt;
+    const uint8_t* wp = lds + pbase + 1024 * ((kt + (lq & 1u)) & 1) + 16u * l16;
+    const uint8_t* sp = lds + sbase + 32u * l16 + 16u * (lq & 1u) + 8u * (lq >> 1);
+    uint4 b[NF];
+#pragma unroll
+    for (int f = 0; f < NF; ++f) {
+      b[f] = *reinterpret_cast<const uint4*>(wp + 256 * f);
+      if (!in) b[f] = make_uint4(0u, 0u, 0u, 0u);
+    }
+#pragma unroll
+    for (int m = 0; m < MF; ++m) {
+      const uint2 v = *reinterpret_cast<const uint2*>(sp + 512 * m);
+      const uint4 x = make_uint4(__builtin_amdgcn_perm(v.x, v.x, 0x01000100u), __builtin_amdgcn_perm(v.x, v.x, 0x03020302u),
+                                 __builtin_amdgcn_perm(v.y, v.y, 0x01000100u), __builtin_amdgcn_perm(v.y, v.y, 0x03020302u));
+#pragma unroll
+      for (int f = 0; f < NF; ++f)
+        acc[m][f] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, x), __builtin_bit_cast(f16x8, b[f]),
+                                                           acc[m][f], 0, 0, 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  };
   const CodeMasks masks = code_masks();
 #pragma unroll
   for (int s = 0; s < kAhead; ++s)
@@ -440,16 +515,23 @@ __device__ __forceinline__ void tile_product(const TileArgs& t, const uint8_t* w
     const int s = 2 * kt;
     mfma_stage<kFmt, BF, MF, NF>(
         lds + here, b0, cur, next, we, masks, acc,
-        [&](int i) { copies(i, s + kAhead, s + 1 + R, kBlocks + R % 2, there, ws); },
+        [&](int i) {
+          // The last pair's sums have been read, a barrier ago at least.
+          if (kFmt == RMOE_FMT_Q4NX && i == 0 && kt % 2 == 0) sums_copy(kt);
+          copies(i, s + kAhead, s + 1 + R, kBlocks + R % 2, there, ws);
+        },
         [&] { next.read(lds + wbase + ws, wp, 1); });
     copies_landed<kEvenEnd>();
     turn();
+    if constexpr (kFmt == RMOE_FMT_Q4NX) {
+      // The next tile's words have landed (past the last tile the operands are not used); those of kt
+      // stay until the coming stage's last copies.
+      convert_words(lds + pbase + 1024 * ((kt + 1) & 1), we_lane, groups - 4 * (kt + 1));
+      if (kt % 2 == 0) add_mins(kt);
+    }
     mfma_stage<kFmt, BF, MF, NF>(
         lds + here, b0, next, cur, we, masks, acc,
         [&](int i) {
-          // The next tile's words have landed (past the last tile the operands are not used).
-          if (kFmt == RMOE_FMT_Q4NX && i == 0)
-            convert_words(lds + pbase + 1024 * ((kt + 1) & 1), we_lane, groups - 4 * (kt + 1));
           copies(i, s + 1 + kAhead, s + 2 + R, kBlocks + 1 - R % 2, there, ws);
         },
         [&] { cur.read(lds + wbase + ws, wp_next, 0); });
@@ -464,7 +546,7 @@ __device__ __forceinline__ void tile_product(const TileArgs& t, const uint8_t* w
 // tiles, and the last of a tile to arrive adds their sums in the order of the slices.
 template <int kFmt, int NF, bool kGated, int BF, int NW, int KS, bool kSplit>
 __global__ __launch_bounds__(64 * NW * KS, BF == 8 ? 2 : BF == 4 ? 3 : 4) void act_tile_kernel(TileArgs t) {
-  constexpr int kLds = kRing * kStage<BF> + NW * kWaveWeights<kFmt>, kTile = 16 * BF;
+  constexpr int kLds = kRing * kStage<BF> + NW * kWaveWeights<kFmt> + kSumBytes<kFmt, BF>, kTile = 16 * BF;
   static_assert(kLds <= 80 * 1024, "two groups a CU");
   __shared__ __attribute__((aligned(16))) uint8_t lds[KS * kLds];
   constexpr int kCols = 16 * NF * NW, kOut = kGated ? kCols / 2 : kCols;
@@ -603,7 +685,7 @@ __global__ __launch_bounds__(64 * NW * KS, BF == 8 ? 2 : BF == 4 ? 3 : 4) void a
 #pragma unroll
           for (int f = 0; f < NF; ++f) {
             float& v = o[at_column(f) ^ (16 * lq)];
-            v = __builtin_amdgcn_ldexpf(KS > 1 ? acc[m][f][i] + v : acc[m][f][i], xe + we[f]) + bias[f];
+            v = __builtin_amdgcn_ldexpf(KS > 1 ? acc[m][f][i] + v : acc[m][f][i], xe + we[f] + kShift<kFmt>) + bias[f];
           }
         }
     }
@@ -706,6 +788,8 @@ hipError_t pick_tiles(const TileArgs& t, hipStream_t st) {
 }
 
 size_t round256(size_t n) { return (n + 255) / 256 * 256; }
+// q4nx's group sums of n rows and the spare ones.
+size_t sum_bytes(int K, size_t n) { return round256((n + kActBM) * (K / kTileCols) * 16); }
 
 }  // namespace
 
@@ -729,7 +813,7 @@ size_t act_tiles_scratch(int fmt, int M, int K, int groups, size_t n) {
   if (!act_tiles_serve(fmt, M, K, groups, n)) return 0;
   const bool tail = groups == 1 && large_tiles(M, n) >= kCus;
   return round256((n + kActBM) * K * 2) + round256(n * 4) + (size_t)groups * M * sizeof(int16_t) +
-         (tail ? kTailBytes + kCus * 4 : 0);
+         (fmt == RMOE_FMT_Q4NX ? sum_bytes(K, n) : 0) + (tail ? kTailBytes + kCus * 4 : 0);
 }
 
 hipError_t launch_act_tiles(const LinAct& a, uint8_t* scratch, size_t bytes, hipStream_t st) {
@@ -738,7 +822,7 @@ hipError_t launch_act_tiles(const LinAct& a, uint8_t* scratch, size_t bytes, hip
   if (groups * 256 >= (size_t)1 << 32) return hipErrorInvalidValue;
   uint16_t* xh = reinterpret_cast<uint16_t*>(scratch);
   int32_t* xe = reinterpret_cast<int32_t*>(scratch + round256(((size_t)a.n + kActBM) * a.K * 2));
-  TileArgs t{a, xh, xe, 0, 0, 1, nullptr, nullptr};
+  TileArgs t{a, xh, xe, nullptr, 0, 0, 1, nullptr, nullptr};
   uint8_t* next = reinterpret_cast<uint8_t*>(xe) + round256((size_t)a.n * 4);
   // Narrower x: the kept exponents count weights that take no part, which may be of any size.  Those
   // of the columns that do are taken for this call.
@@ -750,16 +834,23 @@ hipError_t launch_act_tiles(const LinAct& a, uint8_t* scratch, size_t bytes, hip
     if (e != hipSuccess) return e;
   }
   next += (size_t)rows * sizeof(int16_t);  // M is a multiple of 128
+  const bool q4 = a.fmt == RMOE_FMT_Q4NX;
+  uint16_t* xs = reinterpret_cast<uint16_t*>(next);
+  if (q4) {
+    t.xs = xs;
+    next += sum_bytes(a.K, a.n);
+  }
   const size_t tiles = large_tiles(a.M, a.n);
   if (!a.offsets && (t.slices = (int)split_tail(tiles, a.K_in)) > 1) {
     t.n_whole = (int)(tiles / kCus * kCus);
     t.part = reinterpret_cast<uint64_t*>(next);
     t.arrived = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(t.part) + kTailBytes);
   }
-  hipLaunchKernelGGL(act_prep_kernel, dim3((unsigned)groups), dim3(256), 0, st, a, xh, xe, t.arrived);
+  hipLaunchKernelGGL(q4 ? act_prep_kernel<true> : act_prep_kernel<false>, dim3((unsigned)groups), dim3(256), 0, st, a, xh, xe,
+                     xs, t.arrived);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  return a.fmt == RMOE_FMT_BFP16 ? pick_tiles<RMOE_FMT_BFP16>(t, st) : pick_tiles<RMOE_FMT_Q4NX>(t, st);
+  return q4 ? pick_tiles<RMOE_FMT_Q4NX>(t, st) : pick_tiles<RMOE_FMT_BFP16>(t, st);
 }
 
 }  // namespace rmoe

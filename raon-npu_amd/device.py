@@ -366,9 +366,9 @@ class Matrix:
         ``reserve_act(T)`` first).  x [T, K_in] bfloat16 or int16 bits (K_in <= K a multiple of 8;
         W's columns past it take no part, nor do those past I of an expert's down), bias float32 [M], residual of y's shape (y itself: in
         place).  ``act`` "none", "silu", "gelu", "gelu_tanh": y [T, M]; "swiglu", "situ" (with the
-        betas): y [T, M / 2], the first M / 2 weight rows the gate, the others the up.  Many rows are
-        multiplied in fp16 (q4nx weights rounded to 11 bits), so a row's last bits may depend on T;
-        calls that overlap need a context each."""
+        betas): y [T, M / 2], the first M / 2 weight rows the gate, the others the up.  Many rows
+        are summed in another order, so a row's last bits may depend on T; calls that overlap need a
+        context each."""
         code, gb, vb, gated = _epilogue_act(act, gate_beta, value_beta)
         dev, T, K_in = self.ctx.device, int(T), _shape2(x_dev, "x")[1]
         out = (T, self.M // 2 if gated else self.M)

@@ -1,0 +1,210 @@
+"""GPU: products with an epilogue use the weights as they are, whichever kernel a number of rows selects: each weight
+is seen alone, to fp32's precision, and rows of any size, of zeros, of infinities and NaN go through the kernel of
+many rows as through the one of few.
+
+Bounds.  A q4nx product adds s (n - 8) x, 8 s X and m X (X: a group's sum of x) or 16 s n / 16 x and m X in fp32: with
+T = |s (n - 8)| + 8 |s| + |m| (bfp16: |w|) a sum over K columns is off by at most (K + 64) 2^-23 sum |x| T.  The kernel
+of many rows cuts values of x below 2^-30 of their row's largest by up to 2^-37 of it and is off by up to 2^-35 of a
+row's largest weight in groups far below it, by 2^-28 in bfp16 blocks more than 2^27 below (there are none here):
+K 2^-34 max |x| max |w| together."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+from oracle import bfp16 as B
+from oracle import q4nx as Q
+from raon_npu_amd.geometry import MoeGeometry
+from test_gpu_linear_act import _check
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+
+def _weights(fmt, M, K, seed, std=0.02, live=None):
+    """(bytes, w, T of the bounds) in float64."""
+    rng = np.random.default_rng(seed)
+    w = rng.normal(0.0, std, (M, K)).astype(np.float32)
+    if live is not None:
+        w[:, live:] = 0
+    if fmt == "bfp16":
+        blob = B.pack_gemv(w)
+        wd = torch.from_numpy(B.dequantize_packed(blob, K, M)).double()
+        return blob, wd, wd.abs()
+    c, s, m = Q.quantize(w)
+    c, s, m = (torch.from_numpy(a) for a in (c, s, m))
+    cd, sd, md = c.double(), s.double().repeat_interleave(32, 1), m.double().repeat_interleave(32, 1)
+    return Q.pack_gemv(c.numpy(), s.numpy(), m.numpy()), md + sd * cd, sd.abs() * (cd - 8).abs() + 8 * sd.abs() + md.abs()
+
+
+def _bound(x, w, t):
+    """How far the sums x w^T may be off."""
+    K = x.shape[1]
+    far = K * 2.0 ** -34 * x.abs().amax(1, keepdim=True) * w.abs().amax(1)[None]
+    return (K + 64) * 2.0 ** -23 * (x.abs() @ t.t().contiguous()) + far
+
+
+def _one_by_one(T, K, seed):
+    """Row t holds one power of two, at a column that differs from its neighbours'."""
+    col = (torch.arange(T) * 37 + seed) % K
+    x = torch.zeros(T, K, dtype=torch.bfloat16)
+    x[torch.arange(T), col] = (2.0 ** (torch.arange(T) % 7 - 3)).to(torch.bfloat16)
+    return x, col
+
+
+def _weight_left(x, col, w, t, run):
+    """``run(residual)`` of y = x w^T + residual with the bf16 rounding of each product taken away: what is left of
+    the weight itself comes back.  One column a row: the sum has three nonzero terms (and the kernel's own zeros),
+    off by 4 steps of fp32 of them."""
+    v = x[torch.arange(len(col)), col].double()[:, None]
+    z = (v * w[:, col].t()).contiguous()
+    r = -z.to(torch.bfloat16)
+    y = run(r).cpu().double()
+    ref, terms = z + r.double(), v.abs() * 2 * t[:, col].t()
+    e = 2.0 ** -22 * terms
+    bad = ~((y - ref).abs() <= 2.0 ** -8 * (ref.abs() + e) + e)
+    assert not bad.any(), (bad.nonzero()[:4].tolist(), y[bad][:4].tolist(), ref[bad][:4].tolist(), float(bad.float().mean()))
+
+
+@pytest.mark.parametrize("fmt", ["q4nx", "bfp16"])
+@pytest.mark.parametrize("T", [1, 4, 40, 130, 700, 64 * 64 + 1, 128 * 100, 128 * 129])
+def test_each_weight_of_a_matrix(gpu_ctx, fmt, T):
+    """Tiles of few rows up to 700, 64 x 128 tiles by two groups of K, 128 x 256 tiles, and the last of them cut."""
+    M, K = 512, 1024
+    blob, w, t = _weights(fmt, M, K, 3)
+    mat = gpu_ctx.upload_matrix(blob, M, K, fmt=fmt)
+    mat.reserve_act(T)
+    x, col = _one_by_one(T, K, T)
+    y = torch.zeros(T, M, dtype=torch.bfloat16, device="cuda")
+
+    def run(r):
+        mat.linear_act_dev(x.cuda(), T, y, residual_dev=r.cuda(), stream=torch.cuda.current_stream())
+        return y
+
+    _weight_left(x, col, w, t, run)
+    mat.free()
+
+
+@pytest.mark.parametrize("d_layout", [False, True])
+@pytest.mark.parametrize("part", ["gate_up", "down"])
+def test_each_weight_of_the_experts(gpu_ctx, d_layout, part):
+    """Fewer rows than experts, then 24, 64 and more an expert in the mean."""
+    H, I, E = 512, 320, 5
+    g = MoeGeometry(hidden=H, inter=I, n_routed=E, n_shared=1, top_k=2)
+    gu = [_weights("q4nx", 2 * I, H, e) for e in range(E + 1)]
+    dn = [_weights("bfp16" if d_layout else "q4nx", H, g.inter_pad, 50 + e, live=I) for e in range(E + 1)]
+    if d_layout:
+        lyr = gpu_ctx.create_layer_d(7500, g)
+        lyr.upload_d(1, 0, b"".join(b for b, _, _ in gu[:E]))
+        lyr.upload_d(2, 0, b"".join(b for b, _, _ in dn))
+    else:
+        lyr = gpu_ctx.create_layer(7500, g)
+        lyr.upload_experts(b"".join(b for b, _, _ in gu), b"".join(b for b, _, _ in dn))
+    ws, M, K = (gu, 2 * I, H) if part == "gate_up" else (dn, H, I)
+    for n in (4, 5, 120, 320, 900):
+        lyr.reserve_experts_linear(n)
+        counts = [n // E + (e < n % E) for e in range(E)]
+        offsets = torch.tensor([0] + list(np.cumsum(counts)), dtype=torch.int32)
+        x, col = _one_by_one(n, K, n)
+        y = torch.zeros(n, M, dtype=torch.bfloat16, device="cuda")
+        for e in range(E):
+            a, z = int(offsets[e]), int(offsets[e + 1])
+            if a == z:
+                continue
+            _, w, t = ws[e]
+
+            def run(r):
+                res = torch.zeros(n, M, dtype=torch.bfloat16)
+                res[a:z] = r
+                lyr.experts_linear_dev(part, x.cuda(), offsets.cuda(), y, residual_dev=res.cuda(),
+                                       stream=torch.cuda.current_stream())
+                return y[a:z]
+
+            _weight_left(x[a:z], col[a:z], w[:, :K], t[:, :K], run)
+    lyr.free()
+
+
+MANY = [(512, 64 * 65), (256, 128 * 200)]  # 64 x 128 and 128 x 256 tiles
+
+
+@pytest.mark.parametrize("fmt", ["q4nx", "bfp16"])
+@pytest.mark.parametrize("M,T", MANY)
+def test_ranges_of_values_in_many_rows(gpu_ctx, fmt, M, T):
+    """Rows of 2^-60 to 2^60, of zeros, and with one value far above the others, under weights of 2^-40 to 2^30."""
+    K = 512
+    st = torch.cuda.current_stream()
+    for std in (2.0 ** -40, 1.0, 2.0 ** 30):
+        blob, w, t = _weights(fmt, M, K, 9, std=std)
+        mat = gpu_ctx.upload_matrix(blob, M, K, fmt=fmt)
+        mat.reserve_act(T)
+        x = torch.randn(T, K, generator=torch.Generator().manual_seed(T)) * 2.0 ** torch.linspace(-60, 60, T)[:, None].round()
+        x[T // 2] = 0
+        x[5::64, 5] *= 2.0 ** 20
+        x[6::64, 7] *= 2.0 ** 34  # the others end below fp16's range
+        x = x.to(torch.bfloat16)
+        y = torch.zeros(T, M, dtype=torch.bfloat16, device="cuda")
+        mat.linear_act_dev(x.cuda(), T, y, stream=st)
+        xd, wd = x.cuda().double(), w.cuda()
+        _check(y, (xd @ wd.t().contiguous()).cpu(), _bound(xd, wd, t.cuda()).cpu(), std)
+        assert not y[T // 2].any()
+        mat.free()
+
+
+@pytest.mark.parametrize("fmt", ["q4nx", "bfp16"])
+@pytest.mark.parametrize("M,T", MANY)
+def test_non_finite_rows_among_many_stay_in_their_row(gpu_ctx, fmt, M, T):
+    K = 512
+    blob, _, _ = _weights(fmt, M, K, 9)
+    mat = gpu_ctx.upload_matrix(blob, M, K, fmt=fmt)
+    mat.reserve_act(T)
+    st = torch.cuda.current_stream()
+    x = torch.randn(T, K, generator=torch.Generator().manual_seed(2)).to(torch.bfloat16)
+    want, y = (torch.zeros(T, M, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    mat.linear_act_dev(x.cuda(), T, want, stream=st)
+    bad = [3, 17, 70, T - 1]
+    x[3, 7], x[17, 300], x[70, 0], x[T - 1, K - 1] = (float(v) for v in ("inf", "nan", "-inf", "nan"))
+    x[17, 301] = float("inf")
+    mat.linear_act_dev(x.cuda(), T, y, stream=st)
+    keep = torch.ones(T, dtype=torch.bool)
+    keep[bad] = False
+    assert torch.equal(y[keep.cuda()], want[keep.cuda()])
+    assert not y[bad].isfinite().any()
+    mat.free()
+
+
+@pytest.mark.parametrize("d_layout", [False, True])
+def test_ranges_and_non_finite_rows_by_expert(gpu_ctx, d_layout):
+    """The same by expert, in tiles of 32, 64 and 128 rows."""
+    H, I, E = 512, 320, 3
+    g = MoeGeometry(hidden=H, inter=I, n_routed=E, n_shared=1, top_k=1)
+    fmt = "bfp16" if d_layout else "q4nx"
+    dn = [_weights(fmt, H, g.inter_pad, 60 + e, live=I) for e in range(E + 1)]
+    blob = b"".join(b for b, _, _ in dn)
+    if d_layout:
+        lyr = gpu_ctx.create_layer_d(7501, g)
+        lyr.upload_d(2, 0, blob)
+    else:
+        lyr = gpu_ctx.create_layer(7501, g)
+        c, s, m = Q.quantize(np.zeros((2 * I, H), np.float32))
+        lyr.upload_experts(Q.pack_gemv(c, s, m) * (E + 1), blob)
+    st = torch.cuda.current_stream()
+    for n in (3, 60, 180, 700):
+        lyr.reserve_experts_linear(n)
+        offsets = torch.tensor([0, n // 3, n // 3, n], dtype=torch.int32)
+        x = torch.randn(n, I, generator=torch.Generator().manual_seed(n)) * 2.0 ** torch.linspace(-60, 60, n)[:, None].round()
+        x[n // 2] = 0
+        x[n - 1, 5] *= 2.0 ** 20
+        x = x.to(torch.bfloat16)
+        y, other = (torch.zeros(n, H, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+        lyr.experts_linear_dev("down", x.cuda(), offsets.cuda(), y, stream=st)
+        for e in (0, 2):
+            a, z = int(offsets[e]), int(offsets[e + 1])
+            xd, w, t = x[a:z].double(), dn[e][1][:, :I], dn[e][2][:, :I]
+            _check(y[a:z], xd @ w.t(), _bound(xd, w, t), (n, e))
+        x[0, 7], x[n - 1, 300] = float("inf"), float("nan")
+        lyr.experts_linear_dev("down", x.cuda(), offsets.cuda(), other, stream=st)
+        assert torch.equal(other[1:n - 1], y[1:n - 1])
+        assert not other[[0, n - 1]].isfinite().any()
+    lyr.free()
