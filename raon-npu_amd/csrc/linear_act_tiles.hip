@@ -144,7 +144,8 @@ __global__ __launch_bounds__(256) void row_exponents_kernel(const uint8_t* __res
           if (per * kt + 4 * i + b < nlive) emax = max(emax, (w[i] >> (8 * b)) & 0xffu);
       } else if (per * kt + i < nlive) {
         const float s = __uint_as_float(w[i] << 16), m = __uint_as_float(w[i] & 0xffff0000u);
-        mx = fmaxf(mx, fmaxf(fabsf(m), fabsf(fmaf(15.f, s, m))));
+        // m + 15 s may pass fp32's range where the codes that are taken do not.
+        mx = fmaxf(mx, fmaxf(fabsf(m), fminf(fabsf(fmaf(15.f, s, m)), 0x1.fffffep127f)));
       }
     }
   }

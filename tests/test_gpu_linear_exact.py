@@ -152,6 +152,27 @@ def test_ranges_of_values_in_many_rows(gpu_ctx, fmt, M, T):
         mat.free()
 
 
+@pytest.mark.parametrize("T", [40, 64 * 65])
+def test_weights_at_the_end_of_the_range(gpu_ctx, T):
+    """Groups whose largest possible weight, m + 15 s, is past fp32's range, and whose weights are not."""
+    M, K = 512, 256
+    rng = np.random.default_rng(4)
+    c = rng.integers(0, 3, (M, K)).astype(np.uint8)
+    s, m = np.full((M, K // 32), 1.2e37, np.float32), rng.choice([3e38, -3e38, 1e37], (M, K // 32)).astype(np.float32)
+    blob = Q.pack_gemv(c, s, m)
+    _, s, m = (torch.from_numpy(np.asarray(a)).double() for a in Q.parse_gemv(blob, K, M))
+    cd, sd, md = torch.from_numpy(c).double(), s.repeat_interleave(32, 1), m.repeat_interleave(32, 1)
+    w, t = md + sd * cd, sd * (cd - 8).abs() + 8 * sd + md.abs()
+    assert bool((md + 15 * sd > 3.4028235e38).any()) and float(w.abs().max()) < 3.4028235e38
+    mat = gpu_ctx.upload_matrix(blob, M, K)
+    mat.reserve_act(T)
+    x = (torch.randn(T, K, generator=torch.Generator().manual_seed(1)) * 2.0 ** -118).to(torch.bfloat16)
+    y = torch.zeros(T, M, dtype=torch.bfloat16, device="cuda")
+    mat.linear_act_dev(x.cuda(), T, y, stream=torch.cuda.current_stream())
+    _check(y, x.double() @ w.t(), _bound(x.double(), w, t))
+    mat.free()
+
+
 @pytest.mark.parametrize("fmt", ["q4nx", "bfp16"])
 @pytest.mark.parametrize("M,T", MANY)
 def test_non_finite_rows_among_many_stay_in_their_row(gpu_ctx, fmt, M, T):
