@@ -36,6 +36,15 @@ int fail(int code, const char* fmt, ...) {
 
 hipStream_t pick_stream(rmoe_ctx* ctx, void* stream) { return stream ? (hipStream_t)stream : ctx->stream; }
 
+// Device memory; false if there is not enough.  The failure is reported here: it would otherwise
+// stay behind as the thread's last error, which the next launch's check takes for its own.
+template <typename T>
+bool device_malloc(T** p, size_t bytes) {
+  if (hipMalloc((void**)p, bytes) == hipSuccess) return true;
+  (void)hipGetLastError();
+  return false;
+}
+
 // Grow-only device buffer of n elements of T (zero-filled when (re)allocated).
 template <typename T>
 int grow(T*& p, size_t& cap, size_t n, rmoe_ctx* ctx) {
@@ -48,7 +57,7 @@ int grow(T*& p, size_t& cap, size_t n, rmoe_ctx* ctx) {
   }
   size_t want = std::max<size_t>(n, 1);
   void* q = nullptr;
-  if (hipMalloc(&q, want * sizeof(T)) != hipSuccess) return fail(RMOE_ENOMEM, "hipMalloc of %zu bytes failed", want * sizeof(T));
+  if (!device_malloc(&q, want * sizeof(T))) return fail(RMOE_ENOMEM, "hipMalloc of %zu bytes failed", want * sizeof(T));
   // Zero on the context stream and wait: later launches may use other streams.
   HIP_TRY(hipMemsetAsync(q, 0, want * sizeof(T), ctx->stream));
   HIP_TRY(hipStreamSynchronize(ctx->stream));
@@ -263,7 +272,7 @@ int sync_and_check(rmoe_ctx* ctx, hipStream_t st) {
 
 // The tiles of an [M, K] matrix of `need` bytes, and behind them the exponents of its rows.
 bool alloc_matrix(RmoeMatrix& m, size_t need) {
-  if (hipMalloc((void**)&m.tiles, need + (size_t)m.M * sizeof(int16_t)) != hipSuccess) return false;
+  if (!device_malloc(&m.tiles, need + (size_t)m.M * sizeof(int16_t))) return false;
   m.exps = reinterpret_cast<int16_t*>(m.tiles + need);
   m.live = m.K;
   return true;
@@ -286,15 +295,15 @@ hipError_t dn_exponents(const RmoeLayer& L, size_t e, int n, hipStream_t st) {
 int place_layer(rmoe_ctx* ctx, int layer, RmoeLayer& L) {
   const size_t gub = (size_t)L.gu_experts * L.gu_bytes, gue = (size_t)L.gu_experts * 2 * L.I * sizeof(int16_t);
   const size_t dnb = (size_t)L.dn_experts * L.dn_bytes, dne = (size_t)L.dn_experts * L.H * sizeof(int16_t);
-  if (hipMalloc((void**)&L.gu, gub + gue) != hipSuccess) return fail(RMOE_ENOMEM, "hipMalloc of expert gate_up failed");
-  if (hipMalloc((void**)&L.dn, dnb + dne) != hipSuccess) {
+  if (!device_malloc(&L.gu, gub + gue)) return fail(RMOE_ENOMEM, "hipMalloc of expert gate_up failed");
+  if (!device_malloc(&L.dn, dnb + dne)) {
     hipFree(L.gu);
     return fail(RMOE_ENOMEM, "hipMalloc of expert down failed");
   }
   L.gu_exps = reinterpret_cast<int16_t*>(L.gu + gub);
   L.dn_exps = reinterpret_cast<int16_t*>(L.dn + dnb);
   if (L.dn_fmt == RMOE_FMT_BFP16 &&
-      (hipMalloc((void**)&L.dn_rowexp, (size_t)L.dn_experts * L.H) != hipSuccess ||
+      (!device_malloc(&L.dn_rowexp, (size_t)L.dn_experts * L.H) ||
        hipMemset(L.dn_rowexp, 7, (size_t)L.dn_experts * L.H) != hipSuccess)) {
     hipFree(L.gu);
     hipFree(L.dn);
@@ -469,7 +478,7 @@ int rmoe_create(int device, rmoe_ctx** out) {
     delete ctx;
     return fail(RMOE_EDEVICE, "hipStreamCreate failed");
   }
-  if (hipMalloc((void**)&ctx->s.err, sizeof(int)) != hipSuccess) {
+  if (!device_malloc(&ctx->s.err, sizeof(int))) {
     hipStreamDestroy(ctx->stream);
     delete ctx;
     return fail(RMOE_ENOMEM, "hipMalloc failed");
@@ -1129,13 +1138,13 @@ static int set_router_common(rmoe_ctx* ctx, RmoeLayer* L, const void* w, bool w_
   if (score != RMOE_SCORE_SIGMOID && score != RMOE_SCORE_SOFTMAX) return fail(RMOE_EINVAL, "unknown router score %d", score);
   HIP_TRY(hipSetDevice(ctx->device));
   const size_t wb = (size_t)L->n_routed * L->H * 2;
-  if (!L->router_w && hipMalloc((void**)&L->router_w, wb) != hipSuccess) return fail(RMOE_ENOMEM, "hipMalloc failed");
+  if (!L->router_w && !device_malloc(&L->router_w, wb)) return fail(RMOE_ENOMEM, "hipMalloc failed");
   // The context's stream is ordered with no other: whatever the caller queued that writes w
   // has to end before it is read (the call takes no stream).
   if (w_on_device) HIP_TRY(hipDeviceSynchronize());
   HIP_TRY(hipMemcpyAsync(L->router_w, w, wb, w_on_device ? hipMemcpyDeviceToDevice : hipMemcpyHostToDevice, ctx->stream));
   if (bias) {
-    if (!L->router_bias && hipMalloc((void**)&L->router_bias, L->n_routed * sizeof(float)) != hipSuccess)
+    if (!L->router_bias && !device_malloc(&L->router_bias, L->n_routed * sizeof(float)))
       return fail(RMOE_ENOMEM, "hipMalloc failed");
     HIP_TRY(hipMemcpyAsync(L->router_bias, bias, L->n_routed * sizeof(float), hipMemcpyHostToDevice, ctx->stream));
   } else if (L->router_bias) {
