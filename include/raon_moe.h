@@ -150,7 +150,8 @@ int rmoe_reserve_linear(rmoe_ctx* ctx, int handle, int T);
 int rmoe_linear_act_dev(rmoe_ctx* ctx, int handle, const void* x_dev, int T, int K_in, const float* bias_dev, int act,
                         float gate_beta, float value_beta, const void* residual_dev, void* y_dev, void* stream);
 /* Size the scratch that rmoe_linear_act_dev needs for up to T tokens on this matrix.  Graphs
- * captured before stay valid. */
+ * captured before stay valid: scratch that was too small is kept until rmoe_destroy, and the next
+ * has twice its size where that fits, else what was asked for.  Reserve for the largest call first. */
 int rmoe_reserve_linear_act(rmoe_ctx* ctx, int handle, int T);
 
 /* ------------------------------------------------------------ tokens by expert --

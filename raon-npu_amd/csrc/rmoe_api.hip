@@ -527,7 +527,7 @@ int rmoe_destroy(rmoe_ctx* ctx) {
                   s.chunk_counts, s.staging, s.pf, s.stack, s.stack_cnt, s.act};
   for (void* b : bufs)
     if (b) hipFree(b);
-  for (int i = 0; i < s.n_act_before; ++i) hipFree(s.act_before[i]);
+  for (uint8_t* b : s.act_before) hipFree(b);
   auto it = g_io.find(ctx);
   if (it != g_io.end()) {
     hipFree(it->second.p);
@@ -758,11 +758,13 @@ static int reserve_act(rmoe_ctx* ctx, size_t bytes) {
   HIP_TRY(hipSetDevice(ctx->device));
   if (bytes <= ctx->s.act_bytes) return RMOE_OK;
   // A graph captured before keeps the buffer it was captured with: growing gives a new one, of
-  // at least twice the size, so that the old ones together are smaller.
+  // twice the size where that fits, so that the old ones together are smaller.
   uint8_t* p = nullptr;
   size_t cap = 0;
-  TRY(grow(p, cap, std::max(bytes, 2 * ctx->s.act_bytes), ctx));
-  if (ctx->s.act) ctx->s.act_before[ctx->s.n_act_before++] = ctx->s.act;
+  int r = grow(p, cap, std::max(bytes, 2 * ctx->s.act_bytes), ctx);
+  if (r == RMOE_ENOMEM && bytes < 2 * ctx->s.act_bytes) r = grow(p, cap, bytes, ctx);
+  TRY(r);
+  if (ctx->s.act) ctx->s.act_before.push_back(ctx->s.act);
   ctx->s.act = p;
   ctx->s.act_bytes = cap;
   return RMOE_OK;

@@ -406,8 +406,7 @@ struct RmoeScratch {
   int max_tokens = 0;
   uint8_t* act = nullptr;        // products with an epilogue: fp16 rows, exponents
   size_t act_bytes = 0;
-  uint8_t* act_before[64] = {};  // smaller ones, which captured graphs may hold (each doubles the last)
-  int n_act_before = 0;
+  std::vector<uint8_t*> act_before;  // smaller ones, which captured graphs may hold
   // persistent decode stack (moe_decode_stack.hip)
   uint8_t* stack = nullptr;      // per-layer hand-off buffers
   size_t stack_bytes = 0;

@@ -34,3 +34,32 @@ def test_calls_after_a_reservation_that_does_not_fit(gpu_ctx):
     torch.cuda.synchronize()
     assert torch.equal(y, want) and bool(few.any())
     mat.free()
+
+
+def test_growth_that_fits_only_as_asked(gpu_ctx):
+    """A reservation a little larger than the one before asks for twice that one; where only the size asked for
+    fits, that is what it gets."""
+    from raon_npu_amd import Context
+
+    M, K, gib = 512, 2048, 2 ** 30
+    ctx = Context(0)
+    mat = _matrix(ctx, M, K)
+    rows = 4 * gib // (2 * K)  # 4 GiB of rows in fp16
+    mat.reserve_act(rows)
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    free = torch.cuda.mem_get_info()[0]
+    fill = torch.empty(free - 7 * gib, dtype=torch.uint8, device="cuda")  # 8 GiB and more do not fit, 5 do
+    try:
+        mat.reserve_act(rows * 5 // 4)
+        x = torch.randn(64 * 65, K, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).cuda()
+        y = torch.zeros(64 * 65, M, dtype=torch.bfloat16, device="cuda")
+        mat.linear_act_dev(x, 64 * 65, y, stream=torch.cuda.current_stream())
+        torch.cuda.synchronize()
+        assert bool((y != 0).any(1).all())
+        with pytest.raises(RuntimeError, match="hipMalloc"):
+            mat.reserve_act(2 * rows)
+    finally:
+        del fill
+        torch.cuda.empty_cache()
+    ctx.close()
