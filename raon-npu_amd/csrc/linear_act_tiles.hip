@@ -753,13 +753,16 @@ hipError_t launch_tiles(const TileArgs& t0, hipStream_t st) {
 // Tiles of 128 x 256 and of 64 x 128 weight rows over one matrix of M rows.
 size_t large_tiles(int M, size_t n) { return (n + 127) / 128 * ((M + 255) / 256); }
 size_t small_tiles(int M, size_t n) { return (n + 63) / 64 * (M / 128); }
-constexpr size_t kFillLarge = 200, kFillSmall = 256;
+constexpr size_t kFillLarge = 200;
+// Fewer 64 x 128 tiles than this are left to linear_act_kernel (see act_tiles_serve()).
+constexpr size_t fill_small(int fmt) { return fmt == RMOE_FMT_BFP16 ? 256 : 320; }
 
 // Large tiles past a multiple of 256: a CU takes 50 us for one of [2176, 2560] alone and 72 for
 // two, so a few of them beyond are cut along K into three or four slices, of two K tiles at
-// least, and as many as there are CUs.  4,096 rows of [2176, 2560] (32 beyond) 82 us whole, in 3,
-// 4, 6 and 8 slices 70, 67, 70 and 76; 6,000 of [1536, 2048] (26) 70, and 61, 60, 63 and 66; 5,060
-// of [2176, 2560] (104) 85, in 2 slices 85.  Returns the slices (1: none are cut).
+// least, and as many as there are CUs.  q4nx, 4,096 rows of [2176, 2560] (32 beyond) 87 us
+// whole, in 2, 3 and 4 slices 77, 71 and 70; 6,000 of [1536, 2048] (26) 75, and 68, 64 and 62; 5,060
+// of [2176, 2560] (104) 90, in 2 slices 90.  (Six and eight slices of the 32 were slower than four by
+// 5 and 13 %.)  Returns the slices (1: none are cut).
 constexpr size_t kCus = 256, kMinSlices = 3, kMaxSlices = 4;
 size_t split_tail(size_t tiles, int K_in) {
   const size_t over = tiles % kCus;
@@ -770,12 +773,12 @@ size_t split_tail(size_t tiles, int K_in) {
 constexpr size_t kTailBytes = kCus * kActBM * 256 * 4;  // the sums of at most kCus slices
 
 // By expert: by the rows an expert has in the mean (128 experts, q4nx gate/up [1536, 2048], tiles
-// of 32, 64 and 128 rows: 28 rows 68, 67 and 77 us, 44 rows 108, 81 and 93, 62 rows 135, 113 and
-// 112, 94 rows 184, 139 and 128; bfp16 down [2560, 1088]: 12 rows 100, 108 and 108, 47 rows 147,
+// of 32, 64 and 128 rows: 16 rows 59, 59 and 67 us, 28 rows 74, 72 and 83, 44 rows 110, 86 and 100,
+// 62 rows 132, 113 and 123, 94 rows 180, 147 and 138; bfp16 down [2560, 1088]: 12 rows 100, 108 and 108, 47 rows 147,
 // 138 and 137, 70 rows 180, 164 and 158).
 // One matrix: 128 x 256 from kFillLarge tiles of it on, below that 64 x 128 by two groups of K,
 // which make 3.75 times the workgroups (q4nx [2176, 2560], SwiGLU, 64 x 128 / 128 x 256: 1,024
-// rows 35 / 50 us, 2,048 (144 large tiles) 54 / 54, 3,000 (216) 66 / 58, 4,096 83 / 81).
+// rows 37 / 57 us, 2,048 (144 large tiles) 58 / 61, 3,000 (216) 70 / 62, 4,096 85 / 87).
 template <int kFmt>
 hipError_t pick_tiles(const TileArgs& t, hipStream_t st) {
   const LinAct& a = t.a;
@@ -800,15 +803,17 @@ hipError_t launch_row_exponents(const uint8_t* tiles, int fmt, int M, int K, int
 }
 
 // Which rows this kernel serves, against linear_act_kernel (whose cost grows with every 32 rows).
-// One matrix: from kFillSmall tiles of 64 x 128 on (this kernel / that one, q4nx with SwiGLU:
-// [2176, 2560], 700 rows (187 tiles) 26 / 27 us, 1,024 rows (272) 35 / 40, 1,500 rows 38 / 56;
-// [1536, 2048], 1,024 rows (192) 23 / 23, 1,500 rows (288) 31 / 34; [512, 2048], 3,000 rows (188)
-// 29 / 24).  By expert: from one row an expert on (128 experts, q4nx gate/up [1536, 2048]: 128 rows
-// 39 / 52 us, 2,048 rows 55 / 78, 8,000 rows 112 / 206).
+// One matrix: from fill_small() tiles of 64 x 128 on (this kernel / that one, with SwiGLU.  q4nx:
+// [2176, 2560], 1,100 rows (306 tiles) 39 / 38 us, 1,250 rows (340) 39 / 45; [1536, 2048], 1,500 rows
+// (288) 34 / 31, 1,700 rows (324) 35 / 37; [512, 2048], 4,500 rows (284) 40 / 33, 5,500 rows (344) 39 / 39,
+// 6,500 rows (408) 39 / 44.  bfp16: [2176, 2560], 1,024 rows (272) 34 / 40; [1536, 2048], 1,024 rows (192)
+// 24 / 22, 1,360 rows (264) 31 / 34; [512, 2048], 4,096 rows (256) 31 / 30, 5,500 rows (344) 35 / 41).  By
+// expert: from one row an expert on (128 experts, q4nx gate/up [1536, 2048]: 128 rows 43 / 42 us, 700
+// rows 55 / 69, 8,000 rows 115 / 185; down [2048, 768]: 128 rows 27 / 32).
 bool act_tiles_serve(int fmt, int M, int K, int groups, size_t n) {
   const size_t bytes = fmt == RMOE_FMT_BFP16 ? matrix_bytes_bfp16(M, K) : matrix_bytes(M, K);
   if (bytes >= (size_t)1 << 32) return false;  // 32-bit byte offsets into a matrix
-  return groups > 1 ? n >= (size_t)groups : small_tiles(M, n) >= kFillSmall;
+  return groups > 1 ? n >= (size_t)groups : small_tiles(M, n) >= fill_small(fmt);
 }
 size_t act_tiles_scratch(int fmt, int M, int K, int groups, size_t n) {
   if (!act_tiles_serve(fmt, M, K, groups, n)) return 0;

@@ -69,9 +69,10 @@ def _weight_left(x, col, w, t, run):
 
 
 @pytest.mark.parametrize("fmt", ["q4nx", "bfp16"])
-@pytest.mark.parametrize("T", [1, 4, 40, 130, 700, 64 * 64 + 1, 128 * 100, 128 * 129])
+@pytest.mark.parametrize("T", [1, 4, 40, 130, 700, 64 * 64 + 1, 64 * 80 + 1, 128 * 100, 128 * 129])
 def test_each_weight_of_a_matrix(gpu_ctx, fmt, T):
-    """Tiles of few rows up to 700, 64 x 128 tiles by two groups of K, 128 x 256 tiles, and the last of them cut."""
+    """Tiles of few rows up to 700 (q4nx 4,097), 64 x 128 tiles by two groups of K, 128 x 256 tiles, and the last of them
+    cut."""
     M, K = 512, 1024
     blob, w, t = _weights(fmt, M, K, 3)
     mat = gpu_ctx.upload_matrix(blob, M, K, fmt=fmt)
@@ -126,7 +127,7 @@ def test_each_weight_of_the_experts(gpu_ctx, d_layout, part):
     lyr.free()
 
 
-MANY = [(512, 64 * 65), (256, 128 * 200)]  # 64 x 128 and 128 x 256 tiles
+MANY = [(512, 64 * 81), (256, 128 * 200)]  # 64 x 128 and 128 x 256 tiles
 
 
 @pytest.mark.parametrize("fmt", ["q4nx", "bfp16"])
@@ -152,7 +153,7 @@ def test_ranges_of_values_in_many_rows(gpu_ctx, fmt, M, T):
         mat.free()
 
 
-@pytest.mark.parametrize("T", [40, 64 * 65])
+@pytest.mark.parametrize("T", [40, 64 * 81])
 def test_weights_at_the_end_of_the_range(gpu_ctx, T):
     """Groups whose largest possible weight, m + 15 s, is past fp32's range, and whose weights are not."""
     M, K = 512, 256
@@ -229,3 +230,117 @@ def test_ranges_and_non_finite_rows_by_expert(gpu_ctx, d_layout):
         assert torch.equal(other[1:n - 1], y[1:n - 1])
         assert not other[[0, n - 1]].isfinite().any()
     lyr.free()
+
+
+def _same(a, b):
+    """Two bf16 roundings of sums that differ by their order alone."""
+    a, b = a.double(), b.double()
+    return float((a - b).norm()) <= (2 / 3) ** 0.5 * 2.0 ** -8 * float(b.norm())
+
+
+def test_many_rows_of_weights_of_every_origin(gpu_ctx):
+    """The exponents that many rows use are kept with the weights by every call that writes them: against few rows,
+    which use none, for layers synthesized, quantized and from Q4_K through views of their experts, and for matrices."""
+    st = torch.cuda.current_stream()
+    H, I, E = 512, 256, 2
+    g = MoeGeometry(hidden=H, inter=I, n_routed=E, n_shared=1, top_k=1)
+    T = 64 * 81
+    rng = np.random.default_rng(5)
+
+    def check(mat, K, what):
+        x = torch.randn(T, K, generator=torch.Generator().manual_seed(K)).to(torch.bfloat16).cuda()
+        mat.reserve_act(T)
+        y, few = (torch.zeros(n, mat.M, dtype=torch.bfloat16, device="cuda") for n in (T, 32))
+        mat.linear_act_dev(x, T, y, stream=st)
+        mat.linear_act_dev(x[:32], 32, few, stream=st)
+        assert bool(few.any()) and _same(y[:32], few), what
+        mat.free()
+
+    def q4k(rows, cols, d):  # random 144-byte super-blocks with sane scales
+        b = rng.integers(0, 256, (rows * cols // 256, 144), dtype=np.uint8)
+        b[:, :4] = np.frombuffer(np.array([d, d / 2], dtype=np.float16).tobytes(), dtype=np.uint8)
+        return b.tobytes()
+
+    lyr = gpu_ctx.create_layer(7502, g)
+
+    def check_layer(what):
+        for e in range(E):
+            check(lyr.expert_matrix(e, "gate_up"), H, (what, e, "gate_up"))
+            check(lyr.expert_matrix(e, "down"), I, (what, e, "down"))
+
+    lyr.synthesize(3, std=0.5, stream=st)
+    check_layer("synthesized")
+    for e in range(E):
+        lyr.quantize_expert(e, torch.randn(2 * I, H, device="cuda") * 2.0 ** (13 * e), torch.randn(H, I, device="cuda"))
+    check_layer("quantized")
+    for e in range(E):
+        lyr.upload_expert_q4k(e, "gate", q4k(I, H, 0.01 * 4 ** e))
+        lyr.upload_expert_q4k(e, "up", q4k(I, H, 0.3))
+        lyr.upload_expert_q4k(e, "down", q4k(H, I, 0.002))
+    check_layer("Q4_K")
+    lyr.free()
+    M, K = 512, 768
+    for mat in (gpu_ctx.quantize_matrix(torch.randn(M, K, device="cuda") * 300, M, K),
+                gpu_ctx.upload_matrix(_weights("q4nx", M, K, 1)[0], M, K),
+                gpu_ctx.upload_matrix(_weights("bfp16", M, K, 1, std=2.0 ** -30)[0], M, K, fmt="bfp16"),
+                gpu_ctx.upload_matrix(q4k(M, K, 0.02), M, K, fmt="q4k")):
+        check(mat, K, mat.fmt)
+
+
+@pytest.mark.parametrize("fmt", ["q4nx", "bfp16"])
+def test_groups_of_very_different_sizes_in_many_rows(gpu_ctx, fmt):
+    """Rows whose groups' weights differ by 2^20, met by tokens that are zero where the large ones are."""
+    M, K, T = 512, 512, 64 * 81
+    rng = np.random.default_rng(3)
+    scale = 2.0 ** -rng.integers(0, 21, (M, K // 32))
+    scale[:, 0] = 1.0
+    scale[:, 1:9] = 2.0 ** -20
+    w = (rng.normal(0.0, 0.5, (M, K)) * np.repeat(scale, 32, 1)).astype(np.float32)
+    if fmt == "q4nx":
+        c, s, m = Q.quantize(w)
+        blob = Q.pack_gemv(c, s, m)
+        cd, sd, md = torch.from_numpy(c).double(), *(torch.from_numpy(a).double().repeat_interleave(32, 1) for a in (s, m))
+        wd, t = md + sd * cd, sd.abs() * (cd - 8).abs() + 8 * sd.abs() + md.abs()
+    else:
+        blob = B.pack_gemv(w)
+        wd = torch.from_numpy(B.dequantize_packed(blob, K, M)).double()
+        t = wd.abs()
+    mat = gpu_ctx.upload_matrix(blob, M, K, fmt=fmt)
+    mat.reserve_act(T)
+    x = torch.randn(T, K, generator=torch.Generator().manual_seed(4)).to(torch.bfloat16)
+    x[::2, :32] = 0
+    x[::2, 288:] = 0
+    y = torch.zeros(T, M, dtype=torch.bfloat16, device="cuda")
+    mat.linear_act_dev(x.cuda(), T, y, stream=torch.cuda.current_stream())
+    xd = x.double()
+    _check(y, xd @ wd.t(), (K + 64) * 2.0 ** -23 * (xd.abs() @ t.t()), fmt)
+    mat.free()
+
+
+@pytest.mark.parametrize("fmt", ["q4nx", "bfp16"])
+def test_many_rows_captured_before_a_larger_reserve(gpu_ctx, fmt):
+    """A captured call with its group sums and, for a narrower input, its own exponents in the context's scratch
+    replays as before after calls of other rows and after the scratch has grown."""
+    M, K, K_in, T = 1024, 768, 520, 64 * 41
+    blob, _, _ = _weights(fmt, M, K, 3)
+    mat = gpu_ctx.upload_matrix(blob, M, K, fmt=fmt)
+    mat.reserve_act(T)
+    st = torch.cuda.Stream()
+    x = torch.randn(3 * T, K_in, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).cuda()
+    y, big = (torch.zeros(n, M, dtype=torch.bfloat16, device="cuda") for n in (T, 3 * T))
+    torch.cuda.synchronize()
+    mat.linear_act_dev(x[:T], T, y, act="silu", stream=st)
+    torch.cuda.synchronize()
+    want = y.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=st):
+        mat.linear_act_dev(x[:T], T, y, act="silu", stream=st)
+    for grown in (T, 2 * T, 3 * T):
+        mat.reserve_act(grown)
+        mat.linear_act_dev(x[:grown], grown, big[:grown], act="silu", stream=st)
+        y.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, want)
+    mat.free()

@@ -105,9 +105,9 @@ def test_down_by_expert(gpu_ctx, fmt, kind):
     want.free()
 
 
-# Rows of a dense [512, .] matrix: tiles of few rows up to 4,032, 64 x 128 tiles by two groups of K up to 12,672,
-# 128 x 256 tiles, and (258 tiles) the last two of them cut along K.
-ROWS = (1, 4, 5, 40, 64 * 63, 64 * 63 + 1, 128 * 100, 128 * 129)
+# Rows of a dense [512, .] matrix: tiles of few rows up to 4,032 (q4nx 5,056), 64 x 128 tiles by two groups of K up to
+# 12,672, 128 x 256 tiles, and (258 tiles) the last two of them cut along K.
+ROWS = (1, 4, 5, 40, 64 * 63, 64 * 63 + 1, 64 * 79, 64 * 79 + 1, 128 * 100, 128 * 129)
 
 
 def _many(M, T):

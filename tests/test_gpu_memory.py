@@ -19,7 +19,7 @@ def _matrix(ctx, M, K):
 
 def test_calls_after_a_reservation_that_does_not_fit(gpu_ctx):
     """An allocation that fails is that call's error alone: the next launches do not report it again."""
-    M, K, T = 512, 2048, 64 * 65
+    M, K, T = 512, 2048, 64 * 81
     mat = _matrix(gpu_ctx, M, K)
     mat.reserve_act(T)
     st = torch.cuda.current_stream()
@@ -52,9 +52,9 @@ def test_growth_that_fits_only_as_asked(gpu_ctx):
     fill = torch.empty(free - 7 * gib, dtype=torch.uint8, device="cuda")  # 8 GiB and more do not fit, 5 do
     try:
         mat.reserve_act(rows * 5 // 4)
-        x = torch.randn(64 * 65, K, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).cuda()
-        y = torch.zeros(64 * 65, M, dtype=torch.bfloat16, device="cuda")
-        mat.linear_act_dev(x, 64 * 65, y, stream=torch.cuda.current_stream())
+        x = torch.randn(64 * 81, K, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).cuda()
+        y = torch.zeros(64 * 81, M, dtype=torch.bfloat16, device="cuda")
+        mat.linear_act_dev(x, 64 * 81, y, stream=torch.cuda.current_stream())
         torch.cuda.synchronize()
         assert bool((y != 0).any(1).all())
         with pytest.raises(RuntimeError, match="hipMalloc"):
