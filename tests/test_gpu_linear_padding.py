@@ -53,7 +53,7 @@ def _blobs(fmt, M, K, live, kind, seed):
     return buf.tobytes(), zero, wd
 
 
-def _layers(gpu_ctx, fmt, kind):
+def _layers(gpu_ctx, fmt, kind, I=I):
     """Two layers that differ in the padding of down alone, and down's live weights."""
     g = MoeGeometry(hidden=H, inter=I, n_routed=E, n_shared=1, top_k=2)
     dn = [_blobs(fmt, H, g.inter_pad, I, kind, 10 + e) for e in range(E + 1)]
@@ -101,6 +101,29 @@ def test_down_by_expert(gpu_ctx, fmt, kind):
                 a, z = int(offsets[e]), int(offsets[e + 1])
                 if a < z:
                     _check(ys[0][a:z], *_reference(x[a:z, :I], w[e], None, "none", None, n >= E), (n, width, e))
+    got.free()
+    want.free()
+
+
+@pytest.mark.parametrize("fmt,kind", [(f, k) for f in KINDS for k in KINDS[f]])
+def test_down_that_ends_with_a_tile(gpu_ctx, fmt, kind):
+    """I = 384 of 512: three whole K tiles, the fourth is padding alone."""
+    (got, want), w = _layers(gpu_ctx, fmt, kind, 384)
+    st = torch.cuda.current_stream()
+    for n in (5, 60, 700):
+        offsets = torch.tensor([0, 0, n // 3, n // 3, n, n, n], dtype=torch.int32)
+        for width in (384, 512):
+            x = _rows(n, width, 384, n, True)
+            ys = []
+            for lyr in (got, want):
+                lyr.reserve_experts_linear(n)
+                y = torch.full((n, H), 9.0, dtype=torch.bfloat16, device="cuda")
+                lyr.experts_linear_dev("down", x.cuda(), offsets.cuda(), y, stream=st)
+                ys.append(y)
+            assert torch.equal(*ys), (n, width)
+            for e in (1, 3):
+                a, z = int(offsets[e]), int(offsets[e + 1])
+                _check(ys[0][a:z], *_reference(x[a:z, :384], w[e], None, "none", None, n >= E), (n, width, e))
     got.free()
     want.free()
 
