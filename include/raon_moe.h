@@ -156,10 +156,10 @@ int rmoe_reserve_linear_act(rmoe_ctx* ctx, int handle, int T);
 
 /* ------------------------------------------------------------ tokens by expert --
  * The steps around the experts' products on device operands, for an engine that puts work of
- * its own between them.  T tokens of width H in RMOE_DT_* elements, any H >= 1, contiguous
- * rows at any address of their type; k (1..16) routes per token, A = T k < 2^31 assignments
- * a = t k + r; H at most 2^30.  Asynchronous on `stream`; nothing is allocated and no scratch of the context
- * is used, so that calls on several streams or captured graphs share only the buffers the
+ * its own between them.  T tokens (at least one) of width H in RMOE_DT_* elements, any H from 1 to
+ * 2^30, contiguous rows at any address of their type; k (1..16) routes per token, A = T k < 2^31
+ * assignments a = t k + r.  Asynchronous on `stream`; nothing is allocated and no scratch of the
+ * context is used, so that calls on several streams or captured graphs share only the buffers the
  * caller gives them.  Inputs and outputs of a call must not overlap. */
 
 /* Sort: rows[inv[a]] = x[t] for every assignment whose expert ids[a] is in 0..n_experts-1

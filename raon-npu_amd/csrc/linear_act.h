@@ -14,7 +14,9 @@ __host__ __device__ constexpr bool act_gated(int act) { return act == RMOE_ACT_S
 // their relative accuracy.  exp2 and the reciprocal are the hardware's (1 ulp each); with the
 // exponent's own rounding exp(z) is off by (2 + |z|) 2^-23 of it, far below a bf16 rounding.
 // They are kept short: a product with 4,096 x 1,088 SiTU outputs took 83 us with IEEE
-// divisions, Newton steps and clamps, and 77 without.
+// divisions, Newton steps and clamps, and 77 without.  The calls over whole MoE layers keep
+// act_situ() and act_swiglu() (rmoe_internal.h), which follow the CPU path's operations and whose
+// gate and up are rounded to bf16 first; both are within a few steps of fp32 of the formula.
 __device__ __forceinline__ float recip(float d) { return __builtin_amdgcn_rcpf(d); }
 __device__ __forceinline__ float exp_of(float z) {
   const float t = 1.44269504088896341f * z;
@@ -26,7 +28,7 @@ __device__ __forceinline__ float sigmoid_of(float z) {
   return z >= 0.f ? r : e * r;
 }
 // tanh: 1 - 2 / (1 + exp(2 |z|)), which an infinite exp makes 1, and below 0.3, where that
-// cancels, its power series to z^9 (the next term is 4e-8 of z there).
+// cancels, its power series to z^9 (the next term is (1382 / 155925) z^10 = 5.3e-8 of z there).
 __device__ __forceinline__ float tanh_of(float z) {
   const float a = fabsf(z), q = z * z;
   const float big = fmaf(-2.0f, recip(1.0f + __builtin_amdgcn_exp2f(2.88539008177792681f * a)), 1.0f);

@@ -15,10 +15,10 @@
 // order of the sums leaves.)
 //
 // Bound by the matrix pipes and the vector instructions between them, which form the weights.
-// 53,600 rows of 128 experts' q4nx [1536, 2048], SwiGLU: 360 to 390 us (337 GFLOP, 870 to 940
-// TFLOP/s; torch's bf16 8192^3 reaches 1,210) behind 64 for the rows of x; 8,192 rows of
-// [8192, 4096] 575 us in all (957 TFLOP/s); 128 experts' bfp16 [2560, 1088] of 21 rows each 97 us,
-// in which 425 MB of weights stream at 4.7 TB/s.
+// 53,600 rows of 128 experts' q4nx [1536, 2048], SwiGLU: 395 to 423 us (337 GFLOP, 800 to 850
+// TFLOP/s without the group sums' MFMAs, an eighth more; torch's bf16 8192^3 reaches 1,210) behind 66
+// for the rows of x; 8,192 rows of [8192, 4096] 533 us in all (1,030 TFLOP/s); 128 experts' bfp16
+// [2560, 1088] of 21 rows each 97 to 101 us, in which 425 MB of weights stream at 4.2 to 4.4 TB/s.
 #include <algorithm>
 
 #include "linear_act.h"
@@ -54,8 +54,8 @@ __device__ __forceinline__ uint32_t bf16_pair_to_half(uint32_t v, int e) {
 }
 
 // Rows of x to fp16 (zero past K_in to the end of its pair of K tiles) and their exponents, one wave
-// a row; clears the counters of split tiles (256 at `arrived`, if any).  A copy's work: 53,600 rows of 2,048 (440 MB) take 64
-// us where half of them are in the caches, 90 where not.
+// a row; clears the counters of split tiles (256 at `arrived`, if any).  A copy's work: 53,600 rows
+// of 2,048 (440 MB) take 64 us where half of them are in the caches, 90 where not, 2 more with the sums.
 // kSums: also, per group of 32 columns, the sum of its fp16 values times 2^-4 as two fp16 values (22
 // bits), at xs [n][K / 128 tiles][first, second][4 groups], zero like the columns past K_in.
 template <bool kSums>

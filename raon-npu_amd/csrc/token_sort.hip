@@ -12,11 +12,12 @@
 //
 // Every one of them moves k rows per token and is bound by HBM; small calls are bound by
 // their chain of dependent loads (routes, then rows) and the launch (4 us for four tokens).
-// Each element is read and written once: a wave takes one token and 1 KB of its columns, loads
-// what the k rows share once, and finds the k positions in its own lanes, without LDS or
-// barriers.  6,700 tokens of 8 rows of 4 KB (240 MB), buffers not in the caches: the sort 57 us
-// (10 of them for the positions), the combine 47 (5.1 TB/s); 4,099 tokens: the combine's
-// gradient 59 (286 MB, 4.9 TB/s; a copy reaches 4.8).
+// Each element is read and written once.  The sort and the combine's gradient take a workgroup a
+// token, which keeps the k positions (the dot products' shares) in LDS; the sums take a wave for
+// one token and 1 KB of its columns, which finds the k positions in its own lanes, without LDS or
+// barriers.  6,700 tokens of 8 rows of 4 KB (240 MB), buffers not in the caches: the sort 58 us
+// (10 of them for the positions), the combine 49 (4.9 TB/s); 4,099 tokens: the combine's
+// gradient 60 (286 MB, 4.8 TB/s; a copy reaches 4.8).
 #include <algorithm>
 
 #include "../../include/raon_moe.h"
