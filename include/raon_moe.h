@@ -66,6 +66,13 @@ extern "C" {
 #define RMOE_DT_F16 1
 #define RMOE_DT_F32 2
 
+/* Gates of a block's result in the norms around it: none, one value a column (fp32 [H]), one a row (fp32 [T]), or
+ * one an element (rows' type, [T, H]). */
+#define RMOE_GATE_NONE 0
+#define RMOE_GATE_COLUMN 1
+#define RMOE_GATE_ROW 2
+#define RMOE_GATE_FULL 3
+
 typedef struct rmoe_ctx rmoe_ctx;
 
 /* Message of the last failed call on this thread ("" if none). */
@@ -396,6 +403,71 @@ int rmoe_moe_experts_grouped_dev(rmoe_ctx* ctx, int layer, const void* x_dev, in
 int rmoe_moe_prefill_dev(rmoe_ctx* ctx, int layer, const void* x_dev, int T, void* out_dev, int residual,
                          int act, float gate_beta, float value_beta, void* top_ids_dev,
                          void* top_weights_dev, void* stream);
+
+/* ------------------------------------------------------ microscaled 4-bit rows --
+ * A third weight format and the one quantized form of activations: blocks of 32 columns that share a power of two 2^s,
+ * s = clamp(floor(log2 max|x|) - 2, -127, 127) (zeros: -127), held as the byte s + 127, and per column a 4-bit code, bit
+ * 3 its sign and bits 0..2 an index into 0, 0.5, 1, 1.5, 2, 3, 4, 6: the nearest to x 2^-s, ties to the even index,
+ * magnitudes above 6 to 6.  (The published microscaling format with e2m1 elements and e8m0 scales.)  A block that
+ * holds NaN or an infinity has byte 255 and codes 0 and stands for NaN.  A row of K columns has P = K rounded up to 32 of
+ * them, zeros past K: P/2 bytes of codes, the even column in a byte's low half, and P/32 scale bytes.  Codes and scales
+ * are plain row-major arrays of the caller, weights [M, K] and activations [T, K] alike: weights are quantized by the
+ * same call, and nothing is uploaded or laid out again.  All calls are asynchronous on `stream`, allocate nothing and
+ * use no scratch of the context: calls on several streams and captured graphs share only the buffers the caller gives
+ * them.  At least one row. */
+
+/* x [T, K] in RMOE_DT_* elements, contiguous, at any address of their type, K from 1 to 2^30 -> codes [T, P/2] (16-byte
+ * aligned), scales [T, P/32], and values [T, K] in x's type, what they stand for (exact; NULL: not written; x itself: in
+ * place).  For a forward pass that trains: compute with the values, and pass their gradient on to x unchanged. */
+int rmoe_mx_quantize_dev(rmoe_ctx* ctx, const void* x_dev, int dtype, int T, int K, void* codes_dev, void* scales_dev,
+                         void* values_dev, void* stream);
+/* y[T, M'] = RTNE(act(x W^T + bias) + residual) of quantized rows x [T, K] and weights [M, K], K a multiple of 32 (of
+ * another width: quantized rows end in zeros, so both sides' P is the K here): products exact, sums and epilogue fp32,
+ * rounded once to bf16.  act, bias, residual and M' as in rmoe_linear_act_dev; any M (even when gated).  A scale byte
+ * of 255 in a row of x or W makes its results NaN.  Codes 16-byte aligned.  Sums may be added in another order for
+ * another number of rows, so that a row's last bits may depend on it. */
+int rmoe_mx_linear_dev(rmoe_ctx* ctx, const void* x_codes_dev, const void* x_scales_dev, int T, int K,
+                       const void* w_codes_dev, const void* w_scales_dev, int M, const float* bias_dev, int act,
+                       float gate_beta, float value_beta, const void* residual_dev, void* y_dev, void* stream);
+/* The same over sorted rows, each with the matrix of its expert: for e in 0..n_experts-1 (at most 256) and offsets[e] <=
+ * p < offsets[e+1] (rmoe_sort_tokens_dev's offsets) W_e of codes [n_experts, M, K/2] and scales [n_experts, M, K/32], bias
+ * [n_experts, M] or NULL.  Rows from offsets[n_experts] on stay as they were. */
+int rmoe_mx_experts_linear_dev(rmoe_ctx* ctx, const void* x_codes_dev, const void* x_scales_dev, int n, int K,
+                               const void* w_codes_dev, const void* w_scales_dev, int M, const void* offsets_dev,
+                               int n_experts, const float* bias_dev, int act, float gate_beta, float value_beta,
+                               const void* residual_dev, void* y_dev, void* stream);
+
+/* ------------------------------------------------------- norms around a block --
+ * What stands between two blocks (attention, a dense MLP or the experts) of a residual stream:
+ *   n = (mean_j b_j^2 + eps)^-1/2,  u = n b wpost  (post NULL: u = b)
+ *   y = R(scale r + g u)
+ *   m = (mean_j y_j^2 + eps)^-1/2,  h = R(m y wpre)
+ * block b, residual r, y and h [T, H] in RMOE_DT_* elements at any address of their type, H from 1 to 8192; sums and
+ * products fp32 (rows whose sum of squares passes its range give zeros), R one rounding to the rows' type; h is the
+ * norm of y as stored.  wpost and wpre fp32 [H]; gate g as gate_kind (RMOE_GATE_*) says, NULL for none.  block
+ * NULL: no y, post or gate, and h is the norm of residual (the norm before the first block).  h NULL: not wanted;
+ * codes [T, P/2] (16-byte aligned) and scales [T, P/32], both or neither: h as microscaled 4-bit rows, the bytes that
+ * rmoe_mx_quantize_dev makes of it.  eps > 0.  Asynchronous, allocates nothing, no scratch.  y may be residual or block,
+ * h may be block, nothing else may overlap.  The reference normalises on the host (host/raon.py:904-909). */
+int rmoe_residual_norm_dev(rmoe_ctx* ctx, const void* block_dev, const void* residual_dev, int dtype, int T, int H,
+                           const float* post_weight_dev, const void* gate_dev, int gate_kind, float scale,
+                           const float* pre_weight_dev, float eps, void* y_dev, void* h_dev, void* codes_dev,
+                           void* scales_dev, void* stream);
+/* Floats of work memory that rmoe_residual_norm_backward_dev takes for T rows of width H. */
+int rmoe_norm_backward_work(int T, int H, size_t* floats);
+/* Its gradients from dy (of y where the stream goes on; NULL: none) and dh (of h; NULL: none), at least one of them:
+ *   a = dh wpre,  D = dy + m a - y m^3 (sum_j a_j y_j) / H,  dresidual = scale D,  du = g D,  v = du wpost,
+ *   dblock = n v - b n^3 (sum_j v_j b_j) / H  (post NULL: du),
+ *   dpre_weight = sum_t dh y m,  dpost_weight = sum_t du b n,  dgate = D u summed over what a gate's value is shared by.
+ * block, y (as computed), gate, scale and eps as in the forward call; block NULL: the gradient of the norm of y alone,
+ * with scale 1 for the plain sum dy + norm's.  dpre_weight, dpost_weight fp32 [H], dgate as the gate; NULL: not wanted.
+ * dresidual may be dy, dblock may be dh.  work: fp32, rmoe_norm_backward_work, of the call alone while it runs.  Column
+ * sums are added in a fixed order. */
+int rmoe_residual_norm_backward_dev(rmoe_ctx* ctx, const void* dy_dev, const void* dh_dev, const void* block_dev,
+                                    const void* y_dev, int dtype, int T, int H, const float* post_weight_dev,
+                                    const void* gate_dev, int gate_kind, float scale, const float* pre_weight_dev,
+                                    float eps, void* dblock_dev, void* dresidual_dev, float* dpost_weight_dev,
+                                    void* dgate_dev, float* dpre_weight_dev, float* work_dev, void* stream);
 
 #ifdef __cplusplus
 }

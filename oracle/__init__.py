@@ -14,6 +14,7 @@ Modules and the reference files they restate (paths inside the reference tree):
 * ``oracle.moe``     -- ``host/backend.py:47-62,402-417,466-510``,
                         ``host/raon.py:1224-1247,1288-1330,1565-1621``,
                         ``kernels/moe/reference.py:127-180``
+* ``oracle.mx``      -- no counterpart: microscaled 4-bit rows (e2m1 codes, e8m0 scales)
 * ``oracle.planner`` -- ``kernels/moe_grouped/planner.py:18-322``
 
 How each function is pinned (known answers, golden hashes, closed forms) is

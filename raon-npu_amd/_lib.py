@@ -27,6 +27,10 @@ ACT_GELU_TANH = 5
 DT_BF16 = 0
 DT_F16 = 1
 DT_F32 = 2
+GATE_NONE = 0
+GATE_COLUMN = 1
+GATE_ROW = 2
+GATE_FULL = 3
 SCORE_SIGMOID = 0
 SCORE_SOFTMAX = 1
 FMT_Q4NX = 0
@@ -96,6 +100,12 @@ SIGNATURES: dict[str, list] = {
     "rmoe_moe_prefill_dev": [_p, _i, _p, _i, _p, _i, _i, _f, _f, _p, _p, _p],
     "rmoe_experts_linear_dev": [_p, _i, _i, _p, _i, _i, _p, _p, _i, _f, _f, _p, _p, _p],
     "rmoe_reserve_experts_linear": [_p, _i, _i],
+    "rmoe_mx_quantize_dev": [_p, _p, _i, _i, _i, _p, _p, _p, _p],
+    "rmoe_mx_linear_dev": [_p, _p, _p, _i, _i, _p, _p, _i, _p, _i, _f, _f, _p, _p, _p],
+    "rmoe_mx_experts_linear_dev": [_p, _p, _p, _i, _i, _p, _p, _i, _p, _i, _p, _i, _f, _f, _p, _p, _p],
+    "rmoe_residual_norm_dev": [_p, _p, _p, _i, _i, _i, _p, _p, _i, _f, _p, _f, _p, _p, _p, _p, _p],
+    "rmoe_norm_backward_work": [_i, _i, C.POINTER(_sz)],
+    "rmoe_residual_norm_backward_dev": [_p, _p, _p, _p, _p, _i, _i, _i, _p, _p, _i, _f, _p, _f, _p, _p, _p, _p, _p, _p, _p],
     "rmoe_moe_experts_grouped_dev": [_p, _i, _p, _i, _p, _p, _p, _i, _f, _f, _p, _p, _p],
 }
 _RESTYPES = {"rmoe_last_error": C.c_char_p, "rmoe_version": C.c_char_p, "rmoe_stream": _p}

@@ -411,6 +411,49 @@ int check_linear_act(const rmoe::LinAct& L) {
                         {L.offsets, (size_t)(L.n_experts + 1) * 4}}, {y});
 }
 
+// Microscaled operands of a product: codes aligned to 16 bytes, no output over an input.
+int check_mx(rmoe_ctx* ctx, const rmoe::MxLin& L) {
+  if (!ctx) return fail(RMOE_EINVAL, "null context");
+  if (!L.x || !L.xs || !L.w || !L.ws || !L.y) return fail(RMOE_EINVAL, "null argument");
+  if (L.n < 1) return fail(RMOE_EINVAL, "the number of rows must be >= 1");
+  if (L.K < 32 || L.K % 32 || L.K > 1 << 30) return fail(RMOE_EINVAL, "K (%d) must be a multiple of 32, at most 2^30", L.K);
+  if (L.act < RMOE_ACT_SITU || L.act > RMOE_ACT_GELU_TANH) return fail(RMOE_EINVAL, "unknown activation %d", L.act);
+  const bool gated = L.act == RMOE_ACT_SITU || L.act == RMOE_ACT_SWIGLU;
+  if (L.M < 1 || L.M > 1 << 30 || (gated && L.M % 2))
+    return fail(RMOE_EINVAL, "M (%d) must be 1..2^30, and even for a gated activation", L.M);
+  for (float b : {L.gb, L.vb})
+    if (L.act == RMOE_ACT_SITU && !(fabsf(b) >= 0x1p-100f && fabsf(b) <= 0x1p100f))
+      return fail(RMOE_EINVAL, "SiTU betas must be between 2^-100 and 2^100 in magnitude");
+  if ((reinterpret_cast<uintptr_t>(L.x) | reinterpret_cast<uintptr_t>(L.w)) & 15)
+    return fail(RMOE_EINVAL, "codes must be 16-byte aligned");
+  if ((reinterpret_cast<uintptr_t>(L.y) | reinterpret_cast<uintptr_t>(L.residual)) & 1 ||
+      (reinterpret_cast<uintptr_t>(L.bias) | reinterpret_cast<uintptr_t>(L.offsets)) & 3)
+    return fail(RMOE_EINVAL, "operands must be aligned to their element type");
+  const size_t n = L.n, M = L.M, groups = L.offsets ? L.n_experts : 1;
+  const Span y{L.y, n * (gated ? M / 2 : M) * 2};
+  const Span res{L.residual == L.y ? nullptr : L.residual, y.n};  // y itself: added in place
+  return check_overlap({{L.x, n * (L.K / 2)}, {L.xs, n * (L.K / 32)}, {L.w, groups * M * (L.K / 2)},
+                        {L.ws, groups * M * (L.K / 32)}, res, {L.bias, groups * M * 4},
+                        {L.offsets, (size_t)(L.n_experts + 1) * 4}}, {y});
+}
+
+// Rows, vectors and gate of the norms around a block.
+int check_norm(rmoe_ctx* ctx, const rmoe::NormArgs& a, int dtype, std::initializer_list<const void*> rows,
+               std::initializer_list<const void*> words) {
+  TRY(check_tokens(ctx, dtype, a.T, a.H, 1, rows, words));
+  if (a.H > rmoe::kNormMaxWidth) return fail(RMOE_EINVAL, "H (%d) must be at most %d", a.H, rmoe::kNormMaxWidth);
+  if (!(a.eps > 0.f && a.eps <= 0x1p100f)) return fail(RMOE_EINVAL, "eps must be positive");
+  if (a.gate_kind < RMOE_GATE_NONE || a.gate_kind > RMOE_GATE_FULL)
+    return fail(RMOE_EINVAL, "unknown kind of gate %d", a.gate_kind);
+  if ((a.gate != nullptr) != (a.gate_kind != RMOE_GATE_NONE)) return fail(RMOE_EINVAL, "gate and gate_kind go together");
+  if (!a.block && (a.gate || a.post)) return fail(RMOE_EINVAL, "a gate or a norm after go with a block");
+  return RMOE_OK;
+}
+size_t gate_bytes(const rmoe::NormArgs& a, int dtype) {
+  return a.gate_kind == RMOE_GATE_FULL ? (size_t)a.T * row_bytes(dtype, a.H)
+                                       : 4 * (size_t)(a.gate_kind == RMOE_GATE_ROW ? a.T : a.H);
+}
+
 // ------------------------------------------------------- static decode scratch --
 // rmoe_moe_experts_static_dev runs the routed-expert decode kernels on this file-scope
 // device array instead of context scratch, so it never allocates.  Each GPU holds its
@@ -493,7 +536,7 @@ int rmoe_create(int device, rmoe_ctx** out) {
   bool ok = hipHostMalloc((void**)&ctx->pinned, kPinnedBytes, hipHostMallocDefault) == hipSuccess &&
             hipHostGetDevicePointer((void**)&ctx->pinned_dev, ctx->pinned, 0) == hipSuccess;
   ok = ok && rmoe::prefill_setup() == hipSuccess && rmoe::linear_mfma_setup() == hipSuccess &&
-       rmoe::linear_act_setup() == hipSuccess;
+       rmoe::linear_act_setup() == hipSuccess && rmoe::mx_linear_setup() == hipSuccess;
   for (hipEvent_t& ev : ctx->chunk_done) ok = ok && hipEventCreateWithFlags(&ev, hipEventDisableTiming) == hipSuccess;
   if (!ok) {
     free_base(ctx);
@@ -877,6 +920,115 @@ int rmoe_combine_tokens_backward_dev(rmoe_ctx* ctx, const void* dout, const void
   HIP_TRY(dev.status);
   HIP_TRY(rmoe::launch_combine_grad(dout, rows, dtype, T, H, (const int32_t*)inv, (const float*)weights, k, drows,
                                     (float*)dweights, ctx->s.err, pick_stream(ctx, stream)));
+  return RMOE_OK;
+}
+
+// ------------------------------------------------------- microscaled 4-bit rows --
+int rmoe_mx_quantize_dev(rmoe_ctx* ctx, const void* x, int dtype, int T, int K, void* codes, void* scales, void* values,
+                         void* stream) {
+  TRY(check_tokens(ctx, dtype, T, K, 1, {x, values}, {}));
+  if (!x || !codes || !scales) return fail(RMOE_EINVAL, "null argument");
+  if (reinterpret_cast<uintptr_t>(codes) & 15) return fail(RMOE_EINVAL, "codes must be 16-byte aligned");
+  const size_t rb = row_bytes(dtype, K), P = ((size_t)K + 31) / 32;
+  TRY(check_overlap({{values == x ? nullptr : x, T * rb}}, {{codes, T * P * 16}, {scales, T * P}, {values, T * rb}}));
+  OnDevice dev(ctx);
+  HIP_TRY(dev.status);
+  HIP_TRY(rmoe::launch_mx_quantize(x, dtype, T, K, (uint8_t*)codes, (uint8_t*)scales, values, pick_stream(ctx, stream)));
+  return RMOE_OK;
+}
+
+static int run_mx_linear(rmoe_ctx* ctx, const rmoe::MxLin& L, void* stream) {
+  TRY(check_mx(ctx, L));
+  OnDevice dev(ctx);
+  HIP_TRY(dev.status);
+  const hipError_t e = rmoe::launch_mx_linear(L, pick_stream(ctx, stream));
+  if (e == hipErrorInvalidValue) return fail(RMOE_EINVAL, "%d rows by %d are too many for one call", L.n, L.M);
+  HIP_TRY(e);
+  return RMOE_OK;
+}
+
+int rmoe_mx_linear_dev(rmoe_ctx* ctx, const void* x_codes, const void* x_scales, int T, int K, const void* w_codes,
+                       const void* w_scales, int M, const float* bias, int act, float gate_beta, float value_beta,
+                       const void* residual, void* y, void* stream) {
+  const rmoe::MxLin L{(const uint8_t*)x_codes, (const uint8_t*)x_scales, (const uint8_t*)w_codes,
+                      (const uint8_t*)w_scales, T, M, K, nullptr, 0, bias, act, gate_beta, value_beta,
+                      (const uint16_t*)residual, (uint16_t*)y};
+  return run_mx_linear(ctx, L, stream);
+}
+
+int rmoe_mx_experts_linear_dev(rmoe_ctx* ctx, const void* x_codes, const void* x_scales, int n, int K,
+                               const void* w_codes, const void* w_scales, int M, const void* offsets, int n_experts,
+                               const float* bias, int act, float gate_beta, float value_beta, const void* residual,
+                               void* y, void* stream) {
+  if (!ctx) return fail(RMOE_EINVAL, "null context");
+  if (!offsets) return fail(RMOE_EINVAL, "null argument");
+  if (n_experts < 1 || n_experts > 256) return fail(RMOE_EINVAL, "n_experts (%d) must be in 1..256", n_experts);
+  const rmoe::MxLin L{(const uint8_t*)x_codes, (const uint8_t*)x_scales, (const uint8_t*)w_codes,
+                      (const uint8_t*)w_scales, n, M, K, (const int32_t*)offsets, n_experts, bias, act, gate_beta,
+                      value_beta, (const uint16_t*)residual, (uint16_t*)y};
+  return run_mx_linear(ctx, L, stream);
+}
+
+// -------------------------------------------------------- norms around a block --
+int rmoe_residual_norm_dev(rmoe_ctx* ctx, const void* block, const void* residual, int dtype, int T, int H,
+                           const float* post_weight, const void* gate, int gate_kind, float scale,
+                           const float* pre_weight, float eps, void* y, void* h, void* codes, void* scales,
+                           void* stream) {
+  const rmoe::NormArgs a{block, residual, gate, gate_kind, post_weight, pre_weight, scale, eps, T, H, y, h,
+                         (uint8_t*)codes, (uint8_t*)scales};
+  const bool full = gate_kind == RMOE_GATE_FULL;
+  TRY(check_norm(ctx, a, dtype, {block, residual, y, h, full ? gate : nullptr}, {post_weight, pre_weight, full ? nullptr : gate}));
+  if (!residual || (block != nullptr) != (y != nullptr)) return fail(RMOE_EINVAL, "null argument");
+  if ((codes != nullptr) != (scales != nullptr)) return fail(RMOE_EINVAL, "codes and scales go together");
+  const bool normed = h || codes;
+  if (normed != (pre_weight != nullptr)) return fail(RMOE_EINVAL, "pre_weight goes with h or codes");
+  if (!normed && !block) return fail(RMOE_EINVAL, "neither a block nor an output");
+  if (reinterpret_cast<uintptr_t>(codes) & 15) return fail(RMOE_EINVAL, "codes must be 16-byte aligned");
+  const size_t n = (size_t)T * row_bytes(dtype, H), P = ((size_t)H + 31) / 32, w = (size_t)H * 4;
+  // An output may stand where an input of the same rows does: a row is read before it is written.
+  const bool own_block = block && (block == y || block == h), own_residual = residual == y;
+  const Span b{own_block ? nullptr : block, n}, r{own_residual ? nullptr : residual, n};
+  TRY(check_overlap({b, r, {gate, gate_bytes(a, dtype)}, {post_weight, w}, {pre_weight, w}},
+                    {{y, n}, {h, n}, {codes, (size_t)T * P * 16}, {scales, (size_t)T * P}}));
+  OnDevice dev(ctx);
+  HIP_TRY(dev.status);
+  HIP_TRY(rmoe::launch_norm(a, dtype, pick_stream(ctx, stream)));
+  return RMOE_OK;
+}
+
+int rmoe_norm_backward_work(int T, int H, size_t* floats) {
+  if (!floats) return fail(RMOE_EINVAL, "null argument");
+  if (T < 1 || H < 1 || H > rmoe::kNormMaxWidth)
+    return fail(RMOE_EINVAL, "T (%d) must be >= 1 and H (%d) in 1..%d", T, H, rmoe::kNormMaxWidth);
+  *floats = (size_t)3 * rmoe::norm_groups(T) * H;
+  return RMOE_OK;
+}
+
+int rmoe_residual_norm_backward_dev(rmoe_ctx* ctx, const void* dy, const void* dh, const void* block, const void* y,
+                                    int dtype, int T, int H, const float* post_weight, const void* gate, int gate_kind,
+                                    float scale, const float* pre_weight, float eps, void* dblock, void* dresidual,
+                                    float* dpost_weight, void* dgate, float* dpre_weight, float* work, void* stream) {
+  const rmoe::NormGradArgs a{{block, nullptr, gate, gate_kind, post_weight, pre_weight, scale, eps, T, H,
+                              const_cast<void*>(y), nullptr, nullptr, nullptr},
+                             dy, dh, dblock, dresidual, dgate, dpre_weight, dpost_weight, work};
+  const bool full = gate_kind == RMOE_GATE_FULL;
+  TRY(check_norm(ctx, a.f, dtype, {block, y, dy, dh, dblock, dresidual, full ? gate : nullptr, full ? dgate : nullptr},
+                 {post_weight, pre_weight, dpost_weight, dpre_weight, work, full ? nullptr : gate, full ? nullptr : dgate}));
+  if (!y || !dresidual || !work || (block != nullptr) != (dblock != nullptr)) return fail(RMOE_EINVAL, "null argument");
+  if (!dy && !dh) return fail(RMOE_EINVAL, "neither dy nor dh");
+  if ((dh != nullptr) != (pre_weight != nullptr) || (dpre_weight && !dh))
+    return fail(RMOE_EINVAL, "pre_weight and its gradient go with dh");
+  if ((dgate && !gate) || (dpost_weight && !post_weight))
+    return fail(RMOE_EINVAL, "a gradient goes with its gate or weight");
+  const size_t n = (size_t)T * row_bytes(dtype, H), w = (size_t)H * 4, g = gate_bytes(a.f, dtype);
+  const bool own_dy = dy == dresidual, own_dh = dh && dh == dblock;
+  TRY(check_overlap({{own_dy ? nullptr : dy, n}, {own_dh ? nullptr : dh, n}, {block, n}, {y, n}, {gate, g},
+                     {post_weight, w}, {pre_weight, w}},
+                    {{dblock, n}, {dresidual, n}, {dpost_weight, w}, {dpre_weight, w}, {dgate, g},
+                     {work, (size_t)12 * rmoe::norm_groups(T) * H}}));
+  OnDevice dev(ctx);
+  HIP_TRY(dev.status);
+  HIP_TRY(rmoe::launch_norm_backward(a, dtype, pick_stream(ctx, stream)));
   return RMOE_OK;
 }
 

@@ -566,6 +566,52 @@ size_t act_tiles_scratch(int fmt, int M, int K, int groups, size_t n);
 hipError_t launch_row_exponents(const uint8_t* tiles, int fmt, int M, int K, int K_live, int16_t* exps, hipStream_t st);
 hipError_t launch_act_tiles(const LinAct& a, uint8_t* scratch, size_t bytes, hipStream_t st);
 
+// Rows to microscaled 4-bit codes and scales (mx_quantize.hip, mx.h); values (may be null): what they stand for, in
+// the rows' type.
+hipError_t launch_mx_quantize(const void* x, int dtype, int T, int K, uint8_t* codes, uint8_t* scales, void* values,
+                              hipStream_t st);
+// y = act(x W^T + bias) + residual over n rows of microscaled codes (mx_linear.hip): of one matrix (offsets null),
+// or row p with the matrix of its expert e, offsets[e] <= p < offsets[e + 1].
+struct MxLin {
+  const uint8_t *x, *xs;  // [n, K / 2] 16-byte aligned, [n, K / 32]
+  const uint8_t *w, *ws;  // [n_experts or 1, M, K / 2] 16-byte aligned, [.., M, K / 32]
+  int n, M, K;            // K % 32 == 0
+  const int32_t* offsets;
+  int n_experts;
+  const float* bias;      // [n_experts or 1, M] or null
+  int act;
+  float gb, vb;
+  const uint16_t* residual;
+  uint16_t* y;
+};
+hipError_t mx_linear_setup();  // once per device before the first call
+hipError_t launch_mx_linear(const MxLin& a, hipStream_t st);
+
+// The norms before and after a block (block_norm.hip).  block null: y is not computed, h is the norm of residual.
+struct NormArgs {
+  const void *block, *residual, *gate;  // rows of the call's type; gate as gate_kind says
+  int gate_kind;                        // RMOE_GATE_*
+  const float *post, *pre;              // [H]; post null: no norm after the block
+  float scale, eps;
+  int T, H;                             // H <= kNormMaxWidth
+  void *y, *h;                          // h, codes and scales may be null
+  uint8_t *codes, *scales;
+};
+constexpr int kNormMaxWidth = 8192;
+hipError_t launch_norm(const NormArgs& a, int dtype, hipStream_t st);
+// Its gradient: f as above (y an input, residual, h and codes not read); dy or dh may be null, and without a block
+// dblock, dpost and dgate; a null gradient of a weight or gate is not formed.
+struct NormGradArgs {
+  NormArgs f;
+  const void *dy, *dh;
+  void *dblock, *dresidual, *dgate;
+  float *dpre, *dpost;
+  float* work;  // [3][norm_groups(T)][H]
+};
+// Workgroups of the gradient, each of which leaves its share of the weights' gradients.
+constexpr int norm_groups(int T) { return T < 512 ? T : 512; }
+hipError_t launch_norm_backward(const NormGradArgs& a, int dtype, hipStream_t st);
+
 // Persistent decode of n_layers (<= kMaxStack) layers of one geometry for one token
 // (moe_decode_stack.hip).  One workgroup per CU (grid n_cu).  ids_out/wts_out: [n_layers, k]
 // or null.  Scratch: stack_scratch_bytes / stack_counter_count; counters must be zero.

@@ -13,7 +13,7 @@ import numpy as np
 
 from . import _lib
 from ._lib import (ACT_GELU, ACT_GELU_TANH, ACT_NONE, ACT_SILU, ACT_SITU, ACT_SWIGLU, BUNDLE_B1, BUNDLE_B2, DT_BF16, DT_F16,
-                   DT_F32, PART_DOWN, PART_GATE_UP, SCORE_SIGMOID, SCORE_SOFTMAX, call, check, new_bytes, ptr)
+                   DT_F32, GATE_COLUMN, GATE_FULL, GATE_NONE, GATE_ROW, PART_DOWN, PART_GATE_UP, SCORE_SIGMOID, SCORE_SOFTMAX, call, check, new_bytes, ptr)
 from .geometry import MoeGeometry
 
 
@@ -103,6 +103,33 @@ def _bf16_operand(device: int, t, shape: tuple, name: str) -> int:
     except AttributeError:
         pass
     return _operand(device, t, shape, "int16" if _dtype_name(t) == "int16" else "bfloat16", name)
+
+
+def _byte_operand(device: int, t, shape: tuple, name: str, torch_name: str) -> int:
+    """Bytes of a given shape: uint8, or torch's own type of what they hold."""
+    return _operand(device, t, shape, torch_name if _dtype_name(t) == torch_name else "uint8", name)
+
+
+def _mx_operands(device: int, codes, scales, lead: tuple, K: int, name: str) -> tuple[int, int]:
+    """The addresses of microscaled rows of K columns (a multiple of 32)."""
+    return (_byte_operand(device, codes, (*lead, K // 2), f"{name} codes", "float4_e2m1fn_x2"),
+            _byte_operand(device, scales, (*lead, K // 32), f"{name} scales", "float8_e8m0fnu"))
+
+
+def _optional(device: int, t, shape: tuple, dtype_name: str, name: str) -> int | None:
+    return None if t is None else _operand(device, t, shape, dtype_name, name)
+
+
+def _gate_operand(device: int, gate, T: int, H: int, dt: str, name: str) -> tuple[int | None, int]:
+    """(address, GATE_*) of a gate: float32 [H] by column, float32 [T, 1] by row, [T, H] of the rows' type."""
+    if gate is None:
+        return None, GATE_NONE
+    shape = tuple(getattr(gate, "shape", ()))
+    if shape == (H,):
+        return _operand(device, gate, shape, "float32", name), GATE_COLUMN
+    if shape == (T, 1) and _dtype_name(gate) == "float32":
+        return _operand(device, gate, shape, "float32", name), GATE_ROW
+    return _operand(device, gate, (T, H), dt, name), GATE_FULL
 
 
 def _epilogue_act(act: str, gate_beta, value_beta) -> tuple[int, float, float, bool]:
@@ -309,6 +336,140 @@ class Context:
             _ROW_TYPES[dt], T, H, _operand(dev, inv_dev, (T, k), "int32", "inv"),
             _operand(dev, wts_dev, (T, k), "float32", "wts"), k, _operand(dev, drows_dev, (T * k, H), dt, "drows"),
             _operand(dev, dwts_dev, (T, k), "float32", "dwts"), _stream_ptr(stream)))
+
+    # ----------------------------------------------- microscaled 4-bit rows --
+    def mx_quantize_dev(self, x_dev, codes_dev, scales_dev, values_dev=None, stream=None):
+        """Rows to microscaled 4 bits: x [T, K] bfloat16 (or int16 bits), float16 or float32 -> codes uint8 [T, P / 2]
+        and scales uint8 [T, P / 32], P = K rounded up to 32 (or torch's float4_e2m1fn_x2 and float8_e8m0fnu); values
+        (optional, of x's shape and type; x itself: in place) what they stand for.  Blocks of 32 columns share 2^s, s =
+        floor(log2(max)) - 2, byte s + 127; a code is the e2m1 value nearest to x 2^-s, the even column in a byte's low
+        half.  Weights [M, K] are quantized by the same call.  Asynchronous; allocates nothing and uses no scratch."""
+        dt, dev = _row_type(x_dev, "x"), self.device
+        T, K = _shape2(x_dev, "x")
+        P = -(-K // 32) * 32
+        codes, scales = _mx_operands(dev, codes_dev, scales_dev, (T,), P, "x")
+        check(_lib.load().rmoe_mx_quantize_dev(
+            self._h, _operand(dev, x_dev, (T, K), dt, "x"), _ROW_TYPES[dt], T, K, codes, scales,
+            _optional(dev, values_dev, (T, K), dt, "values"), _stream_ptr(stream)))
+
+    def mx_linear_dev(self, x_codes_dev, x_scales_dev, w_codes_dev, w_scales_dev, y_dev, bias_dev=None, act: str = "none",
+                      residual_dev=None, gate_beta=None, value_beta=None, stream=None):
+        """``y = act(x @ W^T + bias) + residual`` of quantized rows (``mx_quantize_dev``): x codes [T, K / 2] and scales
+        [T, K / 32], W codes [M, K / 2] and scales [M, K / 32], K a multiple of 32; products exact, fp32 sums, rounded
+        once to bf16.  act, bias float32 [M], residual (y itself: in place) and y [T, M] or, gated, [T, M / 2] as in
+        ``Matrix.linear_act_dev``.  Asynchronous; allocates nothing and uses no scratch (capturable, any number of calls
+        at once).  A row's last bits may depend on T."""
+        code, gb, vb, gated = _epilogue_act(act, gate_beta, value_beta)
+        dev, (T, K), M = self.device, _shape2(x_codes_dev, "x codes"), _shape2(w_codes_dev, "w codes")[0]
+        K *= 2
+        x, xs = _mx_operands(dev, x_codes_dev, x_scales_dev, (T,), K, "x")
+        w, ws = _mx_operands(dev, w_codes_dev, w_scales_dev, (M,), K, "w")
+        out = (T, M // 2 if gated else M)
+        check(_lib.load().rmoe_mx_linear_dev(
+            self._h, x, xs, T, K, w, ws, M, _optional(dev, bias_dev, (M,), "float32", "bias"), code, gb, vb,
+            None if residual_dev is None else _bf16_operand(dev, residual_dev, out, "residual"),
+            _bf16_operand(dev, y_dev, out, "y"), _stream_ptr(stream)))
+
+    def mx_experts_linear_dev(self, rows_codes_dev, rows_scales_dev, w_codes_dev, w_scales_dev, offsets_dev, y_dev,
+                              bias_dev=None, act: str = "none", residual_dev=None, gate_beta=None, value_beta=None,
+                              stream=None):
+        """``mx_linear_dev`` over sorted rows, each with its expert's matrix: row p of ``offsets[e] <= p < offsets[e + 1]``
+        (int32 [E + 1], of ``sort_tokens_dev``) with W codes [E, M, K / 2] and scales [E, M, K / 32], bias float32 [E, M].
+        Rows from ``offsets[E]`` on stay as they were."""
+        code, gb, vb, gated = _epilogue_act(act, gate_beta, value_beta)
+        dev, (n, K) = self.device, _shape2(rows_codes_dev, "rows codes")
+        K *= 2
+        try:
+            E, M, _ = w_codes_dev.shape
+        except (AttributeError, ValueError):
+            raise ValueError(f"w codes must be [E, M, K / 2], got shape {tuple(getattr(w_codes_dev, 'shape', ()))}") from None
+        x, xs = _mx_operands(dev, rows_codes_dev, rows_scales_dev, (n,), K, "rows")
+        w, ws = _mx_operands(dev, w_codes_dev, w_scales_dev, (E, M), K, "w")
+        out = (n, M // 2 if gated else M)
+        check(_lib.load().rmoe_mx_experts_linear_dev(
+            self._h, x, xs, n, K, w, ws, M, _operand(dev, offsets_dev, (E + 1,), "int32", "offsets"), E,
+            _optional(dev, bias_dev, (E, M), "float32", "bias"), code, gb, vb,
+            None if residual_dev is None else _bf16_operand(dev, residual_dev, out, "residual"),
+            _bf16_operand(dev, y_dev, out, "y"), _stream_ptr(stream)))
+
+    # ------------------------------------------------- norms around a block --
+    def norm_dev(self, x_dev, weight_dev, h_dev=None, codes_dev=None, scales_dev=None, eps: float = 1e-6, stream=None):
+        """The norm before a block: ``h = x (mean x^2 + eps)^-1/2 weight`` by row, in fp32, rounded once.  x and h [T, H]
+        bfloat16 (or int16 bits), float16 or float32, weight float32 [H], H up to 8192; codes and scales: h as microscaled 4-bit rows
+        (``mx_quantize_dev`` of it), with h or without.  Asynchronous; allocates nothing and uses no scratch."""
+        self._norm(None, x_dev, None, None, None, 1.0, weight_dev, h_dev, codes_dev, scales_dev, eps, stream)
+
+    def residual_norm_dev(self, block_dev, residual_dev, y_dev, post_weight_dev=None, gate_dev=None, scale: float = 1.0,
+                          pre_weight_dev=None, h_dev=None, codes_dev=None, scales_dev=None, eps: float = 1e-6, stream=None):
+        """What stands between two blocks, in one pass: ``y = scale * residual + gate * N(block) post_weight`` and ``h =
+        N(y) pre_weight``, N(v) = v (mean v^2 + eps)^-1/2 by row.  Rows [T, H] of one type; post_weight None: no norm after
+        the block; gate None, float32 [H] (by column), float32 [T, 1] (by row) or [T, H] of the rows' type; pre_weight float32 [H] with h, or
+        codes and scales (h as microscaled 4-bit rows), or both, or none of them.  y may be residual or block, h may be
+        block."""
+        if block_dev is None or y_dev is None:
+            raise ValueError("residual_norm_dev takes a block's result and y")
+        self._norm(block_dev, residual_dev, y_dev, post_weight_dev, gate_dev, scale, pre_weight_dev, h_dev, codes_dev,
+                   scales_dev, eps, stream)
+
+    def _norm(self, block, residual, y, post, gate, scale, pre, h, codes, scales, eps, stream):
+        dt, dev = _row_type(residual, "residual" if block is not None else "x"), self.device
+        T, H = _shape2(residual, "residual" if block is not None else "x")
+        rows = (T, H)
+        if (codes is None) != (scales is None):
+            raise ValueError("codes and scales go together")
+        c, s = (None, None) if codes is None else _mx_operands(dev, codes, scales, (T,), -(-H // 32) * 32, "h")
+        g, kind = _gate_operand(dev, gate, T, H, dt, "gate")
+        check(_lib.load().rmoe_residual_norm_dev(
+            self._h, _optional(dev, block, rows, dt, "block"), _operand(dev, residual, rows, dt, "residual"), _ROW_TYPES[dt],
+            T, H, _optional(dev, post, (H,), "float32", "post weight"), g, kind, float(scale),
+            _optional(dev, pre, (H,), "float32", "pre weight"), float(eps), _optional(dev, y, rows, dt, "y"),
+            _optional(dev, h, rows, dt, "h"), c, s, _stream_ptr(stream)))
+
+    @staticmethod
+    def norm_backward_work(T: int, H: int) -> int:
+        """Float32 elements of work memory that the gradients of the norms take for T rows of width H."""
+        n = C.c_size_t()
+        call("rmoe_norm_backward_work", int(T), int(H), C.byref(n))
+        return n.value
+
+    def norm_backward_dev(self, dh_dev, x_dev, weight_dev, dx_dev, work_dev, dweight_dev=None, dy_dev=None, eps: float = 1e-6,
+                          stream=None):
+        """Gradients of ``norm_dev``: dx, and float32 dweight [H] (optional).  dy (optional) is added to dx: the gradient
+        that x has where the residual stream goes on; dx may be dy.  work as in ``residual_norm_backward_dev``."""
+        self._norm_backward(dy_dev, dh_dev, None, x_dev, None, dx_dev, work_dev, None, None, None, None, 1.0, weight_dev,
+                            dweight_dev, eps, stream)
+
+    def residual_norm_backward_dev(self, dy_dev, dh_dev, block_dev, y_dev, dblock_dev, dresidual_dev, work_dev,
+                                   post_weight_dev=None, dpost_weight_dev=None, gate_dev=None, dgate_dev=None,
+                                   scale: float = 1.0, pre_weight_dev=None, dpre_weight_dev=None, eps: float = 1e-6,
+                                   stream=None):
+        """Gradients of ``residual_norm_dev`` from dy and dh (one of them may be None; without dh no pre_weight), from its
+        block and its y: dblock, dresidual, and where given float32 dpost_weight and dpre_weight [H] and dgate (as the gate).
+        dresidual may be dy, dblock may be dh.  work: float32 [norm_backward_work(T, H)] or more, this call's alone while it runs."""
+        if block_dev is None or dblock_dev is None:
+            raise ValueError("residual_norm_backward_dev takes a block's result and dblock")
+        self._norm_backward(dy_dev, dh_dev, block_dev, y_dev, dblock_dev, dresidual_dev, work_dev, post_weight_dev,
+                            dpost_weight_dev, gate_dev, dgate_dev, scale, pre_weight_dev, dpre_weight_dev, eps, stream)
+
+    def _norm_backward(self, dy, dh, block, y, dblock, dresidual, work, post, dpost, gate, dgate, scale, pre, dpre, eps, stream):
+        dt, dev = _row_type(y, "y"), self.device
+        T, H = _shape2(y, "y")
+        rows, vector = (T, H), (H,)
+        g, kind = _gate_operand(dev, gate, T, H, dt, "gate")
+        if dgate is not None and gate is None:
+            raise ValueError("a gradient goes with its gate")
+        dg = None if dgate is None else _operand(dev, dgate, tuple(gate.shape), _dtype_name(gate), "dgate")
+        shape = tuple(getattr(work, "shape", ()))
+        if len(shape) != 1 or shape[0] < self.norm_backward_work(T, H):
+            raise ValueError(f"work must be float32 [norm_backward_work({T}, {H})] or more, got shape {shape}")
+        check(_lib.load().rmoe_residual_norm_backward_dev(
+            self._h, _optional(dev, dy, rows, dt, "dy"), _optional(dev, dh, rows, dt, "dh"),
+            _optional(dev, block, rows, dt, "block"), _operand(dev, y, rows, dt, "y"), _ROW_TYPES[dt], T, H,
+            _optional(dev, post, vector, "float32", "post weight"), g, kind, float(scale),
+            _optional(dev, pre, vector, "float32", "pre weight"), float(eps), _optional(dev, dblock, rows, dt, "dblock"),
+            _operand(dev, dresidual, rows, dt, "dresidual"), _optional(dev, dpost, vector, "float32", "dpost weight"), dg,
+            _optional(dev, dpre, vector, "float32", "dpre weight"), _operand(dev, work, shape, "float32", "work"),
+            _stream_ptr(stream)))
 
     def dispatch(self, top_ids, n_experts: int) -> tuple[np.ndarray, np.ndarray]:
         ids = np.ascontiguousarray(top_ids, dtype=np.int32)

@@ -1,0 +1,316 @@
+"""GPU: the norms before and after a block with gate and residual scale (csrc/block_norm.hip) against the formulas in 64
+bits, and their gradients also against differences.
+
+Bounds, with u = 2^-24.  A row's sum of H squares: each thread adds up to 16 of them, then 6 + 8 additions join the lanes
+and waves, so it is off by at most 32 u of itself; (.)^-1/2 halves that and adds a division, a root and a division: n and m
+are off by 20 u of themselves.  y is off by 24 u (|g u| + |scale r|), then one rounding (finfo.eps / 2 of the result and half
+the type's least subnormal); h likewise by 24 u |h| and one rounding.  In the gradient D = dy + m a - y m^3 S / H, S = sum a
+y: 128 u of the sum A of its terms' magnitudes (m^3: 60; S: 32 of sum |a y|; products and sums: the rest); dblock by twice
+that bound carried through its own two terms.  Columns' sums over T rows add up to T / 512 + 40 more values: (T / 512 + 168)
+2 u of the sum of the magnitudes."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+TYPES = [torch.bfloat16, torch.float16, torch.float32]
+U = 2.0 ** -24
+EPS = 1e-5
+GATES = ["none", "column", "row", "full"]
+
+
+def _stream():
+    return torch.cuda.current_stream()
+
+
+def _half_step(dtype):
+    f = torch.finfo(dtype)
+    return f.eps / 2, f.smallest_normal * f.eps / 2
+
+
+def _case(T, H, dtype, post, gate, seed):
+    g = torch.Generator().manual_seed(seed)
+    s = {"block": torch.randn(T, H, generator=g).to(dtype), "residual": (3 * torch.randn(T, H, generator=g)).to(dtype),
+         "post": 1 + 0.3 * torch.randn(H, generator=g) if post else None, "pre": 1 + 0.3 * torch.randn(H, generator=g),
+         "dy": torch.randn(T, H, generator=g).to(dtype), "dh": torch.randn(T, H, generator=g).to(dtype)}
+    s["gate"] = {"none": None, "column": 0.5 * torch.randn(H, generator=g), "row": 0.5 * torch.randn(T, 1, generator=g),
+                 "full": (0.5 * torch.randn(T, H, generator=g)).to(dtype)}[gate]
+    return s
+
+
+def _dev(s):
+    return {k: None if v is None else v.cuda() for k, v in s.items()}
+
+
+def _n(x):
+    return (x.square().mean(1, keepdim=True) + EPS).rsqrt()
+
+
+def _forward64(s, scale):
+    """(y, magnitude of its terms) in 64 bits."""
+    b, r = s["block"].double(), s["residual"].double()
+    u = b if s["post"] is None else b * _n(b) * s["post"].double()
+    if s["gate"] is not None:
+        u = u * s["gate"].double()
+    return scale * r + u, u.abs() + (scale * r).abs()
+
+
+def _run(ctx, d, scale, y=None, h=None, codes=None, scales=None, stream=None):
+    y = torch.full_like(d["block"], 7) if y is None else y
+    ctx.residual_norm_dev(d["block"], d["residual"], y, post_weight_dev=d["post"], gate_dev=d["gate"], scale=scale,
+                          pre_weight_dev=None if h is None and codes is None else d["pre"], h_dev=h, codes_dev=codes, scales_dev=scales, eps=EPS,
+                          stream=stream or _stream())
+    return y
+
+
+def _check_h(h, y, pre, dtype):
+    want = y.double() * _n(y.double()) * pre.double()
+    rel, least = _half_step(dtype)
+    off, bound = (h.double() - want).abs(), want.abs() * (24 * U + rel * (1 + 2.0 ** -10)) + least
+    assert bool((off <= bound).all()), float((off / bound).max())
+
+
+SHAPES = [(1, 1), (1, 7), (3, 8), (2, 33), (5, 64), (1, 2048), (17, 511), (9, 520), (445, 2560), (4, 4096), (3, 4097), (2, 8192),
+          (6, 5001), (2, 8191)]
+
+
+@pytest.mark.parametrize("T,H", SHAPES)
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("post,gate", [(True, "column"), (False, "none"), (True, "row"), (False, "full"), (True, "none")])
+def test_forward(gpu_ctx, T, H, dtype, post, gate):
+    s = _case(T, H, dtype, post, gate, T + H)
+    d, scale = _dev(s), 0.75
+    P = -(-H // 32) * 32
+    h = torch.full_like(d["block"], 7)
+    codes = torch.full((T, P // 2), 0xEE, dtype=torch.uint8, device="cuda")
+    scales = torch.full((T, P // 32), 0xEE, dtype=torch.uint8, device="cuda")
+    y = _run(gpu_ctx, d, scale, h=h, codes=codes, scales=scales)
+    want, size = _forward64(s, scale)
+    rel, least = _half_step(dtype)
+    off, bound = (y.cpu().double() - want).abs(), 24 * U * size + want.abs() * rel * (1 + 2.0 ** -10) + least
+    assert bool((off <= bound).all()), float((off / bound).max())
+    _check_h(h.cpu(), y.cpu(), s["pre"], dtype)
+    # The codes are those of the stored rows; by themselves, and without h, the same.
+    c2, s2 = torch.zeros_like(codes), torch.zeros_like(scales)
+    gpu_ctx.mx_quantize_dev(h, c2, s2, stream=_stream())
+    assert torch.equal(codes, c2) and torch.equal(scales, s2)
+    codes.fill_(0xEE), scales.fill_(0xEE)
+    assert torch.equal(_run(gpu_ctx, d, scale, codes=codes, scales=scales), y)
+    assert torch.equal(codes, c2) and torch.equal(scales, s2)
+    # Without a norm before; the norm of the stored rows alone.
+    assert torch.equal(_run(gpu_ctx, d, scale), y)
+    h2 = torch.full_like(h, 7)
+    gpu_ctx.norm_dev(y, d["pre"], h2, eps=EPS, stream=_stream())
+    assert torch.equal(h, h2)
+    codes.fill_(0xEE), scales.fill_(0xEE)
+    gpu_ctx.norm_dev(y, d["pre"], codes_dev=codes, scales_dev=scales, eps=EPS, stream=_stream())
+    assert torch.equal(codes, c2) and torch.equal(scales, s2)
+    # In place: y over the residual and h over the block, y over the block.
+    e = _dev(s)
+    _run(gpu_ctx, e, scale, y=e["residual"], h=e["block"])
+    assert torch.equal(e["residual"], y) and torch.equal(e["block"], h)
+    e = _dev(s)
+    _run(gpu_ctx, e, scale, y=e["block"], h=h2)
+    assert torch.equal(e["block"], y) and torch.equal(h2, h)
+
+
+def test_rows_of_zeros_infinities_and_nan(gpu_ctx):
+    """A row of zeros has the norm 0; NaN and infinities stay in their rows."""
+    for dtype in TYPES:
+        s = _case(6, 96, dtype, True, "none", 1)
+        s["block"][1] = 0.0
+        s["residual"][1] = 0.0
+        s["block"][2, 5], s["block"][3, 7], s["residual"][4, 0] = float("nan"), float("inf"), float("inf")
+        h = torch.empty(6, 96, dtype=dtype, device="cuda")
+        y = _run(gpu_ctx, _dev(s), 1.0, h=h)
+        assert not y[1].any() and not h[1].any()
+        assert bool(torch.isfinite(h[[0, 1, 5]]).all()) and bool(torch.isfinite(y[[0, 1, 5]]).all())
+        assert bool(torch.isnan(y[2]).all()) and bool(torch.isnan(h[2]).all())
+        assert bool(torch.isnan(y[3, 7])) and bool(torch.isnan(h[3]).all())
+        assert bool(torch.isinf(y[4, 0])) and bool(torch.isnan(h[4, 0])) and not h[4, 1:].any()
+
+
+def test_rows_at_any_address(gpu_ctx):
+    """Rows that start inside 16 bytes give the bits of aligned ones; vectors that do, too."""
+    T, H = 5, 136
+    for dtype in TYPES:
+        s = _case(T, H, dtype, True, "full", 3)
+        d = _dev(s)
+        h = torch.empty_like(d["block"])
+        y = _run(gpu_ctx, d, 0.5, h=h)
+
+        def shifted(t):
+            buf = torch.zeros(t.numel() + 9, dtype=t.dtype, device="cuda")
+            v = buf[3:3 + t.numel()].view(t.shape)
+            v.copy_(t)
+            return v
+
+        e = {k: None if v is None else shifted(v) for k, v in d.items()}
+        h2 = shifted(torch.zeros_like(h))
+        assert torch.equal(_run(gpu_ctx, e, 0.5, y=shifted(torch.zeros_like(y)), h=h2), y) and torch.equal(h, h2)
+        a, b = _backward(gpu_ctx, d, y, "full", 0.5), _backward(gpu_ctx, e, shifted(y), "full", 0.5)
+        for k in a:
+            assert torch.equal(a[k], b[k]), k
+
+
+# -------------------------------------------------------------------- gradients --
+def _backward(ctx, d, y, gate, scale, dy=True, dh=True, out=None, stream=None, work=None):
+    T, H = y.shape
+    o = {"dblock": torch.full_like(y, 7), "dresidual": torch.full_like(y, 7)} if out is None else out
+    if dh:
+        o["dpre"] = torch.full((H,), 7.0, device="cuda")
+    if d["post"] is not None:
+        o["dpost"] = torch.full((H,), 7.0, device="cuda")
+    if gate != "none":
+        o["dgate"] = torch.full_like(d["gate"], 7)
+    work = torch.full((ctx.norm_backward_work(T, H),), float("nan"), device="cuda") if work is None else work
+    ctx.residual_norm_backward_dev(d["dy"] if dy else None, d["dh"] if dh else None, d["block"], y, o["dblock"],
+                                   o["dresidual"], work, post_weight_dev=d["post"], dpost_weight_dev=o.get("dpost"),
+                                   gate_dev=d["gate"], dgate_dev=o.get("dgate"), scale=scale,
+                                   pre_weight_dev=d["pre"] if dh else None, dpre_weight_dev=o.get("dpre"), eps=EPS,
+                                   stream=stream or _stream())
+    return o
+
+
+def _backward64(s, y, gate, scale, dy=True, dh=True):
+    """{name: (gradient, magnitude of its terms)} in 64 bits."""
+    b, y = s["block"].double(), y.double()
+    T, H = b.shape
+    zero = torch.zeros_like(b)
+    dyv, dhv = s["dy"].double() if dy else zero, s["dh"].double() if dh else zero
+    out, D, A = {}, dyv, dyv.abs()
+    if dh:
+        m, a = _n(y), dhv * s["pre"].double()
+        D = D + m * a - y * m ** 3 * (a * y).mean(1, keepdim=True)
+        A = A + (m * a).abs() + y.abs() * m ** 3 * (a * y).abs().mean(1, keepdim=True)
+        out["dpre"] = ((dhv * y * m).sum(0), (dhv * y * m).abs().sum(0))
+    out["dresidual"] = (scale * D, scale * A)
+    g = 1.0 if s["gate"] is None else s["gate"].double()
+    ga = 1.0 if s["gate"] is None else g.abs()
+    n, w = (_n(b), s["post"].double()) if s["post"] is not None else (1.0, 1.0)
+    wa = w.abs() if s["post"] is not None else 1.0
+    u = b * n * w
+    if gate != "none":
+        dims = {"column": 0, "row": 1, "full": None}[gate]
+        out["dgate"] = (D * u, A * u.abs()) if dims is None else ((D * u).sum(dims, keepdim=gate == "row"),
+                                                                  (A * u.abs()).sum(dims, keepdim=gate == "row"))
+    du, dA = g * D, ga * A
+    if s["post"] is None:
+        out["dblock"] = (du, dA)
+    else:
+        v, vA = du * w, dA * wa
+        out["dblock"] = (n * v - b * n ** 3 * (v * b).mean(1, keepdim=True),
+                         n * vA + b.abs() * n ** 3 * (vA * b.abs()).mean(1, keepdim=True))
+        out["dpost"] = ((du * b * n).sum(0), (dA * (b * n).abs()).sum(0))
+    return out
+
+
+def _check_gradients(got, want, T, dtype):
+    rel, least = _half_step(dtype)
+    for k, (v, size) in want.items():
+        g = got[k].cpu()
+        if k in ("dpre", "dpost") or g.dtype == torch.float32 and k == "dgate" and dtype != torch.float32:
+            bound = (T / 512 + 168 + (64 if k == "dgate" else 0)) * 2 * U * size + 1e-40
+        else:
+            bound = 512 * U * size + v.abs() * rel * (1 + 2.0 ** -10) + least
+            if k == "dgate":  # fp32 rows: full gates, or sums of them
+                bound = bound + (T / 512 + 232) * 2 * U * size
+        off = (g.double() - v).abs()
+        assert bool((off <= bound).all()), (k, float((off / bound).max()))
+
+
+@pytest.mark.parametrize("T,H", [(1, 1), (1, 7), (2, 33), (5, 64), (1, 2048), (17, 511), (445, 520), (1030, 96), (9, 2560), (3, 4097),
+                                 (2, 8192), (600, 5001)])
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("post,gate", [(True, "column"), (False, "none"), (True, "row"), (False, "full"), (True, "none"),
+                                       (False, "column"), (True, "full")])
+def test_backward(gpu_ctx, T, H, dtype, post, gate):
+    s = _case(T, H, dtype, post, gate, T + H + 1)
+    d, scale = _dev(s), 0.75
+    y = _run(gpu_ctx, d, scale)
+    got = _backward(gpu_ctx, d, y, gate, scale)
+    _check_gradients(got, _backward64(s, y.cpu(), gate, scale), T, dtype)
+    again = _backward(gpu_ctx, d, y, gate, scale)
+    for k in got:
+        assert torch.equal(got[k], again[k]), k
+    if T * H < 10000:
+        for dy, dh in ((True, False), (False, True)):
+            part = _backward(gpu_ctx, d, y, gate, scale, dy=dy, dh=dh)
+            _check_gradients(part, _backward64(s, y.cpu(), gate, scale, dy=dy, dh=dh), T, dtype)
+    # In place: dresidual over dy, dblock over dh.
+    e = _dev(s)
+    _backward(gpu_ctx, e, y, gate, scale, out={"dresidual": e["dy"], "dblock": e["dh"]})
+    assert torch.equal(e["dy"], got["dresidual"]) and torch.equal(e["dh"], got["dblock"])
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("T,H", [(1, 5), (70, 264)])
+def test_norm_backward(gpu_ctx, T, H, dtype):
+    s = _case(T, H, dtype, False, "none", 5)
+    d = _dev(s)
+    x, work = d["residual"], torch.empty(gpu_ctx.norm_backward_work(T, H), device="cuda")
+    dx, dw = torch.empty_like(x), torch.empty(H, device="cuda")
+    for dy in (False, True):
+        gpu_ctx.norm_backward_dev(d["dh"], x, d["pre"], dx, work, dweight_dev=dw, dy_dev=d["dy"] if dy else None, eps=EPS,
+                                  stream=_stream())
+        want = _backward64(s, s["residual"], "none", 1.0, dy=dy)
+        _check_gradients({"dresidual": dx, "dpre": dw}, {k: want[k] for k in ("dresidual", "dpre")}, T, dtype)
+
+
+@pytest.mark.parametrize("post,gate", [(True, "column"), (True, "row"), (False, "full"), (True, "none")])
+def test_gradients_against_differences(gpu_ctx, post, gate):
+    """Along random directions: (L(x + t d) - L(x - t d)) / 2 t in 64 bits, L = <dy, y> + <dh, h>, with fp32 gradients.  The
+    difference is off by O(t^2) (t = 1e-4: under 1e-6 of the terms) and its cancellation (1e-12); the gradients by 2^-14."""
+    T, H, scale, t = 6, 72, 0.75, 1e-4
+    s = _case(T, H, torch.float32, post, gate, 11)
+    d = _dev(s)
+    y64 = _forward64(s, scale)[0]
+    y = y64.float()
+    got = _backward(gpu_ctx, d, y.cuda(), gate, scale)
+
+    def loss(p):
+        y = _forward64(p, scale)[0]
+        return float((s["dy"].double() * y).sum() + (s["dh"].double() * (y * _n(y) * p["pre"].double())).sum())
+
+    g = torch.Generator().manual_seed(2)
+    for name, grad in (("block", "dblock"), ("residual", "dresidual"), ("post", "dpost"), ("pre", "dpre"), ("gate", "dgate")):
+        if s[name] is None:
+            continue
+        direction = torch.randn(s[name].shape, generator=g, dtype=torch.float64)
+        up, down = dict(s), dict(s)
+        up[name], down[name] = s[name].double() + t * direction, s[name].double() - t * direction
+        want = (loss(up) - loss(down)) / (2 * t)
+        along = got[grad].cpu().double() * direction
+        assert abs(float(along.sum()) - want) <= 2.0 ** -14 * float(along.abs().sum()) + 1e-6, name
+
+
+def test_on_other_streams_and_captured(gpu_ctx):
+    """Forward and backward in a graph of another stream, replayed between eager calls with new inputs."""
+    T, H = 37, 320
+    d = _dev(_case(T, H, torch.bfloat16, True, "column", 1))
+    y, h = torch.zeros_like(d["block"]), torch.zeros_like(d["block"])
+    work = torch.empty(gpu_ctx.norm_backward_work(T, H), device="cuda")
+    out = {"dblock": torch.zeros_like(y), "dresidual": torch.zeros_like(y)}
+    st, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=st):
+        _run(gpu_ctx, d, 0.5, y=y, h=h, stream=torch.cuda.current_stream())
+        out = _backward(gpu_ctx, d, y, "column", 0.5, out=out, stream=torch.cuda.current_stream(), work=work)
+    for turn in range(3):
+        new = _case(T, H, torch.bfloat16, True, "column", 100 + turn)
+        for k, v in new.items():
+            d[k].copy_(v)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(st):
+            graph.replay()
+        torch.cuda.synchronize()
+        h2 = torch.empty_like(h)
+        y2 = _run(gpu_ctx, d, 0.5, h=h2)
+        assert torch.equal(y, y2) and torch.equal(h, h2)
+        for k, v in _backward(gpu_ctx, d, y2, "column", 0.5).items():
+            assert torch.equal(out[k], v), k
