@@ -2,6 +2,7 @@
 // matrix or of each row's expert, on the scaled MFMA: codes and scale bytes go into the matrix pipes as they are
 // held, products are exact, sums fp32.
 #include <algorithm>
+#include <type_traits>
 
 #include "linear_act.h"
 #include "mx.h"
@@ -12,12 +13,16 @@ namespace {
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kFp4 = 4;         // the instruction's number of the e2m1 format, for both operands
 constexpr int kScaleOne = 127;  // a scale byte of 2^0
 
 // Codes as the instruction's operand: its upper half belongs to the wider formats.
 __device__ __forceinline__ i32x8 operand(const i32x4& v) { return i32x8{v.x, v.y, v.z, v.w, 0, 0, 0, 0}; }
+
+// bf16 bits of v (RTNE), by the conversion instruction.
+__device__ __forceinline__ uint32_t bf16_bits(float v) { return __builtin_bit_cast(uint16_t, (__bf16)v); }
 
 // Four consecutive outputs of row t from the sums z (and u of the up half).
 struct Epilogue {
@@ -157,11 +162,338 @@ hipError_t launch_few(const MxLin& a, hipStream_t st) {
   return hipGetLastError();
 }
 
+// ----------------------------------------------------------------- many rows --
+// Tiles of 32 MA WA weight rows by 32 NB WB rows of x; a wave takes 32 MA by 32 NB of them as 32 x 32 MFMAs
+// of 64 columns.  K goes by in tiles of 128 columns: 64 bytes of codes and a dword of scale bytes a row, in LDS in
+// three stages.  Codes are copied there past the registers, two tiles ahead of their use; scale bytes are
+// fetched 16 a row (four tiles) at a time and put beside the codes.  A lane's row of a fragment is lane % 32, and
+// of a tile's four blocks it holds 2 h and 2 h + 1, h = lane / 32, for the tile's two MFMA steps.
+// A gated wave's rows are 16 MA gate rows and the up rows of the same outputs.
+constexpr int kStages = 3;
+constexpr int kKTile = 4 * kMxBlock;
+
+template <int MA, int NB, int WA, int WB>
+struct TileShape {
+  static constexpr int kThreads = 64 * WA * WB, BW = 32 * MA * WA, BT = 32 * NB * WB, R = BW + BT;
+  static constexpr int kCodes = R * 64, kStage = kCodes + R * 4;
+  static constexpr int kCopies = R / 16 / (WA * WB);  // a wave's copies of a K tile, 16 rows each
+  static constexpr int kScales = (R + kThreads - 1) / kThreads;
+  static constexpr size_t lds(bool gated) {
+    const size_t out = (size_t)WA * WB * 32 * ((gated ? 16 : 32) * MA + 4) * 4;
+    return out > (size_t)kStages * kStage ? out : (size_t)kStages * kStage;
+  }
+};
+
+// 16 bytes a lane from base + offset to LDS at `lds` + 16 lane.
+__device__ __forceinline__ void copy16(const void* base, uint32_t offset, uint32_t lds) {
+  uint32_t saved;
+  asm volatile(
+      "s_mov_b32 %0, m0\n\t"
+      "s_mov_b32 m0, %3\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dwordx4 %1, %2\n\t"
+      "s_mov_b32 m0, %0"
+      : "=&s"(saved)
+      : "v"(offset), "s"(base), "s"(__builtin_amdgcn_readfirstlane(lds))
+      : "memory");
+}
+// All but this wave's last kPending copies have landed, then the workgroup meets.
+template <int kPending>
+__device__ __forceinline__ void copies_landed() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kPending) : "memory");
+  __syncthreads();
+}
+
+// Scale bytes 16 w .. 16 w + 15 of a row of kb; those past its end are anything.
+__device__ __forceinline__ uint4 load_scales(const uint8_t* row, int w, int kb) {
+  uint4 v = make_uint4(0u, 0u, 0u, 0u);
+  if (16 * w + 16 <= kb) {
+    __builtin_memcpy(&v, row + 16 * w, 16);
+    return v;
+  }
+  uint32_t d[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int b = 16 * w + 4 * i;
+    if (b + 4 <= kb) {
+      __builtin_memcpy(&d[i], row + b, 4);
+    } else if (b < kb) {
+#pragma unroll
+      for (int k = 0; k < 3; ++k) d[i] |= (uint32_t)row[min(b + k, kb - 1)] << (8 * k);
+    }
+  }
+  return make_uint4(d[0], d[1], d[2], d[3]);
+}
+
+template <int MA, int NB, int WA, int WB, bool kGated>
+__global__ __launch_bounds__(64 * WA * WB, 2) void mx_tiles_kernel(MxLin a, int n_nt) {
+  typedef TileShape<MA, NB, WA, WB> S;
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  constexpr int kOut = (kGated ? 16 : 32) * MA;  // outputs of a wave
+  RowTiles<S::BT> rt;
+  const int n_mt = a.offsets ? rt.total(a.offsets, a.n_experts, a.n) : (a.n + S::BT - 1) / S::BT;
+  // XCD x takes a contiguous eighth of the tiles: by expert the weight tiles of a row tile back to back, else
+  // blocks of up to eight row tiles for each weight tile, so that both operands' tiles meet again in its L2.
+  const long total = (long)n_mt * n_nt, per = (total + 7) / 8, slot = blockIdx.x / 8;
+  const long id = (long)(blockIdx.x % 8) * per + slot;
+  if (slot >= per || id >= total) return;
+  int nt, e = 0, row0, nrow;
+  if (a.offsets) {
+    nt = (int)(id % n_nt);
+    rt.find((int)(id / n_nt), e, row0, nrow);
+  } else {
+    constexpr int kBlock = 8;
+    const long group = id / ((long)kBlock * n_nt);
+    const int m0 = (int)group * kBlock, nm = min(kBlock, n_mt - m0), in = (int)(id - group * kBlock * n_nt);
+    nt = in / nm;
+    row0 = (m0 + in % nm) * S::BT;
+    nrow = min(S::BT, a.n - row0);
+  }
+  const int tid = threadIdx.x, lane = tid & 63, wave = wave_id(), l32 = lane & 31, h = lane >> 5;
+  const int wa = wave % WA, wb = wave / WA;
+  const int kb = a.K / kMxBlock, tiles = (kb + 3) / 4, rem = kb % 4;
+  const uint32_t ldb = (uint32_t)a.K / 2;
+  const int width = kGated ? a.M / 2 : a.M;
+  // Row of an LDS row slot: of the weights (e's matrix) or of x; rows past the ends repeat the last one.
+  auto weight_row = [&](int r) {
+    const int w = r / (32 * MA), rr = r % (32 * MA), o = (nt * WA + w) * kOut + rr % kOut;
+    return (kGated && rr >= kOut ? width : 0) + min(o, width - 1);
+  };
+  auto token_row = [&](int r) { return min(r - S::BW, nrow - 1); };
+
+  const uint8_t* cbase[S::kCopies];
+  uint32_t coff[S::kCopies];
+#pragma unroll
+  for (int j = 0; j < S::kCopies; ++j) {
+    const int r0 = 16 * (wave * S::kCopies + j), r = r0 + (lane >> 2);
+    if (r0 < S::BW) {
+      const int first = weight_row(r0);
+      cbase[j] = a.w + ((size_t)e * a.M + first) * ldb;
+      coff[j] = (uint32_t)(weight_row(r) - first) * ldb;
+    } else {
+      const int first = token_row(r0);
+      cbase[j] = a.x + ((size_t)row0 + first) * ldb;
+      coff[j] = (uint32_t)(token_row(r) - first) * ldb;
+    }
+  }
+  // Chunk c of a row's four stands at c ^ (row / 2 % 4): eight rows' chunks of one number are in different banks.
+  const int cchunk = (lane & 3) ^ ((lane >> 3) & 3);
+  auto copies = [&](int t, int stage) {
+    const uint32_t k = (uint32_t)min(4 * t + cchunk, kb - 1) * 16u;
+#pragma unroll
+    for (int j = 0; j < S::kCopies; ++j)
+      copy16(cbase[j], coff[j] + k, (uint32_t)(stage * S::kStage + 16 * (wave * S::kCopies + j) * 64));
+  };
+  const uint8_t* sbase[S::kScales];
+#pragma unroll
+  for (int j = 0; j < S::kScales; ++j) {
+    const int r = min(tid + j * S::kThreads, S::R - 1);
+    sbase[j] = r < S::BW ? a.ws + ((size_t)e * a.M + weight_row(r)) * kb : a.xs + ((size_t)row0 + token_row(r)) * kb;
+  }
+  uint4 q[S::kScales], qn[S::kScales];
+  auto put_scales = [&](int t, int stage) {  // called for t = 0, 1, 2, ...
+    if ((t & 3) == 0) {
+#pragma unroll
+      for (int j = 0; j < S::kScales; ++j) {
+        q[j] = t == 0 ? load_scales(sbase[j], 0, kb) : qn[j];
+        if (t + 4 < tiles) qn[j] = load_scales(sbase[j], t / 4 + 1, kb);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < S::kScales; ++j) {
+      uint32_t v = q[j].x;
+      q[j] = make_uint4(q[j].y, q[j].z, q[j].w, 0u);
+      if (rem && t == tiles - 1) v = (v & ~(~0u << (8 * rem))) | 0x7f7f7f7fu << (8 * rem);  // blocks past the end: 2^0
+      const int r = tid + j * S::kThreads;
+      if (S::R % S::kThreads == 0 || r < S::R) *reinterpret_cast<uint32_t*>(lds + stage * S::kStage + S::kCodes + 4 * r) = v;
+    }
+  };
+
+  f32x16 acc[MA][NB];
+#pragma unroll
+  for (int m = 0; m < MA; ++m)
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[m][n][i] = 0.f;
+
+  struct Frags {
+    i32x4 a[MA], b[NB];
+  } f[2];
+  uint32_t sa[MA], sb[NB];
+  const int arow = wa * 32 * MA + l32, brow = S::BW + wb * 32 * NB + l32;  // multiples of 32 away: l32's place
+  uint32_t at[2];  // of a lane's chunk in step 0 and 1 from its row's start
+#pragma unroll
+  for (int s = 0; s < 2; ++s) at[s] = (uint32_t)((2 * h + s) ^ ((l32 >> 1) & 3)) * 16u;
+  auto read = [&](Frags& g, int stage, int s) {
+    const uint8_t* p = lds + stage * S::kStage + at[s];
+#pragma unroll
+    for (int m = 0; m < MA; ++m) g.a[m] = *reinterpret_cast<const i32x4*>(p + (arow + 32 * m) * 64);
+#pragma unroll
+    for (int n = 0; n < NB; ++n) g.b[n] = *reinterpret_cast<const i32x4*>(p + (brow + 32 * n) * 64);
+  };
+  auto read_scales = [&](int stage) {
+    const uint8_t* p = lds + stage * S::kStage + S::kCodes;
+#pragma unroll
+    for (int m = 0; m < MA; ++m) sa[m] = *reinterpret_cast<const uint32_t*>(p + (arow + 32 * m) * 4) >> (16 * h);
+#pragma unroll
+    for (int n = 0; n < NB; ++n) sb[n] = *reinterpret_cast<const uint32_t*>(p + (brow + 32 * n) * 4) >> (16 * h);
+  };
+  auto multiply = [&](Frags& g, auto step, bool last) {
+    constexpr int s = decltype(step)::value;
+    if (rem && last && 2 * h + s >= rem) {  // blocks past the end: weights of zero
+#pragma unroll
+      for (int m = 0; m < MA; ++m) g.a[m] = i32x4{0, 0, 0, 0};
+    }
+#pragma unroll
+    for (int m = 0; m < MA; ++m)
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+        acc[m][n] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(operand(g.a[m]), operand(g.b[n]), acc[m][n], kFp4, kFp4, s,
+                                                                    (int)sa[m], s, (int)sb[n]);
+  };
+
+#pragma unroll
+  for (int t = 0; t < kStages; ++t)
+    if (t < tiles) {
+      put_scales(t, t);
+      copies(t, t);
+    }
+  if (tiles >= kStages) copies_landed<2 * S::kCopies>();
+  else copies_landed<0>();
+  read(f[0], 0, 0);
+  read_scales(0);
+  int stage = 0;
+  for (int t = 0; t < tiles; ++t) {
+    const int next = stage == kStages - 1 ? 0 : stage + 1;
+    const bool last = t == tiles - 1;
+    read(f[1], stage, 1);
+    multiply(f[0], std::integral_constant<int, 0>(), last);
+    uint32_t ka[MA], kbs[NB];  // this tile's scales, for its second step
+#pragma unroll
+    for (int m = 0; m < MA; ++m) ka[m] = sa[m];
+#pragma unroll
+    for (int n = 0; n < NB; ++n) kbs[n] = sb[n];
+    if (!last) {
+      if (t + 2 < tiles) copies_landed<S::kCopies>();
+      else copies_landed<0>();
+      if (t + kStages < tiles) {
+        put_scales(t + kStages, stage);
+        copies(t + kStages, stage);
+      }
+      read(f[0], next, 0);
+      read_scales(next);
+    }
+    uint32_t na[MA], nb[NB];
+#pragma unroll
+    for (int m = 0; m < MA; ++m) na[m] = sa[m], sa[m] = ka[m];
+#pragma unroll
+    for (int n = 0; n < NB; ++n) nb[n] = sb[n], sb[n] = kbs[n];
+    multiply(f[1], std::integral_constant<int, 1>(), last);
+#pragma unroll
+    for (int m = 0; m < MA; ++m) sa[m] = na[m];
+#pragma unroll
+    for (int n = 0; n < NB; ++n) sb[n] = nb[n];
+    stage = next;
+  }
+  __syncthreads();  // the outputs reuse the stages
+
+  // acc[m][n][i]: weight row 32 m + 8 (i / 4) + 4 h + i % 4, row of x 32 n + l32.  Outputs go through LDS, 32 rows
+  // of x at a time, so that a row's stand together.
+  constexpr int kStride = kOut + 4;
+  float* mine = reinterpret_cast<float*>(lds) + wave * 32 * kStride;
+  const int col0 = (nt * WA + wa) * kOut;
+  const float* bias = a.bias ? a.bias + (size_t)e * a.M : nullptr;
+  const bool wide =
+      width % 8 == 0 && ((reinterpret_cast<uintptr_t>(a.y) | reinterpret_cast<uintptr_t>(a.residual)) & 15) == 0;
+#pragma unroll
+  for (int n = 0; n < NB; ++n) {
+#pragma unroll
+    for (int m = 0; m < (kGated && MA > 1 ? MA / 2 : MA); ++m)
+#pragma unroll
+      for (int g = 0; g < (kGated && MA == 1 ? 2 : 4); ++g) {
+        const int o = 32 * m + 8 * g + 4 * h;
+        f32x4 v;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int c = min(col0 + o + i, width - 1);
+          float z = acc[m][n][4 * g + i];
+          if (bias) z += bias[c];
+          if constexpr (kGated) {
+            float u = MA == 1 ? acc[m][n][4 * (g + 2) + i] : acc[(m + MA / 2) % MA][n][4 * g + i];
+            if (bias) u += bias[width + c];
+            v[i] = act_pair(a.act, z, u, a.gb, a.vb);
+          } else {
+            v[i] = act_single(a.act, z);
+          }
+        }
+        *reinterpret_cast<f32x4*>(mine + l32 * kStride + o) = v;
+      }
+    const int t0 = wb * 32 * NB + 32 * n;
+    constexpr int kLanes = kOut / 8;  // of a row, eight outputs each
+#pragma unroll
+    for (int r = 0; r < 32; r += 64 / kLanes) {
+      const int t = r + lane / kLanes, o = 8 * (lane % kLanes), col = col0 + o;
+      float v[8];
+      *reinterpret_cast<f32x4*>(v) = *reinterpret_cast<const f32x4*>(mine + t * kStride + o);
+      *reinterpret_cast<f32x4*>(v + 4) = *reinterpret_cast<const f32x4*>(mine + t * kStride + o + 4);
+      if (t0 + t >= nrow || col >= width) continue;
+      const size_t to = ((size_t)row0 + t0 + t) * width + col;
+      if (wide) {
+        if (a.residual) {
+          const uint4 r4 = *reinterpret_cast<const uint4*>(a.residual + to);
+          const uint32_t rw[4] = {r4.x, r4.y, r4.z, r4.w};
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[i] += __uint_as_float(i % 2 ? rw[i / 2] & 0xffff0000u : rw[i / 2] << 16);
+        }
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = bf16_bits(v[2 * i]) | bf16_bits(v[2 * i + 1]) << 16;
+        *reinterpret_cast<uint4*>(a.y + to) = make_uint4(w[0], w[1], w[2], w[3]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (col + i < width)
+            a.y[to + i] = (uint16_t)bf16_bits(a.residual ? v[i] + bf16_to_f32(a.residual[to + i]) : v[i]);
+      }
+    }
+  }
+}
+
+template <int MA, int NB, int WA, int WB>
+hipError_t launch_tiles(const MxLin& a, hipStream_t st) {
+  typedef TileShape<MA, NB, WA, WB> S;
+  const bool gated = act_gated(a.act);
+  const int width = gated ? a.M / 2 : a.M, out = S::BW / (gated ? 2 : 1), n_nt = (width + out - 1) / out;
+  const size_t mt = a.offsets ? std::min<size_t>(a.n, (size_t)a.n / S::BT + a.n_experts) : ((size_t)a.n + S::BT - 1) / S::BT;
+  const size_t grid = 8 * ((mt * n_nt + 7) / 8);
+  if (grid * S::kThreads >= (size_t)1 << 32) return hipErrorInvalidValue;
+  auto* kernel = gated ? mx_tiles_kernel<MA, NB, WA, WB, true> : mx_tiles_kernel<MA, NB, WA, WB, false>;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(S::kThreads), S::lds(gated), st, a, n_nt);
+  return hipGetLastError();
+}
+template <int MA, int NB, int WA, int WB>
+hipError_t setup_tiles() {
+  typedef TileShape<MA, NB, WA, WB> S;
+  hipError_t e = hipFuncSetAttribute((const void*)mx_tiles_kernel<MA, NB, WA, WB, true>,
+                                     hipFuncAttributeMaxDynamicSharedMemorySize, (int)S::lds(true));
+  if (e == hipSuccess)
+    e = hipFuncSetAttribute((const void*)mx_tiles_kernel<MA, NB, WA, WB, false>,
+                            hipFuncAttributeMaxDynamicSharedMemorySize, (int)S::lds(false));
+  return e;
+}
+
 }  // namespace
 
-hipError_t mx_linear_setup() { return hipSuccess; }
+hipError_t mx_linear_setup() { return setup_tiles<4, 2, 2, 2>(); }
 
 hipError_t launch_mx_linear(const MxLin& a, hipStream_t st) {
+  if (a.n > 16 && a.K <= 1 << 20) {
+    const int groups = a.offsets ? a.n_experts : 1;
+    if ((size_t)((a.n + 127) / 128) * ((a.M + 255) / 256) >= 512 && a.n / groups >= 64) return launch_tiles<4, 2, 2, 2>(a, st);
+    if ((size_t)((a.n + 127) / 128) * ((a.M + 127) / 128) >= 512 && a.n / groups >= 64) return launch_tiles<2, 2, 2, 2>(a, st);
+    if (a.n / groups > 16) return launch_tiles<1, 1, 2, 2>(a, st);
+  }
   const size_t mt = a.offsets ? std::min<size_t>(a.n, (size_t)a.n / 16 + a.n_experts) : ((size_t)a.n + 15) / 16;
   if (mt * a.M >= (size_t)512 * 256) return launch_few<4, 4>(a, st);
   if (mt * a.M >= (size_t)512 * 32) return launch_few<2, 1>(a, st);
