@@ -18,20 +18,36 @@
 // Bound by HBM.  A row is held in the registers of W waves (eight columns a thread and V of these), which meet in
 // LDS once for each sum: every element is read and written once.
 #include <algorithm>
+#include <type_traits>
 
 #include "mx.h"
 
 namespace rmoe {
 namespace {
 
-constexpr int kMaxWaves = 8;  // of a row: 256 registers a thread
+constexpr int kMaxWaves = 8;  // of a workgroup: up to 256 registers a thread
 
-// Sums of N values over the W waves of a row: a slot per wave, `slots` alternating between calls so that one
-// barrier a call is enough.
+// The sum over the wave's lanes, in every lane: exchanges within the vector unit up to 16 lanes, then the four
+// sixteens' by scalar reads (six exchanges through LDS hardware take 0.3 us, these 0.1).
+__device__ __forceinline__ float lanes_sum(float v) {
+  auto moved = [](float x, auto control) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), decltype(control)::value, 0xF, 0xF, false));
+  };
+  v += moved(v, std::integral_constant<int, 0xB1>());   // lane ^ 1
+  v += moved(v, std::integral_constant<int, 0x4E>());   // lane ^ 2
+  v += moved(v, std::integral_constant<int, 0x141>());  // eight lanes mirrored
+  v += moved(v, std::integral_constant<int, 0x140>());  // sixteen mirrored
+  const int i = __float_as_int(v);
+  return (__int_as_float(__builtin_amdgcn_readlane(i, 0)) + __int_as_float(__builtin_amdgcn_readlane(i, 16))) +
+         (__int_as_float(__builtin_amdgcn_readlane(i, 32)) + __int_as_float(__builtin_amdgcn_readlane(i, 48)));
+}
+
+// Sums of N values over the W waves of a row, the first of which is wave `first` of the workgroup: a slot per wave;
+// calls in turn use different slots, so that one barrier a call is enough (all the workgroup's waves make it).
 template <int N>
-__device__ __forceinline__ void row_sum(float (&v)[N], float (*slots)[N], int wave, int W) {
+__device__ __forceinline__ void row_sum(float (&v)[N], float (*slots)[N], int wave, int first, int W) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = wave_sum(v[i]);
+  for (int i = 0; i < N; ++i) v[i] = lanes_sum(v[i]);
   if (W == 1) return;
   if ((threadIdx.x & 63) == 0) {
 #pragma unroll
@@ -39,10 +55,10 @@ __device__ __forceinline__ void row_sum(float (&v)[N], float (*slots)[N], int wa
   }
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = slots[0][i];
+  for (int i = 0; i < N; ++i) v[i] = slots[first][i];
   for (int w = 1; w < W; ++w) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] += slots[w][i];
+    for (int i = 0; i < N; ++i) v[i] += slots[first + w][i];
   }
 }
 
@@ -52,118 +68,126 @@ __device__ __forceinline__ void to_float(const Chunk<DT>& c, float (&f)[8]) {
   for (int i = 0; i < 8; ++i) f[i] = RowElem<DT>::get(c.v[i]);
 }
 
-// Columns c..c+7 of an fp32 vector of H, zeros past it.
-__device__ __forceinline__ void load_vector(const float* p, int c, int H, float (&f)[8]) {
-  if (c + 8 <= H && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
-    *reinterpret_cast<float4*>(f) = *reinterpret_cast<const float4*>(p + c);
-    *reinterpret_cast<float4*>(f + 4) = *reinterpret_cast<const float4*>(p + c + 4);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = c + i < H ? p[c + i] : 0.f;
-  }
-}
-
 __device__ __forceinline__ float inv_rms(float squares, int H, float eps) {
   return 1.0f / sqrtf(squares / (float)H + eps);
 }
 
-// The gate of columns c..c+7 of row t as fp32.
-template <int DT, bool kWide>
-__device__ __forceinline__ void load_gate(const NormArgs& a, size_t t, int c, float (&g)[8]) {
-  if (a.gate_kind == RMOE_GATE_COLUMN) {
-    load_vector(static_cast<const float*>(a.gate), c, a.H, g);
-  } else if (a.gate_kind == RMOE_GATE_FULL) {
-    to_float<DT>(load_chunk<DT, kWide>(static_cast<const typename RowElem<DT>::T*>(a.gate) + t * a.H, c, a.H), g);
-  } else {
-    const float v = a.gate_kind == RMOE_GATE_ROW ? static_cast<const float*>(a.gate)[t] : 1.f;
+// Where a thread's chunks of a row are.  Of aligned rows (kWide) the threads past the row's end repeat its last chunk,
+// so that loads and stores are free of branches: they compute and store what its owner does, and take no part in sums.
+template <int V, bool kWide>
+struct Columns {
+  int first, step, H;
+  __device__ __forceinline__ Columns(int thread, int W, int H) : first(8 * thread), step(512 * W), H(H) {}
+  __device__ __forceinline__ int raw(int v) const { return first + v * step; }
+  __device__ __forceinline__ int at(int v) const { return kWide ? min(raw(v), H - 8) : raw(v); }
+  __device__ __forceinline__ bool counts(int v, int i) const { return kWide ? raw(v) < H : raw(v) + i < H; }
+};
+
+template <int DT, bool kOnce = false, int V, bool kWide>
+__device__ __forceinline__ void load_row(const void* rows, size_t t, const Columns<V, kWide>& c, Chunk<DT> (&o)[V]) {
+  const auto* p = static_cast<const typename RowElem<DT>::T*>(rows) + t * c.H;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) g[i] = v;
+  for (int v = 0; v < V; ++v) o[v] = load_chunk<DT, kWide, kOnce>(p, c.at(v), c.H);
+}
+template <int DT, int V, bool kWide>
+__device__ __forceinline__ void store_row(void* rows, size_t t, const Columns<V, kWide>& c, int v, const Chunk<DT>& o) {
+  store_chunk<DT, kWide>(static_cast<typename RowElem<DT>::T*>(rows) + t * c.H, c.at(v), c.H, o);
+}
+// A thread's columns of an fp32 vector of H, or ones where there is none.  Of aligned rows without a branch: the
+// vector is a buffer of 4 H bytes, or of none, past whose end the hardware reads zeros.  (With a branch the values are waited
+// for where it ends, before anything behind it is requested: 6,700 rows of 2,560 took 50 us and not 35.)
+template <int V, bool kWide>
+__device__ __forceinline__ void load_columns(const float* p, const Columns<V, kWide>& c, float (&f)[V][8]) {
+  if constexpr (kWide) {
+    const auto buffer = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(p), 0, p ? 4 * c.H : 0, 0x00027000);
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+#pragma unroll
+      for (int i = 0; i < 8; i += 4) {
+        const u32x4_t q = __builtin_amdgcn_raw_buffer_load_b128(buffer, 4 * (c.at(v) + i), 0, 0);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) f[v][i + k] = __uint_as_float(p ? q[k] : 0x3f800000u);
+      }
+  } else {
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[v][i] = p && c.raw(v) + i < c.H ? p[c.raw(v) + i] : 1.f;
   }
 }
 
-template <int DT, int V, bool kWide>
-__global__ __launch_bounds__(64 * kMaxWaves) void norm_kernel(NormArgs a, size_t first) {
-  typedef typename RowElem<DT>::T E;
+// A workgroup is blockDim / (64 W) rows; more than one only of one wave each.
+template <int DT, int V, bool kWide, bool kBlock, bool kFull, bool kOnce>
+__global__ __launch_bounds__(64 * kMaxWaves) void norm_kernel(NormArgs a, int W, size_t first) {
   __shared__ float slots[2][kMaxWaves][1];
-  const size_t t = first + blockIdx.x;
-  const int W = blockDim.x >> 6, wave = wave_id(), H = a.H;
-  auto column = [&](int v) { return 8 * ((int)threadIdx.x + v * (int)blockDim.x); };
-  auto row = [&](const void* p) { return static_cast<const E*>(p) + t * H; };
-  float y[V][8];
-  if (a.block) {
-    Chunk<DT> r[V];
-    float u[V][8], g[V][8];
+  const int wave = wave_id(), H = a.H, group = wave / W;
+  const size_t t = first + (size_t)blockIdx.x * ((blockDim.x >> 6) / W) + group;
+  if (t >= (size_t)a.T) return;
+  const Columns<V, kWide> col((int)threadIdx.x - 64 * W * group, W, H);
+  Chunk<DT> b[V], r[V], fg[V];
+  if constexpr (kBlock) load_row<DT, kOnce>(a.block, t, col, b);
+  load_row<DT, kOnce>(a.residual, t, col, r);
+  if constexpr (kFull) load_row<DT>(a.gate, t, col, fg);
+  float g[V][8], post[V][8], pre[V][8], y[V][8];
+  load_columns(a.post, col, post);
+  load_columns(a.gate_kind == RMOE_GATE_COLUMN ? static_cast<const float*>(a.gate) : nullptr, col, g);
+  load_columns(a.pre, col, pre);
+  if constexpr (kBlock) {
+    float u[V][8];
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const int c = column(v);
-      if (c < H) {
-        to_float<DT>(load_chunk<DT, kWide>(row(a.block), c, H), u[v]);
-        r[v] = load_chunk<DT, kWide>(row(a.residual), c, H);
-        load_gate<DT, kWide>(a, t, c, g[v]);
-      } else {
-        r[v] = Chunk<DT>{};
-#pragma unroll
-        for (int i = 0; i < 8; ++i) u[v][i] = g[v][i] = 0.f;
-      }
-    }
+    for (int v = 0; v < V; ++v) to_float<DT>(b[v], u[v]);
+    const float one = a.gate_kind == RMOE_GATE_ROW ? static_cast<const float*>(a.gate)[t] : 1.f;
     if (a.post) {
       float s[1] = {0.f};
 #pragma unroll
       for (int v = 0; v < V; ++v)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) s[0] = fmaf(u[v][i], u[v][i], s[0]);
-      row_sum<1>(s, slots[0], wave, W);
+        for (int i = 0; i < 8; ++i)
+          if (col.counts(v, i)) s[0] = fmaf(u[v][i], u[v][i], s[0]);
+      row_sum<1>(s, slots[0], wave, 0, W);
       const float n = inv_rms(s[0], H, a.eps);
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        float w[8];
-        load_vector(a.post, column(v), H, w);
+      for (int v = 0; v < V; ++v)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) u[v][i] = u[v][i] * n * w[i];
-      }
+        for (int i = 0; i < 8; ++i) u[v][i] = u[v][i] * n * post[v][i];
     }
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      const int c = column(v);
+      if constexpr (kFull) to_float<DT>(fg[v], g[v]);
       Chunk<DT> o;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        o.v[i] = RowElem<DT>::put(fmaf(g[v][i], u[v][i], a.scale * RowElem<DT>::get(r[v].v[i])));
-        y[v][i] = c + i < H ? RowElem<DT>::get(o.v[i]) : 0.f;
+        o.v[i] = RowElem<DT>::put(fmaf(g[v][i] * one, u[v][i], a.scale * RowElem<DT>::get(r[v].v[i])));
+        y[v][i] = RowElem<DT>::get(o.v[i]);
       }
-      if (c < H) store_chunk<DT, kWide>(static_cast<E*>(a.y) + t * H, c, H, o);
+      store_row<DT>(a.y, t, col, v, o);
     }
   } else {
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      if (column(v) < H) to_float<DT>(load_chunk<DT, kWide>(row(a.residual), column(v), H), y[v]);
-      else
-#pragma unroll
-        for (int i = 0; i < 8; ++i) y[v][i] = 0.f;
-    }
+    for (int v = 0; v < V; ++v) to_float<DT>(r[v], y[v]);
   }
-  if (!a.h && !a.codes) return;
+  if (!a.pre) return;
   float s[1] = {0.f};
 #pragma unroll
   for (int v = 0; v < V; ++v)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) s[0] = fmaf(y[v][i], y[v][i], s[0]);
-  row_sum<1>(s, slots[1], wave, W);
+    for (int i = 0; i < 8; ++i)
+      if (col.counts(v, i)) s[0] = fmaf(y[v][i], y[v][i], s[0]);
+  row_sum<1>(s, slots[1], wave, 0, W);
   const float m = inv_rms(s[0], H, a.eps);
   const int P = (H + kMxBlock - 1) / kMxBlock * kMxBlock;
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    const int c = column(v);
-    float w[8], x[8];
-    load_vector(a.pre, c, H, w);
+    float x[8];
     Chunk<DT> o;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      o.v[i] = RowElem<DT>::put(y[v][i] * m * w[i]);
-      x[i] = c + i < H ? RowElem<DT>::get(o.v[i]) : 0.f;
+      o.v[i] = RowElem<DT>::put(y[v][i] * m * pre[v][i]);
+      x[i] = col.counts(v, i) ? RowElem<DT>::get(o.v[i]) : 0.f;
     }
-    if (a.h && c < H) store_chunk<DT, kWide>(static_cast<E*>(a.h) + t * H, c, H, o);
+    if (a.h) store_row<DT>(a.h, t, col, v, o);
     if (a.codes) {
+      const int c = col.raw(v);
       uint32_t scale;
       const uint32_t q = mx_quantize8(x, scale);
       if (c < P) {
@@ -174,137 +198,187 @@ __global__ __launch_bounds__(64 * kMaxWaves) void norm_kernel(NormArgs a, size_t
   }
 }
 
-// A workgroup takes the rows t = blockIdx.x, + gridDim.x, ...; each thread keeps its columns' shares of the
-// weights' and the column gate's gradients and leaves them at work[which][blockIdx.x][H].
-template <int DT, int V, bool kWide>
-__global__ __launch_bounds__(64 * kMaxWaves) void norm_backward_kernel(NormGradArgs a) {
-  typedef typename RowElem<DT>::T E;
+// A workgroup's waves are blockDim / (64 W) rows at a time, the first ones at blockIdx.x times as many, then
+// gridDim.x times as many further, ...; each thread keeps its columns' shares of the weights' and the column gate's gradients, which
+// the workgroup adds up in LDS at the end and leaves at work[which][blockIdx.x][H].  The next row is under way while one is
+// worked on (one chunk a thread; with two there are no registers for it): its loads come before the row's stores and
+// nothing else is loaded, for a wait for loads is one for every load and store before them.
+template <int DT, int V, bool kWide, bool kBlock, bool kFull>
+__global__ __launch_bounds__(64 * kMaxWaves, 2) void norm_backward_kernel(NormGradArgs a, int W) {
   __shared__ float first_sums[2][kMaxWaves][3], second_sums[2][kMaxWaves][2];
-  const int W = blockDim.x >> 6, wave = wave_id(), H = a.f.H;
-  auto column = [&](int v) { return 8 * ((int)threadIdx.x + v * (int)blockDim.x); };
-  float dpre[V][8], dpost[V][8], dgate[V][8];
+  __shared__ __attribute__((aligned(16))) float shares[kMaxWaves][512];
+  const int wave = wave_id(), H = a.f.H, groups = (int)(blockDim.x >> 6) / W, group = wave / W, own = W * group;
+  const Columns<V, kWide> col((int)threadIdx.x - 64 * own, W, H);
+  const bool by_row = kBlock && a.f.gate_kind == RMOE_GATE_ROW;
+  float pre[V][8], post[V][8], gate[V][8], dpre[V][8], dpost[V][8], dgate[V][8];
+  load_columns(a.f.pre, col, pre);
+  load_columns(kBlock ? a.f.post : nullptr, col, post);
+  load_columns(kBlock && a.f.gate_kind == RMOE_GATE_COLUMN ? static_cast<const float*>(a.f.gate) : nullptr, col, gate);
 #pragma unroll
   for (int v = 0; v < V; ++v)
 #pragma unroll
     for (int i = 0; i < 8; ++i) dpre[v][i] = dpost[v][i] = dgate[v][i] = 0.f;
   const float inv_H = 1.0f / (float)H;
-  int turn = 0;
-  for (size_t t = blockIdx.x; t < (size_t)a.f.T; t += gridDim.x, turn ^= 1) {
-    auto row = [&](const void* p) { return static_cast<const E*>(p) + t * H; };
+
+  struct Row {
+    Chunk<DT> b[V], y[V], d[V], h[V], g[V];
+    float one;
+  };
+  // Operands that are not given read y, and count for nothing.
+  const void *pd = a.dy ? a.dy : a.f.y, *ph = a.dh ? a.dh : a.f.y;
+  const float* prow = by_row ? static_cast<const float*>(a.f.gate) : nullptr;
+  auto load = [&](Row& q, size_t t) {
+    t = min(t, (size_t)a.f.T - 1);
+    if constexpr (kBlock) load_row<DT>(a.f.block, t, col, q.b);
+    load_row<DT>(a.f.y, t, col, q.y);
+    load_row<DT>(pd, t, col, q.d);
+    load_row<DT>(ph, t, col, q.h);
+    if constexpr (kFull) load_row<DT>(a.f.gate, t, col, q.g);
+    if constexpr (kBlock) q.one = prow ? prow[t] : 1.f;
+  };
+  auto work = [&](const Row& now, size_t t, bool live, int turn) {
     float b[V][8], y[V][8], d[V][8], dh[V][8];
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      const int c = column(v);
-      auto load = [&](const void* p, float (&f)[8]) {
-        if (p && c < H) to_float<DT>(load_chunk<DT, kWide>(row(p), c, H), f);
-        else
+      if constexpr (kBlock) to_float<DT>(now.b[v], b[v]);
+      to_float<DT>(now.y[v], y[v]);
+      to_float<DT>(now.d[v], d[v]);
+      to_float<DT>(now.h[v], dh[v]);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) f[i] = 0.f;
-      };
-      load(a.f.block, b[v]);
-      load(a.f.y, y[v]);
-      load(a.dy, d[v]);
-      load(a.dh, dh[v]);
+      for (int i = 0; i < 8; ++i) {
+        if (!a.dy) d[v][i] = 0.f;
+        if (!a.dh) dh[v][i] = 0.f;
+      }
     }
     float s[3] = {0.f, 0.f, 0.f};  // of b^2, y^2, a y
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      float w[8];
-      if (a.dh) load_vector(a.f.pre, column(v), H, w);
+    for (int v = 0; v < V; ++v)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        s[0] = fmaf(b[v][i], b[v][i], s[0]);
-        s[1] = fmaf(y[v][i], y[v][i], s[1]);
-        if (a.dh) s[2] = fmaf(dh[v][i] * w[i], y[v][i], s[2]);
-      }
-    }
-    row_sum<3>(s, first_sums[turn], wave, W);
-    const float n = a.f.post ? inv_rms(s[0], H, a.f.eps) : 1.f;
+      for (int i = 0; i < 8; ++i)
+        if (col.counts(v, i)) {
+          if constexpr (kBlock) s[0] = fmaf(b[v][i], b[v][i], s[0]);
+          s[1] = fmaf(y[v][i], y[v][i], s[1]);
+          s[2] = fmaf(dh[v][i] * pre[v][i], y[v][i], s[2]);
+        }
+    row_sum<3>(s, first_sums[turn], wave, own, W);
+    const float n = kBlock && a.f.post ? inv_rms(s[0], H, a.f.eps) : 1.f;
     if (a.dh) {
       const float m = inv_rms(s[1], H, a.f.eps), k = s[2] * inv_H * m * m * m;
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        float w[8];
-        load_vector(a.f.pre, column(v), H, w);
+      for (int v = 0; v < V; ++v)
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          d[v][i] += fmaf(dh[v][i] * w[i], m, -(y[v][i] * k));
-          dpre[v][i] = fmaf(dh[v][i] * y[v][i], m, dpre[v][i]);
+          d[v][i] += fmaf(dh[v][i] * pre[v][i], m, -(y[v][i] * k));
+          const float p = fmaf(dh[v][i] * y[v][i], m, dpre[v][i]);
+          dpre[v][i] = live ? p : dpre[v][i];
         }
-      }
     }
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       Chunk<DT> o;
 #pragma unroll
       for (int i = 0; i < 8; ++i) o.v[i] = RowElem<DT>::put(a.f.scale * d[v][i]);
-      if (column(v) < H) store_chunk<DT, kWide>(static_cast<E*>(a.dresidual) + t * H, column(v), H, o);
+      if (live) store_row<DT>(a.dresidual, t, col, v, o);
     }
-    if (!a.f.block) continue;
-    float q[2] = {0.f, 0.f};  // of v b, and D u
-    float w[V][8];
+    if constexpr (kBlock) {
+      float q[2] = {0.f, 0.f};  // of v b, and D u
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const int c = column(v);
-      float g[8];
-      if (c < H) load_gate<DT, kWide>(a.f, t, c, g);
-      else
+      for (int v = 0; v < V; ++v) {
+        float g[8];
+        if constexpr (kFull) to_float<DT>(now.g[v], g);
+        Chunk<DT> o;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) g[i] = 0.f;
-      if (a.f.post) load_vector(a.f.post, c, H, w[v]);
-      else
-#pragma unroll
-        for (int i = 0; i < 8; ++i) w[v][i] = 1.f;
-      Chunk<DT> o;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float bn = b[v][i] * n, dg = d[v][i] * (bn * w[v][i]);
-        q[1] += dg;
-        dgate[v][i] += dg;
-        o.v[i] = RowElem<DT>::put(dg);
-        d[v][i] *= g[i];  // du
-        dpost[v][i] = fmaf(d[v][i], bn, dpost[v][i]);
-        q[0] = fmaf(d[v][i] * w[v][i], b[v][i], q[0]);
+        for (int i = 0; i < 8; ++i) {
+          const float bn = b[v][i] * n, dg = d[v][i] * (bn * post[v][i]);
+          o.v[i] = RowElem<DT>::put(dg);
+          d[v][i] *= kFull ? g[i] : gate[v][i] * now.one;  // du
+          if (col.counts(v, i)) {
+            q[0] = fmaf(d[v][i] * post[v][i], b[v][i], q[0]);
+            q[1] += dg;
+          }
+          const float p = fmaf(d[v][i], bn, dpost[v][i]), c = dgate[v][i] + dg;
+          dpost[v][i] = live ? p : dpost[v][i];
+          dgate[v][i] = live ? c : dgate[v][i];
+        }
+        if constexpr (kFull)
+          if (a.dgate && live) store_row<DT>(a.dgate, t, col, v, o);
       }
-      if (a.f.gate_kind == RMOE_GATE_FULL && a.dgate && c < H)
-        store_chunk<DT, kWide>(static_cast<E*>(a.dgate) + t * H, c, H, o);
+      if (a.f.post || by_row) row_sum<2>(q, second_sums[turn], wave, own, W);
+      if (by_row && a.dgate && col.first == 0 && live) static_cast<float*>(a.dgate)[t] = q[1];
+      const float k = q[0] * inv_H * n * n * n;
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        Chunk<DT> o;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          o.v[i] = RowElem<DT>::put(a.f.post ? fmaf(d[v][i] * post[v][i], n, -(b[v][i] * k)) : d[v][i]);
+        if (live) store_row<DT>(a.dblock, t, col, v, o);
+      }
     }
-    if (a.f.post || a.f.gate_kind == RMOE_GATE_ROW) row_sum<2>(q, second_sums[turn], wave, W);
-    if (a.f.gate_kind == RMOE_GATE_ROW && a.dgate && threadIdx.x == 0) static_cast<float*>(a.dgate)[t] = q[1];
-    const float k = a.f.post ? q[0] * inv_H * n * n * n : 0.f;
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      Chunk<DT> o;
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        o.v[i] = RowElem<DT>::put(a.f.post ? fmaf(d[v][i] * w[v][i], n, -(b[v][i] * k)) : d[v][i]);
-      if (column(v) < H) store_chunk<DT, kWide>(static_cast<E*>(a.dblock) + t * H, column(v), H, o);
+  };
+
+  const size_t T = (size_t)a.f.T, step = (size_t)gridDim.x * groups;
+  size_t t = (size_t)blockIdx.x * groups;
+  int turn = 0;
+  Row now;
+  if constexpr (V == 1) {
+    Row ahead;
+    load(now, t + group);
+    for (; t + groups <= T; t += step, turn ^= 1) {
+      load(ahead, t + step + group);
+      work(now, t + group, true, turn);
+      now = ahead;
+    }
+    if (t < T) work(now, t + group, t + group < T, turn);
+  } else {
+    for (; t < T; t += step, turn ^= 1) {
+      load(now, t + group);
+      work(now, t + group, t + group < T, turn);
     }
   }
+
   auto leave = [&](int which, float (&f)[V][8]) {
     float* p = a.work + ((size_t)which * gridDim.x + blockIdx.x) * H;
 #pragma unroll
-    for (int v = 0; v < V; ++v)
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (column(v) + i < H) p[column(v) + i] = f[v][i];
+    for (int v = 0; v < V; ++v) {
+      __syncthreads();
+      *reinterpret_cast<float4*>(&shares[wave][8 * (threadIdx.x & 63)]) = *reinterpret_cast<float4*>(f[v]);
+      *reinterpret_cast<float4*>(&shares[wave][8 * (threadIdx.x & 63) + 4]) = *reinterpret_cast<float4*>(f[v] + 4);
+      __syncthreads();
+      for (int i = threadIdx.x; i < 512 * W; i += blockDim.x) {
+        const int c = 512 * W * v + i;
+        float s = shares[i / 512][i % 512];
+        for (int g = 1; g < groups; ++g) s += shares[g * W + i / 512][i % 512];
+        if (c < H) p[c] = s;
+      }
+    }
   };
   if (a.dpre) leave(0, dpre);
-  if (a.dpost) leave(1, dpost);
-  if (a.f.gate_kind == RMOE_GATE_COLUMN && a.dgate) leave(2, dgate);
+  if constexpr (kBlock) {
+    if (a.dpost) leave(1, dpost);
+    if (a.f.gate_kind == RMOE_GATE_COLUMN && a.dgate) leave(2, dgate);
+  }
 }
 
-// The columns' sums over the workgroups' shares, in their order: 64 columns a workgroup, a wave for each 16th.
+// The columns' sums over the workgroups' shares, in their order: 64 columns a workgroup, a wave for each 16th of the
+// shares, of which kLoads are under way at once.
 __global__ __launch_bounds__(1024) void norm_columns_kernel(const float* __restrict__ work, int groups, int H,
                                                             float* dpre, float* dpost, float* dgate) {
   __shared__ float part[16][64];
+  constexpr int kLoads = 16;
   const int lane = threadIdx.x & 63, wave = wave_id(), c = (int)blockIdx.x * 64 + lane;
   float* out = blockIdx.y == 0 ? dpre : blockIdx.y == 1 ? dpost : dgate;
   if (!out) return;
-  const float* p = work + (size_t)blockIdx.y * groups * H;
+  const float* p = work + (size_t)blockIdx.y * groups * H + min(c, H - 1);
+  const int end = (wave + 1) * groups / 16;
   float s = 0.f;
-  if (c < H)
-    for (int g = wave * groups / 16; g < (wave + 1) * groups / 16; ++g) s += p[(size_t)g * H + c];
+  for (int g = wave * groups / 16; g < end; g += kLoads) {
+    float v[kLoads];
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) v[i] = g + i < end ? p[(size_t)(g + i) * H] : 0.f;
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) s += v[i];
+  }
   part[wave][lane] = s;
   __syncthreads();
   if (wave == 0 && c < H) {
@@ -319,19 +393,27 @@ bool wide_rows(int dtype, int H, std::initializer_list<const void*> ps) {
   return at % 16 == 0 && H % 8 == 0 && (dtype == RMOE_DT_F32 || H * 2 % 16 == 0);
 }
 
-// Waves of a row of eight columns a thread, or of 16 where that takes more than kMaxWaves.
-bool two_chunks(int H) { return H > 512 * kMaxWaves; }
-int waves_for(int H) { return two_chunks(H) ? (H + 1023) / 1024 : (H + 511) / 512; }
-
 template <int DT>
 hipError_t norm_with(const NormArgs& a, hipStream_t st) {
   const bool wide = wide_rows(DT, a.H, {a.block, a.residual, a.y, a.h, a.gate_kind == RMOE_GATE_FULL ? a.gate : nullptr});
-  const int W = waves_for(a.H);
-  auto* kernel = two_chunks(a.H) ? (wide ? norm_kernel<DT, 2, true> : norm_kernel<DT, 2, false>)
-                                 : (wide ? norm_kernel<DT, 1, true> : norm_kernel<DT, 1, false>);
-  const size_t step = ((size_t)1 << 32) / (64 * W) - 1;
+  // Block and residual of 6,700 rows of 2,560 (69 MB): 34.7 us, read past the caches' order 32.2; of 2,000 rows, which are
+  // in the caches from the call before, 11.4 and 12.2.
+  const bool once = wide && (size_t)a.T * a.H * sizeof(typename RowElem<DT>::T) * (a.block ? 2 : 1) >= kOnceBytes;
+  const int V = a.H > 512 * kMaxWaves ? 2 : 1, W = (a.H + 512 * V - 1) / (512 * V);
+  const int rows = W == 1 ? 4 : 1;
+  auto pick = [&](auto block, auto full) {
+    constexpr bool B = decltype(block)::value, F = decltype(full)::value;
+    if (once) return V == 1 ? norm_kernel<DT, 1, true, B, F, true> : norm_kernel<DT, 2, true, B, F, true>;
+    return V == 1 ? (wide ? norm_kernel<DT, 1, true, B, F, false> : norm_kernel<DT, 1, false, B, F, false>)
+                  : (wide ? norm_kernel<DT, 2, true, B, F, false> : norm_kernel<DT, 2, false, B, F, false>);
+  };
+  auto* kernel = a.gate_kind == RMOE_GATE_FULL ? pick(std::true_type(), std::true_type())
+                 : a.block                     ? pick(std::true_type(), std::false_type())
+                                               : pick(std::false_type(), std::false_type());
+  const size_t step = (((size_t)1 << 32) / (64 * W * rows) - 1) * rows;
   for (size_t t = 0; t < (size_t)a.T; t += step) {
-    hipLaunchKernelGGL(kernel, dim3((unsigned)std::min(step, (size_t)a.T - t)), dim3(64 * W), 0, st, a, t);
+    const size_t n = std::min(step, (size_t)a.T - t);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((n + rows - 1) / rows)), dim3(64 * W * rows), 0, st, a, W, t);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
@@ -344,10 +426,18 @@ hipError_t grad_with(const NormGradArgs& a, hipStream_t st) {
   const bool full = f.gate_kind == RMOE_GATE_FULL;
   const bool wide = wide_rows(DT, f.H, {f.block, f.y, a.dy, a.dh, a.dblock, a.dresidual, full ? f.gate : nullptr,
                                         full ? a.dgate : nullptr});
-  const int W = waves_for(f.H), groups = norm_groups(f.T);
-  auto* kernel = two_chunks(f.H) ? (wide ? norm_backward_kernel<DT, 2, true> : norm_backward_kernel<DT, 2, false>)
-                                 : (wide ? norm_backward_kernel<DT, 1, true> : norm_backward_kernel<DT, 1, false>);
-  hipLaunchKernelGGL(kernel, dim3(groups), dim3(64 * W), 0, st, a);
+  const int V = f.H > 512 * kMaxWaves ? 2 : 1;
+  const int W = (f.H + 512 * V - 1) / (512 * V), rows = kMaxWaves / W;
+  const int groups = std::min((f.T + rows - 1) / rows, norm_groups(f.T));
+  auto pick = [&](auto block, auto full) {
+    constexpr bool B = decltype(block)::value, F = decltype(full)::value;
+    return V == 1 ? (wide ? norm_backward_kernel<DT, 1, true, B, F> : norm_backward_kernel<DT, 1, false, B, F>)
+                  : (wide ? norm_backward_kernel<DT, 2, true, B, F> : norm_backward_kernel<DT, 2, false, B, F>);
+  };
+  auto* kernel = full      ? pick(std::true_type(), std::true_type())
+                 : f.block ? pick(std::true_type(), std::false_type())
+                           : pick(std::false_type(), std::false_type());
+  hipLaunchKernelGGL(kernel, dim3(groups), dim3(64 * W * rows), 0, st, a, W);
   hipError_t e = hipGetLastError();
   float* column_gate = f.gate_kind == RMOE_GATE_COLUMN ? static_cast<float*>(a.dgate) : nullptr;
   if (e == hipSuccess && (a.dpre || a.dpost || column_gate)) {

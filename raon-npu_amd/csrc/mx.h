@@ -48,8 +48,10 @@ struct alignas(16) Chunk {
   typename RowElem<DT>::T v[8];
 };
 // Loads and stores of the columns c..c+7 of a row `width` wide: by 16 bytes, or (kWide false: rows that are not
-// aligned to 16 bytes or end inside a chunk) one by one, with zeros past the end.
-template <int DT, bool kWide>
+// aligned to 16 bytes or end inside a chunk) one by one, with zeros past the end.  kOnce: read past the caches' order of
+// use, for rows of kOnceBytes and more that are not read again.
+constexpr size_t kOnceBytes = (size_t)64 << 20;
+template <int DT, bool kWide, bool kOnce = false>
 __device__ __forceinline__ Chunk<DT> load_chunk(const void* row, int c, int width) {
   const auto* p = static_cast<const typename RowElem<DT>::T*>(row) + c;
   Chunk<DT> r;
@@ -57,7 +59,7 @@ __device__ __forceinline__ Chunk<DT> load_chunk(const void* row, int c, int widt
     const uint4* q = reinterpret_cast<const uint4*>(p);
     uint4* o = reinterpret_cast<uint4*>(r.v);
 #pragma unroll
-    for (int i = 0; i < (int)(sizeof(r) / 16); ++i) o[i] = q[i];
+    for (int i = 0; i < (int)(sizeof(r) / 16); ++i) o[i] = kOnce ? load_stream16(reinterpret_cast<const uint8_t*>(q + i)) : q[i];
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) r.v[i] = c + i < width ? p[i] : (typename RowElem<DT>::T)0;

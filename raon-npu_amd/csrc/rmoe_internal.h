@@ -609,7 +609,7 @@ struct NormGradArgs {
   float* work;  // [3][norm_groups(T)][H]
 };
 // Workgroups of the gradient, each of which leaves its share of the weights' gradients.
-constexpr int norm_groups(int T) { return T < 512 ? T : 512; }
+constexpr int norm_groups(int T) { return T < 256 ? T : 256; }
 hipError_t launch_norm_backward(const NormGradArgs& a, int dtype, hipStream_t st);
 
 // Persistent decode of n_layers (<= kMaxStack) layers of one geometry for one token
