@@ -21,6 +21,14 @@ constexpr int kScaleOne = 127;  // a scale byte of 2^0
 // Codes as the instruction's operand: its upper half belongs to the wider formats.
 __device__ __forceinline__ i32x8 operand(const i32x4& v) { return i32x8{v.x, v.y, v.z, v.w, 0, 0, 0, 0}; }
 
+// g sigmoid(g) u with q = exp(g): q / (1 + q) takes an exponential and a reciprocal, few others.  The exponential of half
+// the argument is squared, so that results down to fp32's subnormal ones are formed (the instruction itself gives 0 for
+// those); past exp(87) the quotient is 1.  exp(g) is off by (4 + |g|) 2^-23 of it.
+__device__ __forceinline__ float swiglu(float g, float u) {
+  const float p = __builtin_amdgcn_exp2f(fminf(g * 0.72134752044448170f, 63.f)), q = p * p;
+  return g * (q * recip(1.0f + q)) * u;
+}
+
 // bf16 bits of v (RTNE), by the conversion instruction.
 __device__ __forceinline__ uint32_t bf16_bits(float v) { return __builtin_bit_cast(uint16_t, (__bf16)v); }
 
@@ -45,7 +53,7 @@ struct Epilogue {
       if (bias) z[k] += bias[c];
       if constexpr (kGated) {
         if (bias) u[k] += bias[up + c];
-        z[k] = act_pair(act, z[k], u[k], gb, vb);
+        z[k] = act == RMOE_ACT_SWIGLU ? swiglu(z[k], u[k]) : act_pair(RMOE_ACT_SITU, z[k], u[k], gb, vb);
       } else {
         z[k] = act_single(act, z[k]);
       }
@@ -70,11 +78,32 @@ struct Epilogue {
   }
 };
 
+// Scale bytes at .. at + 15 of a row of kb; those past its end are anything.
+__device__ __forceinline__ uint4 load_scales(const uint8_t* row, int at, int kb) {
+  uint4 v = make_uint4(0u, 0u, 0u, 0u);
+  if (at + 16 <= kb) {
+    __builtin_memcpy(&v, row + at, 16);
+    return v;
+  }
+  uint32_t d[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int b = at + 4 * i;
+    if (b + 4 <= kb) {
+      __builtin_memcpy(&d[i], row + b, 4);
+    } else if (b < kb) {
+#pragma unroll
+      for (int k = 0; k < 3; ++k) d[i] |= (uint32_t)row[min(b + k, kb - 1)] << (8 * k);
+    }
+  }
+  return make_uint4(d[0], d[1], d[2], d[3]);
+}
+
 // ------------------------------------------------------------------ few rows --
 // Tiles of 16 rows of x.  A wave takes NA fragments of 16 weight rows; the workgroup's four waves are WR
 // stripes of them by WK = 4 / WR parts of K, whose sums meet in LDS and are added in their order.
 // A gated stripe holds 8 NA gate rows, then the up rows of the same outputs.
-template <int NA, int WR, bool kGated, bool kTail>
+template <int NA, int WR, bool kGated>
 __global__ __launch_bounds__(256) void mx_few_kernel(MxLin a, int n_nt) {
   constexpr int WK = 4 / WR, kRows = 16 * NA, kOut = kGated ? kRows / 2 : kRows, kStride = kRows + 4;
   __shared__ __attribute__((aligned(16))) float sums[4][16 * kStride];
@@ -114,18 +143,54 @@ __global__ __launch_bounds__(256) void mx_few_kernel(MxLin a, int n_nt) {
   f32x4 acc[NA];
 #pragma unroll
   for (int f = 0; f < NA; ++f) acc[f] = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int s = s0; s < s1; ++s) {
-    const int b = 4 * s + lq, at = kTail ? min(b, kb - 1) : b;
-    const bool in = !kTail || b < kb;
-    i32x4 x = *reinterpret_cast<const i32x4*>(xp + (size_t)at * 16);
-    const int xsc = in ? xsp[at] : kScaleOne;
-    if (!in) x = i32x4{0, 0, 0, 0};
+  // Four steps (512 columns) at once, the next four requested before these are used.  Steps past the wave's part
+  // repeat its last one and are not used; blocks past the row's end repeat its last one as zeros.
+  struct Window {
+    i32x4 w[NA][4], x[4];
+    uint4 ws[NA], xs;
+  };
+  auto load = [&](Window& q, int s) {
+    size_t at[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) at[i] = (size_t)min(4 * min(s + i, s1 - 1) + lq, kb - 1) * 16;
 #pragma unroll
     for (int f = 0; f < NA; ++f) {
-      const i32x4 w = *reinterpret_cast<const i32x4*>(wp[f] + (size_t)at * 16);
-      const int wsc = in ? wsp[f][at] : kScaleOne;
-      acc[f] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(operand(w), operand(x), acc[f], kFp4, kFp4, 0, wsc, 0, xsc);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) q.w[f][i] = *reinterpret_cast<const i32x4*>(wp[f] + at[i]);
     }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) q.x[i] = *reinterpret_cast<const i32x4*>(xp + at[i]);
+#pragma unroll
+    for (int f = 0; f < NA; ++f) q.ws[f] = load_scales(wsp[f], 4 * s, kb);
+    q.xs = load_scales(xsp, 4 * s, kb);
+  };
+  auto work = [&](Window& q, int s) {
+    const uint32_t xs[4] = {q.xs.x, q.xs.y, q.xs.z, q.xs.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (s + i >= s1) break;
+      const bool in = 4 * (s + i) + lq < kb;
+      const int xsc = in ? (int)(xs[i] >> (8 * lq)) : kScaleOne;
+      if (!in) q.x[i] = i32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int f = 0; f < NA; ++f) {
+        const uint32_t ws[4] = {q.ws[f].x, q.ws[f].y, q.ws[f].z, q.ws[f].w};
+        const int wsc = in ? (int)(ws[i] >> (8 * lq)) : kScaleOne;
+        acc[f] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(operand(q.w[f][i]), operand(q.x[i]), acc[f], kFp4, kFp4, 0,
+                                                                  wsc, 0, xsc);
+      }
+    }
+  };
+  if (s0 < s1) {
+    Window now, ahead;
+    load(now, s0);
+    int s = s0;
+    for (; s + 4 < s1; s += 4) {
+      load(ahead, s + 4);
+      work(now, s);
+      now = ahead;
+    }
+    work(now, s);
   }
   // acc[f][i]: weight row 16 f + 4 lq + i, row of x l16.
 #pragma unroll
@@ -151,13 +216,12 @@ __global__ __launch_bounds__(256) void mx_few_kernel(MxLin a, int n_nt) {
 
 template <int NA, int WR>
 hipError_t launch_few(const MxLin& a, hipStream_t st) {
-  const bool gated = act_gated(a.act), tail = a.K % (4 * kMxBlock) != 0;
+  const bool gated = act_gated(a.act);
   const int width = gated ? a.M / 2 : a.M, out = 16 * NA * WR / (gated ? 2 : 1), n_nt = (width + out - 1) / out;
   const size_t mt = a.offsets ? std::min<size_t>(a.n, (size_t)a.n / 16 + a.n_experts) : ((size_t)a.n + 15) / 16;
   const size_t grid = 8 * ((mt * n_nt + 7) / 8);
   if (grid * 256 >= (size_t)1 << 32) return hipErrorInvalidValue;
-  auto* kernel = gated ? (tail ? mx_few_kernel<NA, WR, true, true> : mx_few_kernel<NA, WR, true, false>)
-                       : (tail ? mx_few_kernel<NA, WR, false, true> : mx_few_kernel<NA, WR, false, false>);
+  auto* kernel = gated ? mx_few_kernel<NA, WR, true> : mx_few_kernel<NA, WR, false>;
   hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(256), 0, st, a, n_nt);
   return hipGetLastError();
 }
@@ -172,15 +236,18 @@ hipError_t launch_few(const MxLin& a, hipStream_t st) {
 constexpr int kStages = 3;
 constexpr int kKTile = 4 * kMxBlock;
 
-template <int MA, int NB, int WA, int WB>
+template <int MA, int NB, int WA, int WB, bool kWhole>
 struct TileShape {
-  static constexpr int kThreads = 64 * WA * WB, BW = 32 * MA * WA, BT = 32 * NB * WB, R = BW + BT;
-  static constexpr int kCodes = R * 64, kStage = kCodes + R * 4;
-  static constexpr int kCopies = R / 16 / (WA * WB);  // a wave's copies of a K tile, 16 rows each
+  static constexpr int kWaves = WA * WB, kThreads = 64 * kWaves, BW = 32 * MA * WA, BT = 32 * NB * WB, R = BW + BT;
+  static constexpr int kCodes = R * 64, kStage = kCodes + (kWhole ? 0 : R * 4);  // a stage's bytes
+  static constexpr int kWindow = kStages * kStage;                               // where a window of scales begins
+  static constexpr int kCopies = R / 16 / kWaves;                  // a wave's copies of a K tile, 16 rows each
+  static constexpr int kScaleCopies = (R / 64 + kWaves - 1) / kWaves;  // and of a window of scales, 64 rows each
   static constexpr int kScales = (R + kThreads - 1) / kThreads;
   static constexpr size_t lds(bool gated) {
-    const size_t out = (size_t)WA * WB * 32 * ((gated ? 16 : 32) * MA + 4) * 4;
-    return out > (size_t)kStages * kStage ? out : (size_t)kStages * kStage;
+    const size_t out = (size_t)kWaves * 32 * ((gated ? 16 : 32) * MA + 4) * 4;
+    const size_t in = (size_t)kStages * kStage + (kWhole ? R * 16 : 0);
+    return out > in ? out : in;
   }
 };
 
@@ -204,30 +271,9 @@ __device__ __forceinline__ void copies_landed() {
   __syncthreads();
 }
 
-// Scale bytes 16 w .. 16 w + 15 of a row of kb; those past its end are anything.
-__device__ __forceinline__ uint4 load_scales(const uint8_t* row, int w, int kb) {
-  uint4 v = make_uint4(0u, 0u, 0u, 0u);
-  if (16 * w + 16 <= kb) {
-    __builtin_memcpy(&v, row + 16 * w, 16);
-    return v;
-  }
-  uint32_t d[4] = {0u, 0u, 0u, 0u};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int b = 16 * w + 4 * i;
-    if (b + 4 <= kb) {
-      __builtin_memcpy(&d[i], row + b, 4);
-    } else if (b < kb) {
-#pragma unroll
-      for (int k = 0; k < 3; ++k) d[i] |= (uint32_t)row[min(b + k, kb - 1)] << (8 * k);
-    }
-  }
-  return make_uint4(d[0], d[1], d[2], d[3]);
-}
-
-template <int MA, int NB, int WA, int WB, bool kGated>
+template <int MA, int NB, int WA, int WB, bool kWhole, bool kGated>
 __global__ __launch_bounds__(64 * WA * WB, 2) void mx_tiles_kernel(MxLin a, int n_nt) {
-  typedef TileShape<MA, NB, WA, WB> S;
+  typedef TileShape<MA, NB, WA, WB, kWhole> S;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   constexpr int kOut = (kGated ? 16 : 32) * MA;  // outputs of a wave
   RowTiles<S::BT> rt;
@@ -276,27 +322,55 @@ __global__ __launch_bounds__(64 * WA * WB, 2) void mx_tiles_kernel(MxLin a, int 
       coff[j] = (uint32_t)(token_row(r) - first) * ldb;
     }
   }
-  // Chunk c of a row's four stands at c ^ (row / 2 % 4): eight rows' chunks of one number are in different banks.
-  const int cchunk = (lane & 3) ^ ((lane >> 3) & 3);
+  // Chunk c of a row's four stands at c ^ (row / 4 % 4): sixteen rows' chunks of one number are in different banks.
+    const int cchunk = (lane & 3) ^ (lane >> 4);
   auto copies = [&](int t, int stage) {
     const uint32_t k = (uint32_t)min(4 * t + cchunk, kb - 1) * 16u;
 #pragma unroll
     for (int j = 0; j < S::kCopies; ++j)
       copy16(cbase[j], coff[j] + k, (uint32_t)(stage * S::kStage + 16 * (wave * S::kCopies + j) * 64));
   };
-  const uint8_t* sbase[S::kScales];
+  // Scales of whole windows (K a multiple of 512): copied as the codes are, 16 bytes a row, into the one window there is
+  // once every wave has the one before in its registers.
+  uint32_t soff[S::kScaleCopies];
+  const uint8_t* wbase[S::kScaleCopies];
+  uint32_t wslot[S::kScaleCopies];
+  auto window_copies = [&](int w) {
 #pragma unroll
-  for (int j = 0; j < S::kScales; ++j) {
-    const int r = min(tid + j * S::kThreads, S::R - 1);
-    sbase[j] = r < S::BW ? a.ws + ((size_t)e * a.M + weight_row(r)) * kb : a.xs + ((size_t)row0 + token_row(r)) * kb;
+    for (int j = 0; j < S::kScaleCopies; ++j) copy16(wbase[j], soff[j] + 16 * w, S::kWindow + wslot[j]);
+  };
+  if constexpr (kWhole) {
+#pragma unroll
+    for (int j = 0; j < S::kScaleCopies; ++j) {
+      const int r0 = 64 * ((wave + j * S::kWaves) % (S::R / 64)), r = r0 + lane;  // a wave without a copy repeats another's
+      wslot[j] = 16 * r0;
+      if (r0 < S::BW) {
+        const int first = weight_row(r0);  // the least: a group of 64 begins with gate rows or holds up rows alone
+        wbase[j] = a.ws + ((size_t)e * a.M + first) * kb;
+        soff[j] = (uint32_t)(weight_row(r) - first) * (uint32_t)kb;
+      } else {
+        const int first = token_row(r0);
+        wbase[j] = a.xs + ((size_t)row0 + first) * kb;
+        soff[j] = (uint32_t)(token_row(r) - first) * (uint32_t)kb;
+      }
+    }
   }
+  // Other scales: fetched 16 a row by the registers and put beside a stage's codes, a dword a row.
+  const uint8_t* sbase[S::kScales];
   uint4 q[S::kScales], qn[S::kScales];
+  if constexpr (!kWhole) {
+#pragma unroll
+    for (int j = 0; j < S::kScales; ++j) {
+      const int r = min(tid + j * S::kThreads, S::R - 1);
+      sbase[j] = r < S::BW ? a.ws + ((size_t)e * a.M + weight_row(r)) * kb : a.xs + ((size_t)row0 + token_row(r)) * kb;
+    }
+  }
   auto put_scales = [&](int t, int stage) {  // called for t = 0, 1, 2, ...
     if ((t & 3) == 0) {
 #pragma unroll
       for (int j = 0; j < S::kScales; ++j) {
         q[j] = t == 0 ? load_scales(sbase[j], 0, kb) : qn[j];
-        if (t + 4 < tiles) qn[j] = load_scales(sbase[j], t / 4 + 1, kb);
+        if (t + 4 < tiles) qn[j] = load_scales(sbase[j], 16 * (t / 4 + 1), kb);
       }
     }
 #pragma unroll
@@ -324,7 +398,7 @@ __global__ __launch_bounds__(64 * WA * WB, 2) void mx_tiles_kernel(MxLin a, int 
   const int arow = wa * 32 * MA + l32, brow = S::BW + wb * 32 * NB + l32;  // multiples of 32 away: l32's place
   uint32_t at[2];  // of a lane's chunk in step 0 and 1 from its row's start
 #pragma unroll
-  for (int s = 0; s < 2; ++s) at[s] = (uint32_t)((2 * h + s) ^ ((l32 >> 1) & 3)) * 16u;
+  for (int s = 0; s < 2; ++s) at[s] = (uint32_t)((2 * h + s) ^ (l32 >> 2 & 3)) * 16u;
   auto read = [&](Frags& g, int stage, int s) {
     const uint8_t* p = lds + stage * S::kStage + at[s];
 #pragma unroll
@@ -332,19 +406,35 @@ __global__ __launch_bounds__(64 * WA * WB, 2) void mx_tiles_kernel(MxLin a, int 
 #pragma unroll
     for (int n = 0; n < NB; ++n) g.b[n] = *reinterpret_cast<const i32x4*>(p + (brow + 32 * n) * 64);
   };
+  // The dwords of a tile's scales (kWhole: of a window's four tiles, the next one's first); the lane's two bytes are
+  // brought down where they are used, for a shift here would wait for every read before it.
+  constexpr int kD = kWhole ? 4 : 1;
+  uint32_t da[MA][kD], db[NB][kD];
   auto read_scales = [&](int stage) {
-    const uint8_t* p = lds + stage * S::kStage + S::kCodes;
+    const uint8_t* p = lds + (kWhole ? S::kWindow : stage * S::kStage + S::kCodes);
+    auto get = [&](uint32_t (&d)[kD], int r) {
+      if constexpr (kWhole) *reinterpret_cast<uint4*>(d) = *reinterpret_cast<const uint4*>(p + r * 16);
+      else d[0] = *reinterpret_cast<const uint32_t*>(p + r * 4);
+    };
 #pragma unroll
-    for (int m = 0; m < MA; ++m) sa[m] = *reinterpret_cast<const uint32_t*>(p + (arow + 32 * m) * 4) >> (16 * h);
+    for (int m = 0; m < MA; ++m) get(da[m], arow + 32 * m);
 #pragma unroll
-    for (int n = 0; n < NB; ++n) sb[n] = *reinterpret_cast<const uint32_t*>(p + (brow + 32 * n) * 4) >> (16 * h);
+    for (int n = 0; n < NB; ++n) get(db[n], brow + 32 * n);
   };
-  auto multiply = [&](Frags& g, auto step, bool last) {
-    constexpr int s = decltype(step)::value;
-    if (rem && last && 2 * h + s >= rem) {  // blocks past the end: weights of zero
+  auto take_scales = [&] {
+    auto take = [&](uint32_t (&d)[kD]) {
+      const uint32_t v = d[0] >> (16 * h);
 #pragma unroll
-      for (int m = 0; m < MA; ++m) g.a[m] = i32x4{0, 0, 0, 0};
-    }
+      for (int i = 1; i < kD; ++i) d[i - 1] = d[i];
+      return v;
+    };
+#pragma unroll
+    for (int m = 0; m < MA; ++m) sa[m] = take(da[m]);
+#pragma unroll
+    for (int n = 0; n < NB; ++n) sb[n] = take(db[n]);
+  };
+  auto multiply = [&](const Frags& g, auto step) {
+    constexpr int s = decltype(step)::value;
 #pragma unroll
     for (int m = 0; m < MA; ++m)
 #pragma unroll
@@ -352,152 +442,205 @@ __global__ __launch_bounds__(64 * WA * WB, 2) void mx_tiles_kernel(MxLin a, int 
         acc[m][n] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(operand(g.a[m]), operand(g.b[n]), acc[m][n], kFp4, kFp4, s,
                                                                     (int)sa[m], s, (int)sb[n]);
   };
+  const std::integral_constant<int, 0> first;
+  const std::integral_constant<int, 1> second;
 
+  if constexpr (kWhole) window_copies(0);
 #pragma unroll
   for (int t = 0; t < kStages; ++t)
     if (t < tiles) {
-      put_scales(t, t);
+      if constexpr (!kWhole) put_scales(t, t);
       copies(t, t);
     }
   if (tiles >= kStages) copies_landed<2 * S::kCopies>();
   else copies_landed<0>();
   read(f[0], 0, 0);
   read_scales(0);
+  // A tile's second step is read while its first is multiplied, the next tile's first while its second is.  The
+  // compiler would move the products behind the waits: the scheduling barriers keep them where they are.
   int stage = 0;
-  for (int t = 0; t < tiles; ++t) {
+  for (int t = 0; t < tiles - 1; ++t) {
     const int next = stage == kStages - 1 ? 0 : stage + 1;
-    const bool last = t == tiles - 1;
+    take_scales();
     read(f[1], stage, 1);
-    multiply(f[0], std::integral_constant<int, 0>(), last);
-    uint32_t ka[MA], kbs[NB];  // this tile's scales, for its second step
-#pragma unroll
-    for (int m = 0; m < MA; ++m) ka[m] = sa[m];
-#pragma unroll
-    for (int n = 0; n < NB; ++n) kbs[n] = sb[n];
-    if (!last) {
-      if (t + 2 < tiles) copies_landed<S::kCopies>();
-      else copies_landed<0>();
-      if (t + kStages < tiles) {
-        put_scales(t + kStages, stage);
-        copies(t + kStages, stage);
-      }
-      read(f[0], next, 0);
-      read_scales(next);
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(f[0], first);
+    __builtin_amdgcn_sched_barrier(0);
+    if (t + 2 < tiles) copies_landed<S::kCopies>();
+    else copies_landed<0>();
+    // Every wave has read this stage, and (kWhole) at a window's first tile the window.
+    if constexpr (kWhole)
+      if ((t & 3) == 0 && t + 4 < tiles) window_copies(t / 4 + 1);
+    if (t + kStages < tiles) {
+      if constexpr (!kWhole) put_scales(t + kStages, stage);
+      copies(t + kStages, stage);
     }
-    uint32_t na[MA], nb[NB];
-#pragma unroll
-    for (int m = 0; m < MA; ++m) na[m] = sa[m], sa[m] = ka[m];
-#pragma unroll
-    for (int n = 0; n < NB; ++n) nb[n] = sb[n], sb[n] = kbs[n];
-    multiply(f[1], std::integral_constant<int, 1>(), last);
-#pragma unroll
-    for (int m = 0; m < MA; ++m) sa[m] = na[m];
-#pragma unroll
-    for (int n = 0; n < NB; ++n) sb[n] = nb[n];
+    read(f[0], next, 0);
+    if (!kWhole || (t & 3) == 3) read_scales(next);
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(f[1], second);
+    __builtin_amdgcn_sched_barrier(0);
     stage = next;
   }
+  take_scales();
+  read(f[1], stage, 1);
+  if (!kWhole && rem) {  // blocks past the end: weights of zero
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+      if (2 * h + s >= rem) {
+#pragma unroll
+        for (int m = 0; m < MA; ++m) f[s].a[m] = i32x4{0, 0, 0, 0};
+      }
+  }
+  multiply(f[0], first);
+  multiply(f[1], second);
+#pragma unroll
+  for (int m = 0; m < MA; ++m)
+#pragma unroll
+    for (int n = 0; n < NB; ++n) asm volatile("" : "+v"(acc[m][n]));  // the last products stay in front of what follows
   __syncthreads();  // the outputs reuse the stages
 
   // acc[m][n][i]: weight row 32 m + 8 (i / 4) + 4 h + i % 4, row of x 32 n + l32.  Outputs go through LDS, 32 rows
-  // of x at a time, so that a row's stand together.
+  // of x at a time, so that a row's stand together: gated ones with their activation, others as sums.
   constexpr int kStride = kOut + 4;
   float* mine = reinterpret_cast<float*>(lds) + wave * 32 * kStride;
   const int col0 = (nt * WA + wa) * kOut;
   const float* bias = a.bias ? a.bias + (size_t)e * a.M : nullptr;
   const bool wide =
       width % 8 == 0 && ((reinterpret_cast<uintptr_t>(a.y) | reinterpret_cast<uintptr_t>(a.residual)) & 15) == 0;
-#pragma unroll
-  for (int n = 0; n < NB; ++n) {
+  auto put = [&](int n, auto pair) {
+    int from = col0;
+    asm volatile("" : "+s"(from));  // addresses of biases are formed again: there are no registers to keep them
 #pragma unroll
     for (int m = 0; m < (kGated && MA > 1 ? MA / 2 : MA); ++m)
 #pragma unroll
       for (int g = 0; g < (kGated && MA == 1 ? 2 : 4); ++g) {
         const int o = 32 * m + 8 * g + 4 * h;
         f32x4 v;
+        if constexpr (kGated) {
+          float bz[4] = {0.f, 0.f, 0.f, 0.f}, bu[4] = {0.f, 0.f, 0.f, 0.f};
+          if (bias) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int c = min(col0 + o + i, width - 1);
-          float z = acc[m][n][4 * g + i];
-          if (bias) z += bias[c];
-          if constexpr (kGated) {
-            float u = MA == 1 ? acc[m][n][4 * (g + 2) + i] : acc[(m + MA / 2) % MA][n][4 * g + i];
-            if (bias) u += bias[width + c];
-            v[i] = act_pair(a.act, z, u, a.gb, a.vb);
-          } else {
-            v[i] = act_single(a.act, z);
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t c = (uint32_t)min(from + o + i, width - 1);
+              bz[i] = bias[c];
+              bu[i] = bias[(uint32_t)width + c];
+            }
           }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float u = MA == 1 ? acc[m][n][4 * (g + 2) % 16 + i] : acc[(m + MA / 2) % MA][n][4 * g + i];
+            v[i] = pair(acc[m][n][4 * g + i] + bz[i], u + bu[i]);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v[i] = acc[m][n][4 * g + i];
         }
         *reinterpret_cast<f32x4*>(mine + l32 * kStride + o) = v;
+        __builtin_amdgcn_sched_barrier(0);  // no more than these at once: registers
       }
+  };
+  constexpr int kLanes = kOut / 8;  // of a row, eight outputs each
+  auto take = [&](int t0, int r, bool plain) {
+    const int t = r + lane / kLanes, o = 8 * (lane % kLanes), col = col0 + o;
+    if (t0 + t >= nrow || col >= width) return;
+    float v[8];
+    *reinterpret_cast<f32x4*>(v) = *reinterpret_cast<const f32x4*>(mine + t * kStride + o);
+    *reinterpret_cast<f32x4*>(v + 4) = *reinterpret_cast<const f32x4*>(mine + t * kStride + o + 4);
+    if constexpr (!kGated) {
+      if (bias) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] += bias[min(col + i, width - 1)];
+      }
+      if (!plain) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = act_single(a.act, v[i]);
+      }
+    }
+    const size_t to = ((size_t)row0 + t0 + t) * width + col;
+    if (wide) {
+      if (a.residual) {
+        const uint4 r4 = *reinterpret_cast<const uint4*>(a.residual + to);
+        const uint32_t rw[4] = {r4.x, r4.y, r4.z, r4.w};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] += __uint_as_float(i % 2 ? rw[i / 2] & 0xffff0000u : rw[i / 2] << 16);
+      }
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = bf16_bits(v[2 * i]) | bf16_bits(v[2 * i + 1]) << 16;
+      *reinterpret_cast<uint4*>(a.y + to) = make_uint4(w[0], w[1], w[2], w[3]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (col + i < width)
+          a.y[to + i] = (uint16_t)bf16_bits(a.residual ? v[i] + bf16_to_f32(a.residual[to + i]) : v[i]);
+    }
+  };
+#pragma unroll
+  for (int n = 0; n < NB; ++n) {
+    if (kGated && a.act != RMOE_ACT_SWIGLU)
+      put(n, [&](float g, float u) { return act_pair(RMOE_ACT_SITU, g, u, a.gb, a.vb); });
+    else
+      put(n, [](float g, float u) { return swiglu(g, u); });
     const int t0 = wb * 32 * NB + 32 * n;
-    constexpr int kLanes = kOut / 8;  // of a row, eight outputs each
+    if (kGated || a.act == RMOE_ACT_NONE) {
 #pragma unroll
-    for (int r = 0; r < 32; r += 64 / kLanes) {
-      const int t = r + lane / kLanes, o = 8 * (lane % kLanes), col = col0 + o;
-      float v[8];
-      *reinterpret_cast<f32x4*>(v) = *reinterpret_cast<const f32x4*>(mine + t * kStride + o);
-      *reinterpret_cast<f32x4*>(v + 4) = *reinterpret_cast<const f32x4*>(mine + t * kStride + o + 4);
-      if (t0 + t >= nrow || col >= width) continue;
-      const size_t to = ((size_t)row0 + t0 + t) * width + col;
-      if (wide) {
-        if (a.residual) {
-          const uint4 r4 = *reinterpret_cast<const uint4*>(a.residual + to);
-          const uint32_t rw[4] = {r4.x, r4.y, r4.z, r4.w};
-#pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] += __uint_as_float(i % 2 ? rw[i / 2] & 0xffff0000u : rw[i / 2] << 16);
-        }
-        uint32_t w[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = bf16_bits(v[2 * i]) | bf16_bits(v[2 * i + 1]) << 16;
-        *reinterpret_cast<uint4*>(a.y + to) = make_uint4(w[0], w[1], w[2], w[3]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (col + i < width)
-            a.y[to + i] = (uint16_t)bf16_bits(a.residual ? v[i] + bf16_to_f32(a.residual[to + i]) : v[i]);
-      }
+      for (int r = 0; r < 32; r += 64 / kLanes) take(t0, r, true);
+    } else {
+#pragma unroll 1
+      for (int r = 0; r < 32; r += 64 / kLanes) take(t0, r, false);
     }
   }
 }
 
-template <int MA, int NB, int WA, int WB>
+template <int MA, int NB, int WA, int WB, bool kWhole>
 hipError_t launch_tiles(const MxLin& a, hipStream_t st) {
-  typedef TileShape<MA, NB, WA, WB> S;
+  typedef TileShape<MA, NB, WA, WB, kWhole> S;
   const bool gated = act_gated(a.act);
   const int width = gated ? a.M / 2 : a.M, out = S::BW / (gated ? 2 : 1), n_nt = (width + out - 1) / out;
   const size_t mt = a.offsets ? std::min<size_t>(a.n, (size_t)a.n / S::BT + a.n_experts) : ((size_t)a.n + S::BT - 1) / S::BT;
   const size_t grid = 8 * ((mt * n_nt + 7) / 8);
   if (grid * S::kThreads >= (size_t)1 << 32) return hipErrorInvalidValue;
-  auto* kernel = gated ? mx_tiles_kernel<MA, NB, WA, WB, true> : mx_tiles_kernel<MA, NB, WA, WB, false>;
+  auto* kernel = gated ? mx_tiles_kernel<MA, NB, WA, WB, kWhole, true> : mx_tiles_kernel<MA, NB, WA, WB, kWhole, false>;
   hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(S::kThreads), S::lds(gated), st, a, n_nt);
   return hipGetLastError();
 }
 template <int MA, int NB, int WA, int WB>
+hipError_t pick_tiles(const MxLin& a, hipStream_t st) {
+  const bool whole = a.K % 512 == 0 && ((reinterpret_cast<uintptr_t>(a.xs) | reinterpret_cast<uintptr_t>(a.ws)) & 15) == 0;
+  return whole ? launch_tiles<MA, NB, WA, WB, true>(a, st) : launch_tiles<MA, NB, WA, WB, false>(a, st);
+}
+template <int MA, int NB, int WA, int WB, bool kWhole>
 hipError_t setup_tiles() {
-  typedef TileShape<MA, NB, WA, WB> S;
-  hipError_t e = hipFuncSetAttribute((const void*)mx_tiles_kernel<MA, NB, WA, WB, true>,
+  typedef TileShape<MA, NB, WA, WB, kWhole> S;
+  hipError_t e = hipFuncSetAttribute((const void*)mx_tiles_kernel<MA, NB, WA, WB, kWhole, true>,
                                      hipFuncAttributeMaxDynamicSharedMemorySize, (int)S::lds(true));
   if (e == hipSuccess)
-    e = hipFuncSetAttribute((const void*)mx_tiles_kernel<MA, NB, WA, WB, false>,
+    e = hipFuncSetAttribute((const void*)mx_tiles_kernel<MA, NB, WA, WB, kWhole, false>,
                             hipFuncAttributeMaxDynamicSharedMemorySize, (int)S::lds(false));
   return e;
 }
 
 }  // namespace
 
-hipError_t mx_linear_setup() { return setup_tiles<4, 2, 2, 2>(); }
+// Allow the largest tiles their 78 KB of dynamic LDS (the others stay under 64).
+hipError_t mx_linear_setup() {
+  const hipError_t e = setup_tiles<4, 2, 2, 2, true>();
+  return e == hipSuccess ? setup_tiles<4, 2, 2, 2, false>() : e;
+}
 
 hipError_t launch_mx_linear(const MxLin& a, hipStream_t st) {
   if (a.n > 16 && a.K <= 1 << 20) {
     const int groups = a.offsets ? a.n_experts : 1;
-    if ((size_t)((a.n + 127) / 128) * ((a.M + 255) / 256) >= 512 && a.n / groups >= 64) return launch_tiles<4, 2, 2, 2>(a, st);
-    if ((size_t)((a.n + 127) / 128) * ((a.M + 127) / 128) >= 512 && a.n / groups >= 64) return launch_tiles<2, 2, 2, 2>(a, st);
-    if (a.n / groups > 16) return launch_tiles<1, 1, 2, 2>(a, st);
+    if ((size_t)((a.n + 127) / 128) * ((a.M + 255) / 256) >= 512 && a.n / groups >= 64) return pick_tiles<4, 2, 2, 2>(a, st);
+    if ((size_t)((a.n + 127) / 128) * ((a.M + 127) / 128) >= 512 && a.n / groups >= 64) return pick_tiles<2, 2, 2, 2>(a, st);
+    if (a.n / groups > 16) return pick_tiles<1, 1, 2, 2>(a, st);
   }
-  const size_t mt = a.offsets ? std::min<size_t>(a.n, (size_t)a.n / 16 + a.n_experts) : ((size_t)a.n + 15) / 16;
-  if (mt * a.M >= (size_t)512 * 256) return launch_few<4, 4>(a, st);
-  if (mt * a.M >= (size_t)512 * 32) return launch_few<2, 1>(a, st);
-  return launch_few<1, 1>(a, st);
+  // Weight rows over all row tiles (by expert: of the most tiles there can be).
+  const size_t rows = (size_t)a.M * (a.offsets ? std::min<size_t>(a.n, (size_t)a.n / 16 + a.n_experts) : ((size_t)a.n + 15) / 16);
+  if (rows <= 8192) return launch_few<1, 1>(a, st);
+  if (rows <= (a.offsets ? 49152 : 16384)) return launch_few<2, 2>(a, st);
+  return launch_few<2, 4>(a, st);
 }
 
 }  // namespace rmoe
