@@ -111,16 +111,16 @@ __global__ __launch_bounds__(256) void mx_few_kernel(MxLin a, int n_nt) {
   const int n_mt = a.offsets ? rt.total(a.offsets, a.n_experts, a.n) : (a.n + 15) / 16;
   // XCD x takes a contiguous eighth of the tiles, the row tiles of one weight tile (by expert: the weight
   // tiles of one row tile) back to back.
-  const long total = (long)n_mt * n_nt, per = (total + 7) / 8, slot = blockIdx.x / 8;
-  const long id = (long)(blockIdx.x % 8) * per + slot;
+  const uint32_t total = (uint32_t)n_mt * n_nt, per = (total + 7) / 8, slot = blockIdx.x / 8;  // a launch's fit 24 bits
+  const uint32_t id = blockIdx.x % 8 * per + slot;
   if (slot >= per || id >= total) return;
   int nt, e = 0, row0, nrow;
   if (a.offsets) {
-    nt = (int)(id % n_nt);
-    rt.find((int)(id / n_nt), e, row0, nrow);
+    rt.find((int)(id / (uint32_t)n_nt), e, row0, nrow);
+    nt = (int)(id % (uint32_t)n_nt);
   } else {
-    nt = (int)(id / n_mt);
-    row0 = (int)(id % n_mt) * 16;
+    nt = (int)(id / (uint32_t)n_mt);
+    row0 = (int)(id % (uint32_t)n_mt) * 16;
     nrow = min(16, a.n - row0);
   }
   const int tid = threadIdx.x, lane = tid & 63, wave = wave_id(), l16 = lane & 15, lq = lane >> 4;
@@ -228,22 +228,25 @@ hipError_t launch_few(const MxLin& a, hipStream_t st) {
 
 // ----------------------------------------------------------------- many rows --
 // Tiles of 32 MA WA weight rows by 32 NB WB rows of x; a wave takes 32 MA by 32 NB of them as 32 x 32 MFMAs
-// of 64 columns.  K goes by in tiles of 128 columns: 64 bytes of codes and a dword of scale bytes a row, in LDS in
-// three stages.  Codes are copied there past the registers, two tiles ahead of their use; scale bytes are
-// fetched 16 a row (four tiles) at a time and put beside the codes.  A lane's row of a fragment is lane % 32, and
-// of a tile's four blocks it holds 2 h and 2 h + 1, h = lane / 32, for the tile's two MFMA steps.
+// of 64 columns.  K goes by in stages of KT times 128 columns, 64 KT bytes of codes a row, which are copied to LDS past the
+// registers ahead of their use.  Scale bytes: of whole windows of 512 columns (kWhole) copied likewise, 16 a row;
+// else fetched by the registers and put beside a stage's codes, a dword a row.  A lane's row of a fragment is lane %
+// 32, and of the four blocks of 128 columns it holds 2 h and 2 h + 1, h = lane / 32, for two MFMA steps.
 // A gated wave's rows are 16 MA gate rows and the up rows of the same outputs.
-constexpr int kStages = 3;
 constexpr int kKTile = 4 * kMxBlock;
 
-template <int MA, int NB, int WA, int WB, bool kWhole>
+template <int MA, int NB, int WA, int WB, int KT, bool kWhole>
 struct TileShape {
+  static_assert(KT == 1 || kWhole, "ends of rows inside a stage of 256 columns are not handled");
   static constexpr int kWaves = WA * WB, kThreads = 64 * kWaves, BW = 32 * MA * WA, BT = 32 * NB * WB, R = BW + BT;
-  static constexpr int kCodes = R * 64, kStage = kCodes + (kWhole ? 0 : R * 4);  // a stage's bytes
-  static constexpr int kWindow = kStages * kStage;                               // where a window of scales begins
-  static constexpr int kCopies = R / 16 / kWaves;                  // a wave's copies of a K tile, 16 rows each
+  static constexpr int kStages = KT == 1 ? 3 : 2, kSteps = 2 * KT, kRow = 64 * KT;
+  static constexpr int kCodes = R * kRow, kStage = kCodes + (kWhole ? 0 : R * 4);  // a stage's bytes
+  static constexpr int kWindow = kStages * kStage;                     // where a window of scales begins
+  static constexpr int kCopyRows = 16 / KT;                            // rows of a copy
+  static constexpr int kCopies = R / kCopyRows / kWaves;               // a wave's copies of a stage
   static constexpr int kScaleCopies = (R / 64 + kWaves - 1) / kWaves;  // and of a window of scales, 64 rows each
   static constexpr int kScales = (R + kThreads - 1) / kThreads;
+  static_assert(KT == 1 || kCopies % 2 == 0, "a copy's parity is its number's");
   static constexpr size_t lds(bool gated) {
     const size_t out = (size_t)kWaves * 32 * ((gated ? 16 : 32) * MA + 4) * 4;
     const size_t in = (size_t)kStages * kStage + (kWhole ? R * 16 : 0);
@@ -271,34 +274,34 @@ __device__ __forceinline__ void copies_landed() {
   __syncthreads();
 }
 
-template <int MA, int NB, int WA, int WB, bool kWhole, bool kGated>
+template <int MA, int NB, int WA, int WB, int KT, bool kWhole, bool kGated>
 __global__ __launch_bounds__(64 * WA * WB, 2) void mx_tiles_kernel(MxLin a, int n_nt) {
-  typedef TileShape<MA, NB, WA, WB, kWhole> S;
+  typedef TileShape<MA, NB, WA, WB, KT, kWhole> S;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   constexpr int kOut = (kGated ? 16 : 32) * MA;  // outputs of a wave
   RowTiles<S::BT> rt;
   const int n_mt = a.offsets ? rt.total(a.offsets, a.n_experts, a.n) : (a.n + S::BT - 1) / S::BT;
   // XCD x takes a contiguous eighth of the tiles: by expert the weight tiles of a row tile back to back, else
   // blocks of up to eight row tiles for each weight tile, so that both operands' tiles meet again in its L2.
-  const long total = (long)n_mt * n_nt, per = (total + 7) / 8, slot = blockIdx.x / 8;
-  const long id = (long)(blockIdx.x % 8) * per + slot;
+  const uint32_t total = (uint32_t)n_mt * n_nt, per = (total + 7) / 8, slot = blockIdx.x / 8;  // a launch's fit 24 bits
+  const uint32_t id = blockIdx.x % 8 * per + slot;
   if (slot >= per || id >= total) return;
   int nt, e = 0, row0, nrow;
   if (a.offsets) {
-    nt = (int)(id % n_nt);
-    rt.find((int)(id / n_nt), e, row0, nrow);
+    rt.find((int)(id / (uint32_t)n_nt), e, row0, nrow);
+    nt = (int)(id % (uint32_t)n_nt);
   } else {
-    constexpr int kBlock = 8;
-    const long group = id / ((long)kBlock * n_nt);
-    const int m0 = (int)group * kBlock, nm = min(kBlock, n_mt - m0), in = (int)(id - group * kBlock * n_nt);
-    nt = in / nm;
-    row0 = (m0 + in % nm) * S::BT;
+    constexpr uint32_t kBlock = 8;
+    const uint32_t group = id / (kBlock * n_nt), m0 = group * kBlock, nm = min(kBlock, n_mt - m0);
+    const uint32_t in = id - group * kBlock * n_nt;
+    nt = (int)(in / nm);
+    row0 = (int)(m0 + in % nm) * S::BT;
     nrow = min(S::BT, a.n - row0);
   }
   const int tid = threadIdx.x, lane = tid & 63, wave = wave_id(), l32 = lane & 31, h = lane >> 5;
   const int wa = wave % WA, wb = wave / WA;
-  const int kb = a.K / kMxBlock, tiles = (kb + 3) / 4, rem = kb % 4;
-  const uint32_t ldb = (uint32_t)a.K / 2;
+  const int kb = a.K / kMxBlock, tiles = (kb + 3) / 4, stages = tiles / KT, rem = kb % 4;
+  uint32_t ldb = (uint32_t)a.K / 2;
   const int width = kGated ? a.M / 2 : a.M;
   // Row of an LDS row slot: of the weights (e's matrix) or of x; rows past the ends repeat the last one.
   auto weight_row = [&](int r) {
@@ -307,28 +310,35 @@ __global__ __launch_bounds__(64 * WA * WB, 2) void mx_tiles_kernel(MxLin a, int 
   };
   auto token_row = [&](int r) { return min(r - S::BW, nrow - 1); };
 
+  // A copy's first row, and how many rows behind it there are: those past them repeat the last one.
   const uint8_t* cbase[S::kCopies];
-  uint32_t coff[S::kCopies];
+  int cmore[S::kCopies];
 #pragma unroll
   for (int j = 0; j < S::kCopies; ++j) {
-    const int r0 = 16 * (wave * S::kCopies + j), r = r0 + (lane >> 2);
+    const int r0 = S::kCopyRows * (wave * S::kCopies + j);
     if (r0 < S::BW) {
-      const int first = weight_row(r0);
-      cbase[j] = a.w + ((size_t)e * a.M + first) * ldb;
-      coff[j] = (uint32_t)(weight_row(r) - first) * ldb;
+      const int o = (nt * WA + r0 / (32 * MA)) * kOut + r0 % (32 * MA) % kOut;
+      cbase[j] = a.w + ((size_t)e * a.M + weight_row(r0)) * ldb;
+      cmore[j] = max(width - 1 - o, 0);
     } else {
-      const int first = token_row(r0);
-      cbase[j] = a.x + ((size_t)row0 + first) * ldb;
-      coff[j] = (uint32_t)(token_row(r) - first) * ldb;
+      cbase[j] = a.x + ((size_t)row0 + token_row(r0)) * ldb;
+      cmore[j] = max(nrow - 1 - (r0 - S::BW), 0);
     }
   }
-  // Chunk c of a row's four stands at c ^ (row / 4 % 4): sixteen rows' chunks of one number are in different banks.
-    const int cchunk = (lane & 3) ^ (lane >> 4);
+  // Chunk c of a row's 4 KT stands at c ^ place(row), so that sixteen rows' chunks of one number are in different banks.
+  auto place = [](int row) { return KT == 1 ? (row >> 2) & 3 : (row >> 1) & 7; };
+  const int cchunk = KT == 1 ? (lane & 3) ^ (lane >> 4) : (lane & 7) ^ (lane >> 4);  // of the rows from an even copy's on
+  auto chunk_of = [&](int t) { return (uint32_t)(kWhole ? 4 * KT * t + cchunk : min(4 * t + cchunk, kb - 1)) * 16u; };
+  auto copy = [&](int j, uint32_t chunk, int stage) {
+    // Both factors fit 24 bits: K is at most 2^20.
+    const uint32_t row = __umul24((uint32_t)min(lane / (4 * KT), cmore[j]), ldb);
+    copy16(cbase[j], row + (KT == 2 && j % 2 ? chunk ^ 64u : chunk),
+           (uint32_t)(stage * S::kStage + S::kCopyRows * (wave * S::kCopies + j) * S::kRow));
+  };
   auto copies = [&](int t, int stage) {
-    const uint32_t k = (uint32_t)min(4 * t + cchunk, kb - 1) * 16u;
+    const uint32_t k = chunk_of(t);
 #pragma unroll
-    for (int j = 0; j < S::kCopies; ++j)
-      copy16(cbase[j], coff[j] + k, (uint32_t)(stage * S::kStage + 16 * (wave * S::kCopies + j) * 64));
+    for (int j = 0; j < S::kCopies; ++j) copy(j, k, stage);
   };
   // Scales of whole windows (K a multiple of 512): copied as the codes are, 16 bytes a row, into the one window there is
   // once every wave has the one before in its registers.
@@ -396,15 +406,22 @@ __global__ __launch_bounds__(64 * WA * WB, 2) void mx_tiles_kernel(MxLin a, int 
   } f[2];
   uint32_t sa[MA], sb[NB];
   const int arow = wa * 32 * MA + l32, brow = S::BW + wb * 32 * NB + l32;  // multiples of 32 away: l32's place
-  uint32_t at[2];  // of a lane's chunk in step 0 and 1 from its row's start
+  // A lane's chunk of step 0; that of step s is (4 (s / 2) + s % 2) * 16 away, by exclusive or.
+  uint32_t aat = arow * S::kRow + (2 * h ^ place(l32 & 15)) * 16u, bat = brow * S::kRow + (2 * h ^ place(l32 & 15)) * 16u;
+  // What addresses are formed from is made new in each turn of the loop: kept, they would take a quarter of the registers.
+  auto fresh = [&] { asm volatile("" : "+v"(aat), "+v"(bat), "+s"(ldb)); };
+  // Piece p of a step's fragments, in the order in which the products need them: b0, a0, the other b, the other a.
+  constexpr int kPieces = MA + NB, kProducts = MA * NB;
+  auto read = [&](Frags& g, int stage, int s, int p) {
+    const uint8_t* from = lds + stage * S::kStage;
+    const uint32_t step = (4 * (s / 2) + s % 2) * 16;
+    const int n = p == 0 ? 0 : p <= NB ? p - 1 : -1, m = p == 1 ? 0 : p - NB;
+    if (p == 0 || (p > 1 && p <= NB)) g.b[n] = *reinterpret_cast<const i32x4*>(from + (bat ^ step) + 32 * n * S::kRow);
+    else g.a[m] = *reinterpret_cast<const i32x4*>(from + (aat ^ step) + 32 * m * S::kRow);
+  };
+  auto read_all = [&](Frags& g, int stage, int s) {
 #pragma unroll
-  for (int s = 0; s < 2; ++s) at[s] = (uint32_t)((2 * h + s) ^ (l32 >> 2 & 3)) * 16u;
-  auto read = [&](Frags& g, int stage, int s) {
-    const uint8_t* p = lds + stage * S::kStage + at[s];
-#pragma unroll
-    for (int m = 0; m < MA; ++m) g.a[m] = *reinterpret_cast<const i32x4*>(p + (arow + 32 * m) * 64);
-#pragma unroll
-    for (int n = 0; n < NB; ++n) g.b[n] = *reinterpret_cast<const i32x4*>(p + (brow + 32 * n) * 64);
+    for (int p = 0; p < kPieces; ++p) read(g, stage, s, p);
   };
   // The dwords of a tile's scales (kWhole: of a window's four tiles, the next one's first); the lane's two bytes are
   // brought down where they are used, for a shift here would wait for every read before it.
@@ -432,72 +449,106 @@ __global__ __launch_bounds__(64 * WA * WB, 2) void mx_tiles_kernel(MxLin a, int 
     for (int m = 0; m < MA; ++m) sa[m] = take(da[m]);
 #pragma unroll
     for (int n = 0; n < NB; ++n) sb[n] = take(db[n]);
+    __builtin_amdgcn_sched_barrier(0);
   };
-  auto multiply = [&](const Frags& g, auto step) {
+  // The products of a step, `between(i)` behind the i-th: the reads and copies that go on meanwhile are dealt out
+  // among them, since a wave issues in order and a row of reads would keep the products behind it waiting.  The
+  // scheduling barriers keep the compiler from gathering them.
+  auto multiply = [&](const Frags& g, auto step, auto between) {
     constexpr int s = decltype(step)::value;
 #pragma unroll
-    for (int m = 0; m < MA; ++m)
+    for (int i = 0; i < kProducts; ++i) {
+      const int m = i / NB, n = i % NB;
+      acc[m][n] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(operand(g.a[m]), operand(g.b[n]), acc[m][n], kFp4, kFp4, s,
+                                                                  (int)sa[m], s, (int)sb[n]);
+      between(i);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  // Those of 0..n-1 that are behind the i-th product.
+  auto deal = [&](int i, int n, auto what) {
 #pragma unroll
-      for (int n = 0; n < NB; ++n)
-        acc[m][n] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(operand(g.a[m]), operand(g.b[n]), acc[m][n], kFp4, kFp4, s,
-                                                                    (int)sa[m], s, (int)sb[n]);
+    for (int p = 0; p < n; ++p)
+      if (min(p, kProducts - 1) == i) what(p);
   };
   const std::integral_constant<int, 0> first;
   const std::integral_constant<int, 1> second;
+  auto reading = [&](Frags& g, int stage, int s) {
+    return [&, stage, s](int i) { deal(i, kPieces, [&](int p) { read(g, stage, s, p); }); };
+  };
+  const auto nothing = [](int) {};
+  // Products written before this are not moved behind the branches after it.
+  auto pin = [&] {
+#pragma unroll
+    for (int m = 0; m < MA; ++m)
+#pragma unroll
+      for (int n = 0; n < NB; ++n) asm volatile("" : "+v"(acc[m][n]));
+  };
 
   if constexpr (kWhole) window_copies(0);
 #pragma unroll
-  for (int t = 0; t < kStages; ++t)
-    if (t < tiles) {
+  for (int t = 0; t < S::kStages; ++t)
+    if (t < stages) {
       if constexpr (!kWhole) put_scales(t, t);
       copies(t, t);
     }
-  if (tiles >= kStages) copies_landed<2 * S::kCopies>();
+  if (stages >= S::kStages) copies_landed<(S::kStages - 1) * S::kCopies>();
   else copies_landed<0>();
-  read(f[0], 0, 0);
+  read_all(f[0], 0, 0);
   read_scales(0);
-  // A tile's second step is read while its first is multiplied, the next tile's first while its second is.  The
-  // compiler would move the products behind the waits: the scheduling barriers keep them where they are.
-  int stage = 0;
-  for (int t = 0; t < tiles - 1; ++t) {
-    const int next = stage == kStages - 1 ? 0 : stage + 1;
+  // A step's fragments are read while the step before is multiplied.  A stage is met by the workgroup before its
+  // last step: every wave has read it (and the window, where that is new), the next stage's copies have landed.
+  auto most_steps = [&](int stage) {
     take_scales();
-    read(f[1], stage, 1);
-    __builtin_amdgcn_sched_barrier(0);
-    multiply(f[0], first);
-    __builtin_amdgcn_sched_barrier(0);
-    if (t + 2 < tiles) copies_landed<S::kCopies>();
-    else copies_landed<0>();
-    // Every wave has read this stage, and (kWhole) at a window's first tile the window.
-    if constexpr (kWhole)
-      if ((t & 3) == 0 && t + 4 < tiles) window_copies(t / 4 + 1);
-    if (t + kStages < tiles) {
-      if constexpr (!kWhole) put_scales(t + kStages, stage);
-      copies(t + kStages, stage);
+    multiply(f[0], first, reading(f[1], stage, 1));
+    if constexpr (KT == 2) {
+      multiply(f[1], second, reading(f[0], stage, 2));
+      take_scales();
+      multiply(f[0], first, reading(f[1], stage, 3));
     }
-    read(f[0], next, 0);
-    if (!kWhole || (t & 3) == 3) read_scales(next);
+  };
+  int stage = 0;
+  // Stage t, and the first fragments of the next; kMore: with the copies of the stage that takes its place.
+  auto turn = [&](int t, auto more) {
+    constexpr bool kMore = decltype(more)::value;
+    const int next = stage == S::kStages - 1 ? 0 : stage + 1;
+    fresh();
+    most_steps(stage);
+    pin();
+    if (S::kStages > 2 && t + S::kStages - 1 < stages) copies_landed<(S::kStages - 2) * S::kCopies>();
+    else copies_landed<0>();
+    if constexpr (kWhole) {
+      if (KT * t % 4 == 0 && KT * t + 4 < tiles) window_copies(KT * t / 4 + 1);
+    } else if constexpr (kMore) {
+      put_scales(t + S::kStages, stage);
+    }
+    if (!kWhole || KT * (t + 1) % 4 == 0) read_scales(next);
+    const uint32_t chunk = kMore ? chunk_of(t + S::kStages) : 0u;
     __builtin_amdgcn_sched_barrier(0);
-    multiply(f[1], second);
-    __builtin_amdgcn_sched_barrier(0);
+    multiply(f[1], second, [&](int i) {
+      deal(i, kPieces, [&](int p) { read(f[0], next, 0, p); });
+      if constexpr (kMore) deal(i, S::kCopies, [&](int j) { copy(j, chunk, stage); });
+    });
     stage = next;
-  }
-  take_scales();
-  read(f[1], stage, 1);
-  if (!kWhole && rem) {  // blocks past the end: weights of zero
+  };
+  int t = 0;
+  for (; t < stages - S::kStages; ++t) turn(t, std::true_type());
+  for (; t < stages - 1; ++t) turn(t, std::false_type());
+  if constexpr (kWhole) {
+    most_steps(stage);
+  } else {
+    take_scales();
+    read_all(f[1], stage, 1);
 #pragma unroll
     for (int s = 0; s < 2; ++s)
-      if (2 * h + s >= rem) {
+      if (rem && 2 * h + s >= rem) {  // blocks past the end: weights of zero
 #pragma unroll
         for (int m = 0; m < MA; ++m) f[s].a[m] = i32x4{0, 0, 0, 0};
       }
+    multiply(f[0], first, nothing);
   }
-  multiply(f[0], first);
-  multiply(f[1], second);
-#pragma unroll
-  for (int m = 0; m < MA; ++m)
-#pragma unroll
-    for (int n = 0; n < NB; ++n) asm volatile("" : "+v"(acc[m][n]));  // the last products stay in front of what follows
+  multiply(f[1], second, nothing);
+  pin();
   __syncthreads();  // the outputs reuse the stages
 
   // acc[m][n][i]: weight row 32 m + 8 (i / 4) + 4 h + i % 4, row of x 32 n + l32.  Outputs go through LDS, 32 rows
@@ -593,54 +644,74 @@ __global__ __launch_bounds__(64 * WA * WB, 2) void mx_tiles_kernel(MxLin a, int 
   }
 }
 
-template <int MA, int NB, int WA, int WB, bool kWhole>
+template <int MA, int NB, int WA, int WB, int KT, bool kWhole>
 hipError_t launch_tiles(const MxLin& a, hipStream_t st) {
-  typedef TileShape<MA, NB, WA, WB, kWhole> S;
+  typedef TileShape<MA, NB, WA, WB, KT, kWhole> S;
   const bool gated = act_gated(a.act);
   const int width = gated ? a.M / 2 : a.M, out = S::BW / (gated ? 2 : 1), n_nt = (width + out - 1) / out;
   const size_t mt = a.offsets ? std::min<size_t>(a.n, (size_t)a.n / S::BT + a.n_experts) : ((size_t)a.n + S::BT - 1) / S::BT;
   const size_t grid = 8 * ((mt * n_nt + 7) / 8);
   if (grid * S::kThreads >= (size_t)1 << 32) return hipErrorInvalidValue;
-  auto* kernel = gated ? mx_tiles_kernel<MA, NB, WA, WB, kWhole, true> : mx_tiles_kernel<MA, NB, WA, WB, kWhole, false>;
+  auto* kernel = gated ? mx_tiles_kernel<MA, NB, WA, WB, KT, kWhole, true> : mx_tiles_kernel<MA, NB, WA, WB, KT, kWhole, false>;
   hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(S::kThreads), S::lds(gated), st, a, n_nt);
   return hipGetLastError();
 }
 template <int MA, int NB, int WA, int WB>
 hipError_t pick_tiles(const MxLin& a, hipStream_t st) {
   const bool whole = a.K % 512 == 0 && ((reinterpret_cast<uintptr_t>(a.xs) | reinterpret_cast<uintptr_t>(a.ws)) & 15) == 0;
-  return whole ? launch_tiles<MA, NB, WA, WB, true>(a, st) : launch_tiles<MA, NB, WA, WB, false>(a, st);
+  return whole ? launch_tiles<MA, NB, WA, WB, 2, true>(a, st) : launch_tiles<MA, NB, WA, WB, 1, false>(a, st);
 }
-template <int MA, int NB, int WA, int WB, bool kWhole>
+template <int MA, int NB, int WA, int WB, int KT, bool kWhole>
 hipError_t setup_tiles() {
-  typedef TileShape<MA, NB, WA, WB, kWhole> S;
-  hipError_t e = hipFuncSetAttribute((const void*)mx_tiles_kernel<MA, NB, WA, WB, kWhole, true>,
+  typedef TileShape<MA, NB, WA, WB, KT, kWhole> S;
+  hipError_t e = hipFuncSetAttribute((const void*)mx_tiles_kernel<MA, NB, WA, WB, KT, kWhole, true>,
                                      hipFuncAttributeMaxDynamicSharedMemorySize, (int)S::lds(true));
   if (e == hipSuccess)
-    e = hipFuncSetAttribute((const void*)mx_tiles_kernel<MA, NB, WA, WB, kWhole, false>,
+    e = hipFuncSetAttribute((const void*)mx_tiles_kernel<MA, NB, WA, WB, KT, kWhole, false>,
                             hipFuncAttributeMaxDynamicSharedMemorySize, (int)S::lds(false));
   return e;
 }
 
 }  // namespace
 
-// Allow the largest tiles their 78 KB of dynamic LDS (the others stay under 64).
+// Allow the tiles of more than 64 KB of dynamic LDS theirs (up to 136).
 hipError_t mx_linear_setup() {
-  const hipError_t e = setup_tiles<4, 2, 2, 2, true>();
-  return e == hipSuccess ? setup_tiles<4, 2, 2, 2, false>() : e;
+  for (const hipError_t e : {setup_tiles<4, 2, 2, 4, 2, true>(), setup_tiles<4, 2, 2, 4, 1, false>(),
+                             setup_tiles<2, 2, 2, 2, 2, true>(), setup_tiles<2, 1, 2, 2, 2, true>()})
+    if (e != hipSuccess) return e;
+  return hipSuccess;
 }
 
+// Which kernel serves a call; times in us at 2,560 columns or those given.
+//   Weight rows over all tiles of 16 rows of x, at most kFewRows: the kernel of few rows, for its waves share K.  32 rows of
+//   [4096, 4096] 7.1 and 11.0 with the smallest tiles, 64 rows (16,384) 10.7 and 11.3, 96 rows 14.2 and 11.5.  Fragments
+//   a wave: up to kOneFragment weight rows one (four rows of [4096, 4096] 5.3, two 6.2), above two (64 rows of [1536, 2048] 5.1
+//   and 5.6).  Up to 16 rows of x it serves any matrix, without shared parts of K (16 rows of [24064] 12.6; with two 14.0).
+//   By expert few rows each (under kFewEach) leave the tiles empty: two parts of K, 32 rows of 128 experts' [1536, 2048]
+//   12.1 and 14.8 without, 256 rows 36.7 and 38.4 in tiles of 128 x 64; 512 rows 41.6 and 41.3.
+//   Tiles of 256 x 256 where there are kFillLarge of them (445 rows of [24064] 26.2, in tiles of 128 x 128 27.1; 256 rows
+//   24.2 and 17.9) and, by expert, kFillEach rows each (32,000 rows of 128 experts' [1536, 2048] 110 and 116 in
+//   128 x 64, 16,000 rows 77 and 74).  Else by expert 128 x 64; dense 64 x 64 up to kFillSmall of them (1,024 rows of [4096,
+//   4096] 22.8 and 20.2 in 128 x 128, 2,048 of [1536, 2048] 11.1 and 12.2), above 128 x 128.
+constexpr size_t kOneFragment = 4096, kFewRows = 16384, kFillSmall = 1000, kFillLarge = 180;
+constexpr int kFewEach = 4, kFillEach = 250;
+
 hipError_t launch_mx_linear(const MxLin& a, hipStream_t st) {
-  if (a.n > 16 && a.K <= 1 << 20) {
-    const int groups = a.offsets ? a.n_experts : 1;
-    if ((size_t)((a.n + 127) / 128) * ((a.M + 255) / 256) >= 512 && a.n / groups >= 64) return pick_tiles<4, 2, 2, 2>(a, st);
-    if ((size_t)((a.n + 127) / 128) * ((a.M + 127) / 128) >= 512 && a.n / groups >= 64) return pick_tiles<2, 2, 2, 2>(a, st);
-    if (a.n / groups > 16) return pick_tiles<1, 1, 2, 2>(a, st);
+  const size_t n = a.n, M = a.M, groups = a.offsets ? a.n_experts : 1;
+  auto tiles = [&](size_t weights, size_t rows) { return (n + rows - 1) / rows * ((M + weights - 1) / weights); };
+  const size_t rows = M * (a.offsets ? std::min(n, n / 16 + groups) : (n + 15) / 16);
+  if (rows <= kOneFragment) return launch_few<1, 1>(a, st);
+  if (rows <= kFewRows) return launch_few<2, 1>(a, st);
+  // The tiles' offsets within a matrix's scales and 16 rows' codes take 32 bits.
+  const bool wide = a.K > 1 << 20 || M * (a.K / kMxBlock) >= (size_t)1 << 32;
+  if (a.offsets) {
+    if (wide || n < kFewEach * groups) return launch_few<2, 2>(a, st);
+    if (n >= kFillEach * groups && tiles(256, 256) >= kFillLarge) return pick_tiles<4, 2, 2, 4>(a, st);
+    return pick_tiles<2, 1, 2, 2>(a, st);
   }
-  // Weight rows over all row tiles (by expert: of the most tiles there can be).
-  const size_t rows = (size_t)a.M * (a.offsets ? std::min<size_t>(a.n, (size_t)a.n / 16 + a.n_experts) : ((size_t)a.n + 15) / 16);
-  if (rows <= 8192) return launch_few<1, 1>(a, st);
-  if (rows <= (a.offsets ? 49152 : 16384)) return launch_few<2, 2>(a, st);
-  return launch_few<2, 4>(a, st);
+  if (wide || n <= 16) return launch_few<2, 4>(a, st);
+  if (tiles(256, 256) >= kFillLarge) return pick_tiles<4, 2, 2, 4>(a, st);
+  return tiles(64, 64) < kFillSmall ? pick_tiles<1, 1, 2, 2>(a, st) : pick_tiles<2, 2, 2, 2>(a, st);
 }
 
 }  // namespace rmoe

@@ -215,7 +215,10 @@ def test_product_with_activation(gpu_ctx, act, T, M, K):
 
 
 @pytest.mark.parametrize("T,M,K,act", [(1, 1536, 2048, "swiglu"), (4, 20001, 2560, "none"), (445, 2560, 1088, "none"),
-                                       (1030, 4096, 2048, "swiglu"), (2100, 4100, 992, "none"), (700, 8200, 352, "silu")])
+                                       (1030, 4096, 2048, "swiglu"), (2100, 4100, 992, "none"), (700, 8200, 352, "silu"),
+                                       (1100, 9300, 512, "none"), (1100, 9300, 1056, "swiglu"), (1030, 12000, 1024, "swiglu"),
+                                       (1030, 12001, 1024, "gelu_tanh"), (600, 16000, 96, "none"), (300, 1200, 544, "situ"),
+                                       (300, 1200, 1536, "situ")])
 def test_product_of_size(gpu_ctx, T, M, K, act):
     _check_product(gpu_ctx, T, M, K, act, bias=True, residual=True, seed=5)
 
@@ -322,7 +325,9 @@ def test_experts_with_activation(gpu_ctx, act):
 
 
 @pytest.mark.parametrize("counts,M,K", [([500, 3, 0, 700, 260, 0, 40, 90] * 2, 520, 544), ([130] * 20, 1536, 256),
-                                        ([700, 900], 1030, 288), ([40] * 64, 768, 1088)])
+                                        ([700, 900], 1030, 288), ([40] * 64, 768, 1088),
+                                        ([30, 0, 70] * 3, 520, 1024), ([1, 2] * 12, 2000, 512),
+                                        ([1500, 3, 2100, 500], 3200, 512), ([1000, 1500, 0, 1600], 3200, 352)])
 def test_experts_of_size(gpu_ctx, counts, M, K):
     _check_experts(gpu_ctx, counts, M, K, "swiglu", behind=2)
 
