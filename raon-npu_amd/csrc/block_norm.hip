@@ -73,7 +73,7 @@ __device__ __forceinline__ float inv_rms(float squares, int H, float eps) {
 }
 
 // Where a thread's chunks of a row are.  Of aligned rows (kWide) the threads past the row's end repeat its last chunk,
-// so that loads and stores are free of branches: they compute and store what its owner does, and take no part in sums.
+// so that loads and stores are free of branches: they compute (and store) what its owner does, and take no part in sums.
 template <int V, bool kWide>
 struct Columns {
   int first, step, H;
@@ -89,8 +89,12 @@ __device__ __forceinline__ void load_row(const void* rows, size_t t, const Colum
 #pragma unroll
   for (int v = 0; v < V; ++v) o[v] = load_chunk<DT, kWide, kOnce>(p, c.at(v), c.H);
 }
+// With one chunk a thread the repeating threads are in their owner's wave, whose loads and stores of an address keep
+// their order; with two they may be in another, which would read a row that is written in place too late: they do not store.
 template <int DT, int V, bool kWide>
 __device__ __forceinline__ void store_row(void* rows, size_t t, const Columns<V, kWide>& c, int v, const Chunk<DT>& o) {
+  if constexpr (V > 1)
+    if (!c.counts(v, 0)) return;
   store_chunk<DT, kWide>(static_cast<typename RowElem<DT>::T*>(rows) + t * c.H, c.at(v), c.H, o);
 }
 // A thread's columns of an fp32 vector of H, or ones where there is none.  Of aligned rows without a branch: the

@@ -228,25 +228,25 @@ hipError_t launch_few(const MxLin& a, hipStream_t st) {
 
 // ----------------------------------------------------------------- many rows --
 // Tiles of 32 MA WA weight rows by 32 NB WB rows of x; a wave takes 32 MA by 32 NB of them as 32 x 32 MFMAs
-// of 64 columns.  K goes by in stages of KT times 128 columns, 64 KT bytes of codes a row, which are copied to LDS past the
-// registers ahead of their use.  Scale bytes: of whole windows of 512 columns (kWhole) copied likewise, 16 a row;
-// else fetched by the registers and put beside a stage's codes, a dword a row.  A lane's row of a fragment is lane %
+// of 64 columns.  Codes are copied to LDS past the registers, ahead of their use.  Where K is whole windows of 512 columns
+// (kWhole), in two stages of 256 columns, 128 bytes a row, and the scale bytes of a window likewise, 16 a row; else in three
+// of 128 columns, and scale bytes are fetched by the registers and put beside a stage's codes, a dword a row.  A lane's row of a fragment is lane %
 // 32, and of the four blocks of 128 columns it holds 2 h and 2 h + 1, h = lane / 32, for two MFMA steps.
 // A gated wave's rows are 16 MA gate rows and the up rows of the same outputs.
-constexpr int kKTile = 4 * kMxBlock;
 
-template <int MA, int NB, int WA, int WB, int KT, bool kWhole>
+template <int MA, int NB, int WA, int WB, bool kWhole>
 struct TileShape {
-  static_assert(KT == 1 || kWhole, "ends of rows inside a stage of 256 columns are not handled");
+  static constexpr int KT = kWhole ? 2 : 1;
   static constexpr int kWaves = WA * WB, kThreads = 64 * kWaves, BW = 32 * MA * WA, BT = 32 * NB * WB, R = BW + BT;
-  static constexpr int kStages = KT == 1 ? 3 : 2, kSteps = 2 * KT, kRow = 64 * KT;
+  static constexpr int kStages = kWhole ? 2 : 3, kRow = 64 * KT;
   static constexpr int kCodes = R * kRow, kStage = kCodes + (kWhole ? 0 : R * 4);  // a stage's bytes
   static constexpr int kWindow = kStages * kStage;                     // where a window of scales begins
   static constexpr int kCopyRows = 16 / KT;                            // rows of a copy
   static constexpr int kCopies = R / kCopyRows / kWaves;               // a wave's copies of a stage
   static constexpr int kScaleCopies = (R / 64 + kWaves - 1) / kWaves;  // and of a window of scales, 64 rows each
   static constexpr int kScales = (R + kThreads - 1) / kThreads;
-  static_assert(KT == 1 || kCopies % 2 == 0, "a copy's parity is its number's");
+  static_assert(KT == 1 || kCopies % 2 == 0, "the parity of a copy's rows is its number's");
+  static_assert(R % 64 == 0 && R % (kCopyRows * kWaves) == 0, "whole copies");
   static constexpr size_t lds(bool gated) {
     const size_t out = (size_t)kWaves * 32 * ((gated ? 16 : 32) * MA + 4) * 4;
     const size_t in = (size_t)kStages * kStage + (kWhole ? R * 16 : 0);
@@ -274,9 +274,10 @@ __device__ __forceinline__ void copies_landed() {
   __syncthreads();
 }
 
-template <int MA, int NB, int WA, int WB, int KT, bool kWhole, bool kGated>
+template <int MA, int NB, int WA, int WB, bool kWhole, bool kGated>
 __global__ __launch_bounds__(64 * WA * WB, 2) void mx_tiles_kernel(MxLin a, int n_nt) {
-  typedef TileShape<MA, NB, WA, WB, KT, kWhole> S;
+  typedef TileShape<MA, NB, WA, WB, kWhole> S;
+  constexpr int KT = S::KT;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   constexpr int kOut = (kGated ? 16 : 32) * MA;  // outputs of a wave
   RowTiles<S::BT> rt;
@@ -644,30 +645,30 @@ __global__ __launch_bounds__(64 * WA * WB, 2) void mx_tiles_kernel(MxLin a, int 
   }
 }
 
-template <int MA, int NB, int WA, int WB, int KT, bool kWhole>
+template <int MA, int NB, int WA, int WB, bool kWhole>
 hipError_t launch_tiles(const MxLin& a, hipStream_t st) {
-  typedef TileShape<MA, NB, WA, WB, KT, kWhole> S;
+  typedef TileShape<MA, NB, WA, WB, kWhole> S;
   const bool gated = act_gated(a.act);
   const int width = gated ? a.M / 2 : a.M, out = S::BW / (gated ? 2 : 1), n_nt = (width + out - 1) / out;
   const size_t mt = a.offsets ? std::min<size_t>(a.n, (size_t)a.n / S::BT + a.n_experts) : ((size_t)a.n + S::BT - 1) / S::BT;
   const size_t grid = 8 * ((mt * n_nt + 7) / 8);
   if (grid * S::kThreads >= (size_t)1 << 32) return hipErrorInvalidValue;
-  auto* kernel = gated ? mx_tiles_kernel<MA, NB, WA, WB, KT, kWhole, true> : mx_tiles_kernel<MA, NB, WA, WB, KT, kWhole, false>;
+  auto* kernel = gated ? mx_tiles_kernel<MA, NB, WA, WB, kWhole, true> : mx_tiles_kernel<MA, NB, WA, WB, kWhole, false>;
   hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(S::kThreads), S::lds(gated), st, a, n_nt);
   return hipGetLastError();
 }
 template <int MA, int NB, int WA, int WB>
 hipError_t pick_tiles(const MxLin& a, hipStream_t st) {
   const bool whole = a.K % 512 == 0 && ((reinterpret_cast<uintptr_t>(a.xs) | reinterpret_cast<uintptr_t>(a.ws)) & 15) == 0;
-  return whole ? launch_tiles<MA, NB, WA, WB, 2, true>(a, st) : launch_tiles<MA, NB, WA, WB, 1, false>(a, st);
+  return whole ? launch_tiles<MA, NB, WA, WB, true>(a, st) : launch_tiles<MA, NB, WA, WB, false>(a, st);
 }
-template <int MA, int NB, int WA, int WB, int KT, bool kWhole>
+template <int MA, int NB, int WA, int WB, bool kWhole>
 hipError_t setup_tiles() {
-  typedef TileShape<MA, NB, WA, WB, KT, kWhole> S;
-  hipError_t e = hipFuncSetAttribute((const void*)mx_tiles_kernel<MA, NB, WA, WB, KT, kWhole, true>,
+  typedef TileShape<MA, NB, WA, WB, kWhole> S;
+  hipError_t e = hipFuncSetAttribute((const void*)mx_tiles_kernel<MA, NB, WA, WB, kWhole, true>,
                                      hipFuncAttributeMaxDynamicSharedMemorySize, (int)S::lds(true));
   if (e == hipSuccess)
-    e = hipFuncSetAttribute((const void*)mx_tiles_kernel<MA, NB, WA, WB, KT, kWhole, false>,
+    e = hipFuncSetAttribute((const void*)mx_tiles_kernel<MA, NB, WA, WB, kWhole, false>,
                             hipFuncAttributeMaxDynamicSharedMemorySize, (int)S::lds(false));
   return e;
 }
@@ -676,8 +677,8 @@ hipError_t setup_tiles() {
 
 // Allow the tiles of more than 64 KB of dynamic LDS theirs (up to 136).
 hipError_t mx_linear_setup() {
-  for (const hipError_t e : {setup_tiles<4, 2, 2, 4, 2, true>(), setup_tiles<4, 2, 2, 4, 1, false>(),
-                             setup_tiles<2, 2, 2, 2, 2, true>(), setup_tiles<2, 1, 2, 2, 2, true>()})
+  for (const hipError_t e : {setup_tiles<4, 2, 2, 4, true>(), setup_tiles<4, 2, 2, 4, false>(),
+                             setup_tiles<2, 2, 2, 2, true>()})
     if (e != hipSuccess) return e;
   return hipSuccess;
 }

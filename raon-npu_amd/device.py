@@ -105,15 +105,19 @@ def _bf16_operand(device: int, t, shape: tuple, name: str) -> int:
     return _operand(device, t, shape, "int16" if _dtype_name(t) == "int16" else "bfloat16", name)
 
 
-def _byte_operand(device: int, t, shape: tuple, name: str, torch_name: str) -> int:
-    """Bytes of a given shape: uint8, or torch's own type of what they hold."""
-    return _operand(device, t, shape, torch_name if _dtype_name(t) == torch_name else "uint8", name)
+_CODES = ("uint8", "float4_e2m1fn_x2")  # bytes, or torch's own type of what they hold
+_SCALES = ("uint8", "float8_e8m0fnu")
 
 
-def _mx_operands(device: int, codes, scales, lead: tuple, K: int, name: str) -> tuple[int, int]:
-    """The addresses of microscaled rows of K columns (a multiple of 32)."""
-    return (_byte_operand(device, codes, (*lead, K // 2), f"{name} codes", "float4_e2m1fn_x2"),
-            _byte_operand(device, scales, (*lead, K // 32), f"{name} scales", "float8_e8m0fnu"))
+def _byte_operand(device: int, t, shape: tuple, types: tuple, name: str) -> int:
+    """Bytes of a given shape, of one of two types (one expression, for the reason _operand gives)."""
+    try:
+        if (t.get_device() == device and t.shape == shape and _DTYPE_NAMES.get(t.dtype) in types
+                and t.is_contiguous()):
+            return t.data_ptr()
+    except AttributeError:
+        pass
+    return _operand(device, t, shape, types[1] if _dtype_name(t) == types[1] else types[0], name)
 
 
 def _optional(device: int, t, shape: tuple, dtype_name: str, name: str) -> int | None:
@@ -346,11 +350,12 @@ class Context:
         half.  Weights [M, K] are quantized by the same call.  Asynchronous; allocates nothing and uses no scratch."""
         dt, dev = _row_type(x_dev, "x"), self.device
         T, K = _shape2(x_dev, "x")
-        P = -(-K // 32) * 32
-        codes, scales = _mx_operands(dev, codes_dev, scales_dev, (T,), P, "x")
+        G = (K + 31) // 32
         check(_lib.load().rmoe_mx_quantize_dev(
-            self._h, _operand(dev, x_dev, (T, K), dt, "x"), _ROW_TYPES[dt], T, K, codes, scales,
-            _optional(dev, values_dev, (T, K), dt, "values"), _stream_ptr(stream)))
+            self._h, _operand(dev, x_dev, (T, K), dt, "x"), _ROW_TYPES[dt], T, K,
+            _byte_operand(dev, codes_dev, (T, 16 * G), _CODES, "codes"),
+            _byte_operand(dev, scales_dev, (T, G), _SCALES, "scales"),
+            None if values_dev is None else _operand(dev, values_dev, (T, K), dt, "values"), _stream_ptr(stream)))
 
     def mx_linear_dev(self, x_codes_dev, x_scales_dev, w_codes_dev, w_scales_dev, y_dev, bias_dev=None, act: str = "none",
                       residual_dev=None, gate_beta=None, value_beta=None, stream=None):
@@ -361,12 +366,14 @@ class Context:
         at once).  A row's last bits may depend on T."""
         code, gb, vb, gated = _epilogue_act(act, gate_beta, value_beta)
         dev, (T, K), M = self.device, _shape2(x_codes_dev, "x codes"), _shape2(w_codes_dev, "w codes")[0]
-        K *= 2
-        x, xs = _mx_operands(dev, x_codes_dev, x_scales_dev, (T,), K, "x")
-        w, ws = _mx_operands(dev, w_codes_dev, w_scales_dev, (M,), K, "w")
+        G = K // 16
         out = (T, M // 2 if gated else M)
         check(_lib.load().rmoe_mx_linear_dev(
-            self._h, x, xs, T, K, w, ws, M, _optional(dev, bias_dev, (M,), "float32", "bias"), code, gb, vb,
+            self._h, _byte_operand(dev, x_codes_dev, (T, K), _CODES, "x codes"),
+            _byte_operand(dev, x_scales_dev, (T, G), _SCALES, "x scales"), T, 2 * K,
+            _byte_operand(dev, w_codes_dev, (M, K), _CODES, "w codes"),
+            _byte_operand(dev, w_scales_dev, (M, G), _SCALES, "w scales"), M,
+            None if bias_dev is None else _operand(dev, bias_dev, (M,), "float32", "bias"), code, gb, vb,
             None if residual_dev is None else _bf16_operand(dev, residual_dev, out, "residual"),
             _bf16_operand(dev, y_dev, out, "y"), _stream_ptr(stream)))
 
@@ -378,16 +385,18 @@ class Context:
         Rows from ``offsets[E]`` on stay as they were."""
         code, gb, vb, gated = _epilogue_act(act, gate_beta, value_beta)
         dev, (n, K) = self.device, _shape2(rows_codes_dev, "rows codes")
-        K *= 2
+        G = K // 16
         try:
             E, M, _ = w_codes_dev.shape
         except (AttributeError, ValueError):
             raise ValueError(f"w codes must be [E, M, K / 2], got shape {tuple(getattr(w_codes_dev, 'shape', ()))}") from None
-        x, xs = _mx_operands(dev, rows_codes_dev, rows_scales_dev, (n,), K, "rows")
-        w, ws = _mx_operands(dev, w_codes_dev, w_scales_dev, (E, M), K, "w")
         out = (n, M // 2 if gated else M)
         check(_lib.load().rmoe_mx_experts_linear_dev(
-            self._h, x, xs, n, K, w, ws, M, _operand(dev, offsets_dev, (E + 1,), "int32", "offsets"), E,
+            self._h, _byte_operand(dev, rows_codes_dev, (n, K), _CODES, "rows codes"),
+            _byte_operand(dev, rows_scales_dev, (n, G), _SCALES, "rows scales"), n, 2 * K,
+            _byte_operand(dev, w_codes_dev, (E, M, K), _CODES, "w codes"),
+            _byte_operand(dev, w_scales_dev, (E, M, G), _SCALES, "w scales"), M,
+            _operand(dev, offsets_dev, (E + 1,), "int32", "offsets"), E,
             _optional(dev, bias_dev, (E, M), "float32", "bias"), code, gb, vb,
             None if residual_dev is None else _bf16_operand(dev, residual_dev, out, "residual"),
             _bf16_operand(dev, y_dev, out, "y"), _stream_ptr(stream)))
@@ -412,18 +421,22 @@ class Context:
                    scales_dev, eps, stream)
 
     def _norm(self, block, residual, y, post, gate, scale, pre, h, codes, scales, eps, stream):
-        dt, dev = _row_type(residual, "residual" if block is not None else "x"), self.device
-        T, H = _shape2(residual, "residual" if block is not None else "x")
-        rows = (T, H)
-        if (codes is None) != (scales is None):
-            raise ValueError("codes and scales go together")
-        c, s = (None, None) if codes is None else _mx_operands(dev, codes, scales, (T,), -(-H // 32) * 32, "h")
-        g, kind = _gate_operand(dev, gate, T, H, dt, "gate")
+        name = "x" if block is None else "residual"
+        dt, dev = _row_type(residual, name), self.device
+        rows = T, H = _shape2(residual, name)
+        c = s = None
+        if codes is not None or scales is not None:
+            G = (H + 31) // 32
+            c = _byte_operand(dev, codes, (T, 16 * G), _CODES, "codes")
+            s = _byte_operand(dev, scales, (T, G), _SCALES, "scales")
+        g, kind = (None, GATE_NONE) if gate is None else _gate_operand(dev, gate, T, H, dt, "gate")
         check(_lib.load().rmoe_residual_norm_dev(
-            self._h, _optional(dev, block, rows, dt, "block"), _operand(dev, residual, rows, dt, "residual"), _ROW_TYPES[dt],
-            T, H, _optional(dev, post, (H,), "float32", "post weight"), g, kind, float(scale),
-            _optional(dev, pre, (H,), "float32", "pre weight"), float(eps), _optional(dev, y, rows, dt, "y"),
-            _optional(dev, h, rows, dt, "h"), c, s, _stream_ptr(stream)))
+            self._h, None if block is None else _operand(dev, block, rows, dt, "block"),
+            _operand(dev, residual, rows, dt, name), _ROW_TYPES[dt], T, H,
+            None if post is None else _operand(dev, post, (H,), "float32", "post weight"), g, kind, float(scale),
+            None if pre is None else _operand(dev, pre, (H,), "float32", "pre weight"), float(eps),
+            None if y is None else _operand(dev, y, rows, dt, "y"),
+            None if h is None else _operand(dev, h, rows, dt, "h"), c, s, _stream_ptr(stream)))
 
     @staticmethod
     def norm_backward_work(T: int, H: int) -> int:
@@ -453,8 +466,8 @@ class Context:
 
     def _norm_backward(self, dy, dh, block, y, dblock, dresidual, work, post, dpost, gate, dgate, scale, pre, dpre, eps, stream):
         dt, dev = _row_type(y, "y"), self.device
-        T, H = _shape2(y, "y")
-        rows, vector = (T, H), (H,)
+        rows = T, H = _shape2(y, "y")
+        vector = (H,)
         g, kind = _gate_operand(dev, gate, T, H, dt, "gate")
         if dgate is not None and gate is None:
             raise ValueError("a gradient goes with its gate")

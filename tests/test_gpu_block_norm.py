@@ -76,7 +76,7 @@ def _check_h(h, y, pre, dtype):
 
 
 SHAPES = [(1, 1), (1, 7), (3, 8), (2, 33), (5, 64), (1, 2048), (17, 511), (9, 520), (445, 2560), (4, 4096), (3, 4097), (2, 8192),
-          (6, 5001), (2, 8191)]
+          (6, 5001), (2, 8191), (64, 4104), (33, 7000), (40, 2568)]
 
 
 @pytest.mark.parametrize("T,H", SHAPES)
@@ -225,7 +225,7 @@ def _check_gradients(got, want, T, dtype):
 
 
 @pytest.mark.parametrize("T,H", [(1, 1), (1, 7), (2, 33), (5, 64), (1, 2048), (17, 511), (445, 520), (1030, 96), (9, 2560), (3, 4097),
-                                 (2, 8192), (600, 5001)])
+                                 (2, 8192), (600, 5001), (64, 4104), (300, 7000), (40, 2568)])
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
 @pytest.mark.parametrize("post,gate", [(True, "column"), (False, "none"), (True, "row"), (False, "full"), (True, "none"),
                                        (False, "column"), (True, "full")])
