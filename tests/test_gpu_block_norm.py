@@ -314,3 +314,25 @@ def test_on_other_streams_and_captured(gpu_ctx):
         assert torch.equal(y, y2) and torch.equal(h, h2)
         for k, v in _backward(gpu_ctx, d, y2, "column", 0.5).items():
             assert torch.equal(out[k], v), k
+
+
+def test_past_32_bits(gpu_ctx):
+    """Rows past 2^32 bytes and 2^31 elements: the last ones are normalised, and have the gradients, that they have alone."""
+    T, H, n = 530_000, 4096, 300
+    d = {k: torch.zeros(T, H, dtype=torch.bfloat16, device="cuda") for k in ("block", "residual", "dy", "dh")}
+    few = _dev(_case(n, H, torch.bfloat16, True, "column", 5))
+    for k in d:
+        d[k][-n:] = few[k]
+    d.update({k: few[k] for k in ("post", "pre", "gate")})
+    y, h = torch.zeros_like(d["block"]), torch.zeros_like(d["block"])
+    _run(gpu_ctx, d, 0.75, y=y, h=h)
+    h2 = torch.zeros_like(few["block"])
+    y2 = _run(gpu_ctx, few, 0.75, h=h2)
+    assert torch.equal(y[-n:], y2) and torch.equal(h[-n:], h2) and not y[:-n].any() and not h[:-n].any()
+    del h
+    a, b = _backward(gpu_ctx, d, y, "column", 0.75), _backward(gpu_ctx, few, y2, "column", 0.75)
+    for k in ("dblock", "dresidual"):
+        assert torch.equal(a[k][-n:], b[k]) and not a[k][:-n].any()
+    for k in ("dpre", "dpost", "dgate"):  # the rows are dealt to other groups: another order of the sums
+        size = _backward64({k: None if v is None else v.cpu() for k, v in few.items()}, y2.cpu(), "column", 0.75)[k][1]
+        assert bool(((a[k] - b[k]).abs().cpu().double() <= (T / 512 + 168) * 4 * U * size).all()), k

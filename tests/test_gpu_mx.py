@@ -386,3 +386,85 @@ def test_two_contexts_and_the_contexts_own_stream(gpu_ctx):
         assert torch.equal(y, want)
     finally:
         other.close()
+
+
+# ------------------------------------------------------------ calls at the limits --
+@pytest.mark.parametrize("T,M,K", [(3, 40, 96), (3, 200, 1024), (90, 200, 1024), (90, 200, 96), (1100, 9300, 512)])
+def test_scales_at_any_address(gpu_ctx, T, M, K):
+    x, w = _cuda(_weights((T,), K, 1, 120, 130)), _cuda(_weights((M,), K, 2))
+    want = _product(gpu_ctx, x, w)
+    bound = None
+    for shift in (1, 2, 3, 4, 8):
+        moved = []
+        for s in (x[1], w[1]):
+            buf = torch.zeros(s.numel() + 16, dtype=torch.uint8, device="cuda")
+            moved.append(buf[shift:shift + s.numel()].view(s.shape))
+            moved[-1].copy_(s)
+        got = _product(gpu_ctx, (x[0], moved[0]), (w[0], moved[1]))
+        if bound is None:  # scales that are not aligned take another kernel: the sums' order may be another
+            bound = _plain(_values(*x), _values(*w), None, "none", None)[1]
+        assert bool(((got.cpu().double() - want.cpu().double()).abs() <= 2 * bound).all()), shift
+
+
+@pytest.mark.parametrize("T", [1, 100, 1100])
+def test_swiglu_where_the_exponential_is_subnormal(gpu_ctx, T):
+    """Gates of -80 to -104 give results down to bf16's subnormal ones, 0 only below; gates past 88 give gate times up; -0 and
+    NaN as they come.  g sigmoid(g) u: exp(g) is off by (4 + |g|) 2^-23 of it (its argument's rounding, twice, for it is
+    squared), the rest by 2^-21."""
+    M = 9300
+    sums = torch.tensor([0.0, 0.5, 4.5, 5.0, 5.5, 6.0, 6.5, 7.0, 7.5, 10.0, 12.0])
+    g = torch.Generator().manual_seed(1)
+    pick = torch.randint(0, len(sums), (M // 2,), generator=g)
+    sign = torch.where(torch.rand(M // 2, generator=g) < 0.8, -1.0, 1.0)
+    w = torch.zeros(M, 64)
+    first = sums[pick].clamp(max=6.0)
+    first = torch.where((first == 4.5) | (first == 5.0) | (first == 5.5), 4.0, first)
+    w[:M // 2, 0], w[:M // 2, 1] = sign * first, sign * (sums[pick] - first)
+    w[M // 2:, 32], w[:, 5], w[:, 37] = 1.0, 6.0, 6.0  # the blocks' scales are 2^0; columns 5 and 37 meet zeros
+    x = torch.zeros(T, 64)
+    x[:, :2], x[:, 32] = 16.0, 1.0
+    codes = [tuple(torch.from_numpy(c).cuda() for c in mx.quantize(v.numpy())) for v in (x, w)]
+    assert torch.equal(_values(*codes[1]), w.double()) and torch.equal(_values(*codes[0]), x.double())
+    z = (16 * sign * sums[pick]).double()
+    want = z * torch.sigmoid(z)
+    got = _product(gpu_ctx, *codes, "swiglu").cpu().double()
+    bound = want.abs() * (2.0 ** -8 + (6 + 2 * z.abs()) * 2.0 ** -23 + 2.0 ** -21) + 2.0 ** -133
+    assert bool(((got - want).abs() <= bound).all()), float(((got - want).abs() / bound).max())
+    assert bool((got[:, (z < -70) & (z > -90)] != 0).all())
+
+
+def test_rows_in_front_of_the_first_expert(gpu_ctx):
+    """Offsets that begin past 0 leave the rows in front as they were."""
+    for n, M in ((40, 64), (3000, 4096)):
+        x, w = _cuda(_weights((n,), 64, 1, 120, 130)), _cuda(_weights((2, M), 64, 2))
+        off = torch.tensor([7, n // 2, n - 3], dtype=torch.int32, device="cuda")
+        y = _product(gpu_ctx, x, w, offsets=off)
+        assert bool((y[:7] == 7).all()) and bool((y[n - 3:] == 7).all())
+        for e, (a, b) in enumerate(((7, n // 2), (n // 2, n - 3))):
+            rows = slice(a, b, max(1, (b - a) // 50))
+            want, bound = _plain(_values(x[0][rows], x[1][rows]), _values(w[0][e], w[1][e]), None, "none", None)
+            assert bool(((y[rows].cpu().double() - want).abs() <= bound).all())
+
+
+def test_very_wide_rows_and_many_scales(gpu_ctx):
+    """More columns than the tiles' 32-bit offsets serve, and scales of a matrix past 2^32 bytes: the last weight rows."""
+    for T, M, K in ((20, 8200, (1 << 20) + 32), (20, 4_300_000, 32 * 1024)):
+        w = torch.zeros(M, K // 2, dtype=torch.uint8, device="cuda"), torch.full((M, K // 32), 127, dtype=torch.uint8, device="cuda")
+        few, x = _cuda(_weights((30,), K, 3)), _cuda(_weights((T,), K, 4, 120, 130))
+        w[0][-30:], w[1][-30:] = few
+        y = _product(gpu_ctx, x, w)
+        want, bound = _plain(_values(*x), _values(*few), None, "none", None)
+        assert bool(((y[:, -30:].cpu().double() - want).abs() <= bound).all()) and not y[:, :-30].any()
+        del w, y
+        torch.cuda.empty_cache()
+
+
+def test_the_largest_call_is_refused_or_served(gpu_ctx):
+    """Grids past 2^32 threads are refused; nothing is launched."""
+    held = torch.zeros(64, dtype=torch.uint8, device="cuda")
+    from raon_npu_amd import _lib
+
+    with pytest.raises(ValueError, match="too many"):
+        _lib.call("rmoe_mx_linear_dev", gpu_ctx.handle, 1 << 40, 1 << 50, (1 << 31) - 1, 32, 1 << 45, 1 << 46, 1 << 16, None,
+                  _lib.ACT_NONE, 0.0, 0.0, None, 1 << 52, None)
+    assert not held.any()
