@@ -234,22 +234,28 @@ hipError_t launch_few(const MxLin& a, hipStream_t st) {
 // 32, and of the four blocks of 128 columns it holds 2 h and 2 h + 1, h = lane / 32, for two MFMA steps.
 // A gated wave's rows are 16 MA gate rows and the up rows of the same outputs.
 
-template <int MA, int NB, int WA, int WB, bool kWhole>
+template <int MA, int NB, int WA, int WB, bool kWhole, bool kStays>
 struct TileShape {
+  static_assert(kWhole || !kStays, "whole windows are two stages or more of an even number");
   static constexpr int KT = kWhole ? 2 : 1;
   static constexpr int kWaves = WA * WB, kThreads = 64 * kWaves, BW = 32 * MA * WA, BT = 32 * NB * WB, R = BW + BT;
   static constexpr int kStages = kWhole ? 2 : 3, kRow = 64 * KT;
-  static constexpr int kCodes = R * kRow, kStage = kCodes + (kWhole ? 0 : R * 4);  // a stage's bytes
-  static constexpr int kWindow = kStages * kStage;                     // where a window of scales begins
+  // A stage's codes, behind them a dword of scales a row, or behind the first stage's alone a window of scales.
+  static constexpr int kCodes = R * kRow, kStage = kCodes + R * (kWhole ? 16 : 4);
   static constexpr int kCopyRows = 16 / KT;                            // rows of a copy
   static constexpr int kCopies = R / kCopyRows / kWaves;               // a wave's copies of a stage
   static constexpr int kScaleCopies = (R / 64 + kWaves - 1) / kWaves;  // and of a window of scales, 64 rows each
   static constexpr int kScales = (R + kThreads - 1) / kThreads;
   static_assert(KT == 1 || kCopies % 2 == 0, "the parity of a copy's rows is its number's");
   static_assert(R % 64 == 0 && R % (kCopyRows * kWaves) == 0, "whole copies");
+  // Outputs of a wave, how many of them are in LDS at once (32 rows of them), and where.
+  static constexpr int outputs(bool gated) { return (gated ? 16 : 32) * MA; }
+  static constexpr int part(bool gated) { return kStays && outputs(gated) > 64 ? 64 : outputs(gated); }
+  static constexpr int kOutputs = kStays ? kStage : 0;
+  static constexpr int kTiles = kOutputs + kWaves * 32 * 68 * 4;  // the experts' table of row tiles (kStays)
   static constexpr size_t lds(bool gated) {
-    const size_t out = (size_t)kWaves * 32 * ((gated ? 16 : 32) * MA + 4) * 4;
-    const size_t in = (size_t)kStages * kStage + (kWhole ? R * 16 : 0);
+    const size_t out = kOutputs + (size_t)kWaves * 32 * (part(gated) + 4) * 4 + (kStays ? 64 * sizeof(RowTiles<BT>) : 0);
+    const size_t in = (size_t)(kStages - 1) * kStage + kCodes + (kWhole ? 0 : R * 4);
     return out > in ? out : in;
   }
 };
@@ -274,58 +280,69 @@ __device__ __forceinline__ void copies_landed() {
   __syncthreads();
 }
 
-template <int MA, int NB, int WA, int WB, bool kWhole, bool kGated>
+template <int MA, int NB, int WA, int WB, bool kWhole, bool kStays, bool kGated>
 __global__ __launch_bounds__(64 * WA * WB, 2) void mx_tiles_kernel(MxLin a, int n_nt) {
-  typedef TileShape<MA, NB, WA, WB, kWhole> S;
+  typedef TileShape<MA, NB, WA, WB, kWhole, kStays> S;
   constexpr int KT = S::KT;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-  constexpr int kOut = (kGated ? 16 : 32) * MA;  // outputs of a wave
+  constexpr int kOut = S::outputs(kGated), kPart = S::part(kGated);
   RowTiles<S::BT> rt;
   const int n_mt = a.offsets ? rt.total(a.offsets, a.n_experts, a.n) : (a.n + S::BT - 1) / S::BT;
   // XCD x takes a contiguous eighth of the tiles: by expert the weight tiles of a row tile back to back, else
   // blocks of up to eight row tiles for each weight tile, so that both operands' tiles meet again in its L2.
-  const uint32_t total = (uint32_t)n_mt * n_nt, per = (total + 7) / 8, slot = blockIdx.x / 8;  // a launch's fit 24 bits
-  const uint32_t id = blockIdx.x % 8 * per + slot;
-  if (slot >= per || id >= total) return;
-  int nt, e = 0, row0, nrow;
-  if (a.offsets) {
-    rt.find((int)(id / (uint32_t)n_nt), e, row0, nrow);
-    nt = (int)(id % (uint32_t)n_nt);
-  } else {
-    constexpr uint32_t kBlock = 8;
-    const uint32_t group = id / (kBlock * n_nt), m0 = group * kBlock, nm = min(kBlock, n_mt - m0);
-    const uint32_t in = id - group * kBlock * n_nt;
-    nt = (int)(in / nm);
-    row0 = (int)(m0 + in % nm) * S::BT;
-    nrow = min(S::BT, a.n - row0);
-  }
+  const uint32_t total = (uint32_t)n_mt * n_nt, per = (total + 7) / 8;  // a launch's fit 24 bits
+  struct Tile {
+    int nt, e, row0, nrow;
+  };
+  auto tile_at = [&](uint32_t slot, Tile& q) {  // false: there are no more
+    const uint32_t id = blockIdx.x % 8 * per + slot;
+    if (slot >= per || id >= total) return false;
+    q.e = 0;
+    if (a.offsets) {
+      rt.find((int)(id / (uint32_t)n_nt), q.e, q.row0, q.nrow);
+      q.nt = (int)(id % (uint32_t)n_nt);
+    } else {
+      constexpr uint32_t kBlock = 8;
+      const uint32_t group = id / (kBlock * n_nt), m0 = group * kBlock, nm = min(kBlock, n_mt - m0);
+      const uint32_t in = id - group * kBlock * n_nt;
+      q.nt = (int)(in / nm);
+      q.row0 = (int)(m0 + in % nm) * S::BT;
+      q.nrow = min(S::BT, a.n - q.row0);
+    }
+    return true;
+  };
+  uint32_t slot = blockIdx.x / 8;
+  Tile tile;
+  if (!tile_at(slot, tile)) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = wave_id(), l32 = lane & 31, h = lane >> 5;
   const int wa = wave % WA, wb = wave / WA;
   const int kb = a.K / kMxBlock, tiles = (kb + 3) / 4, stages = tiles / KT, rem = kb % 4;
   uint32_t ldb = (uint32_t)a.K / 2;
   const int width = kGated ? a.M / 2 : a.M;
   // Row of an LDS row slot: of the weights (e's matrix) or of x; rows past the ends repeat the last one.
-  auto weight_row = [&](int r) {
-    const int w = r / (32 * MA), rr = r % (32 * MA), o = (nt * WA + w) * kOut + rr % kOut;
+  auto weight_row = [&](const Tile& q, int r) {
+    const int w = r / (32 * MA), rr = r % (32 * MA), o = (q.nt * WA + w) * kOut + rr % kOut;
     return (kGated && rr >= kOut ? width : 0) + min(o, width - 1);
   };
-  auto token_row = [&](int r) { return min(r - S::BW, nrow - 1); };
+  auto token_row = [&](const Tile& q, int r) { return min(r - S::BW, q.nrow - 1); };
 
   // A copy's first row, and how many rows behind it there are: those past them repeat the last one.
   const uint8_t* cbase[S::kCopies];
   int cmore[S::kCopies];
+  auto aim_copies = [&](const Tile& q) {
 #pragma unroll
-  for (int j = 0; j < S::kCopies; ++j) {
-    const int r0 = S::kCopyRows * (wave * S::kCopies + j);
-    if (r0 < S::BW) {
-      const int o = (nt * WA + r0 / (32 * MA)) * kOut + r0 % (32 * MA) % kOut;
-      cbase[j] = a.w + ((size_t)e * a.M + weight_row(r0)) * ldb;
-      cmore[j] = max(width - 1 - o, 0);
-    } else {
-      cbase[j] = a.x + ((size_t)row0 + token_row(r0)) * ldb;
-      cmore[j] = max(nrow - 1 - (r0 - S::BW), 0);
+    for (int j = 0; j < S::kCopies; ++j) {
+      const int r0 = S::kCopyRows * (wave * S::kCopies + j);
+      if (r0 < S::BW) {
+        const int o = (q.nt * WA + r0 / (32 * MA)) * kOut + r0 % (32 * MA) % kOut;
+        cbase[j] = a.w + ((size_t)q.e * a.M + weight_row(q, r0)) * ldb;
+        cmore[j] = max(width - 1 - o, 0);
+      } else {
+        cbase[j] = a.x + ((size_t)q.row0 + token_row(q, r0)) * ldb;
+        cmore[j] = max(q.nrow - 1 - (r0 - S::BW), 0);
+      }
     }
-  }
+  };
   // Chunk c of a row's 4 KT stands at c ^ place(row), so that sixteen rows' chunks of one number are in different banks.
   auto place = [](int row) { return KT == 1 ? (row >> 2) & 3 : (row >> 1) & 7; };
   const int cchunk = KT == 1 ? (lane & 3) ^ (lane >> 4) : (lane & 7) ^ (lane >> 4);  // of the rows from an even copy's on
@@ -348,24 +365,26 @@ __global__ __launch_bounds__(64 * WA * WB, 2) void mx_tiles_kernel(MxLin a, int 
   uint32_t wslot[S::kScaleCopies];
   auto window_copies = [&](int w) {
 #pragma unroll
-    for (int j = 0; j < S::kScaleCopies; ++j) copy16(wbase[j], soff[j] + 16 * w, S::kWindow + wslot[j]);
+    for (int j = 0; j < S::kScaleCopies; ++j) copy16(wbase[j], soff[j] + 16 * w, S::kCodes + wslot[j]);
   };
-  if constexpr (kWhole) {
+  auto aim_windows = [&](const Tile& q) {
+    int l = lane;
+    asm volatile("" : "+v"(l));
 #pragma unroll
     for (int j = 0; j < S::kScaleCopies; ++j) {
-      const int r0 = 64 * ((wave + j * S::kWaves) % (S::R / 64)), r = r0 + lane;  // a wave without a copy repeats another's
+      const int r0 = 64 * ((wave + j * S::kWaves) % (S::R / 64)), r = r0 + l;  // a wave without a copy repeats another's
       wslot[j] = 16 * r0;
       if (r0 < S::BW) {
-        const int first = weight_row(r0);  // the least: a group of 64 begins with gate rows or holds up rows alone
-        wbase[j] = a.ws + ((size_t)e * a.M + first) * kb;
-        soff[j] = (uint32_t)(weight_row(r) - first) * (uint32_t)kb;
+        const int first = weight_row(q, r0);  // the least: a group of 64 begins with gate rows or holds up rows alone
+        wbase[j] = a.ws + ((size_t)q.e * a.M + first) * kb;
+        soff[j] = (uint32_t)(weight_row(q, r) - first) * (uint32_t)kb;
       } else {
-        const int first = token_row(r0);
-        wbase[j] = a.xs + ((size_t)row0 + first) * kb;
-        soff[j] = (uint32_t)(token_row(r) - first) * (uint32_t)kb;
+        const int first = token_row(q, r0);
+        wbase[j] = a.xs + ((size_t)q.row0 + first) * kb;
+        soff[j] = (uint32_t)(token_row(q, r) - first) * (uint32_t)kb;
       }
     }
-  }
+  };
   // Other scales: fetched 16 a row by the registers and put beside a stage's codes, a dword a row.
   const uint8_t* sbase[S::kScales];
   uint4 q[S::kScales], qn[S::kScales];
@@ -373,7 +392,8 @@ __global__ __launch_bounds__(64 * WA * WB, 2) void mx_tiles_kernel(MxLin a, int 
 #pragma unroll
     for (int j = 0; j < S::kScales; ++j) {
       const int r = min(tid + j * S::kThreads, S::R - 1);
-      sbase[j] = r < S::BW ? a.ws + ((size_t)e * a.M + weight_row(r)) * kb : a.xs + ((size_t)row0 + token_row(r)) * kb;
+      sbase[j] = r < S::BW ? a.ws + ((size_t)tile.e * a.M + weight_row(tile, r)) * kb
+                           : a.xs + ((size_t)tile.row0 + token_row(tile, r)) * kb;
     }
   }
   auto put_scales = [&](int t, int stage) {  // called for t = 0, 1, 2, ...
@@ -395,13 +415,6 @@ __global__ __launch_bounds__(64 * WA * WB, 2) void mx_tiles_kernel(MxLin a, int 
   };
 
   f32x16 acc[MA][NB];
-#pragma unroll
-  for (int m = 0; m < MA; ++m)
-#pragma unroll
-    for (int n = 0; n < NB; ++n)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) acc[m][n][i] = 0.f;
-
   struct Frags {
     i32x4 a[MA], b[NB];
   } f[2];
@@ -429,7 +442,7 @@ __global__ __launch_bounds__(64 * WA * WB, 2) void mx_tiles_kernel(MxLin a, int 
   constexpr int kD = kWhole ? 4 : 1;
   uint32_t da[MA][kD], db[NB][kD];
   auto read_scales = [&](int stage) {
-    const uint8_t* p = lds + (kWhole ? S::kWindow : stage * S::kStage + S::kCodes);
+    const uint8_t* p = lds + (kWhole ? 0 : stage * S::kStage) + S::kCodes;
     auto get = [&](uint32_t (&d)[kD], int r) {
       if constexpr (kWhole) *reinterpret_cast<uint4*>(d) = *reinterpret_cast<const uint4*>(p + r * 16);
       else d[0] = *reinterpret_cast<const uint32_t*>(p + r * 4);
@@ -486,17 +499,6 @@ __global__ __launch_bounds__(64 * WA * WB, 2) void mx_tiles_kernel(MxLin a, int 
       for (int n = 0; n < NB; ++n) asm volatile("" : "+v"(acc[m][n]));
   };
 
-  if constexpr (kWhole) window_copies(0);
-#pragma unroll
-  for (int t = 0; t < S::kStages; ++t)
-    if (t < stages) {
-      if constexpr (!kWhole) put_scales(t, t);
-      copies(t, t);
-    }
-  if (stages >= S::kStages) copies_landed<(S::kStages - 1) * S::kCopies>();
-  else copies_landed<0>();
-  read_all(f[0], 0, 0);
-  read_scales(0);
   // A step's fragments are read while the step before is multiplied.  A stage is met by the workgroup before its
   // last step: every wave has read it (and the window, where that is new), the next stage's copies have landed.
   auto most_steps = [&](int stage) {
@@ -508,10 +510,11 @@ __global__ __launch_bounds__(64 * WA * WB, 2) void mx_tiles_kernel(MxLin a, int 
       multiply(f[0], first, reading(f[1], stage, 3));
     }
   };
-  int stage = 0;
-  // Stage t, and the first fragments of the next; kMore: with the copies of the stage that takes its place.
-  auto turn = [&](int t, auto more) {
-    constexpr bool kMore = decltype(more)::value;
+  int stage;
+  // Stage t, and the first fragments of the next.  kMore: with the copies of the stage that takes its place; kNext: of
+  // the next tile's first, which the copies are already aimed at.
+  auto turn = [&](int t, auto more, auto then) {
+    constexpr bool kNext = decltype(then)::value, kMore = decltype(more)::value || kNext;
     const int next = stage == S::kStages - 1 ? 0 : stage + 1;
     fresh();
     most_steps(stage);
@@ -519,12 +522,13 @@ __global__ __launch_bounds__(64 * WA * WB, 2) void mx_tiles_kernel(MxLin a, int 
     if (S::kStages > 2 && t + S::kStages - 1 < stages) copies_landed<(S::kStages - 2) * S::kCopies>();
     else copies_landed<0>();
     if constexpr (kWhole) {
-      if (KT * t % 4 == 0 && KT * t + 4 < tiles) window_copies(KT * t / 4 + 1);
+      if constexpr (kNext) window_copies(0);
+      else if (KT * t % 4 == 0 && KT * t + 4 < tiles) window_copies(KT * t / 4 + 1);
     } else if constexpr (kMore) {
       put_scales(t + S::kStages, stage);
     }
     if (!kWhole || KT * (t + 1) % 4 == 0) read_scales(next);
-    const uint32_t chunk = kMore ? chunk_of(t + S::kStages) : 0u;
+    const uint32_t chunk = kNext ? chunk_of(0) : kMore ? chunk_of(t + S::kStages) : 0u;
     __builtin_amdgcn_sched_barrier(0);
     multiply(f[1], second, [&](int i) {
       deal(i, kPieces, [&](int p) { read(f[0], next, 0, p); });
@@ -532,153 +536,214 @@ __global__ __launch_bounds__(64 * WA * WB, 2) void mx_tiles_kernel(MxLin a, int 
     });
     stage = next;
   };
-  int t = 0;
-  for (; t < stages - S::kStages; ++t) turn(t, std::true_type());
-  for (; t < stages - 1; ++t) turn(t, std::false_type());
+  aim_copies(tile);
   if constexpr (kWhole) {
-    most_steps(stage);
-  } else {
-    take_scales();
-    read_all(f[1], stage, 1);
-#pragma unroll
-    for (int s = 0; s < 2; ++s)
-      if (rem && 2 * h + s >= rem) {  // blocks past the end: weights of zero
-#pragma unroll
-        for (int m = 0; m < MA; ++m) f[s].a[m] = i32x4{0, 0, 0, 0};
-      }
-    multiply(f[0], first, nothing);
+    aim_windows(tile);
+    window_copies(0);
   }
-  multiply(f[1], second, nothing);
-  pin();
-  __syncthreads();  // the outputs reuse the stages
+#pragma unroll
+  for (int t = 0; t < S::kStages; ++t)
+    if (t < stages) {
+      if constexpr (!kWhole) put_scales(t, t);
+      copies(t, t);
+    }
+  if (stages >= S::kStages) copies_landed<(S::kStages - 1) * S::kCopies>();
+  else copies_landed<0>();
+  if constexpr (kStays)
+    if (a.offsets) reinterpret_cast<RowTiles<S::BT>*>(lds + S::kTiles)[lane] = rt;  // the same by every wave
 
-  // acc[m][n][i]: weight row 32 m + 8 (i / 4) + 4 h + i % 4, row of x 32 n + l32.  Outputs go through LDS, 32 rows
-  // of x at a time, so that a row's stand together: gated ones with their activation, others as sums.
-  constexpr int kStride = kOut + 4;
-  float* mine = reinterpret_cast<float*>(lds) + wave * 32 * kStride;
-  const int col0 = (nt * WA + wa) * kOut;
-  const float* bias = a.bias ? a.bias + (size_t)e * a.M : nullptr;
-  const bool wide =
-      width % 8 == 0 && ((reinterpret_cast<uintptr_t>(a.y) | reinterpret_cast<uintptr_t>(a.residual)) & 15) == 0;
-  auto put = [&](int n, auto pair) {
-    int from = col0;
-    asm volatile("" : "+s"(from));  // addresses of biases are formed again: there are no registers to keep them
+  for (;;) {
 #pragma unroll
-    for (int m = 0; m < (kGated && MA > 1 ? MA / 2 : MA); ++m)
+    for (int m = 0; m < MA; ++m)
 #pragma unroll
-      for (int g = 0; g < (kGated && MA == 1 ? 2 : 4); ++g) {
-        const int o = 32 * m + 8 * g + 4 * h;
-        f32x4 v;
-        if constexpr (kGated) {
-          float bz[4] = {0.f, 0.f, 0.f, 0.f}, bu[4] = {0.f, 0.f, 0.f, 0.f};
-          if (bias) {
+      for (int n = 0; n < NB; ++n)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const uint32_t c = (uint32_t)min(from + o + i, width - 1);
-              bz[i] = bias[c];
-              bu[i] = bias[(uint32_t)width + c];
-            }
-          }
+        for (int i = 0; i < 16; ++i) acc[m][n][i] = 0.f;
+    Tile ahead = tile;
+    bool goes_on = false;
+    if constexpr (kStays) {
+      if (a.offsets) rt = reinterpret_cast<const RowTiles<S::BT>*>(lds + S::kTiles)[lane];
+      slot += gridDim.x / 8;
+      goes_on = tile_at(slot, ahead);
+    }
+    stage = 0;
+    read_all(f[0], 0, 0);
+    read_scales(0);
+    const std::true_type yes;
+    const std::false_type no;
+    int t = 0;
+    for (; t < stages - S::kStages; ++t) turn(t, yes, no);
+    if constexpr (kStays) {
+      // There are two stages or more, of which the last is in the second place: the first is free for the next tile.
+      // Without one this tile's is copied again: copies in a branch cost as much as these, each launch once.
+      aim_copies(ahead);
+      aim_windows(ahead);
+      turn(t, no, yes);
+    } else {
+      for (; t < stages - 1; ++t) turn(t, no, no);
+    }
+    if constexpr (kWhole) {
+      most_steps(stage);
+    } else {
+      take_scales();
+      read_all(f[1], stage, 1);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float u = MA == 1 ? acc[m][n][4 * (g + 2) % 16 + i] : acc[(m + MA / 2) % MA][n][4 * g + i];
-            v[i] = pair(acc[m][n][4 * g + i] + bz[i], u + bu[i]);
-          }
-        } else {
+      for (int s = 0; s < 2; ++s)
+        if (rem && 2 * h + s >= rem) {  // blocks past the end: weights of zero
 #pragma unroll
-          for (int i = 0; i < 4; ++i) v[i] = acc[m][n][4 * g + i];
+          for (int m = 0; m < MA; ++m) f[s].a[m] = i32x4{0, 0, 0, 0};
         }
-        *reinterpret_cast<f32x4*>(mine + l32 * kStride + o) = v;
-        __builtin_amdgcn_sched_barrier(0);  // no more than these at once: registers
-      }
-  };
-  constexpr int kLanes = kOut / 8;  // of a row, eight outputs each
-  auto take = [&](int t0, int r, bool plain) {
-    const int t = r + lane / kLanes, o = 8 * (lane % kLanes), col = col0 + o;
-    if (t0 + t >= nrow || col >= width) return;
-    float v[8];
-    *reinterpret_cast<f32x4*>(v) = *reinterpret_cast<const f32x4*>(mine + t * kStride + o);
-    *reinterpret_cast<f32x4*>(v + 4) = *reinterpret_cast<const f32x4*>(mine + t * kStride + o + 4);
-    if constexpr (!kGated) {
+      multiply(f[0], first, nothing);
+    }
+    multiply(f[1], second, nothing);
+    pin();
+    // The outputs are where the last stage was.  The next tile's first stage has landed: waited for here, not behind
+    // the outputs' stores, which the wait would be one for too.
+    copies_landed<0>();
+
+    // acc[m][n][i]: weight row 32 m + 8 (i / 4) + 4 h + i % 4, row of x 32 n + l32.  Outputs go through LDS, 32 rows
+    // of x at a time, so that a row's stand together: gated ones with their activation, others as sums.
+    constexpr int kStride = kPart + 4;
+    int at = lane;
+    asm volatile("" : "+v"(at));  // what follows is formed for each tile again
+    float* mine = reinterpret_cast<float*>(lds + S::kOutputs) + wave * 32 * kStride;
+    const int col0 = (tile.nt * WA + wa) * kOut;
+    const float* bias = a.bias ? a.bias + (size_t)tile.e * a.M : nullptr;
+    const bool wide =
+        width % 8 == 0 && ((reinterpret_cast<uintptr_t>(a.y) | reinterpret_cast<uintptr_t>(a.residual)) & 15) == 0;
+    if constexpr (kGated) {
       if (bias) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] += bias[min(col + i, width - 1)];
-      }
-      if (!plain) {
+        for (int m = 0; m < MA; ++m)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = act_single(a.act, v[i]);
+          for (int g = 0; g < 4; ++g) {
+            const int r = 32 * m + 8 * g;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float v = bias[(uint32_t)((r >= kOut ? width : 0) + min(col0 + r % kOut + 4 * (at >> 5) + i, width - 1))];
+#pragma unroll
+              for (int n = 0; n < NB; ++n) acc[m][n][4 * g + i] += v;
+            }
+            __builtin_amdgcn_sched_barrier(0);  // no more than these at once: registers
+          }
       }
     }
-    const size_t to = ((size_t)row0 + t0 + t) * width + col;
-    if (wide) {
-      if (a.residual) {
-        const uint4 r4 = *reinterpret_cast<const uint4*>(a.residual + to);
-        const uint32_t rw[4] = {r4.x, r4.y, r4.z, r4.w};
+    auto put = [&](int n, int part, auto pair) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] += __uint_as_float(i % 2 ? rw[i / 2] & 0xffff0000u : rw[i / 2] << 16);
+      for (int k = 0; k < (kGated && MA == 1 ? 2 : kPart / 8); ++k) {
+        const int m = part * (kPart / 32) + k / 4, g = k % 4;
+        f32x4 v;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if constexpr (kGated) {
+            const float u = MA == 1 ? acc[m][n][4 * (g + 2) % 16 + i] : acc[(m + MA / 2) % MA][n][4 * g + i];
+            v[i] = pair(acc[m][n][4 * g + i], u);
+          } else {
+            v[i] = acc[m][n][4 * g + i];
+          }
+        }
+        *reinterpret_cast<f32x4*>(mine + (at & 31) * kStride + 8 * k + 4 * (at >> 5)) = v;
+        __builtin_amdgcn_sched_barrier(0);
       }
-      uint32_t w[4];
+    };
+    constexpr int kLanes = kPart / 8;  // of a row, eight outputs each
+    auto take = [&](int t0, int r, int part, bool plain) {
+      const int t = r + at / kLanes, o = 8 * (at % kLanes), col = col0 + part * kPart + o;
+      if (t0 + t >= tile.nrow || col >= width) return;
+      float v[8];
+      *reinterpret_cast<f32x4*>(v) = *reinterpret_cast<const f32x4*>(mine + t * kStride + o);
+      *reinterpret_cast<f32x4*>(v + 4) = *reinterpret_cast<const f32x4*>(mine + t * kStride + o + 4);
+      if constexpr (!kGated) {
+        if (bias) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = bf16_bits(v[2 * i]) | bf16_bits(v[2 * i + 1]) << 16;
-      *reinterpret_cast<uint4*>(a.y + to) = make_uint4(w[0], w[1], w[2], w[3]);
-    } else {
+          for (int i = 0; i < 8; ++i) v[i] += bias[min(col + i, width - 1)];
+        }
+        if (!plain) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (col + i < width)
-          a.y[to + i] = (uint16_t)bf16_bits(a.residual ? v[i] + bf16_to_f32(a.residual[to + i]) : v[i]);
-    }
-  };
+          for (int i = 0; i < 8; ++i) v[i] = act_single(a.act, v[i]);
+        }
+      }
+      const size_t to = ((size_t)tile.row0 + t0 + t) * width + col;
+      if (wide) {
+        if (a.residual) {
+          const uint4 r4 = *reinterpret_cast<const uint4*>(a.residual + to);
+          const uint32_t rw[4] = {r4.x, r4.y, r4.z, r4.w};
 #pragma unroll
-  for (int n = 0; n < NB; ++n) {
-    if (kGated && a.act != RMOE_ACT_SWIGLU)
-      put(n, [&](float g, float u) { return act_pair(RMOE_ACT_SITU, g, u, a.gb, a.vb); });
-    else
-      put(n, [](float g, float u) { return swiglu(g, u); });
-    const int t0 = wb * 32 * NB + 32 * n;
-    if (kGated || a.act == RMOE_ACT_NONE) {
+          for (int i = 0; i < 8; ++i) v[i] += __uint_as_float(i % 2 ? rw[i / 2] & 0xffff0000u : rw[i / 2] << 16);
+        }
+        uint32_t w[4];
 #pragma unroll
-      for (int r = 0; r < 32; r += 64 / kLanes) take(t0, r, true);
-    } else {
+        for (int i = 0; i < 4; ++i) w[i] = bf16_bits(v[2 * i]) | bf16_bits(v[2 * i + 1]) << 16;
+        *reinterpret_cast<uint4*>(a.y + to) = make_uint4(w[0], w[1], w[2], w[3]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (col + i < width)
+            a.y[to + i] = (uint16_t)bf16_bits(a.residual ? v[i] + bf16_to_f32(a.residual[to + i]) : v[i]);
+      }
+    };
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int part = 0; part < kOut / kPart; ++part) {
+        if (kGated && a.act != RMOE_ACT_SWIGLU)
+          put(n, part, [&](float g, float u) { return act_pair(RMOE_ACT_SITU, g, u, a.gb, a.vb); });
+        else
+          put(n, part, [](float g, float u) { return swiglu(g, u); });
+        const int t0 = wb * 32 * NB + 32 * n;
+        if (kGated || a.act == RMOE_ACT_NONE) {
+#pragma unroll
+          for (int r = 0; r < 32; r += 64 / kLanes) take(t0, r, part, true);
+        } else {
 #pragma unroll 1
-      for (int r = 0; r < 32; r += 64 / kLanes) take(t0, r, false);
-    }
+          for (int r = 0; r < 32; r += 64 / kLanes) take(t0, r, part, false);
+        }
+      }
+    if (!kStays || !goes_on) return;
+    __syncthreads();  // the outputs' place is the second stage's again
+    tile = ahead;
+    copies(1, 1);
   }
 }
 
-template <int MA, int NB, int WA, int WB, bool kWhole>
+constexpr size_t kStaying = 256;  // workgroups that take tile after tile: one a CU, which their LDS fills
+
+template <int MA, int NB, int WA, int WB, bool kWhole, bool kStays>
 hipError_t launch_tiles(const MxLin& a, hipStream_t st) {
-  typedef TileShape<MA, NB, WA, WB, kWhole> S;
+  typedef TileShape<MA, NB, WA, WB, kWhole, kStays> S;
   const bool gated = act_gated(a.act);
   const int width = gated ? a.M / 2 : a.M, out = S::BW / (gated ? 2 : 1), n_nt = (width + out - 1) / out;
   const size_t mt = a.offsets ? std::min<size_t>(a.n, (size_t)a.n / S::BT + a.n_experts) : ((size_t)a.n + S::BT - 1) / S::BT;
-  const size_t grid = 8 * ((mt * n_nt + 7) / 8);
-  if (grid * S::kThreads >= (size_t)1 << 32) return hipErrorInvalidValue;
-  auto* kernel = gated ? mx_tiles_kernel<MA, NB, WA, WB, kWhole, true> : mx_tiles_kernel<MA, NB, WA, WB, kWhole, false>;
+  const size_t all = 8 * ((mt * n_nt + 7) / 8), grid = kStays ? std::min(all, kStaying) : all;
+  if (all * S::kThreads >= (size_t)1 << 32) return hipErrorInvalidValue;
+  auto* kernel = gated ? mx_tiles_kernel<MA, NB, WA, WB, kWhole, kStays, true>
+                       : mx_tiles_kernel<MA, NB, WA, WB, kWhole, kStays, false>;
   hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(S::kThreads), S::lds(gated), st, a, n_nt);
   return hipGetLastError();
 }
-template <int MA, int NB, int WA, int WB>
+// stays: more tiles than kStaying are taken by as many workgroups.
+template <int MA, int NB, int WA, int WB, bool kStays = false>
 hipError_t pick_tiles(const MxLin& a, hipStream_t st) {
   const bool whole = a.K % 512 == 0 && ((reinterpret_cast<uintptr_t>(a.xs) | reinterpret_cast<uintptr_t>(a.ws)) & 15) == 0;
-  return whole ? launch_tiles<MA, NB, WA, WB, true>(a, st) : launch_tiles<MA, NB, WA, WB, false>(a, st);
+  return whole ? launch_tiles<MA, NB, WA, WB, true, kStays>(a, st) : launch_tiles<MA, NB, WA, WB, false, false>(a, st);
 }
-template <int MA, int NB, int WA, int WB, bool kWhole>
+template <int MA, int NB, int WA, int WB, bool kWhole, bool kStays>
 hipError_t setup_tiles() {
-  typedef TileShape<MA, NB, WA, WB, kWhole> S;
-  hipError_t e = hipFuncSetAttribute((const void*)mx_tiles_kernel<MA, NB, WA, WB, kWhole, true>,
+  typedef TileShape<MA, NB, WA, WB, kWhole, kStays> S;
+  hipError_t e = hipFuncSetAttribute((const void*)mx_tiles_kernel<MA, NB, WA, WB, kWhole, kStays, true>,
                                      hipFuncAttributeMaxDynamicSharedMemorySize, (int)S::lds(true));
   if (e == hipSuccess)
-    e = hipFuncSetAttribute((const void*)mx_tiles_kernel<MA, NB, WA, WB, kWhole, false>,
+    e = hipFuncSetAttribute((const void*)mx_tiles_kernel<MA, NB, WA, WB, kWhole, kStays, false>,
                             hipFuncAttributeMaxDynamicSharedMemorySize, (int)S::lds(false));
   return e;
 }
 
 }  // namespace
 
-// Allow the tiles of more than 64 KB of dynamic LDS theirs (up to 136).
+// Allow the tiles of more than 64 KB of dynamic LDS theirs (up to 142).
 hipError_t mx_linear_setup() {
-  for (const hipError_t e : {setup_tiles<4, 2, 2, 4, true>(), setup_tiles<4, 2, 2, 4, false>(),
-                             setup_tiles<2, 2, 2, 2, true>()})
+  for (const hipError_t e : {setup_tiles<4, 2, 2, 4, true, true>(), setup_tiles<4, 2, 2, 4, true, false>(),
+                             setup_tiles<4, 2, 2, 4, false, false>(), setup_tiles<2, 2, 2, 2, true, false>()})
     if (e != hipSuccess) return e;
   return hipSuccess;
 }
@@ -705,13 +770,16 @@ hipError_t launch_mx_linear(const MxLin& a, hipStream_t st) {
   if (rows <= kFewRows) return launch_few<2, 1>(a, st);
   // The tiles' offsets within a matrix's scales and 16 rows' codes take 32 bits.
   const bool wide = a.K > 1 << 20 || M * (a.K / kMxBlock) >= (size_t)1 << 32;
+  auto large = [&] {
+    return tiles(256, 256) > kStaying ? pick_tiles<4, 2, 2, 4, true>(a, st) : pick_tiles<4, 2, 2, 4, false>(a, st);
+  };
   if (a.offsets) {
     if (wide || n < kFewEach * groups) return launch_few<2, 2>(a, st);
-    if (n >= kFillEach * groups && tiles(256, 256) >= kFillLarge) return pick_tiles<4, 2, 2, 4>(a, st);
+    if (n >= kFillEach * groups && tiles(256, 256) >= kFillLarge) return large();
     return pick_tiles<2, 1, 2, 2>(a, st);
   }
   if (wide || n <= 16) return launch_few<2, 4>(a, st);
-  if (tiles(256, 256) >= kFillLarge) return pick_tiles<4, 2, 2, 4>(a, st);
+  if (tiles(256, 256) >= kFillLarge) return large();
   return tiles(64, 64) < kFillSmall ? pick_tiles<1, 1, 2, 2>(a, st) : pick_tiles<2, 2, 2, 2>(a, st);
 }
 

@@ -33,7 +33,7 @@ __global__ __launch_bounds__(256) void mx_quantize_kernel(QuantArgs a, size_t fi
     c = (int)(u - row * per) * 8;
   }
   const E* xr = static_cast<const E*>(a.x) + (kWide ? u * 8 : row * a.K);
-    const Chunk<DT> in = load_chunk<DT, kWide>(xr, c, a.K);
+  const Chunk<DT> in = load_chunk<DT, kWide>(xr, c, a.K);
   float x[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) x[i] = RowElem<DT>::get(in.v[i]);

@@ -468,3 +468,24 @@ def test_the_largest_call_is_refused_or_served(gpu_ctx):
         _lib.call("rmoe_mx_linear_dev", gpu_ctx.handle, 1 << 40, 1 << 50, (1 << 31) - 1, 32, 1 << 45, 1 << 46, 1 << 16, None,
                   _lib.ACT_NONE, 0.0, 0.0, None, 1 << 52, None)
     assert not held.any()
+
+
+@pytest.mark.parametrize("T,M,K,act", [(2100, 9300, 1024, "swiglu"), (4100, 5001, 512, "gelu"), (5200, 4096, 1536, "none"),
+                                       (2304, 8192, 512, "situ")])
+def test_more_tiles_than_workgroups(gpu_ctx, T, M, K, act):
+    """Workgroups that go on to further tiles, their first stage requested while the one before is finished."""
+    _check_product(gpu_ctx, T, M, K, act, True, True)
+
+
+@pytest.mark.parametrize("counts,M,K,act", [([3000, 1, 0, 5000, 257, 2700], 2056, 512, "swiglu"),
+                                            ([300] * 20 + [0, 4000, 1, 255, 256], 1536, 1024, "none")])
+def test_more_experts_tiles_than_workgroups(gpu_ctx, counts, M, K, act):
+    _check_experts(gpu_ctx, counts, M, K, act, True, True, behind=700)
+
+
+def test_further_tiles_are_the_same_each_time(gpu_ctx):
+    """The same rows in one call and in calls of at most as many tiles as workgroups, again and again."""
+    x, w = _cuda(_weights((6144,), 2048, 1, 120, 130)), _cuda(_weights((4096,), 2048, 2))
+    parts = [_product(gpu_ctx, tuple(t[i:i + 2048] for t in x), w, "swiglu") for i in range(0, 6144, 2048)]
+    for _ in range(20):
+        assert torch.equal(_product(gpu_ctx, x, w, "swiglu"), torch.cat(parts))
