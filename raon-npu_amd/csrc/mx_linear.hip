@@ -1,6 +1,12 @@
 // y[n, M'] = RTNE(act(x[n, K] @ W^T + bias) + residual) of microscaled 4-bit rows and weights (mx.h), of one
 // matrix or of each row's expert, on the scaled MFMA: codes and scale bytes go into the matrix pipes as they are
 // held, products are exact, sums fp32.
+//
+// Few rows are bound by the weights' bytes: 4 rows of [260096, 2560] read 354 MB in 67.5 us, 5.2 TB/s (a large copy
+// reaches 4.9, a large write 6.8); the smallest calls by the way from a launch to the first weights and back, 4.3 us
+// for one row of [1536, 2048].  Many rows are bound by the matrix pipes and what feeds them: 6,700 gated rows of
+// [24064, 2560] take 231 us, 3.6 PFLOP/s, 8,192^3 takes 264, 4.2 (the instruction alone, from registers, reaches 6.1 at
+// the power that the card allows; the library's bf16 product 1.2).
 #include <algorithm>
 #include <type_traits>
 
@@ -101,8 +107,11 @@ __device__ __forceinline__ uint4 load_scales(const uint8_t* row, int at, int kb)
 
 // ------------------------------------------------------------------ few rows --
 // Tiles of 16 rows of x.  A wave takes NA fragments of 16 weight rows; the workgroup's four waves are WR
-// stripes of them by WK = 4 / WR parts of K, whose sums meet in LDS and are added in their order.
-// A gated stripe holds 8 NA gate rows, then the up rows of the same outputs.
+// stripes of them by WK = 4 / WR parts of K, whose sums meet in LDS and are added in their order: with one row the card
+// has few workgroups, and shares of K are what keeps enough bytes under way.  Codes go from memory into the operands'
+// registers, 16 bytes a lane; LDS would only delay them, for no wave reads another's weights.  Windows of
+// four steps, the next one requested ahead: 4 rows of [260096, 2560] 67.5 us and 144 without, 32 rows of 128 experts'
+// gated [1536, 2048] 12.1 and 16.8. A gated stripe holds 8 NA gate rows, then the up rows of the same outputs.
 template <int NA, int WR, bool kGated>
 __global__ __launch_bounds__(256) void mx_few_kernel(MxLin a, int n_nt) {
   constexpr int WK = 4 / WR, kRows = 16 * NA, kOut = kGated ? kRows / 2 : kRows, kStride = kRows + 4;
@@ -228,11 +237,17 @@ hipError_t launch_few(const MxLin& a, hipStream_t st) {
 
 // ----------------------------------------------------------------- many rows --
 // Tiles of 32 MA WA weight rows by 32 NB WB rows of x; a wave takes 32 MA by 32 NB of them as 32 x 32 MFMAs
-// of 64 columns.  Codes are copied to LDS past the registers, ahead of their use.  Where K is whole windows of 512 columns
-// (kWhole), in two stages of 256 columns, 128 bytes a row, and the scale bytes of a window likewise, 16 a row; else in three
-// of 128 columns, and scale bytes are fetched by the registers and put beside a stage's codes, a dword a row.  A lane's row of a fragment is lane %
-// 32, and of the four blocks of 128 columns it holds 2 h and 2 h + 1, h = lane / 32, for two MFMA steps.
-// A gated wave's rows are 16 MA gate rows and the up rows of the same outputs.
+// of 64 columns.  Codes are copied to LDS past the registers, ahead of their use.  Where K is whole windows of 512
+// columns (kWhole), in two stages of 256 columns, 128 bytes a row, and the scale bytes of a window likewise, 16 a row;
+// else in three of 128 columns, and scale bytes are fetched by the registers and put beside a stage's codes, a dword a
+// row (pieces of 128 bytes a row are the cheaper ones: in stages of 128 columns 8,192^3 took 345 us, now 264).  A
+// lane's row of a fragment is lane % 32, and of the four blocks of 128 columns it holds 2 h and 2 h + 1, h = lane / 32,
+// for two MFMA steps.  A gated wave's rows are 16 MA gate rows and the up rows of the same outputs.
+//
+// kStays: a workgroup takes tile after tile and requests the next one's first stage before it finishes one, as many
+// workgroups as CUs.  6,700 gated rows of [24064, 2560] take 231 us, with a workgroup a tile 250; 53,600 rows of 128
+// experts' gated [1536, 2048] 138 and 148; 8,192^3 264 and 266.  What is left between tiles is their activation and
+// stores, some 5 us of 22: all the waves are at them at once, for the sums of a second tile have no registers.
 
 template <int MA, int NB, int WA, int WB, bool kWhole, bool kStays>
 struct TileShape {
@@ -422,7 +437,8 @@ __global__ __launch_bounds__(64 * WA * WB, 2) void mx_tiles_kernel(MxLin a, int 
   const int arow = wa * 32 * MA + l32, brow = S::BW + wb * 32 * NB + l32;  // multiples of 32 away: l32's place
   // A lane's chunk of step 0; that of step s is (4 (s / 2) + s % 2) * 16 away, by exclusive or.
   uint32_t aat = arow * S::kRow + (2 * h ^ place(l32 & 15)) * 16u, bat = brow * S::kRow + (2 * h ^ place(l32 & 15)) * 16u;
-  // What addresses are formed from is made new in each turn of the loop: kept, they would take a quarter of the registers.
+  // What addresses are formed from is made new in each turn of the loop: kept, they would take a quarter of the
+  // registers.
   auto fresh = [&] { asm volatile("" : "+v"(aat), "+v"(bat), "+s"(ldb)); };
   // Piece p of a step's fragments, in the order in which the products need them: b0, a0, the other b, the other a.
   constexpr int kPieces = MA + NB, kProducts = MA * NB;
@@ -620,7 +636,8 @@ __global__ __launch_bounds__(64 * WA * WB, 2) void mx_tiles_kernel(MxLin a, int 
             const int r = 32 * m + 8 * g;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const float v = bias[(uint32_t)((r >= kOut ? width : 0) + min(col0 + r % kOut + 4 * (at >> 5) + i, width - 1))];
+              const int c = min(col0 + r % kOut + 4 * (at >> 5) + i, width - 1);
+              const float v = bias[(uint32_t)((r >= kOut ? width : 0) + c)];
 #pragma unroll
               for (int n = 0; n < NB; ++n) acc[m][n][4 * g + i] += v;
             }
@@ -706,7 +723,9 @@ __global__ __launch_bounds__(64 * WA * WB, 2) void mx_tiles_kernel(MxLin a, int 
   }
 }
 
-constexpr size_t kStaying = 256;  // workgroups that take tile after tile: one a CU, which their LDS fills
+// Workgroups that take tile after tile: one a CU, which their LDS fills.  Calls of no more tiles than that do not take
+// them so: the copies for a tile that does not come made 445 rows of [24064, 2560] 27.2 us and not 26.
+constexpr size_t kStaying = 256;
 
 template <int MA, int NB, int WA, int WB, bool kWhole, bool kStays>
 hipError_t launch_tiles(const MxLin& a, hipStream_t st) {
@@ -749,16 +768,16 @@ hipError_t mx_linear_setup() {
 }
 
 // Which kernel serves a call; times in us at 2,560 columns or those given.
-//   Weight rows over all tiles of 16 rows of x, at most kFewRows: the kernel of few rows, for its waves share K.  32 rows of
-//   [4096, 4096] 7.1 and 11.0 with the smallest tiles, 64 rows (16,384) 10.7 and 11.3, 96 rows 14.2 and 11.5.  Fragments
-//   a wave: up to kOneFragment weight rows one (four rows of [4096, 4096] 5.3, two 6.2), above two (64 rows of [1536, 2048] 5.1
-//   and 5.6).  Up to 16 rows of x it serves any matrix, without shared parts of K (16 rows of [24064] 12.6; with two 14.0).
-//   By expert few rows each (under kFewEach) leave the tiles empty: two parts of K, 32 rows of 128 experts' [1536, 2048]
-//   12.1 and 14.8 without, 256 rows 36.7 and 38.4 in tiles of 128 x 64; 512 rows 41.6 and 41.3.
-//   Tiles of 256 x 256 where there are kFillLarge of them (445 rows of [24064] 26.2, in tiles of 128 x 128 27.1; 256 rows
-//   24.2 and 17.9) and, by expert, kFillEach rows each (32,000 rows of 128 experts' [1536, 2048] 110 and 116 in
-//   128 x 64, 16,000 rows 77 and 74).  Else by expert 128 x 64; dense 64 x 64 up to kFillSmall of them (1,024 rows of [4096,
-//   4096] 22.8 and 20.2 in 128 x 128, 2,048 of [1536, 2048] 11.1 and 12.2), above 128 x 128.
+//   Weight rows over all tiles of 16 rows of x, at most kFewRows: the kernel of few rows, for its waves share K.  32
+//   rows of [4096, 4096] 7.1 and 11.0 with the smallest tiles, 64 rows (16,384) 10.7 and 11.3, 96 rows 14.2 and 11.5.
+//   Fragments a wave: up to kOneFragment weight rows one (four rows of [4096, 4096] 5.3, two 6.2), above two (64 rows
+//   of [1536, 2048] 5.1 and 5.6).  Up to 16 rows of x it serves any matrix, without shared parts of K (16 rows of
+//   [24064] 12.6; with two 14.0). By expert few rows each (under kFewEach) leave the tiles empty: two parts of K, 32
+//   rows of 128 experts' [1536, 2048] 12.1 and 14.8 without, 256 rows 36.7 and 38.4 in tiles of 128 x 64; 512 rows 41.6
+//   and 41.3. Tiles of 256 x 256 where there are kFillLarge of them (445 rows of [24064] 26.2, in tiles of 128 x 128
+//   27.1; 256 rows 24.2 and 17.9) and, by expert, kFillEach rows each (32,000 rows of 128 experts' [1536, 2048] 110 and
+//   116 in 128 x 64, 16,000 rows 77 and 74).  Else by expert 128 x 64; dense 64 x 64 up to kFillSmall of them (1,024
+//   rows of [4096, 4096] 22.8 and 20.2 in 128 x 128, 2,048 of [1536, 2048] 11.1 and 12.2), above 128 x 128.
 constexpr size_t kOneFragment = 4096, kFewRows = 16384, kFillSmall = 1000, kFillLarge = 180;
 constexpr int kFewEach = 4, kFillEach = 250;
 
