@@ -772,14 +772,15 @@ hipError_t mx_linear_setup() {
 //   rows of [4096, 4096] 7.1 and 11.0 with the smallest tiles, 64 rows (16,384) 10.7 and 11.3, 96 rows 14.2 and 11.5.
 //   Fragments a wave: up to kOneFragment weight rows one (four rows of [4096, 4096] 5.3, two 6.2), above two (64 rows
 //   of [1536, 2048] 5.1 and 5.6).  Up to 16 rows of x it serves any matrix, without shared parts of K (16 rows of
-//   [24064] 12.6; with two 14.0). By expert few rows each (under kFewEach) leave the tiles empty: two parts of K, 32
+//   [24064] 12.6; with two 14.0).  By expert few rows each (under kFewEach) leave the tiles empty: two parts of K, 32
 //   rows of 128 experts' [1536, 2048] 12.1 and 14.8 without, 256 rows 36.7 and 38.4 in tiles of 128 x 64; 512 rows 41.6
-//   and 41.3. Tiles of 256 x 256 where there are kFillLarge of them (445 rows of [24064] 26.2, in tiles of 128 x 128
-//   27.1; 256 rows 24.2 and 17.9) and, by expert, kFillEach rows each (32,000 rows of 128 experts' [1536, 2048] 110 and
-//   116 in 128 x 64, 16,000 rows 77 and 74).  Else by expert 128 x 64; dense 64 x 64 up to kFillSmall of them (1,024
+//   and 41.3.
+//   Tiles of 256 x 256 where there are kFillLarge of them (445 rows of [24064] 26.2, in tiles of 128 x 128 27.1; 256 rows
+//   24.2 and 17.9) and, by expert, kFillEach rows each (128 experts' gated [1536, 2048]: 24,000 rows 79 and in 128 x 64 98,
+//   16,000 rows 73 and 76, 12,000 rows 72 and 68).  Else by expert 128 x 64; dense 64 x 64 up to kFillSmall of them (1,024
 //   rows of [4096, 4096] 22.8 and 20.2 in 128 x 128, 2,048 of [1536, 2048] 11.1 and 12.2), above 128 x 128.
 constexpr size_t kOneFragment = 4096, kFewRows = 16384, kFillSmall = 1000, kFillLarge = 180;
-constexpr int kFewEach = 4, kFillEach = 250;
+constexpr int kFewEach = 4, kFillEach = 120;
 
 hipError_t launch_mx_linear(const MxLin& a, hipStream_t st) {
   const size_t n = a.n, M = a.M, groups = a.offsets ? a.n_experts : 1;

@@ -478,7 +478,9 @@ def test_more_tiles_than_workgroups(gpu_ctx, T, M, K, act):
 
 
 @pytest.mark.parametrize("counts,M,K,act", [([3000, 1, 0, 5000, 257, 2700], 2056, 512, "swiglu"),
-                                            ([300] * 20 + [0, 4000, 1, 255, 256], 1536, 1024, "none")])
+                                            ([300] * 20 + [0, 4000, 1, 255, 256], 1536, 1024, "none"),
+                                            ([130] * 63 + [0, 256], 1536, 512, "swiglu"),
+                                            ([125] * 70, 1540, 544, "swiglu")])
 def test_more_experts_tiles_than_workgroups(gpu_ctx, counts, M, K, act):
     _check_experts(gpu_ctx, counts, M, K, act, True, True, behind=700)
 
