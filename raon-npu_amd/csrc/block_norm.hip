@@ -17,7 +17,7 @@
 //
 // Bound by HBM.  A row is held in the registers of W waves (eight columns a thread and V of these), which meet in
 // LDS once for each sum: every element is read and written once.  6,700 rows of 2,560 in bf16 through both norms and a
-// gate, 137 MB: 31.4 us, 4.4 TB/s, two copies of as many bytes 29.4; one row 3 us, a launch and a trip to memory.
+// gate, 137 MB: 30 us, 4.6 TB/s, two copies of as many bytes 29.4; one row 3 us, a launch and a trip to memory.
 // Their gradients: 4,099 rows of 2,048 in bf16, 101 MB, 27.6 us and 4 for the weights' sums over the workgroups; 4,099
 // of 2,560 in fp32, 252 MB, 67 us together; 445 of 2,560 in fp32 13 and 4, where two rows a workgroup, one behind the
 // other, are the time.
@@ -64,6 +64,29 @@ __device__ __forceinline__ void row_sum(float (&v)[N], float (*slots)[N], int wa
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] += slots[first + w][i];
   }
+}
+
+// The sum over a row of its chunks' of 512 columns, a wave's s[v] that of chunk v W + wave: each over the lanes, then in
+// the chunks' order, so that no result depends on how many waves a row has.
+template <int V>
+__device__ __forceinline__ float chunks_sum(float (&s)[V], float* slots, int wave, int W) {
+#pragma unroll
+  for (int v = 0; v < V; ++v) s[v] = lanes_sum(s[v]);
+  float sum;
+  if (W == 1) {
+    sum = s[0];
+#pragma unroll
+    for (int v = 1; v < V; ++v) sum += s[v];
+  } else {
+    if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) slots[v * W + wave] = s[v];
+    }
+    __syncthreads();
+    sum = slots[0];
+    for (int i = 1; i < V * W; ++i) sum += slots[i];
+  }
+  return sum;
 }
 
 template <int DT>
@@ -128,7 +151,7 @@ __device__ __forceinline__ void load_columns(const float* p, const Columns<V, kW
 // A workgroup is blockDim / (64 W) rows; more than one only of one wave each.
 template <int DT, int V, bool kWide, bool kBlock, bool kFull, bool kOnce>
 __global__ __launch_bounds__(64 * kMaxWaves) void norm_kernel(NormArgs a, int W, size_t first) {
-  __shared__ float slots[2][kMaxWaves][1];
+  __shared__ float slots[2][kNormMaxWidth / 512 + kMaxWaves];  // the last chunks may be none
   const int wave = wave_id(), H = a.H, group = wave / W;
   const size_t t = first + (size_t)blockIdx.x * ((blockDim.x >> 6) / W) + group;
   if (t >= (size_t)a.T) return;
@@ -147,14 +170,15 @@ __global__ __launch_bounds__(64 * kMaxWaves) void norm_kernel(NormArgs a, int W,
     for (int v = 0; v < V; ++v) to_float<DT>(b[v], u[v]);
     const float one = a.gate_kind == RMOE_GATE_ROW ? static_cast<const float*>(a.gate)[t] : 1.f;
     if (a.post) {
-      float s[1] = {0.f};
+      float s[V];
 #pragma unroll
-      for (int v = 0; v < V; ++v)
+      for (int v = 0; v < V; ++v) {
+        s[v] = 0.f;
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-          if (col.counts(v, i)) s[0] = fmaf(u[v][i], u[v][i], s[0]);
-      row_sum<1>(s, slots[0], wave, 0, W);
-      const float n = inv_rms(s[0], H, a.eps);
+          if (col.counts(v, i)) s[v] = fmaf(u[v][i], u[v][i], s[v]);
+      }
+      const float n = inv_rms(chunks_sum<V>(s, slots[0], wave, W), H, a.eps);
 #pragma unroll
       for (int v = 0; v < V; ++v)
 #pragma unroll
@@ -176,14 +200,15 @@ __global__ __launch_bounds__(64 * kMaxWaves) void norm_kernel(NormArgs a, int W,
     for (int v = 0; v < V; ++v) to_float<DT>(r[v], y[v]);
   }
   if (!a.pre) return;
-  float s[1] = {0.f};
+  float s[V];
 #pragma unroll
-  for (int v = 0; v < V; ++v)
+  for (int v = 0; v < V; ++v) {
+    s[v] = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      if (col.counts(v, i)) s[0] = fmaf(y[v][i], y[v][i], s[0]);
-  row_sum<1>(s, slots[1], wave, 0, W);
-  const float m = inv_rms(s[0], H, a.eps);
+      if (col.counts(v, i)) s[v] = fmaf(y[v][i], y[v][i], s[v]);
+  }
+  const float m = inv_rms(chunks_sum<V>(s, slots[1], wave, W), H, a.eps);
   const int P = (H + kMxBlock - 1) / kMxBlock * kMxBlock;
 #pragma unroll
   for (int v = 0; v < V; ++v) {
@@ -408,13 +433,36 @@ hipError_t norm_with(const NormArgs& a, hipStream_t st) {
   // Block and residual of 6,700 rows of 2,560 (69 MB): 34.7 us, read past the caches' order 32.2; of 2,000 rows, which
   // are in the caches from the call before, 11.4 and 12.2.
   const bool once = wide && (size_t)a.T * a.H * sizeof(typename RowElem<DT>::T) * (a.block ? 2 : 1) >= kOnceBytes;
-  const int V = a.H > 512 * kMaxWaves ? 2 : 1, W = (a.H + 512 * V - 1) / (512 * V);
-  const int rows = W == 1 ? 4 : 1;
-  auto pick = [&](auto block, auto full) {
+  // A row to as many waves as it has chunks for, or of many rows to one wave, or two or four, of up to kManyChunks a
+  // thread: more bytes under way on each CU, fewer waves that meet.  6,700 rows in bf16 through both norms and a gate: of
+  // 2,048 25.6 us and 26.8 in as many waves, of 2,560 30.1 and 32, of 4,096 48 and 49.7; in fp32 of 2,560 58.4 and 63.4; a
+  // norm alone into codes of 2,560 12.3 and 15, of 2,048 10.5 and 11.3.  1,500 rows of 2,560 9.4 and 8.9, a norm alone 5.0
+  // and 5.3; 1,000 rows alone 3.9 and 4.0, one row 3.0 and 2.4.  Without a norm after the block 6,700 rows of 2,560 take
+  // 27.7 and 25, with a gate by element 34.8 and 34.1.
+  constexpr int kManyRows = 3000, kManyAlone = 1500, kManyChunks = 5;
+  const bool many = wide && (a.block ? a.post && a.gate_kind != RMOE_GATE_FULL && a.T >= kManyRows : a.T >= kManyAlone);
+  int V = a.H > 512 * kMaxWaves ? 2 : 1, W = (a.H + 512 * V - 1) / (512 * V);
+  if (many) {
+    for (W = 1; a.H > 512 * kManyChunks * W;) W *= 2;
+    V = (a.H + 512 * W - 1) / (512 * W);
+  }
+  const int rows = W == 1 && !many ? 4 : 1;
+  auto at = [&](auto block, auto full, auto chunks) {
     constexpr bool B = decltype(block)::value, F = decltype(full)::value;
-    if (once) return V == 1 ? norm_kernel<DT, 1, true, B, F, true> : norm_kernel<DT, 2, true, B, F, true>;
-    return V == 1 ? (wide ? norm_kernel<DT, 1, true, B, F, false> : norm_kernel<DT, 1, false, B, F, false>)
-                  : (wide ? norm_kernel<DT, 2, true, B, F, false> : norm_kernel<DT, 2, false, B, F, false>);
+    constexpr int N = decltype(chunks)::value;
+    if constexpr (N <= 2)
+      if (!wide) return norm_kernel<DT, N, false, B, F, false>;
+    return once ? norm_kernel<DT, N, true, B, F, true> : norm_kernel<DT, N, true, B, F, false>;
+  };
+  auto pick = [&](auto block, auto full) {
+    const std::integral_constant<int, 1> one;
+    const std::integral_constant<int, 2> two;
+    if constexpr (!decltype(full)::value) {
+      if (V == 3) return at(block, full, std::integral_constant<int, 3>());
+      if (V == 4) return at(block, full, std::integral_constant<int, 4>());
+      if (V == 5) return at(block, full, std::integral_constant<int, 5>());
+    }
+    return V == 1 ? at(block, full, one) : at(block, full, two);
   };
   auto* kernel = a.gate_kind == RMOE_GATE_FULL ? pick(std::true_type(), std::true_type())
                  : a.block                     ? pick(std::true_type(), std::false_type())

@@ -405,7 +405,8 @@ class Context:
     def norm_dev(self, x_dev, weight_dev, h_dev=None, codes_dev=None, scales_dev=None, eps: float = 1e-6, stream=None):
         """The norm before a block: ``h = x (mean x^2 + eps)^-1/2 weight`` by row, in fp32, rounded once.  x and h [T, H]
         bfloat16 (or int16 bits), float16 or float32, weight float32 [H], H up to 8192; codes and scales: h as microscaled 4-bit rows
-        (``mx_quantize_dev`` of it), with h or without.  Asynchronous; allocates nothing and uses no scratch."""
+        (``mx_quantize_dev`` of it), with h or without.  A row's bits do not depend on the rows beside it.  Asynchronous;
+        allocates nothing and uses no scratch."""
         self._norm(None, x_dev, None, None, None, 1.0, weight_dev, h_dev, codes_dev, scales_dev, eps, stream)
 
     def residual_norm_dev(self, block_dev, residual_dev, y_dev, post_weight_dev=None, gate_dev=None, scale: float = 1.0,

@@ -336,3 +336,41 @@ def test_past_32_bits(gpu_ctx):
     for k in ("dpre", "dpost", "dgate"):  # the rows are dealt to other groups: another order of the sums
         size = _backward64({k: None if v is None else v.cpu() for k, v in few.items()}, y2.cpu(), "column", 0.75)[k][1]
         assert bool(((a[k] - b[k]).abs().cpu().double() <= (T / 512 + 168) * 4 * U * size).all()), k
+
+
+@pytest.mark.parametrize("H", [40, 1000, 1536, 2048, 2560, 2568, 4104, 5000, 5128, 8192, 2559])
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("post,gate", [(True, "column"), (True, "row"), (False, "none"), (True, "full")])
+def test_many_rows(gpu_ctx, H, dtype, post, gate):
+    """Rows of many are held by fewer waves: the same bits as of few, in place too, and right."""
+    T = 3009
+    s = _case(T, H, dtype, post, gate, H)
+    d = _dev(s)
+    h = torch.full_like(d["block"], 7)
+    codes = torch.full((T, -(-H // 32) * 16), 0xEE, dtype=torch.uint8, device="cuda")
+    scales = torch.full((T, -(-H // 32)), 0xEE, dtype=torch.uint8, device="cuda")
+    y = _run(gpu_ctx, d, 0.75, h=h, codes=codes, scales=scales)
+    some = slice(0, T, 100)
+    part = {k: v[some] if v is not None and v.shape[0] == T else v for k, v in s.items()}
+    want, size = _forward64(part, 0.75)
+    rel, least = _half_step(dtype)
+    off, bound = (y[some].cpu().double() - want).abs(), 24 * U * size + want.abs() * rel * (1 + 2.0 ** -10) + least
+    assert bool((off <= bound).all()), float((off / bound).max())
+    _check_h(h[some].cpu(), y[some].cpu(), s["pre"], dtype)
+    for a in range(0, T, 1003):
+        few = {k: v[a:a + 1003].contiguous() if v is not None and v.shape[0] == T else v for k, v in d.items()}
+        h1 = torch.full_like(few["block"], 7)
+        c1, s1 = torch.zeros_like(codes[:1003]), torch.zeros_like(scales[:1003])
+        assert torch.equal(_run(gpu_ctx, few, 0.75, h=h1, codes=c1, scales=s1), y[a:a + 1003])
+        assert torch.equal(h1, h[a:a + 1003]) and torch.equal(c1, codes[a:a + 1003]) and torch.equal(s1, scales[a:a + 1003])
+    h2, c2, s2 = torch.full_like(h, 7), torch.zeros_like(codes), torch.zeros_like(scales)
+    gpu_ctx.norm_dev(y, d["pre"], h2, c2, s2, eps=EPS, stream=_stream())
+    assert torch.equal(h, h2) and torch.equal(codes, c2) and torch.equal(scales, s2)
+    gpu_ctx.norm_dev(y, d["pre"], codes_dev=c2.zero_(), scales_dev=s2.zero_(), eps=EPS, stream=_stream())
+    assert torch.equal(codes, c2) and torch.equal(scales, s2)
+    e = _dev(s)
+    _run(gpu_ctx, e, 0.75, y=e["residual"], h=e["block"])
+    assert torch.equal(e["residual"], y) and torch.equal(e["block"], h)
+    e = _dev(s)
+    _run(gpu_ctx, e, 0.75, y=e["block"], h=h2)
+    assert torch.equal(e["block"], y) and torch.equal(h2, h)
