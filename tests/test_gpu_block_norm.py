@@ -374,3 +374,33 @@ def test_many_rows(gpu_ctx, H, dtype, post, gate):
     e = _dev(s)
     _run(gpu_ctx, e, 0.75, y=e["block"], h=h2)
     assert torch.equal(e["block"], y) and torch.equal(h2, h)
+
+
+def test_vectors_at_any_address_beside_aligned_rows(gpu_ctx):
+    for T in (9, 3001):
+        for dtype in TYPES:
+            d = _dev(_case(T, 264, dtype, True, "column", 7))
+            h = torch.empty_like(d["block"])
+            y = _run(gpu_ctx, d, 0.5, h=h)
+            e = dict(d)
+            for k in ("post", "gate", "pre"):
+                buf = torch.full((264 + 9,), float("nan"), device="cuda")
+                e[k] = buf[3:3 + 264]
+                e[k].copy_(d[k])
+            h2 = torch.empty_like(h)
+            assert torch.equal(_run(gpu_ctx, e, 0.5, h=h2), y) and torch.equal(h, h2)
+            a, b = _backward(gpu_ctx, d, y, "column", 0.5), _backward(gpu_ctx, e, y, "column", 0.5)
+            for k in a:
+                assert torch.equal(a[k], b[k]), k
+
+
+def test_more_rows_than_a_launch_takes(gpu_ctx):
+    T, H, n = (1 << 26) + 70, 8, 200
+    g = torch.Generator().manual_seed(2)
+    few, w = torch.randn(n, H, generator=g).to(torch.bfloat16).cuda(), torch.randn(H, generator=g).cuda()
+    x = torch.zeros(T, H, dtype=torch.bfloat16, device="cuda")
+    x[:n], x[-n:] = few, few
+    h, h2 = torch.full_like(x, 7), torch.full_like(few, 7)
+    gpu_ctx.norm_dev(few, w, h2, eps=EPS, stream=_stream())
+    gpu_ctx.norm_dev(x, w, h, eps=EPS, stream=_stream())
+    assert torch.equal(h[:n], h2) and torch.equal(h[-n:], h2) and not h[n:-n].any()

@@ -491,3 +491,25 @@ def test_further_tiles_are_the_same_each_time(gpu_ctx):
     parts = [_product(gpu_ctx, tuple(t[i:i + 2048] for t in x), w, "swiglu") for i in range(0, 6144, 2048)]
     for _ in range(20):
         assert torch.equal(_product(gpu_ctx, x, w, "swiglu"), torch.cat(parts))
+
+
+def test_many_tiles_captured_with_new_offsets(gpu_ctx):
+    """Products of more tiles than workgroups in a graph: replayed with other rows and other offsets, eager work between."""
+    n, E, M, K = 6000, 4, 4096, 512
+    x, w = _cuda(_weights((n,), K, 1, 120, 130)), _cuda(_weights((E, M), K, 2))
+    off = torch.tensor([0, 1500, 3000, 4500, 6000], dtype=torch.int32, device="cuda")
+    y = torch.zeros(n, M, dtype=torch.bfloat16, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        _product(gpu_ctx, x, w, y=y, offsets=off, stream=torch.cuda.current_stream())
+    for turn, counts in enumerate(([1500] * 4, [6000, 0, 0, 0], [1, 0, 0, 5999], [0, 0, 0, 0], [257, 2000, 3, 600])):
+        for t, s in zip(x, _weights((n,), K, 10 + turn, 120, 130)):
+            t.copy_(s)
+        off.copy_(torch.tensor([0, *np.cumsum(counts)], dtype=torch.int32))
+        y.fill_(7)
+        graph.replay()
+        torch.cuda.synchronize()
+        want = _product(gpu_ctx, x, w, y=torch.full_like(y, 7), offsets=off)
+        assert bool((want[sum(counts):] == 7).all()) and (not counts[0] or not bool((want[0] == 7).all()))
+        assert torch.equal(y, want), counts
