@@ -2,7 +2,7 @@
 // matrix or of each row's expert, on the scaled MFMA: codes and scale bytes go into the matrix pipes as they are
 // held, products are exact, sums fp32.
 //
-// Few rows are bound by the weights' bytes: 4 rows of [260096, 2560] read 354 MB in 67.5 us, 5.2 TB/s (a large copy
+// Few rows are bound by the weights' bytes: 4 rows of [260096, 2560] read 354 MB in 65.7 us, 5.4 TB/s (a large copy
 // reaches 4.9, a large write 6.8); the smallest calls by the way from a launch to the first weights and back, 4.3 us
 // for one row of [1536, 2048].  Many rows are bound by the matrix pipes and what feeds them: 6,700 gated rows of
 // [24064, 2560] take 231 us, 3.6 PFLOP/s, 8,192^3 takes 264, 4.2 (the instruction alone, from registers, reaches 6.1 at
@@ -109,8 +109,8 @@ __device__ __forceinline__ uint4 load_scales(const uint8_t* row, int at, int kb)
 // Tiles of 16 rows of x.  A wave takes NA fragments of 16 weight rows; the workgroup's four waves are WR
 // stripes of them by WK = 4 / WR parts of K, whose sums meet in LDS and are added in their order: with one row the card
 // has few workgroups, and shares of K are what keeps enough bytes under way.  Codes go from memory into the operands'
-// registers, 16 bytes a lane; LDS would only delay them, for no wave reads another's weights.  Windows of
-// four steps, the next one requested ahead: 4 rows of [260096, 2560] 67.5 us and 144 without, 32 rows of 128 experts'
+// registers, 16 bytes a lane; LDS would only delay them, for no wave reads another's weights (from three rows on tiles are
+// the faster ones all the same).  Windows of four steps, the next one requested ahead: 4 rows of [260096, 2560] 67.5 us and 144 without, 32 rows of 128 experts'
 // gated [1536, 2048] 12.1 and 16.8. A gated stripe holds 8 NA gate rows, then the up rows of the same outputs.
 template <int NA, int WR, bool kGated>
 __global__ __launch_bounds__(256) void mx_few_kernel(MxLin a, int n_nt) {
@@ -771,15 +771,19 @@ hipError_t mx_linear_setup() {
 //   Weight rows over all tiles of 16 rows of x, at most kFewRows: the kernel of few rows, for its waves share K.  32
 //   rows of [4096, 4096] 7.1 and 11.0 with the smallest tiles, 64 rows (16,384) 10.7 and 11.3, 96 rows 14.2 and 11.5.
 //   Fragments a wave: up to kOneFragment weight rows one (four rows of [4096, 4096] 5.3, two 6.2), above two (64 rows
-//   of [1536, 2048] 5.1 and 5.6).  Up to 16 rows of x it serves any matrix, without shared parts of K (16 rows of
-//   [24064] 12.6; with two 14.0).  By expert few rows each (under kFewEach) leave the tiles empty: two parts of K, 32
-//   rows of 128 experts' [1536, 2048] 12.1 and 14.8 without, 256 rows 36.7 and 38.4 in tiles of 128 x 64; 512 rows 41.6
-//   and 41.3.
+//   of [1536, 2048] 5.1 and 5.6).  One or two rows of x have it without shared parts of K where there are kFillSmall
+//   tiles of 64 weight rows (one row of [260096] 64.3 and 66.5 in tiles of 128 x 64, four 67.2 and 65.7; one row of
+//   [24064] 10.3 and 9.4 in 64 x 64).
+//   Up to kFlat rows of x the flattest tiles: 128 x 64 where there are kFillSmall of 64 x 64 (32 rows of [260096] 77, in
+//   64 x 64 80, in 256 x 256 102; 65 rows 101, 110 and 111; 128 rows 116, 137 and 116), else 64 x 64 (16 rows of [24064]
+//   9.4 and without LDS 11.8, 32 rows 9.8 and 18).
+//   By expert few rows each (under kFewEach) leave the tiles empty: two parts of K, 32 rows of 128 experts' [1536, 2048]
+//   12.1 and 14.8 without, 256 rows 36.7 and 38.4 in tiles of 128 x 64; 512 rows 41.6 and 41.3.
 //   Tiles of 256 x 256 where there are kFillLarge of them (445 rows of [24064] 26.2, in tiles of 128 x 128 27.1; 256 rows
-//   24.2 and 17.9) and, by expert, kFillEach rows each (128 experts' gated [1536, 2048]: 24,000 rows 79 and in 128 x 64 98,
-//   16,000 rows 73 and 76, 12,000 rows 72 and 68).  Else by expert 128 x 64; dense 64 x 64 up to kFillSmall of them (1,024
-//   rows of [4096, 4096] 22.8 and 20.2 in 128 x 128, 2,048 of [1536, 2048] 11.1 and 12.2), above 128 x 128.
-constexpr size_t kOneFragment = 4096, kFewRows = 16384, kFillSmall = 1000, kFillLarge = 180;
+//   24.2 and 17.9) and, by expert, kFillEach rows each (128 experts' gated [1536, 2048]: 24,000 rows 79 and in 128 x 64
+//   98, 16,000 rows 73 and 76, 12,000 rows 72 and 68).  Else by expert 128 x 64; dense 64 x 64 up to kFillSmall of them
+//   (1,024 rows of [4096, 4096] 22.8 and 20.2 in 128 x 128, 2,048 of [1536, 2048] 11.1 and 12.2), above 128 x 128.
+constexpr size_t kOneFragment = 4096, kFewRows = 16384, kFlat = 96, kFillSmall = 1000, kFillLarge = 180;
 constexpr int kFewEach = 4, kFillEach = 120;
 
 hipError_t launch_mx_linear(const MxLin& a, hipStream_t st) {
@@ -798,9 +802,11 @@ hipError_t launch_mx_linear(const MxLin& a, hipStream_t st) {
     if (n >= kFillEach * groups && tiles(256, 256) >= kFillLarge) return large();
     return pick_tiles<2, 1, 2, 2>(a, st);
   }
-  if (wide || n <= 16) return launch_few<2, 4>(a, st);
+  const bool fill = tiles(64, 64) >= kFillSmall;
+  if (wide || (n <= 2 && fill)) return launch_few<2, 4>(a, st);
+  if (n <= kFlat) return fill ? pick_tiles<2, 1, 2, 2>(a, st) : pick_tiles<1, 1, 2, 2>(a, st);
   if (tiles(256, 256) >= kFillLarge) return large();
-  return tiles(64, 64) < kFillSmall ? pick_tiles<1, 1, 2, 2>(a, st) : pick_tiles<2, 2, 2, 2>(a, st);
+  return fill ? pick_tiles<2, 2, 2, 2>(a, st) : pick_tiles<1, 1, 2, 2>(a, st);
 }
 
 }  // namespace rmoe
