@@ -109,9 +109,10 @@ __device__ __forceinline__ uint4 load_scales(const uint8_t* row, int at, int kb)
 // Tiles of 16 rows of x.  A wave takes NA fragments of 16 weight rows; the workgroup's four waves are WR
 // stripes of them by WK = 4 / WR parts of K, whose sums meet in LDS and are added in their order: with one row the card
 // has few workgroups, and shares of K are what keeps enough bytes under way.  Codes go from memory into the operands'
-// registers, 16 bytes a lane; LDS would only delay them, for no wave reads another's weights (from three rows on tiles are
-// the faster ones all the same).  Windows of four steps, the next one requested ahead: 4 rows of [260096, 2560] 67.5 us and 144 without, 32 rows of 128 experts'
-// gated [1536, 2048] 12.1 and 16.8. A gated stripe holds 8 NA gate rows, then the up rows of the same outputs.
+// registers, 16 bytes a lane, for no wave reads another's weights (of large matrices from three rows on LDS tiles are
+// the faster ones all the same: more bytes under way for their registers).  Windows of four steps, the next one
+// requested ahead: 4 rows of [260096, 2560] 67.5 us and 144 without, 32 rows of 128 experts' gated [1536, 2048] 12.1 and
+// 16.8.  A gated stripe holds 8 NA gate rows, then the up rows of the same outputs.
 template <int NA, int WR, bool kGated>
 __global__ __launch_bounds__(256) void mx_few_kernel(MxLin a, int n_nt) {
   constexpr int WK = 4 / WR, kRows = 16 * NA, kOut = kGated ? kRows / 2 : kRows, kStride = kRows + 4;
