@@ -513,3 +513,9 @@ def test_many_tiles_captured_with_new_offsets(gpu_ctx):
         want = _product(gpu_ctx, x, w, y=torch.full_like(y, 7), offsets=off)
         assert bool((want[sum(counts):] == 7).all()) and (not counts[0] or not bool((want[0] == 7).all()))
         assert torch.equal(y, want), counts
+
+
+@pytest.mark.parametrize("T,M,K,act", [(1, 64010, 96, "swiglu"), (2, 64003, 512, "none"), (3, 64010, 160, "situ"),
+                                       (40, 64010, 512, "swiglu"), (96, 33001, 288, "silu"), (97, 33001, 96, "none")])
+def test_few_rows_of_many_weights(gpu_ctx, T, M, K, act):
+    _check_product(gpu_ctx, T, M, K, act, True, True)
