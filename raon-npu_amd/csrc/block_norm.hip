@@ -13,7 +13,9 @@
 //   dr = c D,   du = g D,   v = du wpost
 //   db = n v - b n^3 (sum_j v_j b_j) / H,               dwpost = sum_t du b n
 //   dg = D u, summed over what g is shared by.
-// n and m are formed again from b and y, which have to be read in any case.
+// n and m are formed again from b and y, which have to be read in any case.  m a - y m^3 S / H, S = sum a y, is formed as
+// m (a - (y m) (m S / H)), and db likewise: y m is at most sqrt(H) and m S / H at most max |a|, where m^3 leaves fp32 for
+// rows past 2^42 and, with an eps as small, for those below 2^-42.
 //
 // Bound by HBM.  A row is held in the registers of W waves (eight columns a thread and V of these), which meet in
 // LDS once for each sum: every element is read and written once.  6,700 rows of 2,560 in bf16 through both norms and a
@@ -297,13 +299,14 @@ __global__ __launch_bounds__(64 * kMaxWaves, 2) void norm_backward_kernel(NormGr
     row_sum<3>(s, first_sums[turn], wave, own, W);
     const float n = kBlock && a.f.post ? inv_rms(s[0], H, a.f.eps) : 1.f;
     if (a.dh) {
-      const float m = inv_rms(s[1], H, a.f.eps), k = s[2] * inv_H * m * m * m;
+      const float m = inv_rms(s[1], H, a.f.eps), k = s[2] * inv_H * m;
 #pragma unroll
       for (int v = 0; v < V; ++v)
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          d[v][i] += fmaf(dh[v][i] * pre[v][i], m, -(y[v][i] * k));
-          const float p = fmaf(dh[v][i] * y[v][i], m, dpre[v][i]);
+          const float ym = y[v][i] * m;
+          d[v][i] = fmaf(fmaf(-ym, k, dh[v][i] * pre[v][i]), m, d[v][i]);
+          const float p = fmaf(dh[v][i], ym, dpre[v][i]);
           dpre[v][i] = live ? p : dpre[v][i];
         }
     }
@@ -339,13 +342,13 @@ __global__ __launch_bounds__(64 * kMaxWaves, 2) void norm_backward_kernel(NormGr
       }
       if (a.f.post || by_row) row_sum<2>(q, second_sums[turn], wave, own, W);
       if (by_row && a.dgate && col.first == 0 && live) static_cast<float*>(a.dgate)[t] = q[1];
-      const float k = q[0] * inv_H * n * n * n;
+      const float k = q[0] * inv_H * n;
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         Chunk<DT> o;
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-          o.v[i] = RowElem<DT>::put(a.f.post ? fmaf(d[v][i] * post[v][i], n, -(b[v][i] * k)) : d[v][i]);
+          o.v[i] = RowElem<DT>::put(a.f.post ? fmaf(-(b[v][i] * n), k, d[v][i] * post[v][i]) * n : d[v][i]);
         if (live) store_row<DT>(a.dblock, t, col, v, o);
       }
     }

@@ -404,3 +404,36 @@ def test_more_rows_than_a_launch_takes(gpu_ctx):
     gpu_ctx.norm_dev(few, w, h2, eps=EPS, stream=_stream())
     gpu_ctx.norm_dev(x, w, h, eps=EPS, stream=_stream())
     assert torch.equal(h[:n], h2) and torch.equal(h[-n:], h2) and not h[n:-n].any()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=str)
+@pytest.mark.parametrize("H", [72, 2560, 4104])
+@pytest.mark.parametrize("row,grad,eps", [(55, 10, 1e-5), (54, -10, 1e-5), (-63, -10, 2.0 ** -126), (-55, -20, 2.0 ** -110)])
+def test_gradients_of_rows_far_from_one(gpu_ctx, dtype, H, row, grad, eps):
+    """Rows of 2^55, and of 2^-63 with an eps as small: the cube of their inverse root, times the row's sum, leaves fp32, the
+    gradients do not.  Rows of 2^row through both norms, dh of 2^grad: dresidual is about 2^(grad - row), dblock 2^(grad - 2 row).
+    Bounds as above: 512 u of the terms' magnitudes and one rounding."""
+    T = 9
+    s = _case(T, H, dtype, True, "none", H)
+    for k, e in (("block", row), ("residual", row), ("dh", grad)):
+        s[k] = (s[k].double() * 2.0 ** e).to(dtype)
+    d = _dev(s)
+    y = s["residual"]
+    dblock, dresidual = torch.full_like(d["block"], 7), torch.full_like(d["block"], 7)
+    dpre, dpost = torch.empty(H, device="cuda"), torch.empty(H, device="cuda")
+    gpu_ctx.residual_norm_backward_dev(None, d["dh"], d["block"], d["residual"], dblock, dresidual,
+                                       torch.empty(gpu_ctx.norm_backward_work(T, H), device="cuda"), post_weight_dev=d["post"],
+                                       dpost_weight_dev=dpost, pre_weight_dev=d["pre"], dpre_weight_dev=dpre, eps=eps,
+                                       stream=_stream())
+    e32 = float(np.float32(eps))
+    b, y, dh, pre, post = (t.double() for t in (s["block"], y, s["dh"], s["pre"], s["post"]))
+    m, n = (y.square().mean(1, keepdim=True) + e32).rsqrt(), (b.square().mean(1, keepdim=True) + e32).rsqrt()
+    a = dh * pre
+    D = m * (a - y * m * (m * (a * y).mean(1, keepdim=True)))
+    A = m * (a.abs() + (y * m).abs() * (m * (a * y).abs().mean(1, keepdim=True)))
+    v, vA = D * post, A * post.abs()
+    db = n * (v - b * n * (n * (v * b).mean(1, keepdim=True)))
+    dbA = n * (vA + (b * n).abs() * (n * (vA * b.abs()).mean(1, keepdim=True)))
+    want = {"dresidual": (D, A), "dblock": (db, dbA), "dpre": ((dh * y * m).sum(0), (dh * y * m).abs().sum(0)),
+            "dpost": ((D * b * n).sum(0), (A * (b * n).abs()).sum(0))}
+    _check_gradients({"dresidual": dresidual, "dblock": dblock, "dpre": dpre, "dpost": dpost}, want, T, dtype)
