@@ -437,3 +437,38 @@ def test_gradients_of_rows_far_from_one(gpu_ctx, dtype, H, row, grad, eps):
     want = {"dresidual": (D, A), "dblock": (db, dbA), "dpre": ((dh * y * m).sum(0), (dh * y * m).abs().sum(0)),
             "dpost": ((D * b * n).sum(0), (A * (b * n).abs()).sum(0))}
     _check_gradients({"dresidual": dresidual, "dblock": dblock, "dpre": dpre, "dpost": dpost}, want, T, dtype)
+
+
+@pytest.mark.parametrize("T,H", [(445, 2560), (4099, 2048), (2500, 264), (2500, 259), (700, 1536), (600, 4096), (600, 4095)])
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("post,gate", [(True, "column"), (True, "row"), (True, "full"), (False, "none")])
+def test_backward_of_more_rows_than_a_pass_takes(gpu_ctx, T, H, dtype, post, gate):
+    """Workgroups that go on to further rows, the next one requested while a row is worked on: of one to eight waves a row,
+    the last pass with rows for some of the workgroups and some of a workgroup's waves; in place too, where the next row's
+    gradients have been read when a row's are written."""
+    s = _case(T, H, dtype, post, gate, T + H + 2)
+    d, scale = _dev(s), 0.75
+    y = _run(gpu_ctx, d, scale)
+    got = _backward(gpu_ctx, d, y, gate, scale)
+    _check_gradients(got, _backward64(s, y.cpu(), gate, scale), T, dtype)
+    e = _dev(s)
+    _backward(gpu_ctx, e, y, gate, scale, out={"dresidual": e["dy"], "dblock": e["dh"]})
+    assert torch.equal(e["dy"], got["dresidual"]) and torch.equal(e["dh"], got["dblock"])
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("T,H", [(300, 2560), (2500, 264), (300, 5000), (40, 8191)])
+def test_norm_backward_of_many_rows(gpu_ctx, T, H, dtype):
+    """Without a block, dx over dy too."""
+    s = _case(T, H, dtype, False, "none", 6)
+    d = _dev(s)
+    x, work = d["residual"], torch.empty(gpu_ctx.norm_backward_work(T, H), device="cuda")
+    dx, dw = torch.empty_like(x), torch.empty(H, device="cuda")
+    for dy in (False, True):
+        gpu_ctx.norm_backward_dev(d["dh"], x, d["pre"], dx, work, dweight_dev=dw, dy_dev=d["dy"] if dy else None, eps=EPS,
+                                  stream=_stream())
+        want = _backward64(s, s["residual"], "none", 1.0, dy=dy)
+        _check_gradients({"dresidual": dx, "dpre": dw}, {k: want[k] for k in ("dresidual", "dpre")}, T, dtype)
+    dw2 = torch.empty_like(dw)
+    gpu_ctx.norm_backward_dev(d["dh"], x, d["pre"], d["dy"], work, dweight_dev=dw2, dy_dev=d["dy"], eps=EPS, stream=_stream())
+    assert torch.equal(d["dy"], dx) and torch.equal(dw2, dw)
