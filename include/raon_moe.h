@@ -424,8 +424,10 @@ int rmoe_mx_quantize_dev(rmoe_ctx* ctx, const void* x_dev, int dtype, int T, int
 /* y[T, M'] = RTNE(act(x W^T + bias) + residual) of quantized rows x [T, K] and weights [M, K], K a multiple of 32 (of
  * another width: quantized rows end in zeros, so both sides' P is the K here): products exact, sums and epilogue fp32,
  * rounded once to bf16.  act, bias, residual and M' as in rmoe_linear_act_dev; any M (even when gated).  A scale byte
- * of 255 in a row of x or W makes its results NaN.  Codes 16-byte aligned.  Sums may be added in another order for
- * another number of rows, so that a row's last bits may depend on it. */
+ * of 255 in a row of x or W makes its results NaN.  Codes 16-byte aligned; scales at any address (at one that is not a
+ * multiple of 16 calls of many rows and of a K that is a multiple of 512 take the kernel of other K, which is slower).
+ * Sums may be added in another order for another number of rows or such scales, so that a row's last bits may depend on
+ * them.  T x M below 2^28 always fits a launch; larger calls whose tiles would take 2^32 threads are refused. */
 int rmoe_mx_linear_dev(rmoe_ctx* ctx, const void* x_codes_dev, const void* x_scales_dev, int T, int K,
                        const void* w_codes_dev, const void* w_scales_dev, int M, const float* bias_dev, int act,
                        float gate_beta, float value_beta, const void* residual_dev, void* y_dev, void* stream);

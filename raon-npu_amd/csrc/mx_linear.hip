@@ -224,16 +224,24 @@ __global__ __launch_bounds__(256) void mx_few_kernel(MxLin a, int n_nt) {
   }
 }
 
+// The launch that serves a call: `fits` says whether its threads are within the 2^32 that a launch takes.
+struct Plan {
+  void (*kernel)(MxLin, int);
+  size_t grid;
+  unsigned threads;
+  size_t lds;
+  int n_nt;
+  bool fits;
+};
+
 template <int NA, int WR>
-hipError_t launch_few(const MxLin& a, hipStream_t st) {
+Plan plan_few(const MxLin& a) {
   const bool gated = act_gated(a.act);
   const int width = gated ? a.M / 2 : a.M, out = 16 * NA * WR / (gated ? 2 : 1), n_nt = (width + out - 1) / out;
   const size_t mt = a.offsets ? std::min<size_t>(a.n, (size_t)a.n / 16 + a.n_experts) : ((size_t)a.n + 15) / 16;
   const size_t grid = 8 * ((mt * n_nt + 7) / 8);
-  if (grid * 256 >= (size_t)1 << 32) return hipErrorInvalidValue;
   auto* kernel = gated ? mx_few_kernel<NA, WR, true> : mx_few_kernel<NA, WR, false>;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(256), 0, st, a, n_nt);
-  return hipGetLastError();
+  return Plan{kernel, grid, 256, 0, n_nt, grid * 256 < (size_t)1 << 32};
 }
 
 // ----------------------------------------------------------------- many rows --
@@ -729,23 +737,22 @@ __global__ __launch_bounds__(64 * WA * WB, 2) void mx_tiles_kernel(MxLin a, int 
 constexpr size_t kStaying = 256;
 
 template <int MA, int NB, int WA, int WB, bool kWhole, bool kStays>
-hipError_t launch_tiles(const MxLin& a, hipStream_t st) {
+Plan plan_tiles(const MxLin& a) {
   typedef TileShape<MA, NB, WA, WB, kWhole, kStays> S;
   const bool gated = act_gated(a.act);
   const int width = gated ? a.M / 2 : a.M, out = S::BW / (gated ? 2 : 1), n_nt = (width + out - 1) / out;
   const size_t mt = a.offsets ? std::min<size_t>(a.n, (size_t)a.n / S::BT + a.n_experts) : ((size_t)a.n + S::BT - 1) / S::BT;
   const size_t all = 8 * ((mt * n_nt + 7) / 8), grid = kStays ? std::min(all, kStaying) : all;
-  if (all * S::kThreads >= (size_t)1 << 32) return hipErrorInvalidValue;
   auto* kernel = gated ? mx_tiles_kernel<MA, NB, WA, WB, kWhole, kStays, true>
                        : mx_tiles_kernel<MA, NB, WA, WB, kWhole, kStays, false>;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(S::kThreads), S::lds(gated), st, a, n_nt);
-  return hipGetLastError();
+  // Of workgroups that stay the tiles count too: their numbers are kept to 24 bits.
+  return Plan{kernel, grid, S::kThreads, S::lds(gated), n_nt, all * S::kThreads < (size_t)1 << 32};
 }
 // stays: more tiles than kStaying are taken by as many workgroups.
 template <int MA, int NB, int WA, int WB, bool kStays = false>
-hipError_t pick_tiles(const MxLin& a, hipStream_t st) {
+Plan pick_tiles(const MxLin& a) {
   const bool whole = a.K % 512 == 0 && ((reinterpret_cast<uintptr_t>(a.xs) | reinterpret_cast<uintptr_t>(a.ws)) & 15) == 0;
-  return whole ? launch_tiles<MA, NB, WA, WB, true, kStays>(a, st) : launch_tiles<MA, NB, WA, WB, false, false>(a, st);
+  return whole ? plan_tiles<MA, NB, WA, WB, true, kStays>(a) : plan_tiles<MA, NB, WA, WB, false, false>(a);
 }
 template <int MA, int NB, int WA, int WB, bool kWhole, bool kStays>
 hipError_t setup_tiles() {
@@ -756,16 +763,6 @@ hipError_t setup_tiles() {
     e = hipFuncSetAttribute((const void*)mx_tiles_kernel<MA, NB, WA, WB, kWhole, kStays, false>,
                             hipFuncAttributeMaxDynamicSharedMemorySize, (int)S::lds(false));
   return e;
-}
-
-}  // namespace
-
-// Allow the tiles of more than 64 KB of dynamic LDS theirs (up to 142).
-hipError_t mx_linear_setup() {
-  for (const hipError_t e : {setup_tiles<4, 2, 2, 4, true, true>(), setup_tiles<4, 2, 2, 4, true, false>(),
-                             setup_tiles<4, 2, 2, 4, false, false>(), setup_tiles<2, 2, 2, 2, true, false>()})
-    if (e != hipSuccess) return e;
-  return hipSuccess;
 }
 
 // Which kernel serves a call; times in us at 2,560 columns or those given.
@@ -787,27 +784,45 @@ hipError_t mx_linear_setup() {
 constexpr size_t kOneFragment = 4096, kFewRows = 16384, kFlat = 96, kFillSmall = 1000, kFillLarge = 180;
 constexpr int kFewEach = 4, kFillEach = 120;
 
-hipError_t launch_mx_linear(const MxLin& a, hipStream_t st) {
+Plan plan_mx_linear(const MxLin& a) {
   const size_t n = a.n, M = a.M, groups = a.offsets ? a.n_experts : 1;
   auto tiles = [&](size_t weights, size_t rows) { return (n + rows - 1) / rows * ((M + weights - 1) / weights); };
   const size_t rows = M * (a.offsets ? std::min(n, n / 16 + groups) : (n + 15) / 16);
-  if (rows <= kOneFragment) return launch_few<1, 1>(a, st);
-  if (rows <= kFewRows) return launch_few<2, 1>(a, st);
+  if (rows <= kOneFragment) return plan_few<1, 1>(a);
+  if (rows <= kFewRows) return plan_few<2, 1>(a);
   // The tiles' offsets within a matrix's scales and 16 rows' codes take 32 bits.
   const bool wide = a.K > 1 << 20 || M * (a.K / kMxBlock) >= (size_t)1 << 32;
   auto large = [&] {
-    return tiles(256, 256) > kStaying ? pick_tiles<4, 2, 2, 4, true>(a, st) : pick_tiles<4, 2, 2, 4, false>(a, st);
+    return tiles(256, 256) > kStaying ? pick_tiles<4, 2, 2, 4, true>(a) : pick_tiles<4, 2, 2, 4, false>(a);
   };
   if (a.offsets) {
-    if (wide || n < kFewEach * groups) return launch_few<2, 2>(a, st);
+    if (wide || n < kFewEach * groups) return plan_few<2, 2>(a);
     if (n >= kFillEach * groups && tiles(256, 256) >= kFillLarge) return large();
-    return pick_tiles<2, 1, 2, 2>(a, st);
+    return pick_tiles<2, 1, 2, 2>(a);
   }
   const bool fill = tiles(64, 64) >= kFillSmall;
-  if (wide || (n <= 2 && fill)) return launch_few<2, 4>(a, st);
-  if (n <= kFlat) return fill ? pick_tiles<2, 1, 2, 2>(a, st) : pick_tiles<1, 1, 2, 2>(a, st);
+  if (wide || (n <= 2 && fill)) return plan_few<2, 4>(a);
+  if (n <= kFlat) return fill ? pick_tiles<2, 1, 2, 2>(a) : pick_tiles<1, 1, 2, 2>(a);
   if (tiles(256, 256) >= kFillLarge) return large();
-  return fill ? pick_tiles<2, 2, 2, 2>(a, st) : pick_tiles<1, 1, 2, 2>(a, st);
+  return fill ? pick_tiles<2, 2, 2, 2>(a) : pick_tiles<1, 1, 2, 2>(a);
+}
+
+}  // namespace
+
+// Allow the tiles of more than 64 KB of dynamic LDS theirs (up to 142).
+hipError_t mx_linear_setup() {
+  for (const hipError_t e : {setup_tiles<4, 2, 2, 4, true, true>(), setup_tiles<4, 2, 2, 4, true, false>(),
+                             setup_tiles<4, 2, 2, 4, false, false>(), setup_tiles<2, 2, 2, 2, true, false>()})
+    if (e != hipSuccess) return e;
+  return hipSuccess;
+}
+
+bool mx_linear_fits(const MxLin& a) { return plan_mx_linear(a).fits; }
+
+hipError_t launch_mx_linear(const MxLin& a, hipStream_t st) {
+  const Plan p = plan_mx_linear(a);
+  hipLaunchKernelGGL(p.kernel, dim3((unsigned)p.grid), dim3(p.threads), p.lds, st, a, p.n_nt);
+  return hipGetLastError();
 }
 
 }  // namespace rmoe

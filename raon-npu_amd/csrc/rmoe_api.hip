@@ -429,6 +429,7 @@ int check_mx(rmoe_ctx* ctx, const rmoe::MxLin& L) {
   if ((reinterpret_cast<uintptr_t>(L.y) | reinterpret_cast<uintptr_t>(L.residual)) & 1 ||
       (reinterpret_cast<uintptr_t>(L.bias) | reinterpret_cast<uintptr_t>(L.offsets)) & 3)
     return fail(RMOE_EINVAL, "operands must be aligned to their element type");
+  if (!rmoe::mx_linear_fits(L)) return fail(RMOE_EINVAL, "%d rows by %d are too many for one call", L.n, L.M);
   const size_t n = L.n, M = L.M, groups = L.offsets ? L.n_experts : 1;
   const Span y{L.y, n * (gated ? M / 2 : M) * 2};
   const Span res{L.residual == L.y ? nullptr : L.residual, y.n};  // y itself: added in place
@@ -941,9 +942,7 @@ static int run_mx_linear(rmoe_ctx* ctx, const rmoe::MxLin& L, void* stream) {
   TRY(check_mx(ctx, L));
   OnDevice dev(ctx);
   HIP_TRY(dev.status);
-  const hipError_t e = rmoe::launch_mx_linear(L, pick_stream(ctx, stream));
-  if (e == hipErrorInvalidValue) return fail(RMOE_EINVAL, "%d rows by %d are too many for one call", L.n, L.M);
-  HIP_TRY(e);
+  HIP_TRY(rmoe::launch_mx_linear(L, pick_stream(ctx, stream)));
   return RMOE_OK;
 }
 

@@ -585,6 +585,7 @@ struct MxLin {
   uint16_t* y;
 };
 hipError_t mx_linear_setup();  // once per device before the first call
+bool mx_linear_fits(const MxLin& a);  // whether a launch takes the call's tiles: sizes and pointers only, no device
 hipError_t launch_mx_linear(const MxLin& a, hipStream_t st);
 
 // The norms before and after a block (block_norm.hip).  block null: y is not computed, h is the norm of residual.

@@ -1,4 +1,4 @@
-"""Which kernel of csrc/mx_linear.hip serves a microscaled product, restated from launch_mx_linear, and product shapes that
+"""Which kernel of csrc/mx_linear.hip serves a microscaled product, restated from plan_mx_linear, and product shapes that
 together reach each of them, gated and not, dense and by expert, with K in whole windows of 512 columns and not."""
 
 from __future__ import annotations

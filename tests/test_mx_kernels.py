@@ -13,8 +13,8 @@ def _shapes(pattern: str, text: str) -> set:
 
 def test_every_kernel_is_reached():
     rule = SOURCE.read_text()
-    rule = rule[rule.index("hipError_t launch_mx_linear("):]
-    few, tiles = _shapes(r"launch_few<([\d, ]+)>", rule), _shapes(r"pick_tiles<([\d, ]+?)(?:, (?:true|false))?>", rule)
+    rule = rule[rule.index("Plan plan_mx_linear("):]
+    few, tiles = _shapes(r"plan_few<([\d, ]+)>", rule), _shapes(r"pick_tiles<([\d, ]+?)(?:, (?:true|false))?>", rule)
     assert few == {(1, 1), (2, 1), (2, 2), (2, 4)} and tiles == {(1, 1, 2, 2), (2, 1, 2, 2), (2, 2, 2, 2), (4, 2, 2, 4)}
     dense = {kernel_of(*s) for s in DENSE}
     experts = {kernel_of(sum(counts), M, K, len(counts)) for counts, M, K in EXPERTS}

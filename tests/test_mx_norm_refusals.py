@@ -208,3 +208,17 @@ def test_null_context():
                     ("rmoe_residual_norm_dev", 16), ("rmoe_residual_norm_backward_dev", 20)):
         with pytest.raises(ValueError, match="null context"):
             _lib.check(getattr(lib, name)(None, *([0] * n)))
+
+
+@pytest.mark.parametrize("n,m,e", [((1 << 31) - 1, 1 << 16, None), (1 << 23, 1 << 18, None), (1000, 1 << 30, 256),
+                                   ((1 << 31) - 1, 1 << 12, 256)])
+@pytest.mark.parametrize("act", [_lib.ACT_NONE, _lib.ACT_SWIGLU])
+def test_more_tiles_than_a_launch_takes(raw, n, m, e, act):  # noqa: F811
+    """Refused before the device is looked at."""
+    far = [1 << (48 + i) for i in range(8)]
+    a = (far[0], far[1], n, 32, far[2], far[3], m, None), (act, 0.0, 0.0, None, far[5])
+    with pytest.raises(ValueError, match="too many"):
+        if e is None:
+            raw("rmoe_mx_linear_dev", *a[0], *a[1], None)
+        else:
+            raw("rmoe_mx_experts_linear_dev", *a[0][:7], far[6], e, None, *a[1], None)
