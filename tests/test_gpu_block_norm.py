@@ -472,3 +472,42 @@ def test_norm_backward_of_many_rows(gpu_ctx, T, H, dtype):
     dw2 = torch.empty_like(dw)
     gpu_ctx.norm_backward_dev(d["dh"], x, d["pre"], d["dy"], work, dweight_dev=dw2, dy_dev=d["dy"], eps=EPS, stream=_stream())
     assert torch.equal(d["dy"], dx) and torch.equal(dw2, dw)
+
+
+@pytest.mark.parametrize("T,H", [(5, 96), (300, 2560), (300, 5001)])
+@pytest.mark.parametrize("gate", ["column", "row", "full"])
+def test_gradients_that_are_not_wanted(gpu_ctx, T, H, gate):
+    """Any of the weights' and the gate's gradients left out: the others keep their bits."""
+    d = _dev(_case(T, H, torch.bfloat16, True, gate, 3))
+    y = _run(gpu_ctx, d, 0.75)
+    want = _backward(gpu_ctx, d, y, gate, 0.75)
+    work = torch.empty(gpu_ctx.norm_backward_work(T, H), device="cuda")
+    for some in range(8):
+        o = {k: torch.full_like(v, 7) for k, v in want.items()}
+        wanted = {k: some >> i & 1 for i, k in enumerate(("dpre", "dpost", "dgate"))}
+        gpu_ctx.residual_norm_backward_dev(
+            d["dy"], d["dh"], d["block"], y, o["dblock"], o["dresidual"], work.fill_(float("nan")), post_weight_dev=d["post"],
+            dpost_weight_dev=o["dpost"] if wanted["dpost"] else None, gate_dev=d["gate"],
+            dgate_dev=o["dgate"] if wanted["dgate"] else None, scale=0.75, pre_weight_dev=d["pre"],
+            dpre_weight_dev=o["dpre"] if wanted["dpre"] else None, eps=EPS, stream=_stream())
+        for k in want:
+            assert torch.equal(o[k], want[k] if wanted.get(k, True) else torch.full_like(o[k], 7)), (k, some)
+
+
+@pytest.mark.parametrize("T,H", [(4, 96), (300, 2560), (3009, 1000)])
+def test_one_tensor_as_block_and_residual(gpu_ctx, T, H):
+    """Inputs may be the same: y = scale x + gate N(x) post, over x too."""
+    for dtype in TYPES:
+        s = _case(T, H, dtype, True, "column", 4)
+        s["residual"] = s["block"]
+        d = _dev(s)
+        d["residual"] = d["block"]
+        h = torch.empty_like(d["block"])
+        y = _run(gpu_ctx, d, 0.75, h=h)
+        want, size = _forward64(s, 0.75)
+        rel, least = _half_step(dtype)
+        off, bound = (y.cpu().double() - want).abs(), 24 * U * size + want.abs() * rel * (1 + 2.0 ** -10) + least
+        assert bool((off <= bound).all()), float((off / bound).max())
+        h2 = torch.empty_like(h)
+        _run(gpu_ctx, d, 0.75, y=d["block"], h=h2)
+        assert torch.equal(d["block"], y) and torch.equal(h2, h)

@@ -519,3 +519,22 @@ def test_many_tiles_captured_with_new_offsets(gpu_ctx):
                                        (40, 64010, 512, "swiglu"), (96, 33001, 288, "silu"), (97, 33001, 96, "none")])
 def test_few_rows_of_many_weights(gpu_ctx, T, M, K, act):
     _check_product(gpu_ctx, T, M, K, act, True, True)
+
+
+def test_quantize_the_widest_rows(gpu_ctx):
+    """Rows of 2^30 columns and of a few fewer (a last block that is filled up): their last and first columns."""
+    few = _rows(4, 4096, 3, torch.bfloat16).cuda()
+    for K in (1 << 30, (1 << 30) - 37):
+        x = torch.zeros(2, K, dtype=torch.bfloat16, device="cuda")
+        P, width = -(-K // 32) * 32, 4096 - (-K % 32)
+        x[:, :4096], x[:, -width:] = few[:2], few[2:, :width]
+        c = torch.full((2, P // 2), 0xEE, dtype=torch.uint8, device="cuda")
+        s = torch.full((2, P // 32), 0xEE, dtype=torch.uint8, device="cuda")
+        gpu_ctx.mx_quantize_dev(x, c, s, stream=_stream())
+        for rows, part, got in ((few[:2], slice(0, 2048), slice(0, 128)),
+                                (few[2:, :width].contiguous(), slice(P // 2 - 2048, None), slice(P // 32 - 128, None))):
+            c1, s1 = _quantize(gpu_ctx, rows)
+            assert torch.equal(c[:, part], c1) and torch.equal(s[:, got], s1)
+        assert not c[:, 2048:-2048].any() and not s[:, 128:-128].any()
+        del x, c, s
+        torch.cuda.empty_cache()
