@@ -20,7 +20,7 @@
 // Bound by HBM.  A row is held in the registers of W waves (eight columns a thread and V of these), which meet in
 // LDS once for each sum: every element is read and written once.  6,700 rows of 2,560 in bf16 through both norms and a
 // gate, 137 MB: 30 us, 4.6 TB/s, two copies of as many bytes 29.4; one row 3 us, a launch and a trip to memory.
-// Their gradients: 4,099 rows of 2,048 in bf16, 101 MB, 27.6 us and 4 for the weights' sums over the workgroups; 4,099
+// Their gradients: 4,099 rows of 2,048 in bf16, 101 MB, 28 us and 4 for the weights' sums over the workgroups; 4,099
 // of 2,560 in fp32, 252 MB, 67 us together; 445 of 2,560 in fp32 13 and 4, where two rows a workgroup, one behind the
 // other, are the time.
 #include <algorithm>

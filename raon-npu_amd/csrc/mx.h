@@ -50,7 +50,6 @@ struct alignas(16) Chunk {
 // Loads and stores of the columns c..c+7 of a row `width` wide: by 16 bytes, or (kWide false: rows that are not
 // aligned to 16 bytes or end inside a chunk) one by one, with zeros past the end.  kOnce: read past the caches' order of
 // use, for rows of kOnceBytes and more that are not read again.
-constexpr size_t kOnceBytes = (size_t)64 << 20;
 template <int DT, bool kWide, bool kOnce = false>
 __device__ __forceinline__ Chunk<DT> load_chunk(const void* row, int c, int width) {
   const auto* p = static_cast<const typename RowElem<DT>::T*>(row) + c;

@@ -2,11 +2,12 @@
 // matrix or of each row's expert, on the scaled MFMA: codes and scale bytes go into the matrix pipes as they are
 // held, products are exact, sums fp32.
 //
-// Few rows are bound by the weights' bytes: 4 rows of [260096, 2560] read 354 MB in 65.7 us, 5.4 TB/s (a large copy
+// Few rows are bound by the weights' bytes: 4 rows of [260096, 2560] read 354 MB in 66.7 us, 5.3 TB/s (a large copy
 // reaches 4.9, a large write 6.8); the smallest calls by the way from a launch to the first weights and back, 4.3 us
 // for one row of [1536, 2048].  Many rows are bound by the matrix pipes and what feeds them: 6,700 gated rows of
-// [24064, 2560] take 231 us, 3.6 PFLOP/s, 8,192^3 takes 264, 4.2 (the instruction alone, from registers, reaches 6.1 at
-// the power that the card allows; the library's bf16 product 1.2).
+// [24064, 2560] take 243 to 250 us (medians on several cards; single runs from 232), 3.3 to 3.4 PFLOP/s, 8,192^3 takes
+// 269 to 275, 4.0 to 4.1 (the instruction alone, from registers, reaches 6.1 at the power that the card allows; the
+// library's bf16 product 1.2).
 #include <algorithm>
 #include <type_traits>
 
@@ -111,8 +112,8 @@ __device__ __forceinline__ uint4 load_scales(const uint8_t* row, int at, int kb)
 // has few workgroups, and shares of K are what keeps enough bytes under way.  Codes go from memory into the operands'
 // registers, 16 bytes a lane, for no wave reads another's weights (of large matrices from three rows on LDS tiles are
 // the faster ones all the same: more bytes under way for their registers).  Windows of four steps, the next one
-// requested ahead: 4 rows of [260096, 2560] 67.5 us and 144 without, 32 rows of 128 experts' gated [1536, 2048] 12.1 and
-// 16.8.  A gated stripe holds 8 NA gate rows, then the up rows of the same outputs.
+// requested ahead: 32 rows of 128 experts' gated [1536, 2048] take 12.1 us, step by step 16.8; one row of [260096, 2560]
+// takes 64 to 66.  A gated stripe holds 8 NA gate rows, then the up rows of the same outputs.
 template <int NA, int WR, bool kGated>
 __global__ __launch_bounds__(256) void mx_few_kernel(MxLin a, int n_nt) {
   constexpr int WK = 4 / WR, kRows = 16 * NA, kOut = kGated ? kRows / 2 : kRows, kStride = kRows + 4;
@@ -249,14 +250,16 @@ Plan plan_few(const MxLin& a) {
 // of 64 columns.  Codes are copied to LDS past the registers, ahead of their use.  Where K is whole windows of 512
 // columns (kWhole), in two stages of 256 columns, 128 bytes a row, and the scale bytes of a window likewise, 16 a row;
 // else in three of 128 columns, and scale bytes are fetched by the registers and put beside a stage's codes, a dword a
-// row (pieces of 128 bytes a row are the cheaper ones: in stages of 128 columns 8,192^3 took 345 us, now 264).  A
+// row (pieces of 128 bytes a row are the cheaper ones: in stages of 128 columns 8,192^3 took 345 us, now 270; 40,200
+// rows of 128 experts' [2560, 1088] take 197 us, of K = 1024 144).  A
 // lane's row of a fragment is lane % 32, and of the four blocks of 128 columns it holds 2 h and 2 h + 1, h = lane / 32,
 // for two MFMA steps.  A gated wave's rows are 16 MA gate rows and the up rows of the same outputs.
 //
 // kStays: a workgroup takes tile after tile and requests the next one's first stage before it finishes one, as many
-// workgroups as CUs.  6,700 gated rows of [24064, 2560] take 231 us, with a workgroup a tile 250; 53,600 rows of 128
-// experts' gated [1536, 2048] 138 and 148; 8,192^3 264 and 266.  What is left between tiles is their activation and
-// stores, some 5 us of 22: all the waves are at them at once, for the sums of a second tile have no registers.
+// workgroups as CUs.  In turn: 6,700 gated rows of [24064, 2560] 249 us, with a workgroup a tile 257; 53,600 rows of 128
+// experts' gated [1536, 2048] 145 and 152; 8,192^3 275 and 278.  What is left between tiles is their activation and
+// stores, some fifth of the time: all the waves are at them at once, for the sums of a second tile have no registers.
+// SiTU's divisions and exponentials make it more: the 6,700 rows take 309 us with it, the 53,600 184.
 
 template <int MA, int NB, int WA, int WB, bool kWhole, bool kStays>
 struct TileShape {

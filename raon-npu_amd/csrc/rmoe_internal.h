@@ -65,6 +65,8 @@ __device__ __forceinline__ uint4 load_stream16(const uint8_t* p) {
   const u32x4_t v = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(p));
   return make_uint4(v.x, v.y, v.z, v.w);
 }
+// Rows of this many bytes in all and more are read so (the callers' comments have what it measured).
+constexpr size_t kOnceBytes = (size_t)64 << 20;
 
 // acc += a.lo*b.lo + a.hi*b.hi with bf16 pairs packed in dwords (v_dot2c_f32_bf16).
 __device__ __forceinline__ float dot2_bf16(uint32_t a, uint32_t b, float acc) {

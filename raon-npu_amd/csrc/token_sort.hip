@@ -59,14 +59,6 @@ struct Elem<RMOE_DT_F32> {
   static __device__ __forceinline__ T put(float v) { return v; }
 };
 
-// Sorted rows of this many bytes and more are summed with non-temporal loads: they are read once
-// and do not fit the caches anyway (6,700 tokens alone, other buffers each time: 58 -> 49 us; the
-// combine's gradient gains nothing).  H 2,048, k 8, sort and combine in turn (the same buffers /
-// others each time): 220 MB of rows 92 / 100 us without the hint, 89 / 93 with it; 67 MB 35 / 36 and
-// 36 / 33; 34 MB 20 / 22 and 23 / 22.  (Storing them so makes the sort alone 60 -> 54 us and the two
-// 100 -> 113: what comes next finds less of them in the cache.)
-constexpr size_t kOnceBytes = (size_t)64 << 20;
-
 // N elements in one load: 16 bytes, or (N = 1) one element where rows are not 16-byte aligned.
 template <int DT, int N>
 struct Pack {
@@ -610,6 +602,12 @@ template <int DT, int N>
 hipError_t sum_with(SumArgs a, hipStream_t st) {
   a.nslab = (a.H + 64 * N - 1) / (64 * N);
   const int total = a.T;
+  // Sorted rows of kOnceBytes and more are summed with non-temporal loads: they are read once
+  // and do not fit the caches anyway (6,700 tokens alone, other buffers each time: 58 -> 49 us; the
+  // combine's gradient gains nothing).  H 2,048, k 8, sort and combine in turn (the same buffers /
+  // others each time): 220 MB of rows 92 / 100 us without the hint, 89 / 93 with it; 67 MB 35 / 36 and
+  // 36 / 33; 34 MB 20 / 22 and 23 / 22.  (Storing them so makes the sort alone 60 -> 54 us and the two
+  // 100 -> 113: what comes next finds less of them in the cache.)
   const bool once = (size_t)a.n * a.H * dtype_bytes(DT) >= kOnceBytes;
   const size_t step = std::max<size_t>(1, kMaxGroups * 4 / a.nslab);
   for (size_t t0 = 0; t0 < (size_t)total; t0 += step) {

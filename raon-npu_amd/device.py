@@ -12,8 +12,9 @@ import ctypes as C
 import numpy as np
 
 from . import _lib
-from ._lib import (ACT_GELU, ACT_GELU_TANH, ACT_NONE, ACT_SILU, ACT_SITU, ACT_SWIGLU, BUNDLE_B1, BUNDLE_B2, DT_BF16, DT_F16,
-                   DT_F32, GATE_COLUMN, GATE_FULL, GATE_NONE, GATE_ROW, PART_DOWN, PART_GATE_UP, SCORE_SIGMOID, SCORE_SOFTMAX, call, check, new_bytes, ptr)
+from ._lib import (ACT_GELU, ACT_GELU_TANH, ACT_NONE, ACT_SILU, ACT_SITU, ACT_SWIGLU, BUNDLE_B1, BUNDLE_B2, DT_BF16,
+                   DT_F16, DT_F32, GATE_COLUMN, GATE_FULL, GATE_NONE, GATE_ROW, PART_DOWN, PART_GATE_UP, SCORE_SIGMOID,
+                   SCORE_SOFTMAX, call, check, new_bytes, ptr)
 from .geometry import MoeGeometry
 
 
@@ -363,7 +364,8 @@ class Context:
         [T, K / 32], W codes [M, K / 2] and scales [M, K / 32], K a multiple of 32; products exact, fp32 sums, rounded
         once to bf16.  act, bias float32 [M], residual (y itself: in place) and y [T, M] or, gated, [T, M / 2] as in
         ``Matrix.linear_act_dev``.  Asynchronous; allocates nothing and uses no scratch (capturable, any number of calls
-        at once).  A row's last bits may depend on T."""
+        at once).  Scales whose address is a multiple of 16 serve many rows of K a multiple of 512 faster.  A row's last
+        bits may depend on T and on that."""
         code, gb, vb, gated = _epilogue_act(act, gate_beta, value_beta)
         dev, (T, K), M = self.device, _shape2(x_codes_dev, "x codes"), _shape2(w_codes_dev, "w codes")[0]
         G = K // 16
@@ -404,18 +406,18 @@ class Context:
     # ------------------------------------------------- norms around a block --
     def norm_dev(self, x_dev, weight_dev, h_dev=None, codes_dev=None, scales_dev=None, eps: float = 1e-6, stream=None):
         """The norm before a block: ``h = x (mean x^2 + eps)^-1/2 weight`` by row, in fp32, rounded once.  x and h [T, H]
-        bfloat16 (or int16 bits), float16 or float32, weight float32 [H], H up to 8192; codes and scales: h as microscaled 4-bit rows
-        (``mx_quantize_dev`` of it), with h or without.  A row's bits do not depend on the rows beside it.  Asynchronous;
-        allocates nothing and uses no scratch."""
+        bfloat16 (or int16 bits), float16 or float32, weight float32 [H], H up to 8192; codes and scales: h as microscaled
+        4-bit rows (``mx_quantize_dev`` of it), with h or without.  A row's bits do not depend on the rows beside it.
+        Asynchronous; allocates nothing and uses no scratch."""
         self._norm(None, x_dev, None, None, None, 1.0, weight_dev, h_dev, codes_dev, scales_dev, eps, stream)
 
     def residual_norm_dev(self, block_dev, residual_dev, y_dev, post_weight_dev=None, gate_dev=None, scale: float = 1.0,
                           pre_weight_dev=None, h_dev=None, codes_dev=None, scales_dev=None, eps: float = 1e-6, stream=None):
         """What stands between two blocks, in one pass: ``y = scale * residual + gate * N(block) post_weight`` and ``h =
         N(y) pre_weight``, N(v) = v (mean v^2 + eps)^-1/2 by row.  Rows [T, H] of one type; post_weight None: no norm after
-        the block; gate None, float32 [H] (by column), float32 [T, 1] (by row) or [T, H] of the rows' type; pre_weight float32 [H] with h, or
-        codes and scales (h as microscaled 4-bit rows), or both, or none of them.  y may be residual or block, h may be
-        block."""
+        the block; gate None, float32 [H] (by column), float32 [T, 1] (by row) or [T, H] of the rows' type; pre_weight
+        float32 [H] with h, or codes and scales (h as microscaled 4-bit rows), or both, or none of them.  y may be
+        residual or block, h may be block."""
         if block_dev is None or y_dev is None:
             raise ValueError("residual_norm_dev takes a block's result and y")
         self._norm(block_dev, residual_dev, y_dev, post_weight_dev, gate_dev, scale, pre_weight_dev, h_dev, codes_dev,
@@ -458,14 +460,16 @@ class Context:
                                    scale: float = 1.0, pre_weight_dev=None, dpre_weight_dev=None, eps: float = 1e-6,
                                    stream=None):
         """Gradients of ``residual_norm_dev`` from dy and dh (one of them may be None; without dh no pre_weight), from its
-        block and its y: dblock, dresidual, and where given float32 dpost_weight and dpre_weight [H] and dgate (as the gate).
-        dresidual may be dy, dblock may be dh.  work: float32 [norm_backward_work(T, H)] or more, this call's alone while it runs."""
+        block and its y: dblock, dresidual, and where given float32 dpost_weight and dpre_weight [H] and dgate (as the
+        gate).  dresidual may be dy, dblock may be dh.  work: float32 [norm_backward_work(T, H)] or more, this call's alone
+        while it runs."""
         if block_dev is None or dblock_dev is None:
             raise ValueError("residual_norm_backward_dev takes a block's result and dblock")
         self._norm_backward(dy_dev, dh_dev, block_dev, y_dev, dblock_dev, dresidual_dev, work_dev, post_weight_dev,
                             dpost_weight_dev, gate_dev, dgate_dev, scale, pre_weight_dev, dpre_weight_dev, eps, stream)
 
-    def _norm_backward(self, dy, dh, block, y, dblock, dresidual, work, post, dpost, gate, dgate, scale, pre, dpre, eps, stream):
+    def _norm_backward(self, dy, dh, block, y, dblock, dresidual, work, post, dpost, gate, dgate, scale, pre, dpre, eps,
+                       stream):
         dt, dev = _row_type(y, "y"), self.device
         rows = T, H = _shape2(y, "y")
         vector = (H,)
